@@ -1,5 +1,5 @@
 """Builds libfklhip.so: the C-ABI runtime plus the ahead-of-time compiled gfx950 kernels of every chain
-signature listed in csrc/aot_signatures.txt.  `python -m fusedkernellibrary_amd.build` rebuilds it in place."""
+signature listed in csrc/aot_signatures.txt and the attention kernels under csrc/attention.  `python -m fusedkernellibrary_amd.build` rebuilds it in place."""
 from __future__ import annotations
 
 import concurrent.futures as cf
@@ -134,7 +134,8 @@ def build_library(verbose: bool = True) -> str:
     sigs = read_signatures()
     units = generate_units(sigs)
     os.makedirs(OBJ_DIR, exist_ok=True)
-    srcs = units + [os.path.join(CSRC, "fklhip_runtime.cpp"), os.path.join(CSRC, "jit.cpp"), generate_jit_sources()]
+    attention = [os.path.join(CSRC, "attention", name) for name in sorted(os.listdir(os.path.join(CSRC, "attention"))) if name.endswith((".hip", ".cpp"))]
+    srcs = attention + units + [os.path.join(CSRC, "fklhip_runtime.cpp"), os.path.join(CSRC, "jit.cpp"), generate_jit_sources()]
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(_compile, srcs))
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB + ".tmp", *objs, "-lhiprtc"]

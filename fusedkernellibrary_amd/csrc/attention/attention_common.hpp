@@ -1,0 +1,70 @@
+// attention_common.hpp -- arguments and launchers of the kernels around a quantised key-value cache.
+#pragma once
+
+#include <stdint.h>
+
+#include <fklhip.h>
+
+namespace fkattn {
+
+// ---- arguments (plain values; the host fills them from the C ABI's structures after its checks) ----------------------
+
+struct Rows {
+    char* data;
+    int64_t token_stride, head_stride;      // bytes
+};
+
+struct Cache {
+    char *k, *v;
+    float *k_scale, *v_scale;
+    uint32_t pages, page_log, kv_heads;
+    int codes;
+};
+
+struct HeadArgs {
+    Rows q, k, v, q_out, k_out;
+    const void *q_weight, *k_weight;
+    const float *cos, *sin;
+    const int32_t *positions, *slots;
+    Cache cache;
+    uint32_t tokens, table_rows;
+    uint32_t q_heads, kv_heads, head_dim, rot_dim;
+    uint32_t q_chunks, k_chunks;            // chunks of kHeads heads; the chunks behind them are values, kQuad heads each
+    int pairs;
+    float eps;
+};
+
+struct ReadArgs {
+    Cache cache;
+    Rows k, v;
+    const int32_t* slots;
+    uint32_t tokens, head_dim, k_chunks;
+};
+
+struct AttentionArgs {
+    Rows q, out;
+    float* lse;
+    const int32_t *page_table, *context, *q_start;
+    const uint64_t* mask;
+    Cache cache;
+    float *partial, *partial_lse;           // [tokens * q_heads][splits](head_dim)
+    int64_t page_table_stride;
+    uint32_t tokens, batch, max_new, max_context, mask_words;
+    uint32_t q_heads, group;                // query heads per key head
+    uint32_t splits, chunk;                 // keys of a sequence are shared out in chunks, one to a split
+    uint32_t group_magic, heads_magic;      // x / group and x / kv_heads as a multiplication (see divide)
+    int type;
+    float scale;
+};
+
+// Launchers (defined next to their kernels). Grids are laid out by the callers' arguments alone.
+struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
+int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
+int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
+int launch_merge(const AttentionArgs& a, uint32_t head_dim, void* stream);
+// Row tiles (of 16 query rows) that a workgroup takes; how a call's keys are shared out.
+struct AttentionPlan { uint32_t row_tiles, row_blocks, splits, chunk; };
+AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim);
+template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
+
+} // namespace fkattn

@@ -1,0 +1,376 @@
+// rows.hip -- the kernels that work on whole heads of tokens: RMS norm and rotation of queries and keys, the quantising
+// write into a paged cache, and the read back.
+//
+// All are bound by memory (a head of 128 elements is 256 bytes in and 256 or 132 out for some 20 operations per element),
+// so what counts is that every access is wide, that all of a lane's rows are requested before the first is used, and
+// that one launch does everything a token needs.
+#include "attention_device.hpp"
+
+namespace fkattn {
+namespace {
+
+// A group of lanes takes a head, eight elements to a lane. Rotation pairs elements half of the rotated part apart; so that
+// both of a pair are in one lane, a lane holds two runs of four elements: i.. and i + rot / 2.. where pairs are halves,
+// eight neighbours where pairs are neighbours or nothing is rotated.
+struct LanePlace {
+    uint32_t at[2];      // first elements of the lane's two runs
+    uint32_t turn;       // first of its four entries in the tables
+    bool live, rotated;
+};
+__device__ __forceinline__ LanePlace place_of(uint32_t lane, uint32_t dim, uint32_t rot, int pairs) {
+    LanePlace p;
+    const uint32_t i = lane * 4;                                 // of dim / 2 pairs, the lane has four
+    p.live = i < dim / 2;
+    p.rotated = i < rot / 2;
+    p.turn = i;
+    const bool halves = p.rotated && !pairs;
+    p.at[0] = halves ? i : 2 * i;
+    p.at[1] = halves ? i + rot / 2 : 2 * i + 4;
+    return p;
+}
+
+template <int TYPE> __device__ __forceinline__ void load4(const char* row, uint32_t at, float* x) {
+    const uint2_t w = *reinterpret_cast<const uint2_t*>(row + at * 2);
+    unpack2<TYPE>(w.x, x[0], x[1]);
+    unpack2<TYPE>(w.y, x[2], x[3]);
+}
+template <int TYPE> __device__ __forceinline__ void store4(char* row, uint32_t at, const float* x) {
+    uint2_t w;
+    w.x = pack2<TYPE>(x[0], x[1]);
+    w.y = pack2<TYPE>(x[2], x[3]);
+    *reinterpret_cast<uint2_t*>(row + at * 2) = w;
+}
+
+// Scale of a row from the bits of its largest magnitude: one that is infinite or NaN makes the row NaN.
+template <int CODES> __device__ __forceinline__ float scale_of(uint32_t bits) {
+    const float top = __builtin_bit_cast(float, bits);
+    return bits >= 0x7f800000u ? __builtin_nanf("") : top / (CODES == FKLHIP_CODES_INT8 ? kTopInt8 : kTopE4M3);
+}
+// Eight values as codes: x / scale, an IEEE division, so that codes are what the definition says bit by bit.
+template <int CODES> __device__ __forceinline__ void encode8(const float* x, float scale, uint32_t* w) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = scale > 0.0f ? x[i] / scale : 0.0f;
+    w[0] = encode4<CODES>(y);
+    w[1] = encode4<CODES>(y + 4);
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// Where a slot is in the cache: its page and its place there; false for a slot outside.
+__device__ __forceinline__ bool locate(const Cache& c, int32_t slot, uint32_t& page, uint32_t& off) {
+    page = uint32_t(slot) >> c.page_log;
+    off = uint32_t(slot) & ((1u << c.page_log) - 1u);
+    return slot >= 0 && page < c.pages;
+}
+__device__ __forceinline__ size_t head_row(const Cache& c, uint32_t page, uint32_t head) {
+    return (size_t(page) * c.kv_heads + head) << c.page_log;     // tokens in front of the head's part of the page
+}
+
+// Tiles of tokens go along y, and along z where there are more than a grid holds.
+constexpr uint32_t kTilesY = 32768;
+__device__ __forceinline__ uint32_t tile_of_grid() { return blockIdx.z * kTilesY + blockIdx.y; }
+
+// LANES to a head of up to 8 * LANES elements, HEADS heads of one token to a group of lanes.
+template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE>
+__global__ __launch_bounds__(256) void k_heads(const HeadArgs a) {
+    const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES;
+    const uint32_t dim = a.head_dim, tile = tile_of_grid();
+    if (TO_CACHE && blockIdx.x >= a.q_chunks + a.k_chunks) {
+        // values: a group takes four tokens of a head, whose bytes lie side by side in the cache where their slots do
+        const uint32_t head = (blockIdx.x - a.q_chunks - a.k_chunks) * 4 + group % 4, at = lane * 8;
+        if (head >= a.kv_heads) return;
+        {
+            const uint32_t first = tile * groups + (group / 4) * 4;
+            uint4_t raw[4];
+            int32_t slot[4];
+            float x[4][8], scale[4];
+            uint32_t code[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool there = first + i < a.tokens;
+                slot[i] = there ? a.slots[first + i] : -1;
+                raw[i] = uint4_t{0, 0, 0, 0};
+                if (there && at < dim) raw[i] = *reinterpret_cast<const uint4_t*>(a.v.data + (first + i) * a.v.token_stride + head * a.v.head_stride + at * 2);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) unpack2<TYPE>(raw[i][k], x[i][2 * k], x[i][2 * k + 1]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[i][k]));
+                scale[i] = scale_of<CODES>(max_lanes<LANES>(top));
+                encode8<CODES>(x[i], scale[i], code[i]);
+            }
+            uint32_t page, off;
+            const bool run = (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+            if (run) {
+                if (!locate(a.cache, slot[0], page, off)) return;
+                const size_t row = head_row(a.cache, page, head) + off;
+                if (lane == 0) *reinterpret_cast<float4_t*>(a.cache.v_scale + row) = float4_t{scale[0], scale[1], scale[2], scale[3]};
+                if (at < dim) {
+                    // 4 x 8 bytes turned: element by element, four tokens each
+                    uint4_t out[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t lo01 = __builtin_amdgcn_perm(code[1][h], code[0][h], 0x05010400u), hi01 = __builtin_amdgcn_perm(code[1][h], code[0][h], 0x07030602u);
+                        const uint32_t lo23 = __builtin_amdgcn_perm(code[3][h], code[2][h], 0x05010400u), hi23 = __builtin_amdgcn_perm(code[3][h], code[2][h], 0x07030602u);
+                        out[h] = uint4_t{__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
+                                         __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
+                    }
+                    uint4_t* to = reinterpret_cast<uint4_t*>(a.cache.v + row * dim + size_t(at) * 4);
+                    to[0] = out[0];
+                    to[1] = out[1];
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!locate(a.cache, slot[i], page, off)) continue;
+                const size_t row = head_row(a.cache, page, head) + off;
+                if (lane == 0) a.cache.v_scale[row] = scale[i];
+                if (at < dim) {
+                    char* to = a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4 + (off & 3);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) to[k * 4] = char(code[i][k / 4] >> (8 * (k % 4)));
+                }
+            }
+        }
+        return;
+    }
+    const bool is_q = blockIdx.x < a.q_chunks;
+    const uint32_t head0 = (is_q ? blockIdx.x : blockIdx.x - a.q_chunks) * HEADS, heads = is_q ? a.q_heads : a.kv_heads;
+    const Rows in = is_q ? a.q : a.k, out = is_q ? a.q_out : a.k_out;
+    const char* weights = static_cast<const char*>(is_q ? a.q_weight : a.k_weight);
+    const LanePlace p = place_of(lane, dim, a.rot_dim, a.pairs);
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = 1.0f;
+    if (weights && p.live) { load4<TYPE>(weights, p.at[0], w); load4<TYPE>(weights, p.at[1], w + 4); }
+    {
+        const uint32_t token = tile * groups + group;
+        if (token >= a.tokens) return;
+        float x[HEADS][8];
+        const char* row = in.data + token * in.token_stride;
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[h][k] = 0.0f;
+            if (p.live && head0 + h < heads) {
+                load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[0], x[h]);
+                load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[1], x[h] + 4);
+            }
+        }
+        float4_t cosine = {1.0f, 1.0f, 1.0f, 1.0f}, sine = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.rotated) {
+            const uint32_t position = uint32_t(a.positions[token]);
+            if (position < a.table_rows) {
+                const size_t at = size_t(position) * (a.rot_dim / 2) + p.turn;
+                cosine = *reinterpret_cast<const float4_t*>(a.cos + at);
+                sine = *reinterpret_cast<const float4_t*>(a.sin + at);
+            } else {
+                cosine = sine = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            }
+        }
+        uint32_t page = 0, off = 0;
+        bool stored = false;
+        if (TO_CACHE && !is_q) stored = locate(a.cache, a.slots[token], page, off);
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            if (head0 + h >= heads) break;
+            if (weights) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(x[h][k], x[h][k], sum);
+                const float r = 1.0f / __builtin_sqrtf(sum_lanes<LANES>(sum) / float(dim) + a.eps);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[h][k] = x[h][k] * r * w[k];
+            }
+            if (p.rotated) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // pairs are (k, k + 4) of the lane's elements as halves, (2k, 2k + 1) as neighbours
+                    float& u = a.pairs ? x[h][2 * k] : x[h][k];
+                    float& v = a.pairs ? x[h][2 * k + 1] : x[h][k + 4];
+                    const float s = u, t = v;
+                    u = s * cosine[k] - t * sine[k];
+                    v = t * cosine[k] + s * sine[k];
+                }
+            }
+            if (is_q || !TO_CACHE) {
+                if (p.live) {
+                    char* to = out.data + token * out.token_stride + (head0 + h) * out.head_stride;
+                    store4<TYPE>(to, p.at[0], x[h]);
+                    store4<TYPE>(to, p.at[1], x[h] + 4);
+                }
+            } else {
+                uint32_t top = 0, code[2];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[h][k]));
+                const float scale = scale_of<CODES>(max_lanes<LANES>(top));
+                encode8<CODES>(x[h], scale, code);
+                if (stored) {
+                    const size_t at = head_row(a.cache, page, head0 + h) + off;
+                    if (lane == 0) a.cache.k_scale[at] = scale;
+                    if (p.live) {
+                        char* to = a.cache.k + at * dim;
+                        *reinterpret_cast<uint32_t*>(to + p.at[0]) = code[0];
+                        *reinterpret_cast<uint32_t*>(to + p.at[1]) = code[1];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Reads slots back, eight elements to a lane: HEADS heads of one token's keys, or four tokens of one head's values (whose
+// bytes lie side by side where the slots do).
+template <int LANES, int HEADS, int TYPE, int CODES>
+__global__ __launch_bounds__(256) void k_read(const ReadArgs a) {
+    const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES, at = lane * 8;
+    const uint32_t dim = a.head_dim, heads = a.cache.kv_heads, tile = tile_of_grid();
+    const bool values = blockIdx.x >= a.k_chunks;
+    {
+        if (!values) {
+            const uint32_t token = tile * groups + group, head0 = blockIdx.x * HEADS;
+            if (token >= a.tokens || at >= dim) return;
+            uint32_t page, off;
+            const bool there = locate(a.cache, a.slots[token], page, off);
+            uint2_t code[HEADS];
+            float scale[HEADS];
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                code[h] = uint2_t{0, 0};
+                scale[h] = 0.0f;
+                if (there && head0 + h < heads) {
+                    const size_t row = head_row(a.cache, page, head0 + h) + off;
+                    code[h] = *reinterpret_cast<const uint2_t*>(a.cache.k + row * dim + at);
+                    scale[h] = a.cache.k_scale[row];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                if (head0 + h >= heads) break;
+                float x[8];
+                decode4<CODES>(code[h].x, x);
+                decode4<CODES>(code[h].y, x + 4);
+                uint4_t w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k] * scale[h], x[2 * k + 1] * scale[h]);
+                *reinterpret_cast<uint4_t*>(a.k.data + token * a.k.token_stride + (head0 + h) * a.k.head_stride + at * 2) = w;
+            }
+        } else {
+            const uint32_t head = (blockIdx.x - a.k_chunks) * 4 + group % 4, first = tile * groups + (group / 4) * 4;
+            if (head >= heads || first >= a.tokens || at >= dim) return;
+            int32_t slot[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) slot[i] = first + i < a.tokens ? a.slots[first + i] : -1;
+            const bool run = (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+            uint32_t page, off;
+            float scale[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t code[8];                                  // of element k: the four tokens' bytes
+#pragma unroll
+            for (int k = 0; k < 8; ++k) code[k] = 0;
+            if (run) {
+                if (locate(a.cache, slot[0], page, off)) {
+                    const size_t row = head_row(a.cache, page, head) + off;
+                    const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + row * dim + size_t(at) * 4);
+                    const uint4_t lo = from[0], hi = from[1];
+                    const float4_t s = *reinterpret_cast<const float4_t*>(a.cache.v_scale + row);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { code[k] = lo[k]; code[k + 4] = hi[k]; scale[k] = s[k]; }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!locate(a.cache, slot[i], page, off)) continue;
+                    const size_t row = head_row(a.cache, page, head) + off;
+                    scale[i] = a.cache.v_scale[row];
+                    // the whole dwords are read: the other bytes are other tokens' of the same page
+                    const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4);
+                    const uint4_t lo = from[0], hi = from[1];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) code[k] |= (((k < 4 ? lo[k & 3] : hi[k & 3]) >> (8 * (off & 3))) & 0xffu) << (8 * i);
+                }
+            }
+            float x[8][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) decode4<CODES>(code[k], x[k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (first + i >= a.tokens) break;
+                uint4_t w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k][i] * scale[i], x[2 * k + 1][i] * scale[i]);
+                *reinterpret_cast<uint4_t*>(a.v.data + (first + i) * a.v.token_stride + head * a.v.head_stride + at * 2) = w;
+            }
+        }
+    }
+}
+
+uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+// Tokens to a workgroup and heads to a group of lanes.
+struct RowShape { uint32_t threads, heads; };
+RowShape row_shape(uint32_t tokens, uint32_t lanes) {
+    // few tokens: one head to a group and small workgroups, so that everything runs at once
+    if (tokens <= 256) return {lanes * 4 < 64 ? 64 : lanes * 4, 1};
+    return {256, 4};
+}
+
+template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE>
+int start_heads(HeadArgs a, uint32_t threads, void* stream, Launched& info) {
+    a.q_chunks = ceil_div(a.q_heads, HEADS);
+    a.k_chunks = ceil_div(a.kv_heads, HEADS);
+    const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
+    const dim3 grid(a.q_chunks + a.k_chunks + (TO_CACHE ? ceil_div(a.kv_heads, 4) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
+    info = {"heads", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
+    k_heads<LANES, HEADS, TYPE, CODES, TO_CACHE><<<grid, dim3(threads), 0, static_cast<hipStream_t>(stream)>>>(a);
+    return int(hipGetLastError());
+}
+template <int LANES, int TYPE> int start_heads(const HeadArgs& a, bool to_cache, void* stream, Launched& info) {
+    const RowShape s = row_shape(a.tokens, LANES);
+    const bool int8 = a.cache.codes == FKLHIP_CODES_INT8;
+    if (s.heads == 1) {
+        if (!to_cache) return start_heads<LANES, 1, TYPE, 0, false>(a, s.threads, stream, info);
+        return int8 ? start_heads<LANES, 1, TYPE, FKLHIP_CODES_INT8, true>(a, s.threads, stream, info)
+                    : start_heads<LANES, 1, TYPE, FKLHIP_CODES_E4M3, true>(a, s.threads, stream, info);
+    }
+    if (!to_cache) return start_heads<LANES, 4, TYPE, 0, false>(a, s.threads, stream, info);
+    return int8 ? start_heads<LANES, 4, TYPE, FKLHIP_CODES_INT8, true>(a, s.threads, stream, info)
+                : start_heads<LANES, 4, TYPE, FKLHIP_CODES_E4M3, true>(a, s.threads, stream, info);
+}
+
+template <int LANES, int HEADS, int TYPE, int CODES> int start_read(ReadArgs a, uint32_t threads, void* stream, Launched& info) {
+    a.k_chunks = ceil_div(a.cache.kv_heads, HEADS);
+    const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
+    const dim3 grid(a.k_chunks + ceil_div(a.cache.kv_heads, 4), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
+    info = {"kv_read", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
+    k_read<LANES, HEADS, TYPE, CODES><<<grid, dim3(threads), 0, static_cast<hipStream_t>(stream)>>>(a);
+    return int(hipGetLastError());
+}
+template <int LANES, int TYPE> int start_read(const ReadArgs& a, void* stream, Launched& info) {
+    const RowShape s = row_shape(a.tokens, LANES);
+    const bool int8 = a.cache.codes == FKLHIP_CODES_INT8;
+    if (s.heads == 1)
+        return int8 ? start_read<LANES, 1, TYPE, FKLHIP_CODES_INT8>(a, s.threads, stream, info) : start_read<LANES, 1, TYPE, FKLHIP_CODES_E4M3>(a, s.threads, stream, info);
+    return int8 ? start_read<LANES, 4, TYPE, FKLHIP_CODES_INT8>(a, s.threads, stream, info) : start_read<LANES, 4, TYPE, FKLHIP_CODES_E4M3>(a, s.threads, stream, info);
+}
+
+} // namespace
+
+int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info) {
+    const bool bf16 = type == FKLHIP_BF16;
+    if (a.head_dim <= 64) return bf16 ? start_heads<8, FKLHIP_BF16>(a, to_cache, stream, info) : start_heads<8, FKLHIP_F16>(a, to_cache, stream, info);
+    if (a.head_dim <= 128) return bf16 ? start_heads<16, FKLHIP_BF16>(a, to_cache, stream, info) : start_heads<16, FKLHIP_F16>(a, to_cache, stream, info);
+    return bf16 ? start_heads<32, FKLHIP_BF16>(a, to_cache, stream, info) : start_heads<32, FKLHIP_F16>(a, to_cache, stream, info);
+}
+
+int launch_read(const ReadArgs& a, int type, void* stream, Launched& info) {
+    const bool bf16 = type == FKLHIP_BF16;
+    if (a.head_dim <= 64) return bf16 ? start_read<8, FKLHIP_BF16>(a, stream, info) : start_read<8, FKLHIP_F16>(a, stream, info);
+    if (a.head_dim <= 128) return bf16 ? start_read<16, FKLHIP_BF16>(a, stream, info) : start_read<16, FKLHIP_F16>(a, stream, info);
+    return bf16 ? start_read<32, FKLHIP_BF16>(a, stream, info) : start_read<32, FKLHIP_F16>(a, stream, info);
+}
+
+} // namespace fkattn

@@ -43,6 +43,10 @@ std::atomic<int>& strip_setting() {
 
 bool strip_enabled() { return strip_setting().load(std::memory_order_relaxed) != 0; }
 
+void note_launch(const char* kernel, const unsigned grid[3], const unsigned block[3], unsigned lds_bytes) {
+    g_last = {kernel, {grid[0], grid[1], grid[2]}, {block[0], block[1], block[2]}, lds_bytes, kernel};
+}
+
 void register_chain(const char* signature, size_t blob_bytes, LaunchFn fn, const void* ctx) {
     Table& t = table();
     std::lock_guard<std::mutex> lock(t.mu);

@@ -26,6 +26,9 @@ bool strip_enabled();
 // Called from static initialisers of the generated instance files, and by the run-time compiler.
 void register_chain(const char* signature, size_t blob_bytes, LaunchFn fn, const void* ctx = nullptr);
 
+// What fklhip_last_launch and fklhip_last_form report for this thread, for kernels that are not chains'.
+void note_launch(const char* kernel, const unsigned grid[3], const unsigned block[3], unsigned lds_bytes);
+
 // Run-time compilation (jit.cpp).  jit_compile_and_register returns FKLHIP_OK after registering the chain, or
 // FKLHIP_EUNKNOWN_SIGNATURE when run-time compilation is switched off or the signature does not compile (the
 // compiler's messages are then available through jit_last_log).

@@ -126,6 +126,98 @@ int fklhip_last_launch(const char **kernel, unsigned grid[3], unsigned block[3],
  * "divergent", ahead of time and compiled at run time alike; "" before the first launch. */
 int fklhip_last_form(const char **form);
 
+/*
+ * Attention over a quantised key-value cache: the operators a language model's server runs for new or drafted tokens.
+ * The reference has them as cooperative kernels of its own beside the fused path (FK/algorithms/attention/: attention,
+ * split decoding, int8 and fp8 cache reads); here they are three kernels behind the five entry points below.
+ *
+ * All pointers are device pointers, all strides count elements, the last dimension of rows is contiguous. 16-bit rows
+ * start at multiples of 16 bytes (head_dim is a multiple of 8; their strides have to be multiples of 8). The calls are
+ * asynchronous on `stream`, allocate nothing, record no memset and may be captured into a graph. A call that returns
+ * FKLHIP_EINVAL has launched nothing; fklhip_argument_error says what was wrong. What only the device can see (slots,
+ * pages, lengths, positions) is held inside its bounds by the kernels, as described at each entry.
+ */
+enum { FKLHIP_BF16 = 0, FKLHIP_F16 = 1 };
+enum { FKLHIP_CODES_INT8 = 0, FKLHIP_CODES_E4M3 = 1 };
+
+/* A paged cache. A cached value is code * scale with one float32 scale per token and head; codes are int8 (-127..127) or
+ * e4m3 (finite, no infinities). Slot s is token s % page_tokens of page s / page_tokens.
+ *   k        [pages][kv_heads][page_tokens][head_dim]          one byte each
+ *   v        [pages][kv_heads][page_tokens / 4][head_dim][4]   four consecutive tokens' bytes of one element side by side
+ *   k_scale  [pages][kv_heads][page_tokens], v_scale the same
+ * page_tokens is 16, 32, 64, 128 or 256; k and v start at multiples of 16 bytes, the scales too. */
+typedef struct fklhip_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t pages;
+    int32_t kv_heads, page_tokens, head_dim, codes;
+} fklhip_kv_cache;
+
+/* Rows [token][head][element] of a 16-bit type. */
+typedef struct fklhip_rows {
+    void *data;
+    int64_t token_stride, head_stride;
+} fklhip_rows;
+
+/* Query, key (and value) heads of `tokens` tokens on their way to attention. */
+typedef struct fklhip_heads {
+    fklhip_rows q, k, v;               /* v is read by fklhip_qkv_to_cache only */
+    fklhip_rows q_out, k_out;          /* k_out is written by fklhip_qk_norm_rope only; outputs may be the inputs */
+    const void *q_weight, *k_weight;   /* [head_dim] of the rows' type; NULL: no norm */
+    const float *cos, *sin;            /* [positions][rot_dim / 2], rows tight; NULL with rot_dim 0 */
+    const int32_t *positions;          /* [tokens]; outside of the table: the token's rotated elements are NaN */
+    const int32_t *slots;              /* [tokens], fklhip_qkv_to_cache only; outside of the cache: the token is not stored */
+    int64_t tokens, table_rows;
+    int32_t q_heads, kv_heads, head_dim, rot_dim;
+    int32_t pairs;                     /* 0: element i turns with i + rot_dim / 2, 1: 2i with 2i + 1 */
+    int32_t type;
+    float eps;
+} fklhip_heads;
+
+/* RMS norm of each query and key head (x * rsqrt(mean(x^2) + eps) * weight) and rotation of its first rot_dim elements by
+ * the token's position ((a, b) -> (a cos - b sin, b cos + a sin)), in 32 bits, rounded once. head_dim: a multiple of 8 up
+ * to 256, rot_dim: a multiple of 8 up to head_dim. */
+int fklhip_qk_norm_rope(const fklhip_heads *heads, void *stream);
+
+/* The same, with the keys (in 32 bits) and the values quantised into the cache in the same launch instead of written out. */
+int fklhip_qkv_to_cache(const fklhip_heads *heads, const fklhip_kv_cache *cache, void *stream);
+
+/* Quantises rows into the cache: scale = max |x| / 127 (448 for e4m3), code = x / scale rounded to the nearest, ties to
+ * even. A row of zeros has scale 0; a row with an infinity or a NaN is stored as NaN (scale NaN, codes 0). Tokens whose
+ * slot is outside of the cache (a negative one, say) are skipped. No two tokens of a call may have the same slot. */
+int fklhip_kv_write(const fklhip_kv_cache *cache, const fklhip_rows *k, const fklhip_rows *v, const int32_t *slots,
+                    int64_t tokens, int type, void *stream);
+
+/* Reads `tokens` slots back as 16-bit rows; a slot outside of the cache gives zeros. */
+int fklhip_kv_read(const fklhip_kv_cache *cache, const int32_t *slots, int64_t tokens, const fklhip_rows *k,
+                   const fklhip_rows *v, int type, void *stream);
+
+/* Attention of new tokens over the cache. Sequence b has context[b] cached tokens and behind them, in the cache too, its
+ * q_start[b + 1] - q_start[b] new ones, whose queries are rows q_start[b].. of q. Token j of the sequence is in slot
+ * page_table[b * page_table_stride + j / page_tokens] * page_tokens + j % page_tokens. Query row r sees the whole context
+ * and new token u if bit u % 64 of mask[r * mask_words + u / 64] is set; without a mask, new token t sees 0..t. Query
+ * heads are shared out to the key heads in order (q_heads a multiple of kv_heads). A row that sees nothing gives zeros and
+ * lse -inf. Lengths above max_new and max_context, and tokens beyond the page table's row, are cut off; pages outside of
+ * the cache are read as its last. head_dim: 64, 96, 128, 192 or 256. */
+typedef struct fklhip_attention {
+    fklhip_rows q, out;
+    float *lse;                        /* [tokens][q_heads] log of the sum of exponentials, or NULL */
+    const int32_t *page_table, *context, *q_start;
+    const uint64_t *mask;              /* [tokens][mask_words] or NULL */
+    void *workspace;                   /* fklhip_tree_attention_workspace bytes; not kept between calls */
+    uint64_t workspace_bytes;
+    int64_t tokens, page_table_stride; /* page_table_stride: entries of a sequence's row, all of them readable */
+    int32_t batch, max_new, max_context, mask_words;
+    int32_t q_heads, type;
+    float scale;                       /* of the scores; usually 1 / sqrt(head_dim) */
+} fklhip_attention;
+
+int fklhip_tree_attention_workspace(const fklhip_attention *call, const fklhip_kv_cache *cache, uint64_t *bytes);
+int fklhip_tree_attention(const fklhip_attention *call, const fklhip_kv_cache *cache, void *stream);
+
+/* What the last of the calls above that returned FKLHIP_EINVAL on this thread found wrong; "" before the first. */
+int fklhip_argument_error(const char **text);
+
 /* Number of chain signatures compiled into the library and the i-th of them with its parameter block size. */
 int fklhip_signature_count(int *count);
 int fklhip_signature_at(int index, const char **signature, size_t *blob_bytes);
