@@ -130,8 +130,8 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, Attention
     return FKLHIP_OK;
 }
 
-uint64_t workspace_of(const fklhip_attention& c, const fklhip_kv_cache& cache, const AttentionPlan& plan) {
-    return plan.splits <= 1 ? 0 : (uint64_t(c.tokens) * c.q_heads * plan.splits * (cache.head_dim + 1) * 4 + 255) / 256 * 256;
+uint64_t workspace_of(const fklhip_kv_cache& cache, const AttentionPlan& plan) {
+    return plan.shares_log == kNoShares ? 0 : (uint64_t(plan.unit_rows) << (plan.shares_log + 1)) * (cache.head_dim + 1) * 4;
 }
 
 } // namespace
@@ -183,7 +183,7 @@ int fklhip_tree_attention_workspace(const fklhip_attention* call, const fklhip_k
     NEED(bytes, "no place for the answer");
     AttentionPlan plan;
     CHECK(plan_call(call, cache, plan));
-    *bytes = workspace_of(*call, *cache, plan);
+    *bytes = workspace_of(*cache, plan);
     return FKLHIP_OK;
 }
 
@@ -197,7 +197,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     NEED(c->context && c->q_start, "no context or no q_start");
     NEED(c->page_table || c->page_table_stride == 0, "no page_table");
     NEED(!c->mask || (c->mask_words >= 1 && int64_t(c->mask_words) * 64 >= c->max_new), "mask_words has to be max_new / 64, rounded up, or more");
-    const uint64_t bytes = workspace_of(*c, *cache, plan);
+    const uint64_t bytes = workspace_of(*cache, plan);
     NEED(bytes == 0 || (c->workspace && c->workspace_bytes >= bytes), "the workspace is smaller than fklhip_tree_attention_workspace says");
     NEED(bytes == 0 || aligned(c->workspace, 16), "the workspace has to start at a multiple of 16 bytes");
     AttentionArgs a{};
@@ -207,12 +207,14 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     a.page_table_stride = c->page_table_stride;
     a.tokens = uint32_t(c->tokens); a.batch = uint32_t(c->batch); a.max_new = uint32_t(c->max_new); a.max_context = uint32_t(c->max_context);
     a.mask_words = uint32_t(c->mask_words); a.q_heads = uint32_t(c->q_heads); a.group = uint32_t(c->q_heads / cache->kv_heads);
-    a.splits = plan.splits; a.chunk = plan.chunk;
-    a.group_magic = magic(a.group); a.heads_magic = magic(uint32_t(cache->kv_heads));
+    a.group_magic = magic(a.group);
+    a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
+    a.unit_rows = plan.unit_rows; a.block_subs = plan.unit_rows >> plan.sub_log; a.sub_log = plan.sub_log;
+    a.granule_log = plan.granule_log; a.shares_log = plan.shares_log;
     a.type = c->type; a.scale = c->scale;
-    if (plan.splits > 1) {
+    if (bytes) {
         a.partial = static_cast<float*>(c->workspace);
-        a.partial_lse = a.partial + uint64_t(a.tokens) * a.q_heads * plan.splits * uint64_t(cache->head_dim);
+        a.partial_lse = a.partial + (uint64_t(plan.unit_rows) << (plan.shares_log + 1)) * uint64_t(cache->head_dim);
     }
     Launched info;
     int rc;
@@ -223,7 +225,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     case 192: rc = launch_attention<192>(a, plan, stream, info); break;
     default: rc = launch_attention<256>(a, plan, stream, info); break;
     }
-    if (rc == FKLHIP_OK && plan.splits > 1) rc = launch_merge(a, uint32_t(cache->head_dim), stream);
+    if (rc == FKLHIP_OK && bytes) rc = launch_merge(a, uint32_t(cache->head_dim), stream);
     return finish(rc, info);
 }
 
@@ -232,16 +234,21 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
 namespace fkattn {
 
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim) {
+    const auto log2_floor = [](uint64_t n) { uint32_t l = 0; while (n >>= 1) ++l; return l; };
     AttentionPlan p;
-    p.row_tiles = rows <= 16 || head_dim > 128 ? 1 : 2;
-    p.row_blocks = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
-    const uint64_t whole = uint64_t(batch) * kv_heads * p.row_blocks;
-    // about four workgroups to each of the 256 compute units, and no fewer than 256 keys to one
-    const uint64_t want = whole ? (1024 + whole - 1) / whole : 1;
-    uint64_t chunk = (keys + want - 1) / want;
-    chunk = std::max<uint64_t>((chunk + 127) / 128 * 128, 256);
-    p.chunk = uint32_t(chunk);
-    p.splits = std::max<uint32_t>(1, uint32_t((keys + chunk - 1) / chunk));
+    // up to 16 (or 32) rows: the waves split the keys; more: they split the rows, 64 or 128 to a workgroup
+    p.split_rows = rows > (head_dim > 128 ? 16 : 32);
+    p.tiles = head_dim > 128 || rows <= 16 || (p.split_rows && rows <= 64) ? 1 : 2;
+    p.unit_rows = p.tiles * (p.split_rows ? 64 : 16);
+    p.sub_log = p.split_rows ? 6 : log2_floor(p.unit_rows);
+    p.granule_log = p.split_rows ? (head_dim > 128 ? 5 : 6) : 7;
+    p.row_blocks = std::max(1u, (rows + p.unit_rows - 1) / p.unit_rows);
+    const uint64_t granules = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log, units = uint64_t(batch) * kv_heads * p.row_blocks;
+    const uint64_t all = units * granules * (p.unit_rows >> p.sub_log);
+    // as many shares as workgroups run at once on 256 compute units, but two granules to each
+    const uint32_t most = p.split_rows ? (head_dim > 128 ? 8 : 9) : p.tiles == 2 || head_dim > 128 ? 9 : 10;
+    p.shares_log = kNoShares;
+    if (granules > 4 && units < (uint64_t(4) << most) && all < (uint64_t(1) << 32)) p.shares_log = std::min(most, log2_floor(all / 2));
     return p;
 }
 

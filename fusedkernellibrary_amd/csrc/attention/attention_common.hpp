@@ -47,23 +47,26 @@ struct AttentionArgs {
     const int32_t *page_table, *context, *q_start;
     const uint64_t* mask;
     Cache cache;
-    float *partial, *partial_lse;           // [tokens * q_heads][splits](head_dim)
+    float *partial, *partial_lse;           // [shares][2][unit_rows](head_dim): a share's parts of row blocks
     int64_t page_table_stride;
+    uint32_t room;                          // tokens that a row of the page table has entries for
     uint32_t tokens, batch, max_new, max_context, mask_words;
     uint32_t q_heads, group;                // query heads per key head
-    uint32_t splits, chunk;                 // keys of a sequence are shared out in chunks, one to a split
-    uint32_t group_magic, heads_magic;      // x / group and x / kv_heads as a multiplication (see divide)
+    uint32_t group_magic;                   // x / group as a multiplication (see divide)
+    uint32_t unit_rows, block_subs, sub_log, granule_log, shares_log;    // how the work is dealt out (work_shares.hpp)
     int type;
     float scale;
 };
+constexpr uint32_t kNoShares = 32;          // shares_log of a launch with a workgroup to each row block
 
 // Launchers (defined next to their kernels). Grids are laid out by the callers' arguments alone.
 struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
 int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, void* stream);
-// Row tiles (of 16 query rows) that a workgroup takes; how a call's keys are shared out.
-struct AttentionPlan { uint32_t row_tiles, row_blocks, splits, chunk; };
+// How a call is run: 16-row tiles to a wave; whether a workgroup's waves split rows or keys; row blocks of a launch without
+// shares; 2^shares_log shares, or none.
+struct AttentionPlan { uint32_t tiles, row_blocks, unit_rows, sub_log, granule_log, shares_log; bool split_rows; };
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim);
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
 

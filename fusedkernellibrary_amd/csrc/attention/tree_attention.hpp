@@ -12,13 +12,26 @@
 // so if the contraction runs over the keys in that order; the cache keeps four tokens' bytes of a value element side by
 // side for that reason. So nothing moves between lanes, and the running maximum is per lane column.
 //
+// Two forms. Few rows to a key head (k_split_keys): the four waves of a workgroup take the same 16 or 32 rows and other keys,
+// which each loads into its registers, and the rows' parts are joined in LDS; the bound is reading the cache. Many rows
+// (k_split_rows): the waves take other rows and the same keys, which pass through LDS, copied there without registers and
+// several stages ahead; the bound is the arithmetic, of which turning codes into halves is shared by a wave's row tiles.
+//
+// How the work is dealt out. The device alone knows the sequences' lengths, so every workgroup adds them up: the keys of all
+// (sequence, key head, block of rows), one behind the other, are cut into equal shares, one to a workgroup, all of which run
+// at the same time. A share may hold parts of two of them and whole ones in between; whole ones are written to the output,
+// parts to the workspace, from where k_merge takes them. Without shares (short sequences, or so many that the order of
+// launch evens them out) a workgroup takes one whole (sequence, key head, block of rows).
+//
 // The running maximum m_r and the largest value scale t are references and not the exact maxima: weights are
 // w = 2^(s - m) * vs / t, and m and t move only when a score leads m by more than 2^kLead or a value scale exceeds t. Only
 // then are scores compared across lanes and the sums rescaled. 2^(s - m) stays below 2^kLead and starts at 2^kStart, so a
 // weight is subnormal in half precision (2^-14) only 2^-(14 + kStart) below the largest of the first keys.
 #pragma once
 
-#include "attention_device.hpp"
+#include <type_traits>
+
+#include "work_shares.hpp"
 
 namespace fkattn {
 
@@ -93,184 +106,194 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint32_t word
     return (lowest_bits(int32_t(below)) | bits << below) & 15u;
 }
 
-// 32 keys: codes and scales of two blocks of 16 as a lane holds them.
-template <int D> struct Tile {
-    using S = Shape<D>;
-    Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
-    float4_t ks[2], vs[2];
+// Keys key0 .. key1 of row block `block` and key head `head` of a sequence; where its parts go.
+struct Segment {
+    Sequence seq;
+    uint32_t b, head, row0, rows;        // rows row0 .. row0 + rows of the sequence's
+    uint32_t key0, key1, all_see;        // every row sees the keys in front of all_see
+    int part;                            // -1: whole, 0 or 1: the share's part
 };
-
-template <int D, int CODES, int R>
-__global__ __launch_bounds__(kWaves * 64, R == 1 && D <= 128 ? 2 : 1) void k_tree_attention(const AttentionArgs a) {
-    using S = Shape<D>;
-    constexpr int kRowFloats = D + 4;                              // of a row in LDS: 16 bytes further round the banks than the last
-    __shared__ __attribute__((aligned(16))) float joined[kWaves][16 * kRowFloats];
-    __shared__ float joined_m[kWaves][16], joined_l[kWaves][16], row_m[16], row_l[16];
-
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col = lane & 15, quarter = lane >> 4;
-    const uint32_t b = blockIdx.z;
-    const uint32_t split = divide(blockIdx.x, a.heads_magic), head = blockIdx.x - split * a.cache.kv_heads;
-    if (split >= a.splits) return;                                 // (the grid's x is padded)
-
-    const int32_t start = a.q_start[b];
-    uint32_t first_token = uint32_t(start < 0 ? 0 : start);
-    if (first_token > a.tokens) first_token = a.tokens;
-    int32_t diff = a.q_start[b + 1] - int32_t(first_token);
-    uint32_t fresh = diff < 0 ? 0 : uint32_t(diff);
-    fresh = min(min(fresh, a.max_new), a.tokens - first_token);
-    int32_t have = a.context[b];
-    uint32_t context = have < 0 ? 0 : min(uint32_t(have), a.max_context);
-    const uint32_t page_mask = (1u << a.cache.page_log) - 1u;
-    const uint64_t room = uint64_t(a.page_table_stride) << a.cache.page_log;
-    context = room < context ? uint32_t(room) : context;
-    const uint32_t total = room < uint64_t(context) + fresh ? uint32_t(room) : context + fresh;
-
-    const uint32_t rows = fresh * a.group, row0 = blockIdx.y * (16 * R);
-    if (row0 >= rows) return;
-    const uint32_t last_row = min(row0 + 16 * R, rows) - 1;
-    // keys that every row of the workgroup sees, and keys that any of them can see
+__device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32_t b, uint32_t head, uint32_t block, uint32_t k0, uint32_t k1, int part) {
+    Segment x;
+    x.seq = s; x.b = b; x.head = head; x.part = part;
+    x.row0 = block * a.unit_rows;
+    x.rows = min(a.unit_rows, s.rows - x.row0);
     const bool causal = a.mask == nullptr;
-    const uint32_t all_see = causal ? min(context + divide(row0, a.group_magic) + 1, total) : context;
-    const uint32_t any_sees = causal ? min(context + divide(last_row, a.group_magic) + 1, total) : total;
-    const uint32_t key0 = split * a.chunk, key1 = min(key0 + a.chunk, any_sees);
+    const uint32_t any_sees = causal ? min(s.context + divide(x.row0 + x.rows - 1, a.group_magic) + 1, s.total) : s.total;
+    x.all_see = causal ? min(s.context + divide(x.row0, a.group_magic) + 1, s.total) : s.context;
+    x.key0 = k0 << a.granule_log;
+    x.key1 = min(k1 << a.granule_log, any_sees);
+    return x;
+}
 
-    // the lane's rows: their new token, and their query elements as the scores want them
-    uint32_t token[R];
+// Calls `run` for every segment of the workgroup.
+template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, F run) {
+    // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
+    uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
+    const bool shared = a.shares_log != kNoShares;
+    if (shared) {
+        const uint32_t share = own_share(a);
+        const Found f = find(a, lane, [&](uint32_t all, uint32_t, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
+        at = share_begin(a, f.all, share);
+        end = share_begin(a, f.all, share + 1);
+        b = f.b;
+        in = at - f.before;
+    }
+    while (at < end && b < kernel_args().batch) {
+        Args& a = kernel_args();
+        const Sequence s = sequence_at(a, b);
+        const uint32_t n = granules_of(a, s), subs = subs_of(a, s);
+        uint32_t head = blockIdx.x, block = blockIdx.y, g0 = 0, g1 = n, count = end - at;
+        int part = -1;
+        if (shared) {
+            if (n * subs == 0 || in >= n * subs * a.cache.kv_heads) {
+                ++b;
+                in = 0;
+                continue;
+            }
+            head = in / (n * subs);
+            const uint32_t in_head = in - head * (n * subs), block_size = n * a.block_subs;
+            block = in_head / block_size;
+            const uint32_t g = in_head - block * block_size, cost = min(a.block_subs, subs - block * a.block_subs), size = n * cost;
+            count = min(size - g, end - at);
+            part = count == size ? -1 : g == 0 ? 1 : 0;
+            g0 = (g + cost - 1) >> (cost - 1);
+            g1 = (g + count + cost - 1) >> (cost - 1);
+        } else if (block * a.block_subs >= subs) {
+            return;
+        }
+        run(segment_of(a, s, b, head, block, g0, g1, part));
+        at += count;
+        in += count;
+    }
+}
+
+// ---- a wave's rows ---------------------------------------------------------------------------------------------------
+
+template <int D, int CODES, int R> struct WaveRows {
+    using S = Shape<D>;
+    uint32_t token[R];                   // the new token of the lane's row
     half8_t q[R][S::kSteps];
     float row_scale[R];
     float4_t o[R][S::kTiles];
     float m[R], l[R];
-    float t = 0.0f, inv_t = 0.0f;
+    float t, inv_t;
+
+    // Rows of the tiles `tile(r)` (16 rows each) of a segment; those behind its last are its last again.
+    template <typename F> __device__ __forceinline__ void start(Args& a, const Segment& x, uint32_t col, uint32_t quarter, F tile) {
+        t = 0.0f;
+        inv_t = 0.0f;
+        uint4_t raw[R][S::kSteps];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const uint32_t row = row0 + r * 16 + col;
-        token[r] = divide(min(row, last_row), a.group_magic);
-        const uint32_t g = min(row, last_row) - token[r] * a.group;
-        const char* from = a.q.data + int64_t(first_token + token[r]) * a.q.token_stride + int64_t(head * a.group + g) * a.q.head_stride;
-        float x[S::kSteps * 8];
-        uint32_t top = 0;
+        for (int r = 0; r < R; ++r) {
+            const uint32_t row = x.row0 + min(tile(r) * 16 + col, x.rows - 1);
+            token[r] = divide(row, a.group_magic);
+            const uint32_t g = row - token[r] * a.group;
+            const char* from = a.q.data + int64_t(x.seq.first_token + token[r]) * a.q.token_stride + int64_t(x.head * a.group + g) * a.q.head_stride;
 #pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-            // the elements that the quarter's codes of this step are of: kChunk / 4 neighbours of each run of kChunk
-            const uint32_t at = S::kChunk == 64 ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
-            const uint4_t w = *reinterpret_cast<const uint4_t*>(from + at * 2);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (a.type == FKLHIP_BF16) unpack2<FKLHIP_BF16>(w[k], x[s * 8 + 2 * k], x[s * 8 + 2 * k + 1]);
-                else unpack2<FKLHIP_F16>(w[k], x[s * 8 + 2 * k], x[s * 8 + 2 * k + 1]);
+            for (int s = 0; s < S::kSteps; ++s) {
+                // the elements that the quarter's codes of this step are of: kChunk / 4 neighbours of each run of kChunk
+                const uint32_t at = S::kChunk == 64 ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
+                raw[r][s] = *reinterpret_cast<const uint4_t*>(from + at * 2);
             }
         }
 #pragma unroll
-        for (int k = 0; k < S::kSteps * 8; ++k) top = max(top, __builtin_bit_cast(uint32_t, x[k]) & 0x7fffffffu);
-        top = max(top, uint32_t(__shfl_xor(int(top), 16)));
-        top = max(top, uint32_t(__shfl_xor(int(top), 32)));
-        // a power of two in front of the row's largest magnitude (finite; a row of zeros is left alone)
-        const int e = top == 0 || top >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
-        row_scale[r] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, e);
+        for (int r = 0; r < R; ++r) {
+            float e[S::kSteps * 8];
+            uint32_t top = 0;
 #pragma unroll
-        for (int s = 0; s < S::kSteps; ++s)
+            for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) q[r][s][k] = _Float16(__builtin_amdgcn_ldexpf(x[s * 8 + k], -e));
+                for (int k = 0; k < 4; ++k) {
+                    if (a.type == FKLHIP_BF16) unpack2<FKLHIP_BF16>(raw[r][s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
+                    else unpack2<FKLHIP_F16>(raw[r][s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
+                }
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        m[r] = kNothing;
-        l[r] = 0.0f;
+            for (int k = 0; k < S::kSteps * 8; ++k) top = max(top, __builtin_bit_cast(uint32_t, e[k]) & 0x7fffffffu);
+            top = max(top, uint32_t(__shfl_xor(int(top), 16)));
+            top = max(top, uint32_t(__shfl_xor(int(top), 32)));
+            // a power of two in front of the row's largest magnitude (a row of zeros, or with an infinity, is left alone)
+            const int p = top == 0 || top >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
+            row_scale[r] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, p);
+#pragma unroll
+            for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) q[r][s][k] = _Float16(__builtin_amdgcn_ldexpf(e[s * 8 + k], -p));
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            m[r] = kNothing;
+            l[r] = 0.0f;
+        }
     }
 
-    const int32_t* pages = a.page_table + int64_t(b) * a.page_table_stride;
-    const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
-    const uint32_t last_entry = total ? (total - 1) >> a.cache.page_log : 0;
-    // The loads of 32 keys: where they are, their codes, and their scales.
-    size_t rows_at[2];
-    Tile<D> tile;
-    auto locate = [&](uint32_t key) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t at = key + h * 16;
-            const uint32_t page = min(uint32_t(pages[min(at >> a.cache.page_log, last_entry)]), a.cache.pages - 1);
-            rows_at[h] = ((size_t(page) * a.cache.kv_heads + head) << a.cache.page_log) + (at & page_mask);
-        }
-    };
-    auto load_k = [&] {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) tile.k[h][i] = load_words<S::kWords>(a.cache.k + rows_at[h] * D + lane_k + i * S::kChunk);
-    };
-    auto load_scales_and_v = [&] {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            tile.ks[h] = *reinterpret_cast<const float4_t*>(a.cache.k_scale + rows_at[h] + quarter * 4);
-            tile.vs[h] = *reinterpret_cast<const float4_t*>(a.cache.v_scale + rows_at[h] + quarter * 4);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) tile.v[h][i] = load_words<S::kWords>(a.cache.v + rows_at[h] * D + lane_v + i * S::kChunk * 4);
-    };
-
-    auto process = [&](auto masked, uint32_t key, bool more) {
-        constexpr bool kMasked = decltype(masked)::value;
-        float4_t s[R][2];
+    // 32 keys from `key` on: get_k(block, load) and get_v have their codes, get_scales(block, ks, vs) their scales;
+    // after_scores runs when the keys are used up.
+    template <bool MASKED, typename K, typename V, typename G, typename A>
+    __device__ __forceinline__ void step(const Segment& x, uint32_t key, uint32_t quarter, K get_k, V get_v, G get_scales, A after_scores) {
+        float4_t y[R][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) s[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < R; ++r) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int st = 0; st < S::kSteps; ++st) {
-                const half8_t k = S::kWords == 4 ? halves8<CODES>(tile.k[h][st / 2].w[(st % 2) * 2], tile.k[h][st / 2].w[(st % 2) * 2 + 1])
-                                                 : halves8<CODES>(tile.k[h][S::kWords == 4 ? 0 : st].w[0], tile.k[h][S::kWords == 4 ? 0 : st].w[1]);
+            for (int i = 0; i < S::kLoads; ++i) {
+                const Words<S::kWords> w = get_k(h, i);
 #pragma unroll
-                for (int r = 0; r < R; ++r) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[r][st], s[r][h], 0, 0, 0);
+                for (int k = 0; k < S::kWords / 2; ++k) {
+                    const half8_t codes = halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[r][i * (S::kWords / 2) + k], y[r][h], 0, 0, 0);
+                }
             }
         }
-        if (more) load_k();                                        // (the keys' registers are free now, the values' at the end)
-        __builtin_amdgcn_sched_barrier(0);
-        uint32_t sees[R][2];                                        // of the quarter's four keys, a bit each
-        if constexpr (kMasked) {
+        after_scores();
+        uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each
+        float4_t ks[2], vs[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+            get_scales(h, ks[h], vs[h]);
+            keep[h] = ~0u;
+            if constexpr (MASKED) {
+                Args& a = kernel_args();
                 const uint32_t at = key + h * 16 + quarter * 4;
-                const uint32_t there = lowest_bits(int32_t(total - at));
+                const uint32_t there = lowest_bits(int32_t(x.seq.total - at));
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const int32_t u = int32_t(at - context);
-                    const uint32_t bits = causal ? lowest_bits(int32_t(token[r]) + 1 - u) : mask_bits(a.mask + int64_t(first_token + token[r]) * a.mask_words, a.mask_words, u);
+                    const int32_t u = int32_t(at - x.seq.context);
+                    const uint32_t bits = a.mask == nullptr ? lowest_bits(int32_t(token[r]) + 1 - u)
+                                                            : mask_bits(a.mask + int64_t(x.seq.first_token + token[r]) * a.mask_words, a.mask_words, u);
                     sees[r][h] = bits & there;
                 }
                 // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
-                uint32_t keep = 0;
+                keep[h] = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    keep |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
-                    tile.vs[h][i] = there >> i & 1 ? tile.vs[h][i] : 0.0f;
+                    keep[h] |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
+                    vs[h][i] = there >> i & 1 ? vs[h][i] : 0.0f;
                 }
-#pragma unroll
-                for (int i = 0; i < S::kLoads; ++i)
-#pragma unroll
-                    for (int k = 0; k < S::kWords; ++k) tile.v[h][i].w[k] &= keep;
             }
         }
-        // scores in units of log2, masked ones -inf
-        float lead = kNothing, scales = 0.0f;
+        // scores in units of log2 from the reference on, masked ones -inf
+        auto score = [&](int r, int h, int i) {
+            float z = __builtin_fmaf(y[r][h][i], row_scale[r], -m[r]);
+            if constexpr (MASKED) z = sees[r][h] >> i & 1 ? z : -__builtin_inff();
+            return z;
+        };
+        float lead = kNothing, scales = 0.0f, z[R][2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) scales = __builtin_fmaxf(scales, tile.vs[h][i]);
+            for (int i = 0; i < 4; ++i) {
+                scales = __builtin_fmaxf(scales, vs[h][i]);
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = s[r][h][i] * tile.ks[h][i] * row_scale[r];
-                    if constexpr (kMasked) x = sees[r][h] >> i & 1 ? x : -__builtin_inff();
-                    s[r][h][i] = x;
-                    lead = __builtin_fmaxf(lead, x - m[r]);
+                for (int r = 0; r < R; ++r) {
+                    y[r][h][i] *= ks[h][i];
+                    z[r][h][i] = score(r, h, i);
+                    lead = __builtin_fmaxf(lead, z[r][h][i]);
                 }
-        }
-        if (__any(lead > kLead || scales > t)) {
-            const float most = __builtin_fmaxf(scales, __shfl_xor(scales, 16));
-            const float largest = __builtin_fmaxf(most, __shfl_xor(most, 32));
+            }
+        if (__builtin_expect(__any(lead > kLead || scales > t), 0)) {
+            const float largest = max_quarters(scales);
             float shrink = 1.0f;
             if (largest > t) {
                 const float now = __builtin_fmaxf(largest, 1.0e-30f);
@@ -284,7 +307,11 @@ __global__ __launch_bounds__(kWaves * 64, R == 1 && D <= 128 ? 2 : 1) void k_tre
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, s[r][h][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        z[r][h][i] = y[r][h][i] * row_scale[r];
+                        if constexpr (MASKED) z[r][h][i] = sees[r][h] >> i & 1 ? z[r][h][i] : -__builtin_inff();
+                        top = __builtin_fmaxf(top, z[r][h][i]);
+                    }
                 top = max_quarters(top);
                 float alpha = 1.0f;
                 if (top - m[r] > kLead) {
@@ -296,6 +323,10 @@ __global__ __launch_bounds__(kWaves * 64, R == 1 && D <= 128 ? 2 : 1) void k_tre
                 alpha *= shrink;
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) o[r][i] *= alpha;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[r][h][i] -= m[r];     // (from the rounded score: at 2^100 it differs from score() by more than an exponent holds)
             }
         }
         half8_t p[R];
@@ -303,112 +334,319 @@ __global__ __launch_bounds__(kWaves * 64, R == 1 && D <= 128 ? 2 : 1) void k_tre
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float scaled = tile.vs[h][i] * inv_t;
+                const float scaled = vs[h][i] * inv_t;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const float e = exp2_fast(s[r][h][i] - m[r]);
+                    const float e = exp2_fast(z[r][h][i]);
                     l[r] += e;
                     float w = e * scaled;
-                    if constexpr (kMasked) w = s[r][h][i] == -__builtin_inff() ? 0.0f : w;   // (a hidden value's scale may be NaN)
+                    if constexpr (MASKED) w = sees[r][h] >> i & 1 ? w : 0.0f;       // (a hidden value's scale may be NaN)
                     p[r][h * 4 + i] = _Float16(w);
                 }
             }
 #pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) {
-            // tile i: elements (i / kWords) * kChunk + column * kWords + i % kWords
-            const half8_t v = halves8<CODES>(tile.v[0][i / S::kWords].w[i % S::kWords], tile.v[1][i / S::kWords].w[i % S::kWords]);
+        for (int c = 0; c < S::kLoads; ++c) {
+            const Words<S::kWords> v0 = get_v(0, c), v1 = get_v(1, c);
 #pragma unroll
-            for (int r = 0; r < R; ++r) o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[r], o[r][i], 0, 0, 0);
-        }
-    };
-
-    uint32_t key = key0 + wave * 32;
-    if (key < key1) {
-        locate(key);
-        load_k();
-        load_scales_and_v();
-    }
-    while (key < key1) {
-        const uint32_t after = key + kWaves * 32;
-        const bool more = after < key1;
-        if (more) locate(after);
-        if (key + 32 <= all_see) process(std::false_type{}, key, more);
-        else process(std::true_type{}, key, more);
-        if (more) load_scales_and_v();
-        __builtin_amdgcn_sched_barrier(0);
-        key = after;
-    }
-
-    // join the waves, 16 rows at a time, and write them
+            for (int k = 0; k < S::kWords; ++k) {
+                // tile c * kWords + k: elements c * kChunk + column * kWords + k
+                const half8_t v = MASKED ? halves8<CODES>(v0.w[k] & keep[0], v1.w[k] & keep[1]) : halves8<CODES>(v0.w[k], v1.w[k]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        l[r] = sum_quarters(l[r]);
-        if (quarter == 0) {
-            joined_m[wave][col] = m[r];
-            joined_l[wave][col] = l[r];
-        }
-        __syncthreads();
-        float top = joined_m[0][col], sum = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][col]);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += joined_l[w][col] * exp2_fast(joined_m[w][col] - top);
-        // l may be NaN (a NaN among the scores), and then the row is
-        const float factor = (sum == 0.0f ? 0.0f : exp2_fast(m[r] - top) / sum) * t;
-#pragma unroll
-        for (int c = 0; c < S::kLoads; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // rows quarter * 4 + i of the kWords tiles of a chunk are neighbouring elements
-                float* to = &joined[wave][col * kRowFloats + c * S::kChunk + (quarter * 4 + i) * S::kWords];
-#pragma unroll
-                for (int k = 0; k < S::kWords; ++k) to[k] = o[r][c * S::kWords + k][i] * factor;
-            }
-        if (wave == 0 && quarter == 0) row_l[col] = sum, row_m[col] = top;
-        __syncthreads();
-        // 16 rows of D elements, four to a thread
-        for (uint32_t at = threadIdx.x; at < 16 * D / 4; at += kWaves * 64) {
-            const uint32_t c = at / (D / 4), d = at % (D / 4) * 4;
-            const uint32_t row = row0 + r * 16 + c;
-            if (row >= rows) continue;
-            float4_t x = *reinterpret_cast<const float4_t*>(&joined[0][c * kRowFloats + d]);
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) x += *reinterpret_cast<const float4_t*>(&joined[w][c * kRowFloats + d]);
-            const uint32_t tok = divide(row, a.group_magic), qh = head * a.group + row - tok * a.group;
-            const size_t place = size_t(first_token + tok) * a.q_heads + qh;
-            const float lse = row_l[c] == 0.0f ? -__builtin_inff() : row_m[c] + __builtin_log2f(row_l[c]);
-            if (a.splits == 1) {
-                uint2_t w;
-                if (a.type == FKLHIP_BF16) { w.x = pack2<FKLHIP_BF16>(x[0], x[1]); w.y = pack2<FKLHIP_BF16>(x[2], x[3]); }
-                else { w.x = pack2<FKLHIP_F16>(x[0], x[1]); w.y = pack2<FKLHIP_F16>(x[2], x[3]); }
-                *reinterpret_cast<uint2_t*>(a.out.data + int64_t(first_token + tok) * a.out.token_stride + int64_t(qh) * a.out.head_stride + d * 2) = w;
-                if (d == 0 && a.lse) a.lse[place] = lse * kLn2;
-            } else {
-                *reinterpret_cast<float4_t*>(a.partial + (place * a.splits + split) * D + d) = x;
-                if (d == 0) a.partial_lse[place * a.splits + split] = lse;
+                for (int r = 0; r < R; ++r) o[r][c * S::kWords + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[r], o[r][c * S::kWords + k], 0, 0, 0);
             }
         }
-        __syncthreads();
+    }
+};
+
+// Four or two neighbouring elements of a row of the result: to the output, or to a share's part.
+template <int D, int N> __device__ __forceinline__ void put(Args& a, const Segment& x, uint32_t share, uint32_t row, uint32_t d, const float* v) {
+    if (x.part < 0) {
+        const uint32_t tok = divide(x.row0 + row, a.group_magic), qh = x.head * a.group + x.row0 + row - tok * a.group;
+        char* to = a.out.data + int64_t(x.seq.first_token + tok) * a.out.token_stride + int64_t(qh) * a.out.head_stride + d * 2;
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) w[k] = a.type == FKLHIP_BF16 ? pack2<FKLHIP_BF16>(v[2 * k], v[2 * k + 1]) : pack2<FKLHIP_F16>(v[2 * k], v[2 * k + 1]);
+        if constexpr (N == 4) *reinterpret_cast<uint2_t*>(to) = uint2_t{w[0], w[1]};
+        else *reinterpret_cast<uint32_t*>(to) = w[0];
+    } else {
+        float* to = a.partial + ((size_t(share) * 2 + x.part) * a.unit_rows + row) * D + d;
+#pragma unroll
+        for (int k = 0; k < N; ++k) to[k] = v[k];
+    }
+}
+// lse is in units of log2.
+__device__ __forceinline__ void put_lse(Args& a, const Segment& x, uint32_t share, uint32_t row, float m, float l) {
+    const float lse = l == 0.0f ? -__builtin_inff() : m + __builtin_log2f(l);
+    if (x.part < 0) {
+        if (!a.lse) return;
+        const uint32_t tok = divide(x.row0 + row, a.group_magic), qh = x.head * a.group + x.row0 + row - tok * a.group;
+        a.lse[size_t(x.seq.first_token + tok) * a.q_heads + qh] = lse * kLn2;
+    } else {
+        a.partial_lse[(size_t(share) * 2 + x.part) * a.unit_rows + row] = lse;
     }
 }
 
-template <int D, int CODES, int R> int start_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) {
-    // workgroups of the same keys and other rows are a multiple of eight apart, which is the same XCD and its L2
-    uint32_t x = a.cache.kv_heads * a.splits;
-    if (plan.row_blocks > 1) x = (x + 7) / 8 * 8;
-    const dim3 grid(x, plan.row_blocks, a.batch);
-    info = {"tree_attention", {grid.x, grid.y, grid.z}, {kWaves * 64, 1, 1}, uint32_t((kWaves * 16 * (D + 4 + 2) + 32) * 4)};
-    k_tree_attention<D, CODES, R><<<grid, dim3(kWaves * 64), 0, static_cast<hipStream_t>(stream)>>>(a);
+// Where 16 keys of a segment are in the cache: tokens in front of them.
+__device__ __forceinline__ size_t place_of_keys(Args& a, const Segment& x, uint32_t key) {
+    const int32_t* pages = a.page_table + int64_t(x.b) * a.page_table_stride;
+    const uint32_t last = (x.seq.total - 1) >> a.cache.page_log;
+    const uint32_t page = min(uint32_t(scalar(pages + min(key >> a.cache.page_log, last))), a.cache.pages - 1);
+    return ((size_t(page) * a.cache.kv_heads + x.head) << a.cache.page_log) + (key & ((1u << a.cache.page_log) - 1u));
+}
+
+// ---- few rows: the waves split the keys -------------------------------------------------------------------------------
+
+template <int D, int CODES, int R>
+__global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_split_keys(const AttentionArgs) {
+    using S = Shape<D>;
+    constexpr int kRowFloats = D + 4;                              // of a row in LDS: 16 bytes further round the banks than the last
+    __shared__ __attribute__((aligned(16))) float joined[kWaves][16 * kRowFloats];
+    __shared__ float joined_m[kWaves][16], joined_l[kWaves][16], row_m[16], row_l[16];
+    walk(kernel_args(), threadIdx.x & 63, [&](const Segment& x) {
+        Args& a = kernel_args();
+        const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
+        const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
+        size_t at[2];
+        Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
+        float4_t ks[2], vs[2];
+        auto locate = [&](uint32_t key) {
+            Args& fresh = kernel_args();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) at[h] = place_of_keys(fresh, x, key + h * 16);
+        };
+        auto load_k = [&] {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < S::kLoads; ++i) k[h][i] = load_words<S::kWords>(a.cache.k + at[h] * D + lane_k + i * S::kChunk);
+        };
+        auto load_scales_and_v = [&] {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ks[h] = *reinterpret_cast<const float4_t*>(a.cache.k_scale + at[h] + quarter * 4);
+                vs[h] = *reinterpret_cast<const float4_t*>(a.cache.v_scale + at[h] + quarter * 4);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < S::kLoads; ++i) v[h][i] = load_words<S::kWords>(a.cache.v + at[h] * D + lane_v + i * S::kChunk * 4);
+        };
+        uint32_t key = x.key0 + wave * 32;
+        WaveRows<D, CODES, R> rows;
+        rows.start(kernel_args(), x, col, quarter, [](int r) { return uint32_t(r); });
+        if (key < x.key1) {
+            locate(key);
+            load_k();
+            load_scales_and_v();
+        }
+        auto get_k = [&](int h, int i) { return k[h][i]; };
+        auto get_v = [&](int h, int i) { return v[h][i]; };
+        auto get_scales = [&](int h, float4_t& s, float4_t& t) { s = ks[h]; t = vs[h]; };
+        // keys that all rows see, then the others
+        auto keys = [&](auto masked, uint32_t end) {
+#pragma unroll 1
+            while (key < end) {
+                const uint32_t next = key + kWaves * 32;
+                const bool more = next < x.key1;
+                if (more) locate(next);
+                // the keys' registers are free for the next once the scores are there, the others' at the end
+                rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [&] {
+                    if (more) load_k();
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                if (more) load_scales_and_v();
+                __builtin_amdgcn_sched_barrier(0);
+                key = next;
+            }
+        };
+        keys(std::false_type{}, min(x.key1, x.all_see & ~31u));
+        keys(std::true_type{}, x.key1);
+        // join the waves, 16 rows at a time, and write them
+        Args& out = kernel_args();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float l = sum_quarters(rows.l[r]), m = rows.m[r];
+            if (quarter == 0) {
+                joined_m[wave][col] = m;
+                joined_l[wave][col] = l;
+            }
+            __syncthreads();
+            float top = joined_m[0][col], sum = 0.0f;
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][col]);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) sum += joined_l[w][col] * exp2_fast(joined_m[w][col] - top);
+            // (a sum that is NaN, from a NaN among the scores, makes the row NaN)
+            const float factor = (sum == 0.0f ? 0.0f : exp2_fast(m - top) / sum) * rows.t;
+#pragma unroll
+            for (int c = 0; c < S::kLoads; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // rows quarter * 4 + i of the kWords tiles of a chunk are neighbouring elements
+                    float* to = &joined[wave][col * kRowFloats + c * S::kChunk + (quarter * 4 + i) * S::kWords];
+#pragma unroll
+                    for (int w = 0; w < S::kWords; ++w) to[w] = rows.o[r][c * S::kWords + w][i] * factor;
+                }
+            if (wave == 0 && quarter == 0) row_l[col] = sum, row_m[col] = top;
+            __syncthreads();
+            for (uint32_t i = thread; i < 16 * D / 4; i += kWaves * 64) {
+                const uint32_t c = i / (D / 4), d = i % (D / 4) * 4, row = r * 16 + c;
+                if (row >= x.rows) continue;
+                float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][c * kRowFloats + d]);
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][c * kRowFloats + d]);
+                const float f[4] = {e[0], e[1], e[2], e[3]};
+                put<D, 4>(out, x, own_share(out), row, d, f);
+                if (d == 0) put_lse(out, x, own_share(out), row, row_m[c], row_l[c]);
+            }
+            __syncthreads();
+        }
+    });
+}
+
+// ---- many rows: the waves split the rows ------------------------------------------------------------------------------
+
+// A stage of keys: per block of 16 their codes, their values' codes, and the scales of both. A wave copies a block, or, where
+// a stage has two (heads of more than 128 elements), the keys' or the values' half of one. Three stages stay under 64 KB.
+template <int D> struct Stage {
+    static constexpr uint32_t kBlocks = D <= 128 ? 4 : 2, kKeys = 16 * kBlocks, kCodes = 16 * D, kBlockBytes = 2 * kCodes + 128, kBytes = kBlocks * kBlockBytes;
+    static constexpr int kStages = 3, kRuns = (kCodes + 1023) / 1024;     // runs of 1 KB (the second of 1536 bytes is half of one)
+    static constexpr int kCopies = kBlocks == 4 ? 2 * kRuns + 1 : kRuns + 1;   // memory operations of a wave
+};
+
+// Copies to LDS without registers, 16 or 4 bytes a lane at `lds` + the same times the lane's number; the count of memory
+// operations in flight says when they are there.
+__device__ __forceinline__ void copy16(const char* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const char* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+// All but the wave's last N memory operations are done; then all waves' are, and nobody reads LDS any more.
+template <int N> __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
+
+template <int D, int CODES, int R>
+__global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(const AttentionArgs) {
+    using S = Shape<D>;
+    using P = Stage<D>;
+    __shared__ __attribute__((aligned(1024))) char ring[P::kStages * P::kBytes];
+    // Runs of 16 bytes a lane are copied so that a lane finds its own at 16 * lane; those of 8 (heads of 96) as they lie.
+    constexpr bool kOwn = S::kWords == 4;
+    constexpr uint32_t kNextK = kOwn ? 1024 : 32, kNextV = kOwn ? 1024 : 128;
+    walk(kernel_args(), threadIdx.x & 63, [&](const Segment& x) {
+        const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
+        const uint32_t from_k = kOwn ? col * D + quarter * 16 : lane * 16, from_v = kOwn ? quarter * (4 * D) + col * 16 : lane * 16;
+        const uint32_t read_k = kOwn ? lane * 16 : col * D + quarter * 8, read_v = kOwn ? lane * 16 : quarter * (4 * D) + col * 8;
+        const uint32_t ring_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring)));
+        const uint32_t stages = x.key1 > x.key0 ? (x.key1 - x.key0 + P::kKeys - 1) / P::kKeys : 0;
+        auto copy = [&](uint32_t stage) {
+            Args& a = kernel_args();
+            const uint32_t block = P::kBlocks == 4 ? wave : wave & 1;
+            const size_t at = place_of_keys(a, x, x.key0 + stage * P::kKeys + block * 16);
+            const uint32_t to = ring_at + (stage % P::kStages) * P::kBytes + block * P::kBlockBytes;
+#pragma unroll
+            for (int i = 0; i < P::kRuns; ++i)
+                if (kOwn || i == 0 || lane < 32) {
+                    if (P::kBlocks == 4 || wave < 2) copy16(a.cache.k + at * D, from_k + i * (kOwn ? 64 : 1024), to + i * 1024);
+                    if (P::kBlocks == 4 || wave >= 2) copy16(a.cache.v + at * D, from_v + i * (kOwn ? 256 : 1024), to + P::kCodes + i * 1024);
+                }
+            // 16 scales of keys and 16 of values side by side: the lanes' offsets cover the distance of the two arrays
+            if (lane < 32) {
+                if (P::kBlocks == 4) {
+                    const char* s = reinterpret_cast<const char*>((lane < 16 ? a.cache.k_scale : a.cache.v_scale) + at) + (lane & 15) * 4;
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to + 2 * P::kCodes), "v"(s) : "memory", "m0");
+                } else if (lane < 16) {
+                    copy4(reinterpret_cast<const char*>((wave < 2 ? a.cache.k_scale : a.cache.v_scale) + at), lane * 4, to + 2 * P::kCodes + (wave < 2 ? 0 : 64));
+                }
+            }
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < P::kStages - 1; ++i)
+            if (i < stages) copy(i);
+        const uint32_t tiles = (x.rows + 15) / 16;
+        auto loop = [&](auto count) {
+            constexpr int kMine = decltype(count)::value;
+            WaveRows<D, CODES, kMine == 0 ? 1 : kMine> rows;
+            if constexpr (kMine > 0) rows.start(kernel_args(), x, col, quarter, [&](int r) { return wave + kWaves * r; });
+            uint32_t stage = 0;
+            // stages whose keys all rows see, then the others
+            auto keys = [&](auto masked, uint32_t end) {
+#pragma unroll 1
+                for (; stage < end; ++stage) {
+                    if (stage + 1 < stages) arrive<P::kCopies>();
+                    else arrive<0>();
+                    if (stage + P::kStages - 1 < stages) copy(stage + P::kStages - 1);
+                    if constexpr (kMine > 0) {
+                        const char* here = ring + (stage % P::kStages) * P::kBytes;
+#pragma unroll 1
+                        for (uint32_t half = 0; half < P::kBlocks / 2; ++half) {
+                            const uint32_t key = x.key0 + stage * P::kKeys + half * 32;
+                            if (decltype(masked)::value && key >= x.key1) break;
+                            const char* piece = here + half * 2 * P::kBlockBytes;
+                            auto get_k = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + read_k + i * kNextK); };
+                            auto get_v = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + P::kCodes + read_v + i * kNextV); };
+                            auto get_scales = [&](int h, float4_t& s, float4_t& t) {
+                                s = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + quarter * 16);
+                                t = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + 64 + quarter * 16);
+                            };
+                            rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [] {});
+                        }
+                    }
+                }
+            };
+            keys(std::false_type{}, min(x.key1, x.all_see) > x.key0 ? (min(x.key1, x.all_see) - x.key0) / P::kKeys : 0);
+            keys(std::true_type{}, stages);
+            if constexpr (kMine > 0) {
+                Args& out = kernel_args();
+                const uint32_t share = own_share(out);
+#pragma unroll
+                for (int r = 0; r < kMine; ++r) {
+                    const uint32_t row = (wave + kWaves * r) * 16 + col;
+                    const float l = sum_quarters(rows.l[r]);
+                    const float factor = l == 0.0f ? 0.0f : rows.t / l;
+                    if (row < x.rows) {
+#pragma unroll
+                        for (int c = 0; c < S::kLoads; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float v[S::kWords];
+#pragma unroll
+                                for (int w = 0; w < S::kWords; ++w) v[w] = rows.o[r][c * S::kWords + w][i] * factor;
+                                put<D, S::kWords>(out, x, share, row, c * S::kChunk + (quarter * 4 + i) * S::kWords, v);
+                            }
+                        if (quarter == 0) put_lse(out, x, share, row, rows.m[r], l);
+                    }
+                }
+            }
+        };
+        if (R == 2 && tiles > wave + kWaves) loop(std::integral_constant<int, R>{});
+        else if (tiles > wave) loop(std::integral_constant<int, 1>{});
+        else loop(std::integral_constant<int, 0>{});
+        arrive<0>();                                               // before the next segment's copies
+    });
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------
+
+template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
+    const dim3 grid = a.shares_log == kNoShares ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(1u << a.shares_log, 1, 1), block(kWaves * 64);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    info = {p.split_rows ? "tree_attention_rows" : "tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1},
+            p.split_rows ? uint32_t(Stage<D>::kStages * Stage<D>::kBytes) : uint32_t((kWaves * 16 * (D + 4 + 2) + 32) * 4)};
+    if constexpr (D <= 128) {
+        if (p.tiles == 2) {
+            if (p.split_rows) k_split_rows<D, CODES, 2><<<grid, block, 0, s>>>(a);
+            else k_split_keys<D, CODES, 2><<<grid, block, 0, s>>>(a);
+            return int(hipGetLastError());
+        }
+    }
+    if (p.split_rows) k_split_rows<D, CODES, 1><<<grid, block, 0, s>>>(a);
+    else k_split_keys<D, CODES, 1><<<grid, block, 0, s>>>(a);
     return int(hipGetLastError());
 }
 
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) {
-    const bool int8 = a.cache.codes == FKLHIP_CODES_INT8;
-    if constexpr (D <= 128) {
-        if (plan.row_tiles == 2)
-            return int8 ? start_attention<D, FKLHIP_CODES_INT8, 2>(a, plan, stream, info) : start_attention<D, FKLHIP_CODES_E4M3, 2>(a, plan, stream, info);
-    }
-    return int8 ? start_attention<D, FKLHIP_CODES_INT8, 1>(a, plan, stream, info) : start_attention<D, FKLHIP_CODES_E4M3, 1>(a, plan, stream, info);
+    return a.cache.codes == FKLHIP_CODES_INT8 ? start_attention<D, FKLHIP_CODES_INT8>(a, plan, stream, info) : start_attention<D, FKLHIP_CODES_E4M3>(a, plan, stream, info);
 }
 
 } // namespace fkattn

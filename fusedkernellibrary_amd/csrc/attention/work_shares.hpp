@@ -1,0 +1,93 @@
+// work_shares.hpp -- how attention's work is dealt out to workgroups: all of them count it the same way.
+#pragma once
+
+#include "attention_device.hpp"
+
+namespace fkattn {
+
+// A kernel's only argument as it lies in the kernel-argument segment. Every call reads its fields anew, by scalar loads where
+// they are used: held in registers from the start they are more than there are scalar registers.
+using Args = const __attribute__((address_space(4))) AttentionArgs;
+__device__ __forceinline__ Args& kernel_args() {
+    auto p = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+// The thread's number, for a part of a kernel that is run again and again: what is computed from it stays in that part (the
+// compiler would move it in front of the loop over segments, and keep it in registers through everything).
+__device__ __forceinline__ uint32_t thread_here() {
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+// What no kernel writes while it runs, at a place that is the same for the whole wave: a scalar load.
+template <typename T> __device__ __forceinline__ T scalar(const T* p) { return *(const __attribute__((address_space(4))) T*)(uintptr_t)p; }
+
+// A sequence as the device finds it, held inside what the host was told.
+struct Sequence { uint32_t first_token, fresh, context, total, rows; };
+__device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t end, int32_t have) {
+    Sequence s;
+    s.first_token = start < 0 ? 0u : min(uint32_t(start), a.tokens);
+    const int32_t diff = end - int32_t(s.first_token);
+    s.fresh = diff < 0 ? 0u : min(min(uint32_t(diff), a.max_new), a.tokens - s.first_token);
+    s.context = have < 0 ? 0u : min(min(uint32_t(have), a.max_context), a.room);
+    s.total = min(s.context + s.fresh, a.room);
+    s.rows = s.fresh * a.group;
+    return s;
+}
+__device__ __forceinline__ Sequence sequence_at(Args& a, uint32_t b) { return sequence_of(a, scalar(a.q_start + b), scalar(a.q_start + b + 1), scalar(a.context + b)); }
+// Work is counted in granules: a.granule keys of one key head and up to a.sub_rows of its rows. A row block has up to
+// a.block_subs times as many rows, and its keys count once for each a.sub_rows of them.
+__device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return (s.total + (1u << a.granule_log) - 1) >> a.granule_log; }
+__device__ __forceinline__ uint32_t subs_of(Args& a, const Sequence& s) { return (s.rows + (1u << a.sub_log) - 1) >> a.sub_log; }
+__device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return subs_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
+
+__device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(v, d);
+        v += lane >= uint32_t(d) ? o : 0u;
+    }
+    return v;
+}
+
+// (of the lane's own sequence)
+__device__ __forceinline__ Sequence sequence_of_lane(Args& a, uint32_t b) { return sequence_of(a, a.q_start[b], a.q_start[b + 1], a.context[b]); }
+__device__ __forceinline__ uint32_t weigh(Args& a, uint32_t b) { return b < a.batch ? weight_of(a, sequence_of_lane(a, b)) : 0u; }
+// The granules of all sequences, and the first of a sequence: that of granule at(all), or that of a token.
+struct Found { uint32_t all, b, before; };
+template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t lane, F is_it) {
+    uint32_t before = 0;
+    Found f{0, a.batch, 0};
+    if (a.batch <= 64) {
+        const uint32_t own = weigh(a, lane), upto = scan_wave(own, lane);
+        f.all = __builtin_amdgcn_readlane(int(upto), 63);
+        const uint64_t hits = __ballot(lane < a.batch && is_it(f.all, lane, upto - own, upto));
+        if (hits) {
+            f.b = __builtin_ctzll(hits);
+            f.before = __builtin_amdgcn_readlane(int(upto - own), int(f.b));
+        }
+        return f;
+    }
+    for (uint32_t b = lane; b < a.batch; b += 64) f.all += weigh(a, b);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) f.all += __shfl_xor(f.all, d);
+    f.all = __builtin_amdgcn_readfirstlane(f.all);
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        const uint32_t own = weigh(a, b0 + lane), upto = before + scan_wave(own, lane);
+        const uint64_t hits = __ballot(b0 + lane < a.batch && is_it(f.all, b0 + lane, upto - own, upto));
+        if (hits) {
+            const int hit = __builtin_ctzll(hits);
+            f.b = b0 + hit;
+            f.before = __builtin_amdgcn_readlane(int(upto - own), hit);
+            return f;
+        }
+        before = __builtin_amdgcn_readlane(int(upto), 63);
+    }
+    return f;
+}
+__device__ __forceinline__ uint32_t share_begin(Args& a, uint32_t all, uint32_t share) { return uint32_t((uint64_t(share) * all) >> a.shares_log); }
+// Neighbouring shares, which may be of the same keys, are on the same XCD (workgroups go round the eight).
+__device__ __forceinline__ uint32_t own_share(Args& a) { return a.shares_log >= 3 ? (blockIdx.x & 7u) << (a.shares_log - 3) | blockIdx.x >> 3 : blockIdx.x; }
+
+} // namespace fkattn
