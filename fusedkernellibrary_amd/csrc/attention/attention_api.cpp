@@ -131,7 +131,7 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, Attention
 }
 
 uint64_t workspace_of(const fklhip_kv_cache& cache, const AttentionPlan& plan) {
-    return plan.shares_log == kNoShares ? 0 : (uint64_t(plan.unit_rows) << (plan.shares_log + 1)) * (cache.head_dim + 1) * 4;
+    return uint64_t(plan.shares()) * 2 * plan.unit_rows * (cache.head_dim + 1) * 4;
 }
 
 } // namespace
@@ -210,11 +210,11 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     a.group_magic = magic(a.group);
     a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
     a.unit_rows = plan.unit_rows; a.block_subs = plan.unit_rows >> plan.sub_log; a.sub_log = plan.sub_log;
-    a.granule_log = plan.granule_log; a.shares_log = plan.shares_log;
+    a.granule_log = plan.granule_log; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
     a.type = c->type; a.scale = c->scale;
     if (bytes) {
         a.partial = static_cast<float*>(c->workspace);
-        a.partial_lse = a.partial + (uint64_t(plan.unit_rows) << (plan.shares_log + 1)) * uint64_t(cache->head_dim);
+        a.partial_lse = a.partial + uint64_t(plan.shares()) * 2 * plan.unit_rows * uint64_t(cache->head_dim);
     }
     Launched info;
     int rc;
@@ -225,7 +225,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     case 192: rc = launch_attention<192>(a, plan, stream, info); break;
     default: rc = launch_attention<256>(a, plan, stream, info); break;
     }
-    if (rc == FKLHIP_OK && bytes) rc = launch_merge(a, uint32_t(cache->head_dim), stream);
+    if (rc == FKLHIP_OK && bytes) rc = launch_merge(a, uint32_t(cache->head_dim), plan.many_parts, stream);
     return finish(rc, info);
 }
 
@@ -245,10 +245,13 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     p.row_blocks = std::max(1u, (rows + p.unit_rows - 1) / p.unit_rows);
     const uint64_t granules = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log, units = uint64_t(batch) * kv_heads * p.row_blocks;
     const uint64_t all = units * granules * (p.unit_rows >> p.sub_log);
-    // as many shares as workgroups run at once on 256 compute units, but two granules to each
-    const uint32_t most = p.split_rows ? (head_dim > 128 ? 8 : 9) : p.tiles == 2 || head_dim > 128 ? 9 : 10;
-    p.shares_log = kNoShares;
-    if (granules > 4 && units < (uint64_t(4) << most) && all < (uint64_t(1) << 32)) p.shares_log = std::min(most, log2_floor(all / 2));
+    // as many shares as workgroups run at once on 256 compute units, or a power of two that leaves two granules to each
+    const uint32_t at_once = head_dim > 128 ? 1 : p.split_rows || p.tiles == 2 ? 2 : 3;
+    p.share_log = 8 + (at_once == 2);
+    p.share_odd = at_once == 3 ? 3 : 1;
+    if (granules <= 4 || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
+    else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
+    p.many_parts = p.shares() > 16 * units;
     return p;
 }
 

@@ -1,50 +1,107 @@
 // merge.hip -- joins the parts of a row's attention that several shares of the work computed (work_shares.hpp).
 //
-// o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max). A workgroup to a row: its threads take the parts' weights first, then
-// groups of lanes take a part each, so that many parts are read at once. Bound by latency: counting the work, reading a
-// few weights, reading the parts (4 bytes an element), one after another.
+// o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max). Bound by latency: counting the work, reading the parts' weights,
+// reading the parts (4 bytes an element), one after another. Few parts to a row: a group of lanes takes a row (k_merge_few).
+// Many: a workgroup does, whose groups of lanes take a part each, so that many parts are read at once (k_merge_many).
 #include "work_shares.hpp"
 
 namespace fkattn {
 namespace {
 
 constexpr uint32_t kThreads = 256, kMostParts = 1025;         // (a row's parts are of neighbouring shares)
+template <int D> struct Lanes { static constexpr uint32_t kRow = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = kThreads / kRow; };
 
-template <int D> __global__ __launch_bounds__(kThreads) void k_merge(const AttentionArgs) {
-    Args& a = kernel_args();
-    constexpr uint32_t kLanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = kThreads / kLanes;
-    __shared__ float weight[kMostParts], tops[4], sums[4];
-    __shared__ __attribute__((aligned(16))) float joined[kGroups][D];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t head = blockIdx.x, token = blockIdx.y + blockIdx.z * 32768u;
-    if (token >= a.tokens) return;
-    const Found f = find(a, lane, [&](uint32_t, uint32_t b, uint32_t, uint32_t) {
+// The sequence of a token, with the granules in front of it.
+struct TokenOf { Sequence s; Found f; };
+__device__ __forceinline__ TokenOf sequence_of_token(Args& a, uint32_t token) {
+    TokenOf x;
+    x.f = find(a, threadIdx.x & 63, [&](uint32_t, uint32_t b, uint32_t, uint32_t) {
         const Sequence s = sequence_of_lane(a, b);
         return token >= s.first_token && token - s.first_token < s.fresh;
     });
-    if (f.b >= a.batch) return;                               // a row of no sequence
-    const Sequence s = sequence_at(a, f.b);
-    const uint32_t n = granules_of(a, s), subs = subs_of(a, s);
-    const uint32_t kv_head = divide(head, a.group_magic), row = (token - s.first_token) * a.group + head - kv_head * a.group;
-    const uint32_t block = row / a.unit_rows, size = n * min(a.block_subs, subs - block * a.block_subs);
-    const uint32_t first = f.before + kv_head * (n * subs) + block * a.block_subs * n;
-    char* out = a.out.data + int64_t(token) * a.out.token_stride + int64_t(head) * a.out.head_stride;
-    const uint32_t at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = at * 4;
-    if (size == 0) {                                          // no keys: nobody had it
-        if (group == 0 && d < D) *reinterpret_cast<uint2_t*>(out + d * 2) = uint2_t{0, 0};
-        if (threadIdx.x == 0 && a.lse) a.lse[size_t(token) * a.q_heads + head] = -__builtin_inff();
-        return;
+    if (x.f.b < a.batch) x.s = sequence_at(a, x.f.b);
+    return x;
+}
+// A row's parts: those of shares share0 .. share0 + count. None: nobody had any of it. One: it has been written.
+struct Parts {
+    uint32_t share0, count, row;
+    __device__ __forceinline__ size_t place(Args& a, uint32_t part) const { return (size_t(share0 + part) * 2 + (part == 0 ? 1 : 0)) * a.unit_rows + row; }
+    // (a share of nothing, between others where there are more shares than granules, wrote nothing)
+    __device__ __forceinline__ float lse(Args& a, uint32_t all, uint32_t part) const {
+        return share_begin(a, all, share0 + part) == share_begin(a, all, share0 + part + 1) ? -__builtin_inff() : a.partial_lse[place(a, part)];
     }
-    // the share of a granule g: the largest i with i * all / shares <= g
-    const auto share_of = [&](uint32_t g) { return uint32_t((((uint64_t(g) + 1) << a.shares_log) + f.all - 1) / f.all) - 1; };
-    const uint32_t share0 = share_of(first), share1 = share_of(first + size - 1);
-    if (share0 == share1) return;                             // written by the one share that had all of it
-    const uint32_t parts = share1 - share0 + 1, in_block = row - block * a.unit_rows;
-    const auto place = [&](uint32_t part) { return (size_t(share0 + part) * 2 + (part == 0 ? 1 : 0)) * a.unit_rows + in_block; };
+};
+__device__ __forceinline__ Parts parts_of(Args& a, const TokenOf& x, uint32_t token, uint32_t head) {
+    const uint32_t n = granules_of(a, x.s), subs = subs_of(a, x.s);
+    const uint32_t kv_head = divide(head, a.group_magic), row = (token - x.s.first_token) * a.group + head - kv_head * a.group;
+    const uint32_t block = row / a.unit_rows, size = n * min(a.block_subs, subs - block * a.block_subs);
+    if (size == 0) return {0, 0, 0};
+    const uint32_t first = x.f.before + kv_head * (n * subs) + block * a.block_subs * n;
+    const uint32_t share0 = share_of(a, x.f.all, first);
+    return {share0, share_of(a, x.f.all, first + size - 1) - share0 + 1, row - block * a.unit_rows};
+}
+// Four elements of a row, and its lse (in units of log2).
+__device__ __forceinline__ void put4(Args& a, uint32_t token, uint32_t head, uint32_t d, float4_t x) {
+    uint2_t w;
+    if (a.type == FKLHIP_BF16) { w.x = pack2<FKLHIP_BF16>(x[0], x[1]); w.y = pack2<FKLHIP_BF16>(x[2], x[3]); }
+    else { w.x = pack2<FKLHIP_F16>(x[0], x[1]); w.y = pack2<FKLHIP_F16>(x[2], x[3]); }
+    *reinterpret_cast<uint2_t*>(a.out.data + int64_t(token) * a.out.token_stride + int64_t(head) * a.out.head_stride + d * 2) = w;
+}
+__device__ __forceinline__ void put_lse(Args& a, uint32_t token, uint32_t head, float lse) {
+    if (a.lse) a.lse[size_t(token) * a.q_heads + head] = lse * 0.6931471805599453f;
+}
+
+template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const AttentionArgs) {
+    constexpr uint32_t kLanes = Lanes<D>::kRow;
+    Args& a = kernel_args();
+    const uint32_t at = threadIdx.x % kLanes, head = blockIdx.x * Lanes<D>::kGroups + threadIdx.x / kLanes, d = at * 4;
+    const uint32_t token = blockIdx.y + blockIdx.z * 32768u;
+    if (token >= a.tokens) return;
+    const TokenOf x = sequence_of_token(a, token);
+    if (x.f.b >= a.batch || head >= a.q_heads) return;        // a row of no sequence, or none
+    const Parts p = parts_of(a, x, token, head);
+    if (p.count == 1) return;
+    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (uint32_t i0 = 0; i0 < p.count; i0 += kLanes) {
+        const float mine = i0 + at < p.count ? p.lse(a, x.f.all, i0 + at) : -__builtin_inff();
+        float most = mine;
+#pragma unroll
+        for (uint32_t i = kLanes / 2; i; i >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, i, kLanes));
+        const float now = __builtin_fmaxf(top, most), base = now == -__builtin_inff() ? 0.0f : now, alpha = __builtin_amdgcn_exp2f(top - base);
+        top = now;
+        o *= alpha;
+        const float weight = __builtin_amdgcn_exp2f(mine - base);
+        float all = weight;
+#pragma unroll
+        for (uint32_t i = kLanes / 2; i; i >>= 1) all += __shfl_xor(all, i, kLanes);
+        sum = sum * alpha + all;                              // NaN where a part's is
+        const uint32_t count = min(kLanes, p.count - i0);
+#pragma unroll 4
+        for (uint32_t i = 0; i < count; ++i) {
+            const float w = __shfl(weight, i, kLanes);
+            if (d < D && w != 0.0f) o += *reinterpret_cast<const float4_t*>(a.partial + p.place(a, i0 + i) * D + d) * w;
+        }
+    }
+    if (d < D) put4(a, token, head, d, o * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (at == 0) put_lse(a, token, head, top + __builtin_log2f(sum));
+}
+
+template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const AttentionArgs) {
+    constexpr uint32_t kLanes = Lanes<D>::kRow, kGroups = Lanes<D>::kGroups;
+    __shared__ float weight[kMostParts], tops[4], sums[4];
+    __shared__ __attribute__((aligned(16))) float joined[kGroups][D];
+    Args& a = kernel_args();
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = at * 4;
+    const uint32_t head = blockIdx.x, token = blockIdx.y + blockIdx.z * 32768u;
+    if (token >= a.tokens) return;
+    const TokenOf t = sequence_of_token(a, token);
+    if (t.f.b >= a.batch) return;
+    const Parts p = parts_of(a, t, token, head);
+    if (p.count == 1) return;
     float top = -__builtin_inff();
-    for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
-        const uint32_t share = share0 + i;
-        const float x = share_begin(a, f.all, share) == share_begin(a, f.all, share + 1) ? -__builtin_inff() : a.partial_lse[place(i)];   // (shares of nothing)
+    for (uint32_t i = threadIdx.x; i < p.count; i += kThreads) {
+        const float x = p.lse(a, t.f.all, i);
         weight[i] = x;
         top = __builtin_fmaxf(top, x);
     }
@@ -55,7 +112,7 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge(const Atten
     top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
     const float base = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
-    for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < p.count; i += kThreads) {
         const float w = __builtin_amdgcn_exp2f(weight[i] - base);
         weight[i] = w;
         sum += w;
@@ -64,13 +121,13 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge(const Atten
     for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
-    sum = sums[0] + sums[1] + sums[2] + sums[3];              // NaN where a part's is
+    sum = sums[0] + sums[1] + sums[2] + sums[3];
     float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
     if (d < D) {
 #pragma unroll 4
-        for (uint32_t i = group; i < parts; i += kGroups) {
+        for (uint32_t i = group; i < p.count; i += kGroups) {
             const float w = weight[i];
-            if (w != 0.0f) x += *reinterpret_cast<const float4_t*>(a.partial + place(i) * D + d) * w;
+            if (w != 0.0f) x += *reinterpret_cast<const float4_t*>(a.partial + p.place(a, i) * D + d) * w;
         }
         *reinterpret_cast<float4_t*>(&joined[group][d]) = x;
     }
@@ -78,29 +135,29 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge(const Atten
     if (group == 0 && d < D) {
 #pragma unroll
         for (uint32_t i = 1; i < kGroups; ++i) x += *reinterpret_cast<const float4_t*>(&joined[i][d]);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        x *= inv;
-        uint2_t w;
-        if (a.type == FKLHIP_BF16) { w.x = pack2<FKLHIP_BF16>(x[0], x[1]); w.y = pack2<FKLHIP_BF16>(x[2], x[3]); }
-        else { w.x = pack2<FKLHIP_F16>(x[0], x[1]); w.y = pack2<FKLHIP_F16>(x[2], x[3]); }
-        *reinterpret_cast<uint2_t*>(out + d * 2) = w;
-        if (at == 0 && a.lse) a.lse[size_t(token) * a.q_heads + head] = (top + __builtin_log2f(sum)) * 0.6931471805599453f;
+        put4(a, token, head, d, x * (sum == 0.0f ? 0.0f : 1.0f / sum));
+        if (at == 0) put_lse(a, token, head, top + __builtin_log2f(sum));
     }
+}
+
+template <int D> int start_merge(const AttentionArgs& a, bool many_parts, hipStream_t s) {
+    const uint32_t y = a.tokens < 32768u ? a.tokens : 32768u, z = (a.tokens + 32767u) / 32768u;
+    if (many_parts) k_merge_many<D><<<dim3(a.q_heads, y, z), kThreads, 0, s>>>(a);
+    else k_merge_few<D><<<dim3((a.q_heads + Lanes<D>::kGroups - 1) / Lanes<D>::kGroups, y, z), kThreads, 0, s>>>(a);
+    return int(hipGetLastError());
 }
 
 } // namespace
 
-int launch_merge(const AttentionArgs& a, uint32_t head_dim, void* stream) {
-    const dim3 grid(a.q_heads, a.tokens < 32768u ? a.tokens : 32768u, (a.tokens + 32767u) / 32768u);
+int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream) {
     const hipStream_t s = static_cast<hipStream_t>(stream);
     switch (head_dim) {
-    case 64: k_merge<64><<<grid, kThreads, 0, s>>>(a); break;
-    case 96: k_merge<96><<<grid, kThreads, 0, s>>>(a); break;
-    case 128: k_merge<128><<<grid, kThreads, 0, s>>>(a); break;
-    case 192: k_merge<192><<<grid, kThreads, 0, s>>>(a); break;
-    default: k_merge<256><<<grid, kThreads, 0, s>>>(a); break;
+    case 64: return start_merge<64>(a, many_parts, s);
+    case 96: return start_merge<96>(a, many_parts, s);
+    case 128: return start_merge<128>(a, many_parts, s);
+    case 192: return start_merge<192>(a, many_parts, s);
+    default: return start_merge<256>(a, many_parts, s);
     }
-    return int(hipGetLastError());
 }
 
 } // namespace fkattn

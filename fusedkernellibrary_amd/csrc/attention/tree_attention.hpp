@@ -130,7 +130,7 @@ __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32
 template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, F run) {
     // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
     uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
-    const bool shared = a.shares_log != kNoShares;
+    const bool shared = a.share_odd != 0;
     if (shared) {
         const uint32_t share = own_share(a);
         const Found f = find(a, lane, [&](uint32_t all, uint32_t, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
@@ -232,11 +232,13 @@ template <int D, int CODES, int R> struct WaveRows {
     __device__ __forceinline__ void step(const Segment& x, uint32_t key, uint32_t quarter, K get_k, V get_v, G get_scales, A after_scores) {
         float4_t y[R][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < R; ++r) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) {
+        for (int i = 0; i < S::kLoads; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 const Words<S::kWords> w = get_k(h, i);
 #pragma unroll
                 for (int k = 0; k < S::kWords / 2; ++k) {
@@ -245,6 +247,7 @@ template <int D, int CODES, int R> struct WaveRows {
                     for (int r = 0; r < R; ++r) y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[r][i * (S::kWords / 2) + k], y[r][h], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);                      // (all codes at once as halves would take 32 registers)
         }
         after_scores();
         uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each
@@ -629,7 +632,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
 // ---- launches ---------------------------------------------------------------------------------------------------------
 
 template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
-    const dim3 grid = a.shares_log == kNoShares ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(1u << a.shares_log, 1, 1), block(kWaves * 64);
+    const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(kWaves * 64);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     info = {p.split_rows ? "tree_attention_rows" : "tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1},
             p.split_rows ? uint32_t(Stage<D>::kStages * Stage<D>::kBytes) : uint32_t((kWaves * 16 * (D + 4 + 2) + 32) * 4)};

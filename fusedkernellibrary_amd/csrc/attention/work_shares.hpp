@@ -42,13 +42,17 @@ __device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { re
 __device__ __forceinline__ uint32_t subs_of(Args& a, const Sequence& s) { return (s.rows + (1u << a.sub_log) - 1) >> a.sub_log; }
 __device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return subs_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
 
-__device__ __forceinline__ uint32_t scan_wave(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d);
-        v += lane >= uint32_t(d) ? o : 0u;
-    }
-    return v;
+// Sums of a wave's lanes up to and with each.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t v) {
+    v = add_dpp<0x111, 0xf>(v);                               // row_shr 1, 2, 4, 8: within sixteen lanes
+    v = add_dpp<0x112, 0xf>(v);
+    v = add_dpp<0x114, 0xf>(v);
+    v = add_dpp<0x118, 0xf>(v);
+    v = add_dpp<0x142, 0xa>(v);                               // row_bcast 15: the second and fourth sixteen get the one before
+    return add_dpp<0x143, 0xc>(v);                            // row_bcast 31: the upper half gets the lower
 }
 
 // (of the lane's own sequence)
@@ -60,7 +64,7 @@ template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t la
     uint32_t before = 0;
     Found f{0, a.batch, 0};
     if (a.batch <= 64) {
-        const uint32_t own = weigh(a, lane), upto = scan_wave(own, lane);
+        const uint32_t own = weigh(a, lane), upto = scan_wave(own);
         f.all = __builtin_amdgcn_readlane(int(upto), 63);
         const uint64_t hits = __ballot(lane < a.batch && is_it(f.all, lane, upto - own, upto));
         if (hits) {
@@ -69,12 +73,11 @@ template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t la
         }
         return f;
     }
-    for (uint32_t b = lane; b < a.batch; b += 64) f.all += weigh(a, b);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) f.all += __shfl_xor(f.all, d);
-    f.all = __builtin_amdgcn_readfirstlane(f.all);
+    uint32_t sum = 0;
+    for (uint32_t b = lane; b < a.batch; b += 64) sum += weigh(a, b);
+    f.all = __builtin_amdgcn_readlane(int(scan_wave(sum)), 63);
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint32_t own = weigh(a, b0 + lane), upto = before + scan_wave(own, lane);
+        const uint32_t own = weigh(a, b0 + lane), upto = before + scan_wave(own);
         const uint64_t hits = __ballot(b0 + lane < a.batch && is_it(f.all, b0 + lane, upto - own, upto));
         if (hits) {
             const int hit = __builtin_ctzll(hits);
@@ -86,8 +89,16 @@ template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t la
     }
     return f;
 }
-__device__ __forceinline__ uint32_t share_begin(Args& a, uint32_t all, uint32_t share) { return uint32_t((uint64_t(share) * all) >> a.shares_log); }
+// There are share_odd << share_log shares, share_odd being 1 or 3; all granules times the shares fit 42 bits.
+__device__ __forceinline__ uint32_t share_begin(Args& a, uint32_t all, uint32_t share) {
+    const uint32_t x = uint32_t((uint64_t(share) * all) >> a.share_log);
+    return a.share_odd == 3 ? x / 3 : x;
+}
+// The share that a granule is of: the last to begin at or in front of it.
+__device__ __forceinline__ uint32_t share_of(Args& a, uint32_t all, uint32_t granule) {
+    return uint32_t((((uint64_t(granule) + 1) * a.share_odd << a.share_log) + all - 1) / all) - 1;
+}
 // Neighbouring shares, which may be of the same keys, are on the same XCD (workgroups go round the eight).
-__device__ __forceinline__ uint32_t own_share(Args& a) { return a.shares_log >= 3 ? (blockIdx.x & 7u) << (a.shares_log - 3) | blockIdx.x >> 3 : blockIdx.x; }
+__device__ __forceinline__ uint32_t own_share(Args& a) { return a.share_log >= 3 ? (blockIdx.x & 7u) * (a.share_odd << (a.share_log - 3)) + (blockIdx.x >> 3) : blockIdx.x; }
 
 } // namespace fkattn
