@@ -246,7 +246,7 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     const uint64_t granules = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log, units = uint64_t(batch) * kv_heads * p.row_blocks;
     const uint64_t all = units * granules * (p.unit_rows >> p.sub_log);
     // as many shares as workgroups run at once on 256 compute units, or a power of two that leaves two granules to each
-    const uint32_t at_once = head_dim > 128 ? 1 : p.split_rows || p.tiles == 2 ? 2 : 3;
+    const uint32_t at_once = head_dim > 128 ? 1 : p.tiles == 2 ? 2 : 3;
     p.share_log = 8 + (at_once == 2);
     p.share_odd = at_once == 3 ? 3 : 1;
     if (granules <= 4 || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;

@@ -97,11 +97,17 @@ __device__ __forceinline__ float sum_quarters(float v) {
 
 // The lowest n of four bits.
 __device__ __forceinline__ uint32_t lowest_bits(int32_t n) { return n >= 4 ? 15u : n <= 0 ? 0u : (1u << n) - 1u; }
-// Bits u .. u + 3 of a row of a mask, where those below 0 (the context's) are set and those behind the row are not.
-__device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint32_t words, int32_t u) {
+// Bits u .. u + 3 of a row of a mask, where those below 0 (the context's) are set and those behind the row are not; `first` is
+// the row's first word.
+__device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint64_t first, uint32_t words, int32_t u) {
     const uint32_t below = u >= 0 ? 0u : u <= -4 ? 4u : uint32_t(-u), from = u >= 0 ? uint32_t(u) : 0u;
-    const uint32_t lo_at = from >> 6, hi_at = (from + 3) >> 6, shift = from & 63u;
-    const uint64_t lo = lo_at < words ? row[lo_at] : 0, hi = hi_at < words && hi_at != lo_at ? row[hi_at] : 0;
+    const uint32_t shift = from & 63u;
+    uint64_t lo = from < 64u ? first : 0, hi = 0;
+    if (words > 1) {                                          // (the same for the whole wave)
+        const uint32_t lo_at = from >> 6, hi_at = (from + 3) >> 6;
+        lo = lo_at < words ? row[lo_at] : 0;
+        hi = hi_at < words && hi_at != lo_at ? row[hi_at] : 0;
+    }
     const uint32_t bits = uint32_t(lo >> shift) | (shift ? uint32_t(hi << (64u - shift)) : 0u);
     return (lowest_bits(int32_t(below)) | bits << below) & 15u;
 }
@@ -124,6 +130,11 @@ __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32
     x.key0 = k0 << a.granule_log;
     x.key1 = min(k1 << a.granule_log, any_sees);
     return x;
+}
+
+__device__ __forceinline__ uint32_t to_vector(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // Calls `run` for every segment of the workgroup.
@@ -162,9 +173,13 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         } else if (block * a.block_subs >= subs) {
             return;
         }
+        // (a segment needs all scalar registers: what the walk goes on with waits in vector registers)
+        const uint32_t next_at = to_vector(at + count), next_in = to_vector(in + count), next_end = to_vector(end), next_b = to_vector(b);
         run(segment_of(a, s, b, head, block, g0, g1, part));
-        at += count;
-        in += count;
+        at = __builtin_amdgcn_readfirstlane(next_at);
+        in = __builtin_amdgcn_readfirstlane(next_in);
+        end = __builtin_amdgcn_readfirstlane(next_end);
+        b = __builtin_amdgcn_readfirstlane(next_b);
     }
 }
 
@@ -173,6 +188,7 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
 template <int D, int CODES, int R> struct WaveRows {
     using S = Shape<D>;
     uint32_t token[R];                   // the new token of the lane's row
+    uint64_t sees_first[R];              // and the first word of its mask: fetched in good time, a word is all that trees of up to 64 have
     half8_t q[R][S::kSteps];
     float row_scale[R];
     float4_t o[R][S::kTiles];
@@ -188,6 +204,7 @@ template <int D, int CODES, int R> struct WaveRows {
         for (int r = 0; r < R; ++r) {
             const uint32_t row = x.row0 + min(tile(r) * 16 + col, x.rows - 1);
             token[r] = divide(row, a.group_magic);
+            sees_first[r] = a.mask ? a.mask[int64_t(x.seq.first_token + token[r]) * a.mask_words] : 0;
             const uint32_t g = row - token[r] * a.group;
             const char* from = a.q.data + int64_t(x.seq.first_token + token[r]) * a.q.token_stride + int64_t(x.head * a.group + g) * a.q.head_stride;
 #pragma unroll
@@ -264,7 +281,7 @@ template <int D, int CODES, int R> struct WaveRows {
                 for (int r = 0; r < R; ++r) {
                     const int32_t u = int32_t(at - x.seq.context);
                     const uint32_t bits = a.mask == nullptr ? lowest_bits(int32_t(token[r]) + 1 - u)
-                                                            : mask_bits(a.mask + int64_t(x.seq.first_token + token[r]) * a.mask_words, a.mask_words, u);
+                                                            : mask_bits(a.mask + int64_t(x.seq.first_token + token[r]) * a.mask_words, sees_first[r], a.mask_words, u);
                     sees[r][h] = bits & there;
                 }
                 // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
@@ -389,13 +406,23 @@ __device__ __forceinline__ void put_lse(Args& a, const Segment& x, uint32_t shar
     }
 }
 
-// Where 16 keys of a segment are in the cache: tokens in front of them.
-__device__ __forceinline__ size_t place_of_keys(Args& a, const Segment& x, uint32_t key) {
-    const int32_t* pages = a.page_table + int64_t(x.b) * a.page_table_stride;
-    const uint32_t last = (x.seq.total - 1) >> a.cache.page_log;
-    const uint32_t page = min(uint32_t(scalar(pages + min(key >> a.cache.page_log, last))), a.cache.pages - 1);
-    return ((size_t(page) * a.cache.kv_heads + x.head) << a.cache.page_log) + (key & ((1u << a.cache.page_log) - 1u));
-}
+// A wave's way through the page table: 64 entries at a time, one to a lane. (A scalar load for each block of keys would have
+// every wave wait for it; places are asked for in ascending order.)
+struct Pages {
+    uint32_t first, entry;
+    __device__ __forceinline__ void fetch(Args& a, const Segment& x, uint32_t page, uint32_t lane) {
+        first = page;
+        const int32_t* entries = a.page_table + int64_t(x.b) * a.page_table_stride;
+        entry = min(uint32_t(entries[min(page + lane, (x.seq.total - 1) >> a.cache.page_log)]), a.cache.pages - 1);
+    }
+    // Where 16 keys of the segment are in the cache: tokens in front of them.
+    __device__ __forceinline__ size_t place(Args& a, const Segment& x, uint32_t key, uint32_t lane) {
+        const uint32_t page = key >> a.cache.page_log;
+        if (__builtin_expect(page - first >= 64, 0)) fetch(a, x, page, lane);
+        const uint32_t at = __builtin_amdgcn_readlane(entry, page - first);
+        return ((size_t(at) * a.cache.kv_heads + x.head) << a.cache.page_log) + (key & ((1u << a.cache.page_log) - 1u));
+    }
+};
 
 // ---- few rows: the waves split the keys -------------------------------------------------------------------------------
 
@@ -412,10 +439,10 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
         size_t at[2];
         Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
         float4_t ks[2], vs[2];
+        Pages pages{0, 0};
         auto locate = [&](uint32_t key) {
-            Args& fresh = kernel_args();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) at[h] = place_of_keys(fresh, x, key + h * 16);
+            for (int h = 0; h < 2; ++h) at[h] = pages.place(a, x, key + h * 16, lane);
         };
         auto load_k = [&] {
 #pragma unroll
@@ -435,6 +462,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
                 for (int i = 0; i < S::kLoads; ++i) v[h][i] = load_words<S::kWords>(a.cache.v + at[h] * D + lane_v + i * S::kChunk * 4);
         };
         uint32_t key = x.key0 + wave * 32;
+        if (key < x.key1) pages.fetch(a, x, key >> a.cache.page_log, lane);
         WaveRows<D, CODES, R> rows;
         rows.start(kernel_args(), x, col, quarter, [](int r) { return uint32_t(r); });
         if (key < x.key1) {
@@ -542,10 +570,12 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
         const uint32_t read_k = kOwn ? lane * 16 : col * D + quarter * 8, read_v = kOwn ? lane * 16 : quarter * (4 * D) + col * 8;
         const uint32_t ring_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring)));
         const uint32_t stages = x.key1 > x.key0 ? (x.key1 - x.key0 + P::kKeys - 1) / P::kKeys : 0;
+        Pages pages{0, 0};
+        const uint32_t block = P::kBlocks == 4 ? wave : wave & 1;
+        if (stages) pages.fetch(kernel_args(), x, (x.key0 + block * 16) >> kernel_args().cache.page_log, lane);
         auto copy = [&](uint32_t stage) {
             Args& a = kernel_args();
-            const uint32_t block = P::kBlocks == 4 ? wave : wave & 1;
-            const size_t at = place_of_keys(a, x, x.key0 + stage * P::kKeys + block * 16);
+            const size_t at = pages.place(a, x, x.key0 + stage * P::kKeys + block * 16, lane);
             const uint32_t to = ring_at + (stage % P::kStages) * P::kBytes + block * P::kBlockBytes;
 #pragma unroll
             for (int i = 0; i < P::kRuns; ++i)
