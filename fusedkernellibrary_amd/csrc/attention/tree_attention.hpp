@@ -23,10 +23,10 @@
 // parts to the workspace, from where k_merge takes them. Without shares (short sequences, or so many that the order of
 // launch evens them out) a workgroup takes one whole (sequence, key head, block of rows).
 //
-// The running maximum m_r and the largest value scale t are references and not the exact maxima: weights are
-// w = 2^(s - m) * vs / t, and m and t move only when a score leads m by more than 2^kLead or a value scale exceeds t. Only
-// then are scores compared across lanes and the sums rescaled. 2^(s - m) stays below 2^kLead and starts at 2^kStart, so a
-// weight is subnormal in half precision (2^-14) only 2^-(14 + kStart) below the largest of the first keys.
+// The running maximum is a reference m_r and not the exact maximum: weights are w = 2^(s - m) * vs, sums those of 2^(s - m), and
+// m moves only when a weight exceeds 2^kLead. Only then are scores compared across lanes and the sums rescaled. The largest
+// weight starts at 2^kStart, so one is subnormal in half precision (below 2^-14) only 2^-(14 + kStart) below the largest of
+// the first keys. (Value scales below kLeastScale count as that: values of 10^-22 and less lose accuracy.)
 #pragma once
 
 #include <type_traits>
@@ -36,7 +36,7 @@
 namespace fkattn {
 
 constexpr int kWaves = 4;                    // of a workgroup: they share out a chunk's keys, 32 at a time
-constexpr float kStart = 6.0f, kLead = 14.0f;
+constexpr float kStart = 6.0f, kLead = 14.0f, kLargest = 16384.0f, kLeastScale = 0x1p-80f, kMostSum = 0x1p98f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -1.0e30f;         // the reference of a row that has seen no key
 
@@ -193,12 +193,10 @@ template <int D, int CODES, int R> struct WaveRows {
     float row_scale[R];
     float4_t o[R][S::kTiles];
     float m[R], l[R];
-    float t, inv_t;
+    float limit[R];                      // the largest weight that is fine as it is: kLargest, or -1 while the row has seen no key
 
     // Rows of the tiles `tile(r)` (16 rows each) of a segment; those behind its last are its last again.
     template <typename F> __device__ __forceinline__ void start(Args& a, const Segment& x, uint32_t col, uint32_t quarter, F tile) {
-        t = 0.0f;
-        inv_t = 0.0f;
         uint4_t raw[R][S::kSteps];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -238,10 +236,13 @@ template <int D, int CODES, int R> struct WaveRows {
                 for (int k = 0; k < 8; ++k) q[r][s][k] = _Float16(__builtin_amdgcn_ldexpf(e[s * 8 + k], -p));
 #pragma unroll
             for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            m[r] = kNothing;
+            m[r] = 0.0f;
             l[r] = 0.0f;
+            limit[r] = -1.0f;
         }
     }
+    // The reference at the end, for comparison with others'.
+    __device__ __forceinline__ float reference(int r) const { return limit[r] < 0.0f ? kNothing : m[r]; }
 
     // 32 keys from `key` on: get_k(block, load) and get_v have their codes, get_scales(block, ks, vs) their scales;
     // after_scores runs when the keys are used up.
@@ -267,12 +268,11 @@ template <int D, int CODES, int R> struct WaveRows {
             __builtin_amdgcn_sched_barrier(0);                      // (all codes at once as halves would take 32 registers)
         }
         after_scores();
-        uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each
+        uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each; bytes that are a token's
         float4_t ks[2], vs[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             get_scales(h, ks[h], vs[h]);
-            keep[h] = ~0u;
             if constexpr (MASKED) {
                 Args& a = kernel_args();
                 const uint32_t at = key + h * 16 + quarter * 4;
@@ -287,83 +287,77 @@ template <int D, int CODES, int R> struct WaveRows {
                 // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
                 keep[h] = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    keep[h] |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
-                    vs[h][i] = there >> i & 1 ? vs[h][i] : 0.0f;
-                }
+                for (int i = 0; i < 4; ++i) keep[h] |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
             }
         }
-        // scores in units of log2 from the reference on, masked ones -inf
-        auto score = [&](int r, int h, int i) {
-            float z = __builtin_fmaf(y[r][h][i], row_scale[r], -m[r]);
-            if constexpr (MASKED) z = sees[r][h] >> i & 1 ? z : -__builtin_inff();
-            return z;
+        // Weights, and a look at whether a reference has to move: where a weight is too large for half precision, or where the
+        // row has seen no key yet.
+        float w[R][2][4], sum[R];
+        bool move = false;
+        auto weigh = [&](int r, int h, int i, float score) {
+            float e = exp2_fast(score);
+            float weight = e * vs[h][i];
+            if constexpr (MASKED) {
+                e = sees[r][h] >> i & 1 ? e : 0.0f;
+                weight = sees[r][h] >> i & 1 ? weight : 0.0f;       // (a hidden value's scale may be NaN)
+            }
+            sum[r] += e;
+            return weight;
         };
-        float lead = kNothing, scales = 0.0f, z[R][2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < R; ++r) {
+            float top = 0.0f;
+            sum[r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                scales = __builtin_fmaxf(scales, vs[h][i]);
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
+                for (int i = 0; i < 4; ++i) {
                     y[r][h][i] *= ks[h][i];
-                    z[r][h][i] = score(r, h, i);
-                    lead = __builtin_fmaxf(lead, z[r][h][i]);
+                    w[r][h][i] = weigh(r, h, i, __builtin_fmaf(y[r][h][i], row_scale[r], -m[r]));
+                    top = __builtin_fmaxf(top, w[r][h][i]);
                 }
-            }
-        if (__builtin_expect(__any(lead > kLead || scales > t), 0)) {
-            const float largest = max_quarters(scales);
-            float shrink = 1.0f;
-            if (largest > t) {
-                const float now = __builtin_fmaxf(largest, 1.0e-30f);
-                shrink = t / now;
-                t = now;
-                inv_t = 1.0f / now;
-            }
+            move |= top > limit[r] || sum[r] > kMostSum;
+        }
+        if (__builtin_expect(__any(move), 0)) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                // the largest weight there would be, in units of log2
                 float top = -__builtin_inff();
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        z[r][h][i] = y[r][h][i] * row_scale[r];
-                        if constexpr (MASKED) z[r][h][i] = sees[r][h] >> i & 1 ? z[r][h][i] : -__builtin_inff();
-                        top = __builtin_fmaxf(top, z[r][h][i]);
+                        float v = y[r][h][i] * row_scale[r] + __builtin_log2f(__builtin_fmaxf(vs[h][i], kLeastScale));
+                        if constexpr (MASKED) v = sees[r][h] >> i & 1 ? v : -__builtin_inff();
+                        top = __builtin_fmaxf(top, v);
                     }
                 top = max_quarters(top);
                 float alpha = 1.0f;
-                if (top - m[r] > kLead) {
-                    const float now = top - kStart;
-                    alpha = exp2_fast(m[r] - now);
-                    m[r] = now;
+                if (limit[r] < 0.0f ? top > -__builtin_inff() : top - m[r] > kLead) {
+                    alpha = limit[r] < 0.0f ? 0.0f : exp2_fast(m[r] + kStart - top);
+                    m[r] = top - kStart;
+                    limit[r] = kLargest;
                 }
                 l[r] *= alpha;
-                alpha *= shrink;
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) o[r][i] *= alpha;
+                // (from the rounded scores: those of 2^100 differ from their reference by more than an exponent holds)
+                sum[r] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) z[r][h][i] -= m[r];     // (from the rounded score: at 2^100 it differs from score() by more than an exponent holds)
+                    for (int i = 0; i < 4; ++i) w[r][h][i] = weigh(r, h, i, y[r][h][i] * row_scale[r] - m[r]);
             }
         }
         half8_t p[R];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < R; ++r) {
+            l[r] += sum[r];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float scaled = vs[h][i] * inv_t;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float e = exp2_fast(z[r][h][i]);
-                    l[r] += e;
-                    float w = e * scaled;
-                    if constexpr (MASKED) w = sees[r][h] >> i & 1 ? w : 0.0f;       // (a hidden value's scale may be NaN)
-                    p[r][h * 4 + i] = _Float16(w);
-                }
-            }
+                for (int i = 0; i < 4; ++i) p[r][h * 4 + i] = _Float16(w[r][h][i]);
+        }
 #pragma unroll
         for (int c = 0; c < S::kLoads; ++c) {
             const Words<S::kWords> v0 = get_v(0, c), v1 = get_v(1, c);
@@ -496,7 +490,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
         Args& out = kernel_args();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float l = sum_quarters(rows.l[r]), m = rows.m[r];
+            const float l = sum_quarters(rows.l[r]), m = rows.reference(r);
             if (quarter == 0) {
                 joined_m[wave][col] = m;
                 joined_l[wave][col] = l;
@@ -508,7 +502,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) sum += joined_l[w][col] * exp2_fast(joined_m[w][col] - top);
             // (a sum that is NaN, from a NaN among the scores, makes the row NaN)
-            const float factor = (sum == 0.0f ? 0.0f : exp2_fast(m - top) / sum) * rows.t;
+            const float factor = sum == 0.0f ? 0.0f : exp2_fast(m - top) / sum;
 #pragma unroll
             for (int c = 0; c < S::kLoads; ++c)
 #pragma unroll
@@ -547,11 +541,17 @@ template <int D> struct Stage {
 
 // Copies to LDS without registers, 16 or 4 bytes a lane at `lds` + the same times the lane's number; the count of memory
 // operations in flight says when they are there.
+// (the compiler is told that a value is the wave's and not the lane's)
+__device__ __forceinline__ uint32_t of_wave(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const char* of_wave(const char* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const char*>(uint64_t(of_wave(uint32_t(v >> 32))) << 32 | of_wave(uint32_t(v)));
+}
 __device__ __forceinline__ void copy16(const char* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(of_wave(lds)), "v"(offset), "s"(of_wave(base)) : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(const char* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(of_wave(lds)), "v"(offset), "s"(of_wave(base)) : "memory", "m0");
 }
 // All but the wave's last N memory operations are done; then all waves' are, and nobody reads LDS any more.
 template <int N> __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
             if (lane < 32) {
                 if (P::kBlocks == 4) {
                     const char* s = reinterpret_cast<const char*>((lane < 16 ? a.cache.k_scale : a.cache.v_scale) + at) + (lane & 15) * 4;
-                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to + 2 * P::kCodes), "v"(s) : "memory", "m0");
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(of_wave(to + 2 * P::kCodes)), "v"(s) : "memory", "m0");
                 } else if (lane < 16) {
                     copy4(reinterpret_cast<const char*>((wave < 2 ? a.cache.k_scale : a.cache.v_scale) + at), lane * 4, to + 2 * P::kCodes + (wave < 2 ? 0 : 64));
                 }
@@ -601,34 +601,40 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
             constexpr int kMine = decltype(count)::value;
             WaveRows<D, CODES, kMine == 0 ? 1 : kMine> rows;
             if constexpr (kMine > 0) rows.start(kernel_args(), x, col, quarter, [&](int r) { return wave + kWaves * r; });
-            uint32_t stage = 0;
-            // stages whose keys all rows see, then the others
-            auto keys = [&](auto masked, uint32_t end) {
-#pragma unroll 1
-                for (; stage < end; ++stage) {
+            uint32_t key = x.key0, stage = 0;
+            const char* piece = ring;
+            // (every stage's first step; waves without rows take part in the copies and the waiting)
+            auto begin = [&](uint32_t key) {
+                if ((key & (P::kKeys - 1)) == 0) {
                     if (stage + 1 < stages) arrive<P::kCopies>();
                     else arrive<0>();
                     if (stage + P::kStages - 1 < stages) copy(stage + P::kStages - 1);
-                    if constexpr (kMine > 0) {
-                        const char* here = ring + (stage % P::kStages) * P::kBytes;
-#pragma unroll 1
-                        for (uint32_t half = 0; half < P::kBlocks / 2; ++half) {
-                            const uint32_t key = x.key0 + stage * P::kKeys + half * 32;
-                            if (decltype(masked)::value && key >= x.key1) break;
-                            const char* piece = here + half * 2 * P::kBlockBytes;
-                            auto get_k = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + read_k + i * kNextK); };
-                            auto get_v = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + P::kCodes + read_v + i * kNextV); };
-                            auto get_scales = [&](int h, float4_t& s, float4_t& t) {
-                                s = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + quarter * 16);
-                                t = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + 64 + quarter * 16);
-                            };
-                            rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [] {});
-                        }
-                    }
+                    piece = ring + (stage % P::kStages) * P::kBytes;
+                    ++stage;
+                } else {
+                    piece += 2 * P::kBlockBytes;
                 }
             };
-            keys(std::false_type{}, min(x.key1, x.all_see) > x.key0 ? (min(x.key1, x.all_see) - x.key0) / P::kKeys : 0);
-            keys(std::true_type{}, stages);
+            if constexpr (kMine > 0) {
+                auto get_k = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + read_k + i * kNextK); };
+                auto get_v = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + P::kCodes + read_v + i * kNextV); };
+                auto get_scales = [&](int h, float4_t& s, float4_t& t) {
+                    s = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + quarter * 16);
+                    t = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + 64 + quarter * 16);
+                };
+                // keys that all rows see, then the others
+                auto keys = [&](auto masked, uint32_t end) {
+#pragma unroll 1
+                    for (; key < end; key += 32) {
+                        begin(key);
+                        rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [] {});
+                    }
+                };
+                keys(std::false_type{}, min(x.key1, x.all_see & ~31u));
+                keys(std::true_type{}, x.key1);
+            } else {
+                for (; key < x.key1; key += P::kKeys) begin(key);
+            }
             if constexpr (kMine > 0) {
                 Args& out = kernel_args();
                 const uint32_t share = own_share(out);
@@ -636,7 +642,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
                 for (int r = 0; r < kMine; ++r) {
                     const uint32_t row = (wave + kWaves * r) * 16 + col;
                     const float l = sum_quarters(rows.l[r]);
-                    const float factor = l == 0.0f ? 0.0f : rows.t / l;
+                    const float factor = l == 0.0f ? 0.0f : 1.0f / l;
                     if (row < x.rows) {
 #pragma unroll
                         for (int c = 0; c < S::kLoads; ++c)
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
                                 for (int w = 0; w < S::kWords; ++w) v[w] = rows.o[r][c * S::kWords + w][i] * factor;
                                 put<D, S::kWords>(out, x, share, row, c * S::kChunk + (quarter * 4 + i) * S::kWords, v);
                             }
-                        if (quarter == 0) put_lse(out, x, share, row, rows.m[r], l);
+                        if (quarter == 0) put_lse(out, x, share, row, rows.reference(r), l);
                     }
                 }
             }
