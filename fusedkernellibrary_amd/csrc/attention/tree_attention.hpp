@@ -118,6 +118,7 @@ struct Segment {
     uint32_t b, head, row0, rows;        // rows row0 .. row0 + rows of the sequence's
     uint32_t key0, key1, all_see;        // every row sees the keys in front of all_see
     int part;                            // -1: whole, 0 or 1: the share's part
+    uint32_t behind, quarter;            // keys of the share behind the segment's, and a quarter of them all
 };
 __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32_t b, uint32_t head, uint32_t block, uint32_t k0, uint32_t k1, int part) {
     Segment x;
@@ -150,6 +151,7 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         b = f.b;
         in = at - f.before;
     }
+    const uint32_t whole = end - at;
     while (at < end && b < kernel_args().batch) {
         Args& a = kernel_args();
         const Sequence s = sequence_at(a, b);
@@ -175,12 +177,26 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         }
         // (a segment needs all scalar registers: what the walk goes on with waits in vector registers)
         const uint32_t next_at = to_vector(at + count), next_in = to_vector(in + count), next_end = to_vector(end), next_b = to_vector(b);
-        run(segment_of(a, s, b, head, block, g0, g1, part));
+        Segment x = segment_of(a, s, b, head, block, g0, g1, part);
+        x.quarter = whole << a.granule_log >> 2;
+        x.behind = (end - at - count) << a.granule_log;
+        if (!shared) x.behind = 0, x.quarter = (x.key1 - x.key0) >> 2;
+        run(x);
         at = __builtin_amdgcn_readfirstlane(next_at);
         in = __builtin_amdgcn_readfirstlane(next_in);
         end = __builtin_amdgcn_readfirstlane(next_end);
         b = __builtin_amdgcn_readfirstlane(next_b);
     }
+}
+
+// A wave's priority falls as its share gets done: left alone, the oldest of the workgroups on a compute unit runs ahead, and the
+// last one ends alone, without others to fill its gaps.
+__device__ __forceinline__ void set_priority(const Segment& x, uint32_t key) {
+    const uint32_t left = x.behind + x.key1 - key;
+    if (left > 3 * x.quarter) __builtin_amdgcn_s_setprio(3);
+    else if (left > 2 * x.quarter) __builtin_amdgcn_s_setprio(2);
+    else if (left > x.quarter) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
 }
 
 // ---- a wave's rows ---------------------------------------------------------------------------------------------------
@@ -473,6 +489,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
             while (key < end) {
                 const uint32_t next = key + kWaves * 32;
                 const bool more = next < x.key1;
+                set_priority(x, key);
                 if (more) locate(next);
                 // the keys' registers are free for the next once the scores are there, the others' at the end
                 rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [&] {
@@ -606,6 +623,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
             // (every stage's first step; waves without rows take part in the copies and the waiting)
             auto begin = [&](uint32_t key) {
                 if ((key & (P::kKeys - 1)) == 0) {
+                    set_priority(x, key);
                     if (stage + 1 < stages) arrive<P::kCopies>();
                     else arrive<0>();
                     if (stage + P::kStages - 1 < stages) copy(stage + P::kStages - 1);
