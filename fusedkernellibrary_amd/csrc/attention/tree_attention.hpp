@@ -40,6 +40,19 @@ constexpr float kStart = 6.0f, kLead = 14.0f, kLargest = 16384.0f, kLeastScale =
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -1.0e30f;         // the reference of a row that has seen no key
 
+// How a key's product with the queries is taken. The matrix unit has products of 8-bit codes themselves, for runs of 64 (int8) or
+// 128 (e4m3) elements: a query row is then a sum of two or three rows of such codes, and no key is converted.
+//   int8: in fixed point, 256 * hi + lo (bfloat16: exact for elements from 2^-7 of the row's largest on) or with a third
+//         part behind them (half precision: exact from 2^-11 on); smaller elements are off by 2^-15 (2^-22) of the largest.
+//   e4m3: what four bits hold of each element, and of what is left, twice (8 bits, all that bfloat16 has) or three times;
+//         elements below 2^-9 of the largest are off by 2^-17 of it.
+// Heads of other sizes: keys as halves.
+template <int D, int CODES> constexpr bool kCodeProducts = CODES == FKLHIP_CODES_INT8 ? D % 64 == 0 : D % 128 == 0;
+
+using int2_t = int __attribute__((ext_vector_type(2)));
+using int4_t = int __attribute__((ext_vector_type(4)));
+using int8_t8 = int __attribute__((ext_vector_type(8)));
+
 template <int D> struct Shape {
     static constexpr int kChunk = D % 64 == 0 ? 64 : 32;   // elements of a row that one load of a lane's quarter row covers
     static constexpr int kLoads = D / kChunk;              // of a block of 16 keys (or values)
@@ -201,11 +214,13 @@ __device__ __forceinline__ void set_priority(const Segment& x, uint32_t key) {
 
 // ---- a wave's rows ---------------------------------------------------------------------------------------------------
 
-template <int D, int CODES, int R> struct WaveRows {
+// PARTS: rows of codes that a query row is the sum of, or 0: halves.
+template <int D, int CODES, int R, int PARTS> struct WaveRows {
     using S = Shape<D>;
+    static constexpr int kQueryRegs = PARTS == 0 ? S::kSteps * 4 : PARTS * S::kSteps * 2;     // dwords of a lane's quarter row
     uint32_t token[R];                   // the new token of the lane's row
     uint64_t sees_first[R];              // and the first word of its mask: fetched in good time, a word is all that trees of up to 64 have
-    half8_t q[R][S::kSteps];
+    uint32_t q[R][kQueryRegs];           // halves, or the parts one behind the other
     float row_scale[R];
     float4_t o[R][S::kTiles];
     float m[R], l[R];
@@ -244,12 +259,57 @@ template <int D, int CODES, int R> struct WaveRows {
             top = max(top, uint32_t(__shfl_xor(int(top), 16)));
             top = max(top, uint32_t(__shfl_xor(int(top), 32)));
             // a power of two in front of the row's largest magnitude (a row of zeros, or with an infinity, is left alone)
-            const int p = top == 0 || top >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
-            row_scale[r] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, p);
+            const bool plain = top == 0 || top >= 0x7f800000u;
+            const int p = plain ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
+            float unit = a.scale * kLog2e;
+            if constexpr (PARTS == 0) {
 #pragma unroll
-            for (int s = 0; s < S::kSteps; ++s)
+                for (int k = 0; k < S::kSteps * 4; ++k)
+                    q[r][k] = pack2<FKLHIP_F16>(__builtin_amdgcn_ldexpf(e[2 * k], -p), __builtin_amdgcn_ldexpf(e[2 * k + 1], -p));
+            } else if constexpr (CODES == FKLHIP_CODES_INT8) {
+                // A power of two in front of the largest magnitude that leaves it below 127.5 * 2^8 (or 2^14); a row with an
+                // infinity or a NaN has scores that are NaN.
+                constexpr int kBits = PARTS == 2 ? 14 : 21;
+                const int up = kBits - p - (__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, top), -p) >= 1.9921875f ? 1 : 0);
+                unit = top >= 0x7f800000u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(unit, -up - p);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) q[r][s][k] = _Float16(__builtin_amdgcn_ldexpf(e[s * 8 + k], -p));
+                for (int k = 0; k < S::kSteps * 2; ++k) {
+                    uint32_t w[PARTS];
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) w[part] = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        int v = int(__builtin_rintf(__builtin_amdgcn_ldexpf(e[4 * k + i], up)));
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part) {      // the last digit of -128 .. 127, then the rest
+                            const int digit = int(uint32_t(v) << 24) >> 24;
+                            w[part] |= uint32_t(digit & 0xff) << (8 * i);
+                            v = (v - digit) >> 8;
+                        }
+                    }
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) q[r][part * S::kSteps * 2 + k] = w[part];
+                }
+            } else {
+                unit = top >= 0x7f800000u ? __builtin_nanf("") : unit * 0x1p-7f;
+#pragma unroll
+                for (int k = 0; k < S::kSteps * 2; ++k) {
+                    float left[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) left[i] = __builtin_amdgcn_ldexpf(e[4 * k + i], 7 - p);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        int w = __builtin_amdgcn_cvt_pk_fp8_f32(left[0], left[1], 0, false);
+                        w = __builtin_amdgcn_cvt_pk_fp8_f32(left[2], left[3], w, true);
+                        q[r][part * S::kSteps * 2 + k] = uint32_t(w);
+                        float taken[4];
+                        decode4<FKLHIP_CODES_E4M3>(uint32_t(w), taken);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) left[i] -= taken[i];
+                    }
+                }
+            }
+            row_scale[r] = __builtin_amdgcn_ldexpf(unit, p);
 #pragma unroll
             for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
             m[r] = 0.0f;
@@ -260,29 +320,84 @@ template <int D, int CODES, int R> struct WaveRows {
     // The reference at the end, for comparison with others'.
     __device__ __forceinline__ float reference(int r) const { return limit[r] < 0.0f ? kNothing : m[r]; }
 
+    // Products of a block of 16 keys with the rows, four keys to a quarter; the codes' scales are not in them.
+    template <typename K> __device__ __forceinline__ void products(K get_k, float4_t (&y)[R][2]) {
+        if constexpr (PARTS == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < R; ++r) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < S::kLoads; ++i) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Words<S::kWords> w = get_k(h, i);
+#pragma unroll
+                    for (int k = 0; k < S::kWords / 2; ++k) {
+                        const half8_t codes = halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const uint32_t* from = &q[r][(i * (S::kWords / 2) + k) * 4];
+                            y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8_t, uint4_t{from[0], from[1], from[2], from[3]}), y[r][h], 0, 0, 0);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);                  // (all codes at once as halves would take 32 registers)
+            }
+        } else if constexpr (CODES == FKLHIP_CODES_INT8) {
+            // the first two parts as one whole number, the third by itself: with it, 32 bits would not do
+            int4_t sum[PARTS - 1][R][2];
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int i = 0; i < S::kLoads; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const Words<S::kWords> w = get_k(h, i);
+                        const int4_t codes = {int(w.w[0]), int(w.w[1]), int(w.w[2]), int(w.w[3])};
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const uint32_t* from = &q[r][part * S::kSteps * 2 + i * 4];
+                            int4_t& to = sum[part < 2 ? 0 : 1][r][h];
+                            const int4_t before = i > 0 ? to : part == 1 ? to << 8 : int4_t{0, 0, 0, 0};
+                            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes, int4_t{int(from[0]), int(from[1]), int(from[2]), int(from[3])}, before, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[r][h][i] = float(sum[0][r][h][i]);
+                        if constexpr (PARTS == 3) y[r][h][i] = __builtin_fmaf(y[r][h][i], 256.0f, float(sum[1][r][h][i]));
+                    }
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kLoads; i += 2)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Words<S::kWords> lo = get_k(h, i), hi = get_k(h, i + 1);
+                    const int8_t8 codes = {int(lo.w[0]), int(lo.w[1]), int(lo.w[2]), int(lo.w[3]), int(hi.w[0]), int(hi.w[1]), int(hi.w[2]), int(hi.w[3])};
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part) {
+                            const uint32_t* from = &q[r][part * S::kSteps * 2 + i * 4];
+                            const int8_t8 row = {int(from[0]), int(from[1]), int(from[2]), int(from[3]), int(from[4]), int(from[5]), int(from[6]), int(from[7])};
+                            const float4_t before = i == 0 && part == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : y[r][h];
+                            y[r][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, row, before, 0, 0, 0, 0, 0, 0);   // (e4m3 both, no scales)
+                        }
+                }
+        }
+    }
+
     // 32 keys from `key` on: get_k(block, load) and get_v have their codes, get_scales(block, ks, vs) their scales;
     // after_scores runs when the keys are used up.
     template <bool MASKED, typename K, typename V, typename G, typename A>
     __device__ __forceinline__ void step(const Segment& x, uint32_t key, uint32_t quarter, K get_k, V get_v, G get_scales, A after_scores) {
         float4_t y[R][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < R; ++r) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const Words<S::kWords> w = get_k(h, i);
-#pragma unroll
-                for (int k = 0; k < S::kWords / 2; ++k) {
-                    const half8_t codes = halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]);
-#pragma unroll
-                    for (int r = 0; r < R; ++r) y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[r][i * (S::kWords / 2) + k], y[r][h], 0, 0, 0);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);                      // (all codes at once as halves would take 32 registers)
-        }
+        products(get_k, y);
         after_scores();
         uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each; bytes that are a token's
         float4_t ks[2], vs[2];
@@ -436,7 +551,7 @@ struct Pages {
 
 // ---- few rows: the waves split the keys -------------------------------------------------------------------------------
 
-template <int D, int CODES, int R>
+template <int D, int CODES, int R, int PARTS>
 __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_split_keys(const AttentionArgs) {
     using S = Shape<D>;
     constexpr int kRowFloats = D + 4;                              // of a row in LDS: 16 bytes further round the banks than the last
@@ -473,7 +588,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
         };
         uint32_t key = x.key0 + wave * 32;
         if (key < x.key1) pages.fetch(a, x, key >> a.cache.page_log, lane);
-        WaveRows<D, CODES, R> rows;
+        WaveRows<D, CODES, R, PARTS> rows;
         rows.start(kernel_args(), x, col, quarter, [](int r) { return uint32_t(r); });
         if (key < x.key1) {
             locate(key);
@@ -573,7 +688,7 @@ __device__ __forceinline__ void copy4(const char* base, uint32_t offset, uint32_
 // All but the wave's last N memory operations are done; then all waves' are, and nobody reads LDS any more.
 template <int N> __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
 
-template <int D, int CODES, int R>
+template <int D, int CODES, int R, int PARTS>
 __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(const AttentionArgs) {
     using S = Shape<D>;
     using P = Stage<D>;
@@ -616,7 +731,7 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
         const uint32_t tiles = (x.rows + 15) / 16;
         auto loop = [&](auto count) {
             constexpr int kMine = decltype(count)::value;
-            WaveRows<D, CODES, kMine == 0 ? 1 : kMine> rows;
+            WaveRows<D, CODES, kMine == 0 ? 1 : kMine, PARTS> rows;
             if constexpr (kMine > 0) rows.start(kernel_args(), x, col, quarter, [&](int r) { return wave + kWaves * r; });
             uint32_t key = x.key0, stage = 0;
             const char* piece = ring;
@@ -685,25 +800,35 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 
-template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
+template <int D, int CODES, int PARTS> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
     const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(kWaves * 64);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     info = {p.split_rows ? "tree_attention_rows" : "tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1},
             p.split_rows ? uint32_t(Stage<D>::kStages * Stage<D>::kBytes) : uint32_t((kWaves * 16 * (D + 4 + 2) + 32) * 4)};
     if constexpr (D <= 128) {
         if (p.tiles == 2) {
-            if (p.split_rows) k_split_rows<D, CODES, 2><<<grid, block, 0, s>>>(a);
-            else k_split_keys<D, CODES, 2><<<grid, block, 0, s>>>(a);
+            if (p.split_rows) k_split_rows<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
+            else k_split_keys<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
             return int(hipGetLastError());
         }
     }
-    if (p.split_rows) k_split_rows<D, CODES, 1><<<grid, block, 0, s>>>(a);
-    else k_split_keys<D, CODES, 1><<<grid, block, 0, s>>>(a);
+    if (p.split_rows) k_split_rows<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
+    else k_split_keys<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
     return int(hipGetLastError());
 }
 
+template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
+    if constexpr (kCodeProducts<D, CODES>) {
+        if (a.type == FKLHIP_F16) return start_attention<D, CODES, 3>(a, p, stream, info);
+        return start_attention<D, CODES, 2>(a, p, stream, info);
+    } else {
+        return start_attention<D, CODES, 0>(a, p, stream, info);
+    }
+}
+
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) {
-    return a.cache.codes == FKLHIP_CODES_INT8 ? start_attention<D, FKLHIP_CODES_INT8>(a, plan, stream, info) : start_attention<D, FKLHIP_CODES_E4M3>(a, plan, stream, info);
+    if (a.cache.codes == FKLHIP_CODES_INT8) return start_attention<D, FKLHIP_CODES_INT8>(a, plan, stream, info);
+    return start_attention<D, FKLHIP_CODES_E4M3>(a, plan, stream, info);
 }
 
 } // namespace fkattn

@@ -124,8 +124,10 @@ def attention(q, slots, page, page_table, context, q_start, mask, scale, dtype):
             mean = torch.where(seen, w, 0.0) @ vh.abs().nan_to_num(0.0)
             # Weights rounded to half precision (2^-11 each), the scores' sums in 32 bits (dim products and the rounding of
             # their scaling, on the sum of magnitudes), exponentials and sums in 32 bits, weights below half precision's
-            # normal numbers (2^-25 of a scale, against a sum of at least 2^6), the result's own rounding.
-            slack = 2.0 ** -11 + 2.0 ** -18 + 2 * (dim + 8) * 2.0 ** -24 * size.amax(-1, keepdim=True)
+            # normal numbers (2^-25 of a scale, against a sum of at least 2^6), the result's own rounding. Query elements are
+            # held to 2^-16 of their row's largest (half of that, rounded) where products are taken on codes.
+            fixed = 2.0 ** -17 * q[lo:hi, h].double().abs().amax(-1, keepdim=True) * kh.abs().sum(-1).nan_to_num(0.0).max() * abs(scale)
+            slack = 2.0 ** -11 + 2.0 ** -18 + 2 * (dim + 8) * 2.0 ** -24 * size.amax(-1, keepdim=True) + 2 * fixed
             bound[lo:hi, h] = out[lo:hi, h].abs() * ROUND[dtype] + slack * mean + 2.0 ** -31 * n * vh.abs().nan_to_num(0.0).max() + LEAST[dtype]
             lse[lo:hi, h] = torch.where(total[:, 0] == 0, -math.inf, top[:, 0] + total[:, 0].log())
     return out, bound, lse
