@@ -209,7 +209,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     a.mask_words = uint32_t(c->mask_words); a.q_heads = uint32_t(c->q_heads); a.group = uint32_t(c->q_heads / cache->kv_heads);
     a.group_magic = magic(a.group);
     a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
-    a.unit_rows = plan.unit_rows; a.block_subs = plan.unit_rows >> plan.sub_log; a.sub_log = plan.sub_log;
+    a.unit_rows = plan.unit_rows;
     a.granule_log = plan.granule_log; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
     a.type = c->type; a.scale = c->scale;
     if (bytes) {
@@ -236,17 +236,15 @@ namespace fkattn {
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim) {
     const auto log2_floor = [](uint64_t n) { uint32_t l = 0; while (n >>= 1) ++l; return l; };
     AttentionPlan p;
-    // up to 16 (or 32) rows: the waves split the keys; more: they split the rows, 64 or 128 to a workgroup
-    p.split_rows = rows > (head_dim > 128 ? 16 : 32);
-    p.tiles = head_dim > 128 || rows <= 16 || (p.split_rows && rows <= 64) ? 1 : 2;
-    p.unit_rows = p.tiles * (p.split_rows ? 64 : 16);
-    p.sub_log = p.split_rows ? 6 : log2_floor(p.unit_rows);
-    p.granule_log = p.split_rows ? (head_dim > 128 ? 5 : 6) : 7;
+    // 16-row tiles to a workgroup: as few as hold the rows; each takes registers
+    p.tiles = rows <= 16 ? 1 : rows <= 32 || head_dim > 128 ? 2 : 4;
+    p.unit_rows = 16 * p.tiles;
+    p.granule_log = 7;
     p.row_blocks = std::max(1u, (rows + p.unit_rows - 1) / p.unit_rows);
     const uint64_t granules = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log, units = uint64_t(batch) * kv_heads * p.row_blocks;
-    const uint64_t all = units * granules * (p.unit_rows >> p.sub_log);
+    const uint64_t all = units * granules;
     // as many shares as workgroups run at once on 256 compute units, or a power of two that leaves two granules to each
-    const uint32_t at_once = head_dim > 128 ? 1 : p.tiles == 2 ? 2 : 3;
+    const uint32_t at_once = head_dim > 128 ? 1 : p.tiles == 1 ? 3 : 2;
     p.share_log = 8 + (at_once == 2);
     p.share_odd = at_once == 3 ? 3 : 1;
     if (granules <= 4 || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;

@@ -53,7 +53,7 @@ struct AttentionArgs {
     uint32_t tokens, batch, max_new, max_context, mask_words;
     uint32_t q_heads, group;                // query heads per key head
     uint32_t group_magic;                   // x / group as a multiplication (see divide)
-    uint32_t unit_rows, block_subs, sub_log, granule_log, share_log, share_odd;    // how the work is dealt out (work_shares.hpp)
+    uint32_t unit_rows, granule_log, share_log, share_odd;    // how the work is dealt out (work_shares.hpp)
     int type;
     float scale;
 };
@@ -64,11 +64,11 @@ struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
 int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream);
-// How a call is run: 16-row tiles to a wave; whether a workgroup's waves split rows or keys; row blocks of a launch without
-// shares; share_odd << share_log shares, or none; whether rows have so many parts that a workgroup joins one.
+// How a call is run: 16-row tiles (and so rows) to a workgroup; row blocks of a sequence; share_odd << share_log shares, or none;
+// whether rows have so many parts that a workgroup joins one.
 struct AttentionPlan {
-    uint32_t tiles, row_blocks, unit_rows, sub_log, granule_log, share_log, share_odd;
-    bool split_rows, many_parts;
+    uint32_t tiles, row_blocks, unit_rows, granule_log, share_log, share_odd;
+    bool many_parts;
     uint32_t shares() const { return share_odd << share_log; }
 };
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim);

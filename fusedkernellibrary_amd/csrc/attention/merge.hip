@@ -32,13 +32,13 @@ struct Parts {
     }
 };
 __device__ __forceinline__ Parts parts_of(Args& a, const TokenOf& x, uint32_t token, uint32_t head) {
-    const uint32_t n = granules_of(a, x.s), subs = subs_of(a, x.s);
+    const uint32_t n = granules_of(a, x.s);
     const uint32_t kv_head = divide(head, a.group_magic), row = (token - x.s.first_token) * a.group + head - kv_head * a.group;
-    const uint32_t block = row / a.unit_rows, size = n * min(a.block_subs, subs - block * a.block_subs);
-    if (size == 0) return {0, 0, 0};
-    const uint32_t first = x.f.before + kv_head * (n * subs) + block * a.block_subs * n;
+    const uint32_t block = row >> __builtin_ctz(a.unit_rows);
+    if (n == 0) return {0, 0, 0};
+    const uint32_t first = x.f.before + (kv_head * blocks_of(a, x.s) + block) * n;
     const uint32_t share0 = share_of(a, x.f.all, first);
-    return {share0, share_of(a, x.f.all, first + size - 1) - share0 + 1, row - block * a.unit_rows};
+    return {share0, share_of(a, x.f.all, first + n - 1) - share0 + 1, row - block * a.unit_rows};
 }
 // Four elements of a row, and its lse (in units of log2).
 __device__ __forceinline__ void put4(Args& a, uint32_t token, uint32_t head, uint32_t d, float4_t x) {

@@ -63,19 +63,6 @@ template <int D> struct Shape {
 
 template <int WORDS> struct Words { uint32_t w[WORDS]; };
 
-template <int WORDS> __device__ __forceinline__ Words<WORDS> load_words(const char* p) {
-    Words<WORDS> r;
-    if constexpr (WORDS == 4) {
-        const uint4_t v = *reinterpret_cast<const uint4_t*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.w[i] = v[i];
-    } else {
-        const uint2_t v = *reinterpret_cast<const uint2_t*>(p);
-        r.w[0] = v.x; r.w[1] = v.y;
-    }
-    return r;
-}
-
 // Four codes of a dword as half precision, exactly.
 template <int CODES> __device__ __forceinline__ void halves4(uint32_t w, half2_t& lo, half2_t& hi) {
     if constexpr (CODES == FKLHIP_CODES_INT8) {
@@ -98,15 +85,17 @@ template <int CODES> __device__ __forceinline__ half8_t halves8(uint32_t a, uint
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The larger of a lane column's four quarters (lanes l, l ^ 16, l ^ 32, l ^ 48), and their sum.
-__device__ __forceinline__ float max_quarters(float v) {
-    v = __builtin_fmaxf(v, __shfl_xor(v, 16));
-    return __builtin_fmaxf(v, __shfl_xor(v, 32));
+// The larger of a lane column's four quarters (lanes l, l ^ 16, l ^ 32, l ^ 48), and their sum: rows of sixteen lanes, then
+// halves of the wave change places.
+template <typename F> __device__ __forceinline__ float join_quarters(float v, F f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t w = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, uint32_t(rows[0])), __builtin_bit_cast(float, uint32_t(rows[1]))));
+    const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return f(__builtin_bit_cast(float, uint32_t(halves[0])), __builtin_bit_cast(float, uint32_t(halves[1])));
 }
-__device__ __forceinline__ float sum_quarters(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
+__device__ __forceinline__ float max_quarters(float v) { return join_quarters(v, [](float a, float b) { return __builtin_fmaxf(a, b); }); }
+__device__ __forceinline__ float sum_quarters(float v) { return join_quarters(v, [](float a, float b) { return a + b; }); }
 
 // The lowest n of four bits.
 __device__ __forceinline__ uint32_t lowest_bits(int32_t n) { return n >= 4 ? 15u : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -146,13 +135,9 @@ __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32
     return x;
 }
 
-__device__ __forceinline__ uint32_t to_vector(uint32_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
-// Calls `run` for every segment of the workgroup.
-template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, F run) {
+// Calls `run` for every segment of the workgroup. `kept` is the wave's place in LDS for what the walk goes on with: a segment
+// needs all registers.
+template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, uint32_t* kept, F run) {
     // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
     uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
     const bool shared = a.share_odd != 0;
@@ -164,41 +149,37 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         b = f.b;
         in = at - f.before;
     }
-    const uint32_t whole = end - at;
+    uint32_t whole = end - at;
     while (at < end && b < kernel_args().batch) {
         Args& a = kernel_args();
         const Sequence s = sequence_at(a, b);
-        const uint32_t n = granules_of(a, s), subs = subs_of(a, s);
-        uint32_t head = blockIdx.x, block = blockIdx.y, g0 = 0, g1 = n, count = end - at;
+        const uint32_t n = granules_of(a, s), blocks = blocks_of(a, s);
+        uint32_t head = blockIdx.x, block = blockIdx.y, g = 0, count = n;
         int part = -1;
         if (shared) {
-            if (n * subs == 0 || in >= n * subs * a.cache.kv_heads) {
+            const uint32_t unit = n ? in / n : 0;
+            if (unit >= blocks * a.cache.kv_heads || n == 0) {
                 ++b;
                 in = 0;
                 continue;
             }
-            head = in / (n * subs);
-            const uint32_t in_head = in - head * (n * subs), block_size = n * a.block_subs;
-            block = in_head / block_size;
-            const uint32_t g = in_head - block * block_size, cost = min(a.block_subs, subs - block * a.block_subs), size = n * cost;
-            count = min(size - g, end - at);
-            part = count == size ? -1 : g == 0 ? 1 : 0;
-            g0 = (g + cost - 1) >> (cost - 1);
-            g1 = (g + count + cost - 1) >> (cost - 1);
-        } else if (block * a.block_subs >= subs) {
+            head = unit / blocks;
+            block = unit - head * blocks;
+            g = in - unit * n;
+            count = min(n - g, end - at);
+            part = count == n ? -1 : g == 0 ? 1 : 0;
+        } else if (block >= blocks) {
             return;
         }
-        // (a segment needs all scalar registers: what the walk goes on with waits in vector registers)
-        const uint32_t next_at = to_vector(at + count), next_in = to_vector(in + count), next_end = to_vector(end), next_b = to_vector(b);
-        Segment x = segment_of(a, s, b, head, block, g0, g1, part);
+        kept[0] = at + count; kept[1] = in + count; kept[2] = end; kept[3] = b; kept[4] = whole;
+        Segment x = segment_of(a, s, b, head, block, g, g + count, part);
         x.quarter = whole << a.granule_log >> 2;
         x.behind = (end - at - count) << a.granule_log;
         if (!shared) x.behind = 0, x.quarter = (x.key1 - x.key0) >> 2;
         run(x);
-        at = __builtin_amdgcn_readfirstlane(next_at);
-        in = __builtin_amdgcn_readfirstlane(next_in);
-        end = __builtin_amdgcn_readfirstlane(next_end);
-        b = __builtin_amdgcn_readfirstlane(next_b);
+        if (!shared) return;
+        at = __builtin_amdgcn_readfirstlane(kept[0]); in = __builtin_amdgcn_readfirstlane(kept[1]); end = __builtin_amdgcn_readfirstlane(kept[2]);
+        b = __builtin_amdgcn_readfirstlane(kept[3]); whole = __builtin_amdgcn_readfirstlane(kept[4]);
     }
 }
 
@@ -212,293 +193,273 @@ __device__ __forceinline__ void set_priority(const Segment& x, uint32_t key) {
     else __builtin_amdgcn_s_setprio(0);
 }
 
-// ---- a wave's rows ---------------------------------------------------------------------------------------------------
+// ---- query rows ------------------------------------------------------------------------------------------------------
 
-// PARTS: rows of codes that a query row is the sum of, or 0: halves.
-template <int D, int CODES, int R, int PARTS> struct WaveRows {
+// Row `row` of a segment; those behind its last are its last again.
+struct RowPlace { uint32_t token, head; };
+__device__ __forceinline__ RowPlace place_of_row(Args& a, const Segment& x, uint32_t row) {
+    const uint32_t at = x.row0 + min(row, x.rows - 1), token = divide(at, a.group_magic);
+    return {token, x.head * a.group + at - token * a.group};
+}
+
+// A lane's quarter of a query row as the products want it (halves, or PARTS rows of codes one behind the other), and what its
+// scores have to be multiplied with to be in units of log2.
+template <int D, int PARTS> constexpr int kQueryRegs = PARTS == 0 ? D / 8 : PARTS * D / 16;
+template <int D> __device__ __forceinline__ void load_query(Args& a, const Segment& x, uint32_t row, uint32_t quarter, uint4_t (&raw)[D / 32]) {
+    const RowPlace place = place_of_row(a, x, row);
+    const char* from = a.q.data + int64_t(x.seq.first_token + place.token) * a.q.token_stride + int64_t(place.head) * a.q.head_stride;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        // the elements that the quarter's codes of this step are of: kChunk / 4 neighbours of each run of kChunk
+        const uint32_t at = Shape<D>::kChunk == 64 ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
+        raw[s] = *reinterpret_cast<const uint4_t*>(from + at * 2);
+    }
+}
+template <int D, int CODES, int PARTS> __device__ __forceinline__ float prepare_query(Args& a, const uint4_t (&raw)[D / 32], uint32_t (&q)[kQueryRegs<D, PARTS>]) {
     using S = Shape<D>;
-    static constexpr int kQueryRegs = PARTS == 0 ? S::kSteps * 4 : PARTS * S::kSteps * 2;     // dwords of a lane's quarter row
-    uint32_t token[R];                   // the new token of the lane's row
-    uint64_t sees_first[R];              // and the first word of its mask: fetched in good time, a word is all that trees of up to 64 have
-    uint32_t q[R][kQueryRegs];           // halves, or the parts one behind the other
-    float row_scale[R];
-    float4_t o[R][S::kTiles];
-    float m[R], l[R];
-    float limit[R];                      // the largest weight that is fine as it is: kLargest, or -1 while the row has seen no key
-
-    // Rows of the tiles `tile(r)` (16 rows each) of a segment; those behind its last are its last again.
-    template <typename F> __device__ __forceinline__ void start(Args& a, const Segment& x, uint32_t col, uint32_t quarter, F tile) {
-        uint4_t raw[R][S::kSteps];
+    float e[S::kSteps * 8];
+    uint32_t top = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint32_t row = x.row0 + min(tile(r) * 16 + col, x.rows - 1);
-            token[r] = divide(row, a.group_magic);
-            sees_first[r] = a.mask ? a.mask[int64_t(x.seq.first_token + token[r]) * a.mask_words] : 0;
-            const uint32_t g = row - token[r] * a.group;
-            const char* from = a.q.data + int64_t(x.seq.first_token + token[r]) * a.q.token_stride + int64_t(x.head * a.group + g) * a.q.head_stride;
+    for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
-            for (int s = 0; s < S::kSteps; ++s) {
-                // the elements that the quarter's codes of this step are of: kChunk / 4 neighbours of each run of kChunk
-                const uint32_t at = S::kChunk == 64 ? (s / 2) * 64 + quarter * 16 + (s % 2) * 8 : s * 32 + quarter * 8;
-                raw[r][s] = *reinterpret_cast<const uint4_t*>(from + at * 2);
-            }
+        for (int k = 0; k < 4; ++k) {
+            if (a.type == FKLHIP_BF16) unpack2<FKLHIP_BF16>(raw[s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
+            else unpack2<FKLHIP_F16>(raw[s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float e[S::kSteps * 8];
-            uint32_t top = 0;
+    for (int k = 0; k < S::kSteps * 8; ++k) top = max(top, __builtin_bit_cast(uint32_t, e[k]) & 0x7fffffffu);
+    top = max(top, uint32_t(__shfl_xor(int(top), 16)));
+    top = max(top, uint32_t(__shfl_xor(int(top), 32)));
+    // a power of two in front of the row's largest magnitude (a row of zeros, or with an infinity, is left alone)
+    const bool plain = top == 0 || top >= 0x7f800000u;
+    const int p = plain ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
+    // (a negative scale turns the queries round: scores are multiplied with what is above 0)
+    float unit = __builtin_fabsf(a.scale) * kLog2e;
+    if (a.scale < 0.0f)
 #pragma unroll
-            for (int s = 0; s < S::kSteps; ++s)
+        for (int k = 0; k < S::kSteps * 8; ++k) e[k] = -e[k];
+    if constexpr (PARTS == 0) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (a.type == FKLHIP_BF16) unpack2<FKLHIP_BF16>(raw[r][s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
-                    else unpack2<FKLHIP_F16>(raw[r][s][k], e[s * 8 + 2 * k], e[s * 8 + 2 * k + 1]);
-                }
+        for (int k = 0; k < S::kSteps * 4; ++k)
+            q[k] = pack2<FKLHIP_F16>(__builtin_amdgcn_ldexpf(e[2 * k], -p), __builtin_amdgcn_ldexpf(e[2 * k + 1], -p));
+    } else if constexpr (CODES == FKLHIP_CODES_INT8) {
+        // A power of two in front of the largest magnitude that leaves it below 127.5 * 2^8 (or 2^14); a row with an
+        // infinity or a NaN has scores that are NaN.
+        constexpr int kBits = PARTS == 2 ? 14 : 21;
+        const int up = kBits - p - (__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, top), -p) >= 1.9921875f ? 1 : 0);
+        unit = top >= 0x7f800000u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(unit, -up - p);
 #pragma unroll
-            for (int k = 0; k < S::kSteps * 8; ++k) top = max(top, __builtin_bit_cast(uint32_t, e[k]) & 0x7fffffffu);
-            top = max(top, uint32_t(__shfl_xor(int(top), 16)));
-            top = max(top, uint32_t(__shfl_xor(int(top), 32)));
-            // a power of two in front of the row's largest magnitude (a row of zeros, or with an infinity, is left alone)
-            const bool plain = top == 0 || top >= 0x7f800000u;
-            const int p = plain ? 0 : __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) - 1;
-            float unit = a.scale * kLog2e;
-            if constexpr (PARTS == 0) {
+        for (int k = 0; k < S::kSteps * 2; ++k) {
+            uint32_t w[PARTS];
 #pragma unroll
-                for (int k = 0; k < S::kSteps * 4; ++k)
-                    q[r][k] = pack2<FKLHIP_F16>(__builtin_amdgcn_ldexpf(e[2 * k], -p), __builtin_amdgcn_ldexpf(e[2 * k + 1], -p));
-            } else if constexpr (CODES == FKLHIP_CODES_INT8) {
-                // A power of two in front of the largest magnitude that leaves it below 127.5 * 2^8 (or 2^14); a row with an
-                // infinity or a NaN has scores that are NaN.
-                constexpr int kBits = PARTS == 2 ? 14 : 21;
-                const int up = kBits - p - (__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, top), -p) >= 1.9921875f ? 1 : 0);
-                unit = top >= 0x7f800000u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(unit, -up - p);
+            for (int part = 0; part < PARTS; ++part) w[part] = 0;
 #pragma unroll
-                for (int k = 0; k < S::kSteps * 2; ++k) {
-                    uint32_t w[PARTS];
+            for (int i = 0; i < 4; ++i) {
+                int v = int(__builtin_rintf(__builtin_amdgcn_ldexpf(e[4 * k + i], up)));
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part) w[part] = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        int v = int(__builtin_rintf(__builtin_amdgcn_ldexpf(e[4 * k + i], up)));
-#pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part) {      // the last digit of -128 .. 127, then the rest
-                            const int digit = int(uint32_t(v) << 24) >> 24;
-                            w[part] |= uint32_t(digit & 0xff) << (8 * i);
-                            v = (v - digit) >> 8;
-                        }
-                    }
-#pragma unroll
-                    for (int part = 0; part < PARTS; ++part) q[r][part * S::kSteps * 2 + k] = w[part];
-                }
-            } else {
-                unit = top >= 0x7f800000u ? __builtin_nanf("") : unit * 0x1p-7f;
-#pragma unroll
-                for (int k = 0; k < S::kSteps * 2; ++k) {
-                    float left[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) left[i] = __builtin_amdgcn_ldexpf(e[4 * k + i], 7 - p);
-#pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
-                        int w = __builtin_amdgcn_cvt_pk_fp8_f32(left[0], left[1], 0, false);
-                        w = __builtin_amdgcn_cvt_pk_fp8_f32(left[2], left[3], w, true);
-                        q[r][part * S::kSteps * 2 + k] = uint32_t(w);
-                        float taken[4];
-                        decode4<FKLHIP_CODES_E4M3>(uint32_t(w), taken);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) left[i] -= taken[i];
-                    }
+                for (int part = PARTS - 1; part >= 0; --part) {      // the last digit of -128 .. 127, then the rest
+                    const int digit = int(uint32_t(v) << 24) >> 24;
+                    w[part] |= uint32_t(digit & 0xff) << (8 * i);
+                    v = (v - digit) >> 8;
                 }
             }
-            row_scale[r] = __builtin_amdgcn_ldexpf(unit, p);
 #pragma unroll
-            for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            m[r] = 0.0f;
-            l[r] = 0.0f;
-            limit[r] = -1.0f;
+            for (int part = 0; part < PARTS; ++part) q[part * S::kSteps * 2 + k] = w[part];
+        }
+    } else {
+        unit = top >= 0x7f800000u ? __builtin_nanf("") : unit * 0x1p-7f;
+#pragma unroll
+        for (int k = 0; k < S::kSteps * 2; ++k) {
+            float left[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) left[i] = __builtin_amdgcn_ldexpf(e[4 * k + i], 7 - p);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                int w = __builtin_amdgcn_cvt_pk_fp8_f32(left[0], left[1], 0, false);
+                w = __builtin_amdgcn_cvt_pk_fp8_f32(left[2], left[3], w, true);
+                q[part * S::kSteps * 2 + k] = uint32_t(w);
+                float taken[4];
+                decode4<FKLHIP_CODES_E4M3>(uint32_t(w), taken);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) left[i] -= taken[i];
+            }
         }
     }
-    // The reference at the end, for comparison with others'.
-    __device__ __forceinline__ float reference(int r) const { return limit[r] < 0.0f ? kNothing : m[r]; }
+    unit = __builtin_amdgcn_ldexpf(unit, p);
+    return unit < 1.0e-37f ? 1.0e-37f : unit;                      // (above 0, as masked scores are -inf; NaN stays)
+}
 
-    // Products of a block of 16 keys with the rows, four keys to a quarter; the codes' scales are not in them.
-    template <typename K> __device__ __forceinline__ void products(K get_k, float4_t (&y)[R][2]) {
+// ---- 32 keys ---------------------------------------------------------------------------------------------------------
+
+// What a wave has summed up for its rows: R tiles of 16, one to a lane column; a quarter of each sum.
+template <int D, int CODES, int R, int PARTS> struct Sums {
+    using S = Shape<D>;
+    float4_t o[R][S::kTiles];
+    float m[R], l[R];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) o[r][i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            m[r] = kNothing;                                        // (which the first key that a row sees leads by more than kLead)
+            l[r] = 0.0f;
+        }
+    }
+
+    // Products of two blocks of 16 keys with a tile's rows, four keys of each to a quarter; the codes' scales are not in them.
+    template <typename K, typename Q> __device__ __forceinline__ void products(K get_k, Q get_q, float4_t (&y)[2]) {
         if constexpr (PARTS == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int r = 0; r < R; ++r) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int h = 0; h < 2; ++h) y[h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < S::kLoads; ++i) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const Words<S::kWords> w = get_k(h, i);
 #pragma unroll
-                    for (int k = 0; k < S::kWords / 2; ++k) {
-                        const half8_t codes = halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]);
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            const uint32_t* from = &q[r][(i * (S::kWords / 2) + k) * 4];
-                            y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8_t, uint4_t{from[0], from[1], from[2], from[3]}), y[r][h], 0, 0, 0);
-                        }
-                    }
+                    for (int k = 0; k < S::kWords / 2; ++k)
+                        y[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]), __builtin_bit_cast(half8_t, get_q(i * (S::kWords / 2) + k)), y[h], 0, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);                  // (all codes at once as halves would take 32 registers)
             }
         } else if constexpr (CODES == FKLHIP_CODES_INT8) {
             // the first two parts as one whole number, the third by itself: with it, 32 bits would not do
-            int4_t sum[PARTS - 1][R][2];
+            int4_t sum[PARTS - 1][2];
 #pragma unroll
             for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-                for (int i = 0; i < S::kLoads; ++i)
+                for (int i = 0; i < S::kLoads; ++i) {
+                    const int4_t row = __builtin_bit_cast(int4_t, get_q(part * S::kLoads + i));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const Words<S::kWords> w = get_k(h, i);
-                        const int4_t codes = {int(w.w[0]), int(w.w[1]), int(w.w[2]), int(w.w[3])};
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            const uint32_t* from = &q[r][part * S::kSteps * 2 + i * 4];
-                            int4_t& to = sum[part < 2 ? 0 : 1][r][h];
-                            const int4_t before = i > 0 ? to : part == 1 ? to << 8 : int4_t{0, 0, 0, 0};
-                            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes, int4_t{int(from[0]), int(from[1]), int(from[2]), int(from[3])}, before, 0, 0, 0);
-                        }
+                        int4_t& to = sum[part < 2 ? 0 : 1][h];
+                        const int4_t before = i > 0 ? to : part == 1 ? to << 8 : int4_t{0, 0, 0, 0};
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(int4_t{int(w.w[0]), int(w.w[1]), int(w.w[2]), int(w.w[3])}, row, before, 0, 0, 0);
                     }
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        y[r][h][i] = float(sum[0][r][h][i]);
-                        if constexpr (PARTS == 3) y[r][h][i] = __builtin_fmaf(y[r][h][i], 256.0f, float(sum[1][r][h][i]));
-                    }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::kLoads; i += 2)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const Words<S::kWords> lo = get_k(h, i), hi = get_k(h, i + 1);
-                    const int8_t8 codes = {int(lo.w[0]), int(lo.w[1]), int(lo.w[2]), int(lo.w[3]), int(hi.w[0]), int(hi.w[1]), int(hi.w[2]), int(hi.w[3])};
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
-                            const uint32_t* from = &q[r][part * S::kSteps * 2 + i * 4];
-                            const int8_t8 row = {int(from[0]), int(from[1]), int(from[2]), int(from[3]), int(from[4]), int(from[5]), int(from[6]), int(from[7])};
-                            const float4_t before = i == 0 && part == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : y[r][h];
-                            y[r][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, row, before, 0, 0, 0, 0, 0, 0);   // (e4m3 both, no scales)
-                        }
+                    if constexpr (PARTS == 3) __builtin_amdgcn_sched_barrier(0);    // (one part's registers at a time)
                 }
-        }
-    }
-
-    // 32 keys from `key` on: get_k(block, load) and get_v have their codes, get_scales(block, ks, vs) their scales;
-    // after_scores runs when the keys are used up.
-    template <bool MASKED, typename K, typename V, typename G, typename A>
-    __device__ __forceinline__ void step(const Segment& x, uint32_t key, uint32_t quarter, K get_k, V get_v, G get_scales, A after_scores) {
-        float4_t y[R][2];
-        products(get_k, y);
-        after_scores();
-        uint32_t sees[R][2], keep[2];                               // of the quarter's four keys, a bit each; bytes that are a token's
-        float4_t ks[2], vs[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            get_scales(h, ks[h], vs[h]);
-            if constexpr (MASKED) {
-                Args& a = kernel_args();
-                const uint32_t at = key + h * 16 + quarter * 4;
-                const uint32_t there = lowest_bits(int32_t(x.seq.total - at));
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const int32_t u = int32_t(at - x.seq.context);
-                    const uint32_t bits = a.mask == nullptr ? lowest_bits(int32_t(token[r]) + 1 - u)
-                                                            : mask_bits(a.mask + int64_t(x.seq.first_token + token[r]) * a.mask_words, sees_first[r], a.mask_words, u);
-                    sees[r][h] = bits & there;
-                }
-                // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
-                keep[h] = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) keep[h] |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
-            }
-        }
-        // Weights, and a look at whether a reference has to move: where a weight is too large for half precision, or where the
-        // row has seen no key yet.
-        float w[R][2][4], sum[R];
-        bool move = false;
-        auto weigh = [&](int r, int h, int i, float score) {
-            float e = exp2_fast(score);
-            float weight = e * vs[h][i];
-            if constexpr (MASKED) {
-                e = sees[r][h] >> i & 1 ? e : 0.0f;
-                weight = sees[r][h] >> i & 1 ? weight : 0.0f;       // (a hidden value's scale may be NaN)
-            }
-            sum[r] += e;
-            return weight;
-        };
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float top = 0.0f;
-            sum[r] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    y[r][h][i] *= ks[h][i];
-                    w[r][h][i] = weigh(r, h, i, __builtin_fmaf(y[r][h][i], row_scale[r], -m[r]));
-                    top = __builtin_fmaxf(top, w[r][h][i]);
+                    y[h][i] = float(sum[0][h][i]);
+                    if constexpr (PARTS == 3) y[h][i] = __builtin_fmaf(y[h][i], 256.0f, float(sum[1][h][i]));
                 }
-            move |= top > limit[r] || sum[r] > kMostSum;
-        }
-        if (__builtin_expect(__any(move), 0)) {
+        } else {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+            for (int i = 0; i < S::kLoads; i += 2)
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    const uint4_t u = get_q(part * S::kLoads + i), v = get_q(part * S::kLoads + i + 1);
+                    const int8_t8 row = {int(u[0]), int(u[1]), int(u[2]), int(u[3]), int(v[0]), int(v[1]), int(v[2]), int(v[3])};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const Words<S::kWords> lo = get_k(h, i), hi = get_k(h, i + 1);
+                        const int8_t8 codes = {int(lo.w[0]), int(lo.w[1]), int(lo.w[2]), int(lo.w[3]), int(hi.w[0]), int(hi.w[1]), int(hi.w[2]), int(hi.w[3])};
+                        const float4_t before = i == 0 && part == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : y[h];
+                        y[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, row, before, 0, 0, 0, 0, 0, 0);   // (e4m3 both, no scales)
+                    }
+                    if constexpr (PARTS == 3) __builtin_amdgcn_sched_barrier(0);    // (one part's registers at a time)
+                }
+        }
+    }
+
+    // 32 keys: get_k(block, load) and get_v have their codes, get_scales(ks, vs) the scales of the quarter's four keys of each
+    // block, get_q(tile, run) the queries, get_unit(tile) what their scores are multiplied with. after_scores runs when the
+    // keys are used up. Where `masked`, sees(tile, block) has a bit for each of the quarter's four keys that the lane's row
+    // sees, and hide() clears the values that are no token's. (The masked way is a branch around the scores and no second copy
+    // of the loop: between two loops the sums would be held twice.)
+    template <typename K, typename V, typename Q, typename U, typename G, typename M, typename H, typename A>
+    __device__ __forceinline__ void step(bool masked, K get_k, V get_v, Q get_q, U get_unit, G get_scales, M sees, H hide, A after_scores) {
+        half8_t p[R];
+        float4_t y[2], next[2];
+        // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of three parts of int8 take
+        // all registers without that.)
+        constexpr bool kAhead = !(R == 4 && PARTS == 3 && CODES == FKLHIP_CODES_INT8);
+        if (kAhead) products(get_k, [&](int run) { return get_q(0, run); }, y);
+        if (R == 1) after_scores();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (!kAhead) products(get_k, [&](int run) { return get_q(r, run); }, y);
+            else if (r + 1 < R) products(get_k, [&](int run) { return get_q(r + 1, run); }, next);
+            if (kAhead ? r + 2 == R : r + 1 == R) after_scores();
+            const float unit = get_unit(r);
+            float4_t ks[2], vs[2];
+            get_scales(ks, vs);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) y[h] *= ks[h];
+            if (__builtin_expect(masked, 0)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t seen = sees(r, h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[h][i] = seen >> i & 1 ? y[h][i] : -__builtin_inff();
+                        vs[h][i] = seen >> i & 1 ? vs[h][i] : 0.0f;          // (a hidden value's scale may be NaN)
+                    }
+                }
+            }
+            // Weights, and a look at whether the reference has to move: where a weight is too large for half precision.
+            float w[2][4], sum = 0.0f, top = 0.0f;
+            auto weigh = [&](int h, int i, float score) {
+                const float e = exp2_fast(score);
+                w[h][i] = e * vs[h][i];
+                sum += e;
+            };
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    weigh(h, i, __builtin_fmaf(y[h][i], unit, -m[r]));
+                    top = __builtin_fmaxf(top, w[h][i]);
+                }
+            if (__builtin_expect(__any(top > kLargest || sum > kMostSum), 0)) {
                 // the largest weight there would be, in units of log2
-                float top = -__builtin_inff();
+                top = -__builtin_inff();
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float v = y[r][h][i] * row_scale[r] + __builtin_log2f(__builtin_fmaxf(vs[h][i], kLeastScale));
-                        if constexpr (MASKED) v = sees[r][h] >> i & 1 ? v : -__builtin_inff();
-                        top = __builtin_fmaxf(top, v);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        top = __builtin_fmaxf(top, y[h][i] * unit + __builtin_amdgcn_logf(__builtin_fmaxf(vs[h][i], kLeastScale)));
                 top = max_quarters(top);
                 float alpha = 1.0f;
-                if (limit[r] < 0.0f ? top > -__builtin_inff() : top - m[r] > kLead) {
-                    alpha = limit[r] < 0.0f ? 0.0f : exp2_fast(m[r] + kStart - top);
+                if (top - m[r] > kLead) {
+                    alpha = exp2_fast(m[r] + kStart - top);
                     m[r] = top - kStart;
-                    limit[r] = kLargest;
                 }
                 l[r] *= alpha;
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) o[r][i] *= alpha;
                 // (from the rounded scores: those of 2^100 differ from their reference by more than an exponent holds)
-                sum[r] = 0.0f;
+                sum = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[r][h][i] = weigh(r, h, i, y[r][h][i] * row_scale[r] - m[r]);
+                    for (int i = 0; i < 4; ++i) weigh(h, i, y[h][i] * unit - m[r]);
             }
+            l[r] += sum;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[r][h * 4 + i] = _Float16(w[h][i]);
+                if (kAhead && r + 1 < R) y[h] = next[h];
+            }
+            if constexpr (R > 1) __builtin_amdgcn_sched_barrier(0);     // (more tiles' scores at once take more registers than there are)
         }
-        half8_t p[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            l[r] += sum[r];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[r][h * 4 + i] = _Float16(w[r][h][i]);
-        }
+        if (__builtin_expect(masked, 0)) hide();
 #pragma unroll
         for (int c = 0; c < S::kLoads; ++c) {
             const Words<S::kWords> v0 = get_v(0, c), v1 = get_v(1, c);
 #pragma unroll
             for (int k = 0; k < S::kWords; ++k) {
                 // tile c * kWords + k: elements c * kChunk + column * kWords + k
-                const half8_t v = MASKED ? halves8<CODES>(v0.w[k] & keep[0], v1.w[k] & keep[1]) : halves8<CODES>(v0.w[k], v1.w[k]);
+                const half8_t v = halves8<CODES>(v0.w[k], v1.w[k]);
 #pragma unroll
                 for (int r = 0; r < R; ++r) o[r][c * S::kWords + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[r], o[r][c * S::kWords + k], 0, 0, 0);
             }
+            if constexpr (R > 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -531,6 +492,27 @@ __device__ __forceinline__ void put_lse(Args& a, const Segment& x, uint32_t shar
     }
 }
 
+// Loads from an address that is the same for the whole wave, in scalar registers, and 32 bits of the lane's.
+using Global = const __attribute__((address_space(1))) char*;
+__device__ __forceinline__ Global of_wave(const void* p) {
+    uint64_t v = reinterpret_cast<uint64_t>(p);
+    asm volatile("" : "+s"(v));
+    return (Global)v;
+}
+template <typename T> __device__ __forceinline__ T load_at(Global base, uint32_t lane_part) { return *(const __attribute__((address_space(1))) T*)(base + size_t(lane_part)); }
+template <int WORDS> __device__ __forceinline__ Words<WORDS> load_words_at(Global base, uint32_t lane_part) {
+    Words<WORDS> r;
+    if constexpr (WORDS == 4) {
+        const uint4_t v = load_at<uint4_t>(base, lane_part);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = v[i];
+    } else {
+        const uint2_t v = load_at<uint2_t>(base, lane_part);
+        r.w[0] = v.x; r.w[1] = v.y;
+    }
+    return r;
+}
+
 // A wave's way through the page table: 64 entries at a time, one to a lane. (A scalar load for each block of keys would have
 // every wave wait for it; places are asked for in ascending order.)
 struct Pages {
@@ -549,21 +531,104 @@ struct Pages {
     }
 };
 
-// ---- few rows: the waves split the keys -------------------------------------------------------------------------------
+// ---- the kernel -------------------------------------------------------------------------------------------------------
+
+template <int D, int R> constexpr int kResident = D > 128 ? 1 : R == 1 ? 3 : 2;      // workgroups of a compute unit
+
+// Joins a workgroup's waves, kAtOnce<D, R> tiles at a time, and writes the rows.
+template <int D, int R> constexpr int kAtOnce = R > 1 && D <= 128 ? 2 : 1;
+template <int D> constexpr int kRowFloats = D + 4;                 // of a row in LDS: 16 bytes further round the banks than the last
+template <int D, int CODES, int R, int PARTS>
+__device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, PARTS>& sums, char* space, float (&joined_m)[kWaves][R * 16], float (&joined_l)[kWaves][R * 16]) {
+    using S = Shape<D>;
+    Args& a = kernel_args();
+    const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
+    const uint32_t share = own_share(a);
+    constexpr int kTilesAtOnce = kAtOnce<D, R>, kRows = kTilesAtOnce * 16;
+    float(*joined)[kRows * kRowFloats<D>] = reinterpret_cast<float(*)[kRows * kRowFloats<D>]>(space);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float l = sum_quarters(sums.l[r]);
+        if (quarter == 0) {
+            joined_m[wave][r * 16 + col] = sums.m[r];
+            joined_l[wave][r * 16 + col] = l;
+        }
+    }
+    __syncthreads();
+    // what a row's waves together lead, and sum up to
+    auto row_of = [&](uint32_t row, float& top, float& sum) {
+        top = joined_m[0][row];
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][row]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += joined_l[w][row] * exp2_fast(joined_m[w][row] - top);
+    };
+#pragma unroll
+    for (int r0 = 0; r0 < R; r0 += kTilesAtOnce) {
+        if (r0 > 0) __syncthreads();
+#pragma unroll
+        for (int r = r0; r < r0 + kTilesAtOnce; ++r) {
+            float top, sum;
+            row_of(r * 16 + col, top, sum);
+            // (a sum that is NaN, from a NaN among the scores, makes the row NaN)
+            const float factor = sum == 0.0f ? 0.0f : exp2_fast(joined_m[wave][r * 16 + col] - top) / sum;
+#pragma unroll
+            for (int c = 0; c < S::kLoads; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // rows quarter * 4 + i of the kWords tiles of a chunk are neighbouring elements
+                    float* to = &joined[wave][((r - r0) * 16 + col) * kRowFloats<D> + c * S::kChunk + (quarter * 4 + i) * S::kWords];
+#pragma unroll
+                    for (int w = 0; w < S::kWords; ++w) to[w] = sums.o[r][c * S::kWords + w][i] * factor;
+                }
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (uint32_t i = thread; i < kRows * D / 4; i += kWaves * 64) {
+            const uint32_t c = i / (D / 4), d = i % (D / 4) * 4, row = r0 * 16 + c;
+            if (row >= x.rows) break;
+            float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][c * kRowFloats<D> + d]);
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][c * kRowFloats<D> + d]);
+            const float f[4] = {e[0], e[1], e[2], e[3]};
+            put<D, 4>(a, x, share, row, d, f);
+        }
+    }
+    if (thread < x.rows) {
+        float top, sum;
+        row_of(thread, top, sum);
+        put_lse(a, x, share, thread, top, sum);
+    }
+    __syncthreads();
+}
 
 template <int D, int CODES, int R, int PARTS>
-__global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_split_keys(const AttentionArgs) {
+__global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attention(const AttentionArgs) {
     using S = Shape<D>;
-    constexpr int kRowFloats = D + 4;                              // of a row in LDS: 16 bytes further round the banks than the last
-    __shared__ __attribute__((aligned(16))) float joined[kWaves][16 * kRowFloats];
-    __shared__ float joined_m[kWaves][16], joined_l[kWaves][16], row_m[16], row_l[16];
-    walk(kernel_args(), threadIdx.x & 63, [&](const Segment& x) {
+    constexpr int kRegs = kQueryRegs<D, PARTS>, kRuns = kRegs / 4;
+    // One tile's rows: in registers. More: in LDS, whose place the joining of the waves takes afterwards.
+    constexpr bool kInLds = R > 1;
+    constexpr uint32_t kJoin = kWaves * kAtOnce<D, R> * 16 * kRowFloats<D> * 4, kQueries = kInLds ? R * kRuns * 1024 : 0;
+    __shared__ __attribute__((aligned(16))) char space[kJoin > kQueries ? kJoin : kQueries];
+    __shared__ float joined_m[kWaves][R * 16], joined_l[kWaves][R * 16];
+    __shared__ float units[R * 16];
+    __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
+    __shared__ __attribute__((aligned(16))) float scales[kWaves][2][64];
+    uint4_t* queries = reinterpret_cast<uint4_t*>(space);
+
+    __shared__ uint32_t walks[kWaves][8];
+    walk(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
         Args& a = kernel_args();
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
+        // The queries are asked for first, then keys and values, and while those are on their way the queries are made ready.
+        uint4_t raw[S::kSteps];
+        const uint32_t tile = kInLds ? wave : 0;
+        if (tile < R) load_query<D>(a, x, tile * 16 + col, quarter, raw);
         size_t at[2];
         Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
-        float4_t ks[2], vs[2];
+        float4_t k_scales[2], v_scales[2];
         Pages pages{0, 0};
         auto locate = [&](uint32_t key) {
 #pragma unroll
@@ -571,230 +636,114 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : R == 1 ? 2 : 2) void k_s
         };
         auto load_k = [&] {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                const Global from = of_wave(a.cache.k + at[h] * D);
 #pragma unroll
-                for (int i = 0; i < S::kLoads; ++i) k[h][i] = load_words<S::kWords>(a.cache.k + at[h] * D + lane_k + i * S::kChunk);
+                for (int i = 0; i < S::kLoads; ++i) k[h][i] = load_words_at<S::kWords>(from + i * S::kChunk, lane_k);
+            }
         };
-        auto load_scales_and_v = [&] {
+        // Scales of several tiles' steps are used again and again, and would take 16 registers: those go to LDS, two of the keys' and
+        // two of the values' blocks of 16 side by side, for this step and the next.
+        const uint32_t scales_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float*)&scales[wave][0][0])));
+        auto load_scales_and_v = [&](uint32_t step) {
+            if constexpr (kInLds) {
+                const float* from = (lane < 32 ? a.cache.k_scale : a.cache.v_scale) + at[lane >> 4 & 1] + col;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(scales_at + (step & 1) * 256), "v"(from) : "memory", "m0");
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    k_scales[h] = load_at<float4_t>(of_wave(a.cache.k_scale + at[h]), quarter * 16);
+                    v_scales[h] = load_at<float4_t>(of_wave(a.cache.v_scale + at[h]), quarter * 16);
+                }
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                ks[h] = *reinterpret_cast<const float4_t*>(a.cache.k_scale + at[h] + quarter * 4);
-                vs[h] = *reinterpret_cast<const float4_t*>(a.cache.v_scale + at[h] + quarter * 4);
+                const Global from = of_wave(a.cache.v + at[h] * D);
+#pragma unroll
+                for (int i = 0; i < S::kLoads; ++i) v[h][i] = load_words_at<S::kWords>(from + i * S::kChunk * 4, lane_v);
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < S::kLoads; ++i) v[h][i] = load_words<S::kWords>(a.cache.v + at[h] * D + lane_v + i * S::kChunk * 4);
         };
-        uint32_t key = x.key0 + wave * 32;
-        if (key < x.key1) pages.fetch(a, x, key >> a.cache.page_log, lane);
-        WaveRows<D, CODES, R, PARTS> rows;
-        rows.start(kernel_args(), x, col, quarter, [](int r) { return uint32_t(r); });
+        uint32_t key = x.key0 + wave * 32, step = 0;
         if (key < x.key1) {
+            pages.fetch(a, x, key >> a.cache.page_log, lane);
             locate(key);
             load_k();
-            load_scales_and_v();
+            load_scales_and_v(0);
         }
+        uint32_t q[kRegs];
+        uint64_t mask = 0;                                         // (of one tile's rows, like the queries)
+        float unit = 0.0f;
+        if (tile < R) {
+            Args& b = kernel_args();
+            if (b.mask) mask = b.mask[int64_t(x.seq.first_token + place_of_row(b, x, tile * 16 + col).token) * b.mask_words];
+            unit = prepare_query<D, CODES, PARTS>(b, raw, q);
+            if constexpr (kInLds) {
+#pragma unroll
+                for (int run = 0; run < kRuns; ++run) queries[(tile * kRuns + run) * 64 + lane] = uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
+                if (quarter == 0) {
+                    units[tile * 16 + col] = unit;
+                    masks[tile * 16 + col] = mask;
+                }
+            }
+        }
+        Sums<D, CODES, R, PARTS> sums;
+        sums.clear();
+        if constexpr (kInLds) __syncthreads();
         auto get_k = [&](int h, int i) { return k[h][i]; };
         auto get_v = [&](int h, int i) { return v[h][i]; };
-        auto get_scales = [&](int h, float4_t& s, float4_t& t) { s = ks[h]; t = vs[h]; };
-        // keys that all rows see, then the others
-        auto keys = [&](auto masked, uint32_t end) {
+        auto get_q = [&](int r, int run) {
+            if constexpr (kInLds) return queries[(r * kRuns + run) * 64 + lane];
+            else return uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
+        };
+        auto get_unit = [&](int r) { return kInLds ? units[r * 16 + col] : unit; };
+        auto get_scales = [&](float4_t (&ks)[2], float4_t (&vs)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ks[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][step & 1][h * 16 + quarter * 4]) : k_scales[h];
+                vs[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][step & 1][32 + h * 16 + quarter * 4]) : v_scales[h];
+            }
+        };
+        auto sees = [&](int r, int h) {
+            Args& b = kernel_args();
+            const uint32_t first = key + h * 16 + quarter * 4, there = lowest_bits(int32_t(x.seq.total - first));
+            const int32_t u = int32_t(first - x.seq.context);
+            const uint32_t token = place_of_row(b, x, r * 16 + col).token;
+            if (b.mask == nullptr) return lowest_bits(int32_t(token) + 1 - u) & there;
+            const uint64_t word = kInLds ? masks[r * 16 + col] : mask;
+            return mask_bits(b.mask + int64_t(x.seq.first_token + token) * b.mask_words, word, b.mask_words, u) & there;
+        };
+        // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
+        auto hide = [&] {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t there = lowest_bits(int32_t(x.seq.total - (key + h * 16 + quarter * 4)));
+                uint32_t keep = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) keep |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
+#pragma unroll
+                for (int i = 0; i < S::kLoads; ++i)
+#pragma unroll
+                    for (int w = 0; w < S::kWords; ++w) v[h][i].w[w] &= keep;
+            }
+        };
 #pragma unroll 1
-            while (key < end) {
-                const uint32_t next = key + kWaves * 32;
-                const bool more = next < x.key1;
-                set_priority(x, key);
-                if (more) locate(next);
-                // the keys' registers are free for the next once the scores are there, the others' at the end
-                rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [&] {
-                    if (more) load_k();
-                    __builtin_amdgcn_sched_barrier(0);
-                });
-                if (more) load_scales_and_v();
+        while (key < x.key1) {
+            const uint32_t next = key + kWaves * 32;
+            const bool more = next < x.key1;
+            set_priority(x, key);
+            if (more) locate(next);
+            if constexpr (kInLds) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * S::kLoads) : "memory");    // (the scales: only values have been asked for since)
+            // the keys' registers are free for the next once the scores are there, the others' at the end
+            sums.step(key + 32 > x.all_see, get_k, get_v, get_q, get_unit, get_scales, sees, hide, [&] {
+                if (more) load_k();
                 __builtin_amdgcn_sched_barrier(0);
-                key = next;
-            }
-        };
-        keys(std::false_type{}, min(x.key1, x.all_see & ~31u));
-        keys(std::true_type{}, x.key1);
-        // join the waves, 16 rows at a time, and write them
-        Args& out = kernel_args();
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float l = sum_quarters(rows.l[r]), m = rows.reference(r);
-            if (quarter == 0) {
-                joined_m[wave][col] = m;
-                joined_l[wave][col] = l;
-            }
-            __syncthreads();
-            float top = joined_m[0][col], sum = 0.0f;
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][col]);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += joined_l[w][col] * exp2_fast(joined_m[w][col] - top);
-            // (a sum that is NaN, from a NaN among the scores, makes the row NaN)
-            const float factor = sum == 0.0f ? 0.0f : exp2_fast(m - top) / sum;
-#pragma unroll
-            for (int c = 0; c < S::kLoads; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // rows quarter * 4 + i of the kWords tiles of a chunk are neighbouring elements
-                    float* to = &joined[wave][col * kRowFloats + c * S::kChunk + (quarter * 4 + i) * S::kWords];
-#pragma unroll
-                    for (int w = 0; w < S::kWords; ++w) to[w] = rows.o[r][c * S::kWords + w][i] * factor;
-                }
-            if (wave == 0 && quarter == 0) row_l[col] = sum, row_m[col] = top;
-            __syncthreads();
-            for (uint32_t i = thread; i < 16 * D / 4; i += kWaves * 64) {
-                const uint32_t c = i / (D / 4), d = i % (D / 4) * 4, row = r * 16 + c;
-                if (row >= x.rows) continue;
-                float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][c * kRowFloats + d]);
-#pragma unroll
-                for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][c * kRowFloats + d]);
-                const float f[4] = {e[0], e[1], e[2], e[3]};
-                put<D, 4>(out, x, own_share(out), row, d, f);
-                if (d == 0) put_lse(out, x, own_share(out), row, row_m[c], row_l[c]);
-            }
-            __syncthreads();
+            });
+            if (more) load_scales_and_v(step + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            key = next;
+            ++step;
         }
-    });
-}
-
-// ---- many rows: the waves split the rows ------------------------------------------------------------------------------
-
-// A stage of keys: per block of 16 their codes, their values' codes, and the scales of both. A wave copies a block, or, where
-// a stage has two (heads of more than 128 elements), the keys' or the values' half of one. Three stages stay under 64 KB.
-template <int D> struct Stage {
-    static constexpr uint32_t kBlocks = D <= 128 ? 4 : 2, kKeys = 16 * kBlocks, kCodes = 16 * D, kBlockBytes = 2 * kCodes + 128, kBytes = kBlocks * kBlockBytes;
-    static constexpr int kStages = 3, kRuns = (kCodes + 1023) / 1024;     // runs of 1 KB (the second of 1536 bytes is half of one)
-    static constexpr int kCopies = kBlocks == 4 ? 2 * kRuns + 1 : kRuns + 1;   // memory operations of a wave
-};
-
-// Copies to LDS without registers, 16 or 4 bytes a lane at `lds` + the same times the lane's number; the count of memory
-// operations in flight says when they are there.
-// (the compiler is told that a value is the wave's and not the lane's)
-__device__ __forceinline__ uint32_t of_wave(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ const char* of_wave(const char* p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<const char*>(uint64_t(of_wave(uint32_t(v >> 32))) << 32 | of_wave(uint32_t(v)));
-}
-__device__ __forceinline__ void copy16(const char* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(of_wave(lds)), "v"(offset), "s"(of_wave(base)) : "memory", "m0");
-}
-__device__ __forceinline__ void copy4(const char* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(of_wave(lds)), "v"(offset), "s"(of_wave(base)) : "memory", "m0");
-}
-// All but the wave's last N memory operations are done; then all waves' are, and nobody reads LDS any more.
-template <int N> __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
-
-template <int D, int CODES, int R, int PARTS>
-__global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(const AttentionArgs) {
-    using S = Shape<D>;
-    using P = Stage<D>;
-    __shared__ __attribute__((aligned(1024))) char ring[P::kStages * P::kBytes];
-    // Runs of 16 bytes a lane are copied so that a lane finds its own at 16 * lane; those of 8 (heads of 96) as they lie.
-    constexpr bool kOwn = S::kWords == 4;
-    constexpr uint32_t kNextK = kOwn ? 1024 : 32, kNextV = kOwn ? 1024 : 128;
-    walk(kernel_args(), threadIdx.x & 63, [&](const Segment& x) {
-        const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
-        const uint32_t from_k = kOwn ? col * D + quarter * 16 : lane * 16, from_v = kOwn ? quarter * (4 * D) + col * 16 : lane * 16;
-        const uint32_t read_k = kOwn ? lane * 16 : col * D + quarter * 8, read_v = kOwn ? lane * 16 : quarter * (4 * D) + col * 8;
-        const uint32_t ring_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)ring)));
-        const uint32_t stages = x.key1 > x.key0 ? (x.key1 - x.key0 + P::kKeys - 1) / P::kKeys : 0;
-        Pages pages{0, 0};
-        const uint32_t block = P::kBlocks == 4 ? wave : wave & 1;
-        if (stages) pages.fetch(kernel_args(), x, (x.key0 + block * 16) >> kernel_args().cache.page_log, lane);
-        auto copy = [&](uint32_t stage) {
-            Args& a = kernel_args();
-            const size_t at = pages.place(a, x, x.key0 + stage * P::kKeys + block * 16, lane);
-            const uint32_t to = ring_at + (stage % P::kStages) * P::kBytes + block * P::kBlockBytes;
-#pragma unroll
-            for (int i = 0; i < P::kRuns; ++i)
-                if (kOwn || i == 0 || lane < 32) {
-                    if (P::kBlocks == 4 || wave < 2) copy16(a.cache.k + at * D, from_k + i * (kOwn ? 64 : 1024), to + i * 1024);
-                    if (P::kBlocks == 4 || wave >= 2) copy16(a.cache.v + at * D, from_v + i * (kOwn ? 256 : 1024), to + P::kCodes + i * 1024);
-                }
-            // 16 scales of keys and 16 of values side by side: the lanes' offsets cover the distance of the two arrays
-            if (lane < 32) {
-                if (P::kBlocks == 4) {
-                    const char* s = reinterpret_cast<const char*>((lane < 16 ? a.cache.k_scale : a.cache.v_scale) + at) + (lane & 15) * 4;
-                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(of_wave(to + 2 * P::kCodes)), "v"(s) : "memory", "m0");
-                } else if (lane < 16) {
-                    copy4(reinterpret_cast<const char*>((wave < 2 ? a.cache.k_scale : a.cache.v_scale) + at), lane * 4, to + 2 * P::kCodes + (wave < 2 ? 0 : 64));
-                }
-            }
-        };
-#pragma unroll
-        for (uint32_t i = 0; i < P::kStages - 1; ++i)
-            if (i < stages) copy(i);
-        const uint32_t tiles = (x.rows + 15) / 16;
-        auto loop = [&](auto count) {
-            constexpr int kMine = decltype(count)::value;
-            WaveRows<D, CODES, kMine == 0 ? 1 : kMine, PARTS> rows;
-            if constexpr (kMine > 0) rows.start(kernel_args(), x, col, quarter, [&](int r) { return wave + kWaves * r; });
-            uint32_t key = x.key0, stage = 0;
-            const char* piece = ring;
-            // (every stage's first step; waves without rows take part in the copies and the waiting)
-            auto begin = [&](uint32_t key) {
-                if ((key & (P::kKeys - 1)) == 0) {
-                    set_priority(x, key);
-                    if (stage + 1 < stages) arrive<P::kCopies>();
-                    else arrive<0>();
-                    if (stage + P::kStages - 1 < stages) copy(stage + P::kStages - 1);
-                    piece = ring + (stage % P::kStages) * P::kBytes;
-                    ++stage;
-                } else {
-                    piece += 2 * P::kBlockBytes;
-                }
-            };
-            if constexpr (kMine > 0) {
-                auto get_k = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + read_k + i * kNextK); };
-                auto get_v = [&](int h, int i) { return load_words<S::kWords>(piece + h * P::kBlockBytes + P::kCodes + read_v + i * kNextV); };
-                auto get_scales = [&](int h, float4_t& s, float4_t& t) {
-                    s = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + quarter * 16);
-                    t = *reinterpret_cast<const float4_t*>(piece + h * P::kBlockBytes + 2 * P::kCodes + 64 + quarter * 16);
-                };
-                // keys that all rows see, then the others
-                auto keys = [&](auto masked, uint32_t end) {
-#pragma unroll 1
-                    for (; key < end; key += 32) {
-                        begin(key);
-                        rows.template step<decltype(masked)::value>(x, key, quarter, get_k, get_v, get_scales, [] {});
-                    }
-                };
-                keys(std::false_type{}, min(x.key1, x.all_see & ~31u));
-                keys(std::true_type{}, x.key1);
-            } else {
-                for (; key < x.key1; key += P::kKeys) begin(key);
-            }
-            if constexpr (kMine > 0) {
-                Args& out = kernel_args();
-                const uint32_t share = own_share(out);
-#pragma unroll
-                for (int r = 0; r < kMine; ++r) {
-                    const uint32_t row = (wave + kWaves * r) * 16 + col;
-                    const float l = sum_quarters(rows.l[r]);
-                    const float factor = l == 0.0f ? 0.0f : 1.0f / l;
-                    if (row < x.rows) {
-#pragma unroll
-                        for (int c = 0; c < S::kLoads; ++c)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float v[S::kWords];
-#pragma unroll
-                                for (int w = 0; w < S::kWords; ++w) v[w] = rows.o[r][c * S::kWords + w][i] * factor;
-                                put<D, S::kWords>(out, x, share, row, c * S::kChunk + (quarter * 4 + i) * S::kWords, v);
-                            }
-                        if (quarter == 0) put_lse(out, x, share, row, rows.reference(r), l);
-                    }
-                }
-            }
-        };
-        if (R == 2 && tiles > wave + kWaves) loop(std::integral_constant<int, R>{});
-        else if (tiles > wave) loop(std::integral_constant<int, 1>{});
-        else loop(std::integral_constant<int, 0>{});
-        arrive<0>();                                               // before the next segment's copies
+        join_waves<D, CODES, R, PARTS>(x, sums, space, joined_m, joined_l);
     });
 }
 
@@ -803,20 +752,17 @@ __global__ __launch_bounds__(kWaves * 64, D > 128 ? 1 : 2) void k_split_rows(con
 template <int D, int CODES, int PARTS> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
     const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(kWaves * 64);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    info = {p.split_rows ? "tree_attention_rows" : "tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1},
-            p.split_rows ? uint32_t(Stage<D>::kStages * Stage<D>::kBytes) : uint32_t((kWaves * 16 * (D + 4 + 2) + 32) * 4)};
+    info = {"tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1}, 0};
     if constexpr (D <= 128) {
-        if (p.tiles == 2) {
-            if (p.split_rows) k_split_rows<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
-            else k_split_keys<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
+        if (p.tiles == 4) {
+            k_tree_attention<D, CODES, 4, PARTS><<<grid, block, 0, s>>>(a);
             return int(hipGetLastError());
         }
     }
-    if (p.split_rows) k_split_rows<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
-    else k_split_keys<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
+    if (p.tiles == 2) k_tree_attention<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
+    else k_tree_attention<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
     return int(hipGetLastError());
 }
-
 template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
     if constexpr (kCodeProducts<D, CODES>) {
         if (a.type == FKLHIP_F16) return start_attention<D, CODES, 3>(a, p, stream, info);

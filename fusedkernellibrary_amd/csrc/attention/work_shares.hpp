@@ -36,11 +36,10 @@ __device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t 
     return s;
 }
 __device__ __forceinline__ Sequence sequence_at(Args& a, uint32_t b) { return sequence_of(a, scalar(a.q_start + b), scalar(a.q_start + b + 1), scalar(a.context + b)); }
-// Work is counted in granules: a.granule keys of one key head and up to a.sub_rows of its rows. A row block has up to
-// a.block_subs times as many rows, and its keys count once for each a.sub_rows of them.
+// Work is counted in granules: 2^granule_log keys of one key head and one block of its rows.
 __device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return (s.total + (1u << a.granule_log) - 1) >> a.granule_log; }
-__device__ __forceinline__ uint32_t subs_of(Args& a, const Sequence& s) { return (s.rows + (1u << a.sub_log) - 1) >> a.sub_log; }
-__device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return subs_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
+__device__ __forceinline__ uint32_t blocks_of(Args& a, const Sequence& s) { return (s.rows + a.unit_rows - 1) >> __builtin_ctz(a.unit_rows); }
+__device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return blocks_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
 
 // Sums of a wave's lanes up to and with each.
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
