@@ -210,7 +210,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     a.group_magic = magic(a.group);
     a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
     a.unit_rows = plan.unit_rows;
-    a.granule_log = plan.granule_log; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
+    a.granule_log = plan.granule_log; a.lead = plan.lead; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
     a.type = c->type; a.scale = c->scale;
     if (bytes) {
         a.partial = static_cast<float*>(c->workspace);
@@ -240,14 +240,15 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     p.tiles = rows <= 16 ? 1 : rows <= 32 || head_dim > 128 ? 2 : 4;
     p.unit_rows = 16 * p.tiles;
     p.granule_log = 7;
+    p.lead = p.tiles == 1 ? 1 : p.tiles == 2 ? 3 : 5;
     p.row_blocks = std::max(1u, (rows + p.unit_rows - 1) / p.unit_rows);
-    const uint64_t granules = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log, units = uint64_t(batch) * kv_heads * p.row_blocks;
+    const uint64_t granules = p.lead + ((uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log), units = uint64_t(batch) * kv_heads * p.row_blocks;
     const uint64_t all = units * granules;
     // as many shares as workgroups run at once on 256 compute units, or a power of two that leaves two granules to each
     const uint32_t at_once = head_dim > 128 ? 1 : p.tiles == 1 ? 3 : 2;
     p.share_log = 8 + (at_once == 2);
     p.share_odd = at_once == 3 ? 3 : 1;
-    if (granules <= 4 || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
+    if (granules <= 4 + p.lead || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
     else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
     p.many_parts = p.shares() > 16 * units;
     return p;

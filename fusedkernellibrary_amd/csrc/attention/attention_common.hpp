@@ -53,7 +53,7 @@ struct AttentionArgs {
     uint32_t tokens, batch, max_new, max_context, mask_words;
     uint32_t q_heads, group;                // query heads per key head
     uint32_t group_magic;                   // x / group as a multiplication (see divide)
-    uint32_t unit_rows, granule_log, share_log, share_odd;    // how the work is dealt out (work_shares.hpp)
+    uint32_t unit_rows, granule_log, lead, share_log, share_odd;    // how the work is dealt out (work_shares.hpp)
     int type;
     float scale;
 };
@@ -67,7 +67,7 @@ int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, voi
 // How a call is run: 16-row tiles (and so rows) to a workgroup; row blocks of a sequence; share_odd << share_log shares, or none;
 // whether rows have so many parts that a workgroup joins one.
 struct AttentionPlan {
-    uint32_t tiles, row_blocks, unit_rows, granule_log, share_log, share_odd;
+    uint32_t tiles, row_blocks, unit_rows, granule_log, lead, share_log, share_odd;
     bool many_parts;
     uint32_t shares() const { return share_odd << share_log; }
 };

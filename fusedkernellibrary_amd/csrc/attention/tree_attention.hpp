@@ -172,11 +172,16 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
             return;
         }
         kept[0] = at + count; kept[1] = in + count; kept[2] = end; kept[3] = b; kept[4] = whole;
-        Segment x = segment_of(a, s, b, head, block, g, g + count, part);
+        Segment x = segment_of(a, s, b, head, block, max(g, a.lead) - a.lead, max(g + count, a.lead) - a.lead, part);
         x.quarter = whole << a.granule_log >> 2;
         x.behind = (end - at - count) << a.granule_log;
         if (!shared) x.behind = 0, x.quarter = (x.key1 - x.key0) >> 2;
-        run(x);
+        if (part >= 0 && g + count <= a.lead) {
+            // nothing but a block's beginning
+            if (threadIdx.x < x.rows) a.partial_lse[(size_t(own_share(a)) * 2 + part) * a.unit_rows + threadIdx.x] = -__builtin_inff();
+        } else {
+            run(x);
+        }
         if (!shared) return;
         at = __builtin_amdgcn_readfirstlane(kept[0]); in = __builtin_amdgcn_readfirstlane(kept[1]); end = __builtin_amdgcn_readfirstlane(kept[2]);
         b = __builtin_amdgcn_readfirstlane(kept[3]); whole = __builtin_amdgcn_readfirstlane(kept[4]);

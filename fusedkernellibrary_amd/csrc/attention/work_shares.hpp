@@ -36,8 +36,9 @@ __device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t 
     return s;
 }
 __device__ __forceinline__ Sequence sequence_at(Args& a, uint32_t b) { return sequence_of(a, scalar(a.q_start + b), scalar(a.q_start + b + 1), scalar(a.context + b)); }
-// Work is counted in granules: 2^granule_log keys of one key head and one block of its rows.
-__device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return (s.total + (1u << a.granule_log) - 1) >> a.granule_log; }
+// Work is counted in granules: 2^granule_log keys of one key head and one block of its rows. In front of a block's keys stand
+// `lead` granules for what it takes to begin and to end it.
+__device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return s.total ? a.lead + ((s.total + (1u << a.granule_log) - 1) >> a.granule_log) : 0u; }
 __device__ __forceinline__ uint32_t blocks_of(Args& a, const Sequence& s) { return (s.rows + a.unit_rows - 1) >> __builtin_ctz(a.unit_rows); }
 __device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return blocks_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
 
