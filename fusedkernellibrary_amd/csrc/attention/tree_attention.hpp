@@ -469,21 +469,12 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
     }
 };
 
-// Four or two neighbouring elements of a row of the result: to the output, or to a share's part.
-template <int D, int N> __device__ __forceinline__ void put(Args& a, const Segment& x, uint32_t share, uint32_t row, uint32_t d, const float* v) {
-    if (x.part < 0) {
-        const uint32_t tok = divide(x.row0 + row, a.group_magic), qh = x.head * a.group + x.row0 + row - tok * a.group;
-        char* to = a.out.data + int64_t(x.seq.first_token + tok) * a.out.token_stride + int64_t(qh) * a.out.head_stride + d * 2;
-        uint32_t w[N / 2];
-#pragma unroll
-        for (int k = 0; k < N / 2; ++k) w[k] = a.type == FKLHIP_BF16 ? pack2<FKLHIP_BF16>(v[2 * k], v[2 * k + 1]) : pack2<FKLHIP_F16>(v[2 * k], v[2 * k + 1]);
-        if constexpr (N == 4) *reinterpret_cast<uint2_t*>(to) = uint2_t{w[0], w[1]};
-        else *reinterpret_cast<uint32_t*>(to) = w[0];
-    } else {
-        float* to = a.partial + ((size_t(share) * 2 + x.part) * a.unit_rows + row) * D + d;
-#pragma unroll
-        for (int k = 0; k < N; ++k) to[k] = v[k];
-    }
+// Four neighbouring elements of a row of the result.
+__device__ __forceinline__ void put4(Args& a, const Segment& x, uint32_t row, uint32_t d, float4_t v) {
+    const uint32_t tok = divide(x.row0 + row, a.group_magic), qh = x.head * a.group + x.row0 + row - tok * a.group;
+    const uint2_t w = a.type == FKLHIP_BF16 ? uint2_t{pack2<FKLHIP_BF16>(v[0], v[1]), pack2<FKLHIP_BF16>(v[2], v[3])}
+                                            : uint2_t{pack2<FKLHIP_F16>(v[0], v[1]), pack2<FKLHIP_F16>(v[2], v[3])};
+    *reinterpret_cast<uint2_t*>(a.out.data + int64_t(x.seq.first_token + tok) * a.out.token_stride + int64_t(qh) * a.out.head_stride + d * 2) = w;
 }
 // lse is in units of log2.
 __device__ __forceinline__ void put_lse(Args& a, const Segment& x, uint32_t share, uint32_t row, float m, float l) {
@@ -589,15 +580,21 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
                 }
         }
         __syncthreads();
-#pragma unroll 2
-        for (uint32_t i = thread; i < kRows * D / 4; i += kWaves * 64) {
-            const uint32_t c = i / (D / 4), d = i % (D / 4) * 4, row = r0 * 16 + c;
-            if (row >= x.rows) break;
-            float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][c * kRowFloats<D> + d]);
+        auto sum_of = [&](uint32_t i) {
+            const uint32_t at = i / (D / 4) * kRowFloats<D> + i % (D / 4) * 4;
+            float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][at]);
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][c * kRowFloats<D> + d]);
-            const float f[4] = {e[0], e[1], e[2], e[3]};
-            put<D, 4>(a, x, share, row, d, f);
+            for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][at]);
+            return e;
+        };
+        const uint32_t count = min(uint32_t(kRows), x.rows - min(x.rows, uint32_t(r0 * 16))) * (D / 4);
+        if (x.part < 0) {
+#pragma unroll 2
+            for (uint32_t i = thread; i < count; i += kWaves * 64) put4(a, x, r0 * 16 + i / (D / 4), i % (D / 4) * 4, sum_of(i));
+        } else {
+            float4_t* to = reinterpret_cast<float4_t*>(a.partial + ((size_t(share) * 2 + x.part) * a.unit_rows + r0 * 16) * D);
+#pragma unroll 4
+            for (uint32_t i = thread; i < count; i += kWaves * 64) to[i] = sum_of(i);
         }
     }
     if (thread < x.rows) {
@@ -630,7 +627,11 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attenti
         // The queries are asked for first, then keys and values, and while those are on their way the queries are made ready.
         uint4_t raw[S::kSteps];
         const uint32_t tile = kInLds ? wave : 0;
-        if (tile < R) load_query<D>(a, x, tile * 16 + col, quarter, raw);
+        uint64_t mask = 0;                                         // (of one tile's rows, like the queries)
+        if (tile < R) {
+            load_query<D>(a, x, tile * 16 + col, quarter, raw);
+            if (a.mask) mask = a.mask[int64_t(x.seq.first_token + place_of_row(a, x, tile * 16 + col).token) * a.mask_words];
+        }
         size_t at[2];
         Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
         float4_t k_scales[2], v_scales[2];
@@ -676,12 +677,9 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attenti
             load_scales_and_v(0);
         }
         uint32_t q[kRegs];
-        uint64_t mask = 0;                                         // (of one tile's rows, like the queries)
         float unit = 0.0f;
         if (tile < R) {
-            Args& b = kernel_args();
-            if (b.mask) mask = b.mask[int64_t(x.seq.first_token + place_of_row(b, x, tile * 16 + col).token) * b.mask_words];
-            unit = prepare_query<D, CODES, PARTS>(b, raw, q);
+            unit = prepare_query<D, CODES, PARTS>(kernel_args(), raw, q);
             if constexpr (kInLds) {
 #pragma unroll
                 for (int run = 0; run < kRuns; ++run) queries[(tile * kRuns + run) * 64 + lane] = uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
