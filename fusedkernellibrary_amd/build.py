@@ -1,12 +1,15 @@
 """Builds libfklhip.so: the C-ABI runtime plus the ahead-of-time compiled gfx950 kernels of every chain
-signature listed in csrc/aot_signatures.txt and the attention kernels under csrc/attention.  `python -m fusedkernellibrary_amd.build` rebuilds it in place."""
+signature listed in csrc/aot_signatures.txt and the attention kernels under csrc/attention, and _attention.so, the
+attention operators' torch binding.  `python -m fusedkernellibrary_amd.build` rebuilds it in place."""
 from __future__ import annotations
 
 import concurrent.futures as cf
 import hashlib
+import importlib.util
 import os
 import shlex
 import subprocess
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -134,7 +137,7 @@ def build_library(verbose: bool = True) -> str:
     sigs = read_signatures()
     units = generate_units(sigs)
     os.makedirs(OBJ_DIR, exist_ok=True)
-    attention = [os.path.join(CSRC, "attention", name) for name in sorted(os.listdir(os.path.join(CSRC, "attention"))) if name.endswith((".hip", ".cpp"))]
+    attention = [os.path.join(CSRC, "attention", name) for name in sorted(os.listdir(os.path.join(CSRC, "attention"))) if name.endswith((".hip", ".cpp")) and name != "torch_binding.cpp"]
     srcs = attention + units + [os.path.join(CSRC, "fklhip_runtime.cpp"), os.path.join(CSRC, "jit.cpp"), generate_jit_sources()]
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(_compile, srcs))
@@ -148,5 +151,29 @@ def build_library(verbose: bool = True) -> str:
     return LIB
 
 
+def build_torch_binding(verbose: bool = True) -> str | None:
+    """_attention.so: host code only, so the host compiler builds it. Without torch there is nothing to bind, and
+    libfklhip.so does not need it."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    torch_dir = spec.submodule_search_locations[0]
+    out = os.path.join(PKG, "_attention.so")
+    rocm = os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")
+    include = [INCLUDE, os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), rocm,
+               sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++20", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-w", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1",
+           *[f"-I{d}" for d in include], os.path.join(CSRC, "attention", "torch_binding.cpp"), "-o", out + ".tmp",
+           "-L", PKG, "-lfklhip", "-L", os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on torch_binding.cpp:\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+    if verbose:
+        print(f"built {out}")
+    return out
+
+
 if __name__ == "__main__":
     build_library()
+    build_torch_binding()
