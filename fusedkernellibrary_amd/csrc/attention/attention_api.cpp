@@ -236,21 +236,44 @@ namespace fkattn {
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim) {
     const auto log2_floor = [](uint64_t n) { uint32_t l = 0; while (n >>= 1) ++l; return l; };
     AttentionPlan p;
-    // 16-row tiles to a workgroup: as few as hold the rows; each takes registers
-    p.tiles = rows <= 16 ? 1 : rows <= 32 || head_dim > 128 ? 2 : 4;
-    p.unit_rows = 16 * p.tiles;
     p.granule_log = 7;
+    const uint64_t length = (uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log;     // of the longest sequence there may be
+    const auto blocks = [&](uint32_t tiles) { return std::max(1u, (rows + 16 * tiles - 1) / (16 * tiles)); };
+    const auto units = [&](uint32_t tiles) { return uint64_t(batch) * kv_heads * blocks(tiles); };
+    const uint32_t most_tiles = rows <= 16 ? 1 : rows <= 32 || head_dim > 128 ? 2 : 4;         // (each takes registers)
+    const uint32_t slots = head_dim > 128 ? 256 : 512;                                       // workgroups at once on 256 compute units
+    // A workgroup to each row block, if all run at once and none is long: joining shares' parts costs 6 us and more. Small blocks
+    // are the faster ones then, whose keys come from the L2 cache again; one tile's has eight waves if each has a compute unit.
+    // Measured, 8 key heads of 128 (4 waves, 8 waves, shares, in us): one sequence of 1000 keys 12.1, 11.7, 14.4; 2000 17.8, 16.9,
+    // 16.3; 3000 23.4, 22.2, 16.2: a compute unit reads 50 GB/s and no more. 2 key heads of 64, 2000 keys: 14.5, 11.6, 14.5.
+    // 16 tokens, 16 sequences of 1000 keys: one tile 18.7, two 18.8, four 27.2, shares of two tiles 26.8; one sequence of
+    // 1000: 12.5, 16.8, 25.3 and 16.8.
+    p.tiles = 1;
+    while (p.tiles < most_tiles && units(p.tiles) > slots) p.tiles *= 2;
+    p.waves = p.tiles == 1 && units(1) <= 256 ? 8 : 4;
+    const uint64_t worth = (p.waves == 8 ? 16 : p.tiles == 4 ? 6 : 8) * 128 / head_dim;
+    p.share_log = 0;
+    p.share_odd = 0;
+    // (sequences are taken to be half as long as the longest in the mean: shares use the compute units that ended early)
+    const bool whole = units(p.tiles) <= slots ? length * (2 * slots - units(p.tiles)) <= worth * 2 * slots : length <= 8;
+    if (!whole) {
+        // shares: the fewer blocks the less is converted and read, unless a share has so little that beginning and ending it counts more
+        p.tiles = most_tiles;
+        p.waves = 4;
+        while (p.tiles > 1 && units(p.tiles) * length < uint64_t(p.tiles == 4 ? 8 : 4) * slots) p.tiles /= 2;
+    }
+    p.unit_rows = 16 * p.tiles;
+    p.row_blocks = blocks(p.tiles);
     p.lead = p.tiles == 1 ? 1 : p.tiles == 2 ? 3 : 5;
-    p.row_blocks = std::max(1u, (rows + p.unit_rows - 1) / p.unit_rows);
-    const uint64_t granules = p.lead + ((uint64_t(keys) + (1u << p.granule_log) - 1) >> p.granule_log), units = uint64_t(batch) * kv_heads * p.row_blocks;
-    const uint64_t all = units * granules;
-    // as many shares as workgroups run at once on 256 compute units, or a power of two that leaves two granules to each
-    const uint32_t at_once = head_dim > 128 ? 1 : p.tiles == 1 ? 3 : 2;
-    p.share_log = 8 + (at_once == 2);
-    p.share_odd = at_once == 3 ? 3 : 1;
-    if (granules <= 4 + p.lead || units >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
-    else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
-    p.many_parts = p.shares() > 16 * units;
+    if (!whole) {
+        // as many shares as workgroups run at once, or a power of two that leaves two granules to each
+        const uint64_t all = units(p.tiles) * (p.lead + length);
+        p.share_odd = slots == 512 && p.tiles == 1 ? 3 : 1;
+        p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
+        if (units(p.tiles) >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
+        else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
+    }
+    p.many_parts = p.shares() > 16 * units(p.tiles);
     return p;
 }
 

@@ -64,10 +64,10 @@ struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
 int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream);
-// How a call is run: 16-row tiles (and so rows) to a workgroup; row blocks of a sequence; share_odd << share_log shares, or none;
-// whether rows have so many parts that a workgroup joins one.
+// How a call is run: 16-row tiles (and so rows) and waves to a workgroup; row blocks of a sequence; share_odd << share_log
+// shares, or none; whether rows have so many parts that a workgroup joins one.
 struct AttentionPlan {
-    uint32_t tiles, row_blocks, unit_rows, granule_log, lead, share_log, share_odd;
+    uint32_t tiles, waves, row_blocks, unit_rows, granule_log, lead, share_log, share_odd;
     bool many_parts;
     uint32_t shares() const { return share_odd << share_log; }
 };

@@ -35,7 +35,6 @@
 
 namespace fkattn {
 
-constexpr int kWaves = 4;                    // of a workgroup: they share out a chunk's keys, 32 at a time
 constexpr float kStart = 6.0f, kLead = 14.0f, kLargest = 16384.0f, kLeastScale = 0x1p-80f, kMostSum = 0x1p98f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -1.0e30f;         // the reference of a row that has seen no key
@@ -529,13 +528,14 @@ struct Pages {
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 
-template <int D, int R> constexpr int kResident = D > 128 ? 1 : R == 1 ? 3 : 2;      // workgroups of a compute unit
+// Workgroups of a compute unit. Their waves share out a segment's keys, 32 at a time.
+template <int D, int R, int WAVES> constexpr int kResident = D > 128 || WAVES == 8 ? 1 : R == 1 ? 3 : 2;
 
 // Joins a workgroup's waves, kAtOnce<D, R> tiles at a time, and writes the rows.
 template <int D, int R> constexpr int kAtOnce = R > 1 && D <= 128 ? 2 : 1;
 template <int D> constexpr int kRowFloats = D + 4;                 // of a row in LDS: 16 bytes further round the banks than the last
-template <int D, int CODES, int R, int PARTS>
-__device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, PARTS>& sums, char* space, float (&joined_m)[kWaves][R * 16], float (&joined_l)[kWaves][R * 16]) {
+template <int WAVES, int D, int CODES, int R, int PARTS>
+__device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, PARTS>& sums, char* space, float (&joined_m)[WAVES][R * 16], float (&joined_l)[WAVES][R * 16]) {
     using S = Shape<D>;
     Args& a = kernel_args();
     const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
@@ -556,9 +556,9 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
         top = joined_m[0][row];
         sum = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, joined_m[w][row]);
+        for (int w = 1; w < WAVES; ++w) top = __builtin_fmaxf(top, joined_m[w][row]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += joined_l[w][row] * exp2_fast(joined_m[w][row] - top);
+        for (int w = 0; w < WAVES; ++w) sum += joined_l[w][row] * exp2_fast(joined_m[w][row] - top);
     };
 #pragma unroll
     for (int r0 = 0; r0 < R; r0 += kTilesAtOnce) {
@@ -584,17 +584,17 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
             const uint32_t at = i / (D / 4) * kRowFloats<D> + i % (D / 4) * 4;
             float4_t e = *reinterpret_cast<const float4_t*>(&joined[0][at]);
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][at]);
+            for (int w = 1; w < WAVES; ++w) e += *reinterpret_cast<const float4_t*>(&joined[w][at]);
             return e;
         };
         const uint32_t count = min(uint32_t(kRows), x.rows - min(x.rows, uint32_t(r0 * 16))) * (D / 4);
         if (x.part < 0) {
 #pragma unroll 2
-            for (uint32_t i = thread; i < count; i += kWaves * 64) put4(a, x, r0 * 16 + i / (D / 4), i % (D / 4) * 4, sum_of(i));
+            for (uint32_t i = thread; i < count; i += WAVES * 64) put4(a, x, r0 * 16 + i / (D / 4), i % (D / 4) * 4, sum_of(i));
         } else {
             float4_t* to = reinterpret_cast<float4_t*>(a.partial + ((size_t(share) * 2 + x.part) * a.unit_rows + r0 * 16) * D);
 #pragma unroll 4
-            for (uint32_t i = thread; i < count; i += kWaves * 64) to[i] = sum_of(i);
+            for (uint32_t i = thread; i < count; i += WAVES * 64) to[i] = sum_of(i);
         }
     }
     if (thread < x.rows) {
@@ -605,21 +605,21 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
     __syncthreads();
 }
 
-template <int D, int CODES, int R, int PARTS>
-__global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attention(const AttentionArgs) {
+template <int D, int CODES, int R, int PARTS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_attention(const AttentionArgs) {
     using S = Shape<D>;
     constexpr int kRegs = kQueryRegs<D, PARTS>, kRuns = kRegs / 4;
     // One tile's rows: in registers. More: in LDS, whose place the joining of the waves takes afterwards.
     constexpr bool kInLds = R > 1;
-    constexpr uint32_t kJoin = kWaves * kAtOnce<D, R> * 16 * kRowFloats<D> * 4, kQueries = kInLds ? R * kRuns * 1024 : 0;
+    constexpr uint32_t kJoin = WAVES * kAtOnce<D, R> * 16 * kRowFloats<D> * 4, kQueries = kInLds ? R * kRuns * 1024 : 0;
     __shared__ __attribute__((aligned(16))) char space[kJoin > kQueries ? kJoin : kQueries];
-    __shared__ float joined_m[kWaves][R * 16], joined_l[kWaves][R * 16];
+    __shared__ float joined_m[WAVES][R * 16], joined_l[WAVES][R * 16];
     __shared__ float units[R * 16];
     __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
-    __shared__ __attribute__((aligned(16))) float scales[kWaves][2][64];
+    __shared__ __attribute__((aligned(16))) float scales[WAVES][2][64];
     uint4_t* queries = reinterpret_cast<uint4_t*>(space);
 
-    __shared__ uint32_t walks[kWaves][8];
+    __shared__ uint32_t walks[WAVES][8];
     walk(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
         Args& a = kernel_args();
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
@@ -731,7 +731,7 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attenti
         };
 #pragma unroll 1
         while (key < x.key1) {
-            const uint32_t next = key + kWaves * 32;
+            const uint32_t next = key + WAVES * 32;
             const bool more = next < x.key1;
             set_priority(x, key);
             if (more) locate(next);
@@ -746,24 +746,25 @@ __global__ __launch_bounds__(kWaves * 64, (kResident<D, R>)) void k_tree_attenti
             key = next;
             ++step;
         }
-        join_waves<D, CODES, R, PARTS>(x, sums, space, joined_m, joined_l);
+        join_waves<WAVES>(x, sums, space, joined_m, joined_l);
     });
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 
 template <int D, int CODES, int PARTS> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
-    const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(kWaves * 64);
+    const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(p.waves * 64);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     info = {"tree_attention", {grid.x, grid.y, grid.z}, {block.x, 1, 1}, 0};
-    if constexpr (D <= 128) {
-        if (p.tiles == 4) {
-            k_tree_attention<D, CODES, 4, PARTS><<<grid, block, 0, s>>>(a);
-            return int(hipGetLastError());
-        }
+    if (p.tiles == 4) {
+        if constexpr (D <= 128) k_tree_attention<D, CODES, 4, PARTS, 4><<<grid, block, 0, s>>>(a);
+    } else if (p.tiles == 2) {
+        k_tree_attention<D, CODES, 2, PARTS, 4><<<grid, block, 0, s>>>(a);
+    } else if (p.waves == 8) {
+        k_tree_attention<D, CODES, 1, PARTS, 8><<<grid, block, 0, s>>>(a);
+    } else {
+        k_tree_attention<D, CODES, 1, PARTS, 4><<<grid, block, 0, s>>>(a);
     }
-    if (p.tiles == 2) k_tree_attention<D, CODES, 2, PARTS><<<grid, block, 0, s>>>(a);
-    else k_tree_attention<D, CODES, 1, PARTS><<<grid, block, 0, s>>>(a);
     return int(hipGetLastError());
 }
 template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
