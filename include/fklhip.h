@@ -119,6 +119,8 @@ int fklhip_strip_form(int enable);
  * kernel receives "rows", "gather" or "strip", each with "_jit" behind it for chains compiled at run time, or "rows_unaligned": the
  * kernel for rows that do not all start on dword boundaries, of the chains compiled ahead of time that have one of its own for
  * them (padding, deinterlacing, planar and circular reads; the others have one kernel for rows at every alignment).
+ * The operators around a key-value cache are "heads" (norms, rotations and writes), "kv_read" and "tree_attention_TxW", with T tiles
+ * of 16 rows and W waves to a workgroup; their lds_bytes are 0, as they ask for none at run time.
  * grid/block receive 3 values each. */
 int fklhip_last_launch(const char **kernel, unsigned grid[3], unsigned block[3], unsigned *lds_bytes);
 /* The same launch's kernel by its own name, which fklhip_last_launch gives by the form it took the place of: "rows", "flat" (planes whose rows

@@ -122,6 +122,40 @@ def test_cache_write_and_read(ops, device, kind, dtype, tokens, heads, dim, page
         assert torch.equal(got.cpu(), want.float().to(dtype))                          # one rounding of a float32 product
 
 
+@pytest.mark.parametrize("kind,dim", [(INT8, 64), (E4M3, 128), (INT8, 192)])
+def test_writes_of_runs_that_begin_anywhere(ops, device, kind, dim):
+    """Stretches of all lengths that begin at any place of four, in any order, some slots outside, over the edges of workgroups."""
+    g = gen(dim)
+    page, pages, heads = 16, 40, 3
+    left, slots = list(range(pages * page)), []
+    while len(left) > 60:
+        n, at = int(torch.randint(1, 24, (1,), generator=g)), int(torch.randint(0, len(left), (1,), generator=g))
+        slots += left[at:at + n]                                                    # (with gaps where something has been taken out)
+        del left[at:at + n]
+        if n % 5 == 0:
+            slots += [-1, pages * page + n, -4, -3, -2, -1][:n % 7]
+    slots = torch.tensor(slots, dtype=torch.int32)
+    tokens, there = len(slots), (slots >= 0) & (slots < pages * page)
+    cache = ops.KvCache.allocate(pages, heads, page, dim, codes=kind, device=device)
+    for t in (cache.k, cache.v):
+        t.view(torch.int8).fill_(0x55)
+    for t in (cache.k_scale, cache.v_scale):
+        t.fill_(-7.0)
+    x = torch.randn((2, tokens, heads, dim), generator=g).to(BF16)
+    ops.kv_write(cache, x[0].to(device), x[1].to(device), slots.to(device))
+    have = ref.Slots.of(cache)
+    untouched = torch.ones(pages * page, dtype=torch.bool)
+    untouched[slots[there].long()] = False
+    for codes, scale, rows in ((have.k, have.ks, x[0]), (have.v, have.vs, x[1])):
+        want, want_scale = ref.quantise(rows[there], kind)
+        assert torch.equal(scale[slots[there].long()], want_scale)
+        assert torch.equal(ref.values_of(codes[slots[there].long()], kind, want_scale), ref.values_of(want, kind, want_scale))
+        assert (codes[untouched] == 0x55).all() and (scale[untouched] == -7.0).all()
+    k, v = ops.kv_read(cache, slots.to(device))
+    for got, want in ((k, have.keys), (v, have.values)):
+        assert torch.equal(got.cpu()[there], want(slots[there].long()).float().to(BF16)) and (got.cpu()[~there] == 0).all()
+
+
 @pytest.mark.parametrize("kind", [INT8, E4M3])
 def test_rows_with_infinities_slots_outside_and_strides(ops, device, kind):
     g = gen(1)
@@ -175,7 +209,7 @@ def tree_mask(new, words, g):
     return torch.tensor(rows, dtype=torch.int64).view(-1, words)
 
 
-def run_attention(ops, device, *, context, new, hq, hkv, dim, page, kind, dtype, mask=None, scale=None, q=None, slots=None, seed=0, poison=True, table=None, **more):
+def run_attention(ops, device, *, context, new, hq, hkv, dim, page, kind, dtype, mask=None, scale=None, q=None, slots=None, seed=0, poison=True, table=None, said=None, **more):
     g = gen(seed)
     lengths = [c + n for c, n in zip(context, new)]
     if table is None:
@@ -196,7 +230,9 @@ def run_attention(ops, device, *, context, new, hq, hkv, dim, page, kind, dtype,
     cache = ops.KvCache(*slots.tensors(page, device))
     lse = torch.full((sum(new), hq), 5.0, dtype=torch.float32, device=device)
     context = torch.tensor(context, dtype=torch.int32)
-    out = ops.tree_attention(q.to(device), cache, table.to(device), context.to(device), q_start.to(device), max_new=max(new), max_context=int(context.max()),
+    if said is not None:                                                           # the longest context there might be
+        table = torch.nn.functional.pad(table, (0, -(-(said + max(new)) // page) - table.shape[1]), value=-1)
+    out = ops.tree_attention(q.to(device), cache, table.to(device), context.to(device), q_start.to(device), max_new=max(new), max_context=int(context.max()) if said is None else said,
                              mask=None if mask is None else mask.to(device), scale=scale, lse=lse, **more)
     want, bound, want_lse = ref.attention(q, slots, page, table, context, q_start, mask, dim ** -0.5 if scale is None else scale, dtype)
     ref.check(out, want, bound, "out")
@@ -302,6 +338,30 @@ def test_long_contexts_are_shared_out(ops, device, kind, dim, new):
     """One long and some short sequences: the long one's keys go to many workgroups, whose parts are joined."""
     out = run_attention(ops, device, context=[5003, 0, 40, 1999], new=[new, 1, new, 1], hq=6, hkv=2, dim=dim, page=64, kind=kind, dtype=F16, seed=dim + new)
     assert out.isfinite().all()
+
+
+def ragged(n, top, g):
+    return [int(x) for x in torch.randint(0, top, (n,), generator=g)]
+
+
+@pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, BF16), (INT8, F16), (E4M3, F16)])
+@pytest.mark.parametrize("form,dim,batch,new,hq,hkv,said,shared", [
+    ("1x8", 128, 7, 3, 4, 2, None, False), ("1x4", 64, 150, 2, 4, 2, None, False), ("2x4", 128, 130, 9, 6, 2, None, False), ("4x4", 64, 65, 64, 8, 8, None, False),
+    ("4x4", 128, 33, 64, 16, 16, None, False), ("1x4", 128, 40, 5, 2, 1, 20000, True), ("1x4", 256, 30, 4, 6, 2, 30000, True), ("2x4", 64, 19, 9, 6, 2, 9000, True),
+    ("2x4", 256, 9, 8, 8, 2, 70000, True), ("2x4", 192, 150, 20, 2, 2, None, False), ("4x4", 128, 11, 33, 6, 3, 20000, True), ("4x4", 96, 9, 50, 4, 2, 70000, True),
+    ("4x4", 64, 70, 40, 8, 4, 4000, True)])
+def test_every_form(ops, device, kind, dtype, form, dim, batch, new, hq, hkv, said, shared):
+    """The tiles and waves of a workgroup, and shares or none, that sizes lead to: with sequences of all lengths, some without new tokens."""
+    import fusedkernellibrary_amd as fkl
+    g = gen(batch)
+    some = ragged(batch, new + 1, g)
+    some[batch // 2] = new
+    context = ragged(batch, 200, g)
+    run_attention(ops, device, context=context, new=some, hq=hq, hkv=hkv, dim=dim, page=16, kind=kind, dtype=dtype, seed=batch, said=said,
+                  mask=tree_mask(some, 1, g) if new > 1 else None)
+    last = fkl.last_launch()
+    assert last["form"] == "tree_attention_" + form
+    assert (last["grid"][1:] == [1, 1] and last["grid"][0] >= 64) if shared else last["grid"][2] == batch
 
 
 def test_results_do_not_change_from_call_to_call(ops, device):
@@ -444,4 +504,4 @@ def test_last_launch_names_the_kernels(ops, device):
     ops.kv_read(cache, ints(0))
     assert fkl.last_launch()["form"] == "kv_read"
     ops.tree_attention(x, cache, ints(0, 1).view(1, 2), ints(0), ints(0, 1), max_new=1, max_context=0)
-    assert fkl.last_launch()["form"] == "tree_attention"
+    assert fkl.last_launch()["form"] == "tree_attention_1x8"
