@@ -651,11 +651,17 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         // Scales of several tiles' steps are used again and again, and would take 16 registers: those go to LDS, two of the keys' and
         // two of the values' blocks of 16 side by side, for this step and the next.
         const uint32_t scales_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float*)&scales[wave][0][0])));
-        auto load_scales_and_v = [&](uint32_t step) {
+        auto copy_scales = [&](uint32_t step) {
             if constexpr (kInLds) {
-                const float* from = (lane < 32 ? a.cache.k_scale : a.cache.v_scale) + at[lane >> 4 & 1] + col;
+                Args& b = kernel_args();
+                const uint32_t l = thread_here();
+                const size_t first = at[0], second = at[1];
+                const float* from = (l & 32 ? b.cache.v_scale : b.cache.k_scale) + (l & 16 ? second : first) + (l & 15);
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(scales_at + (step & 1) * 256), "v"(from) : "memory", "m0");
-            } else {
+            }
+        };
+        auto load_scales_and_v = [&] {
+            if constexpr (!kInLds) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     k_scales[h] = load_at<float4_t>(of_wave(a.cache.k_scale + at[h]), quarter * 16);
@@ -673,8 +679,13 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         if (key < x.key1) {
             pages.fetch(a, x, key >> a.cache.page_log, lane);
             locate(key);
+            // (in the order of the steps to come: a first step that had asked for values first would have every step wait for its values)
+            __builtin_amdgcn_sched_barrier(0);
+            copy_scales(0);
             load_k();
-            load_scales_and_v(0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_scales_and_v();
+            __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t q[kRegs];
         float unit = 0.0f;
@@ -706,8 +717,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 vs[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][step & 1][32 + h * 16 + quarter * 4]) : v_scales[h];
             }
         };
+        // (from the thread's number anew, and so in the next: what both compute would be kept in registers through the loop)
         auto sees = [&](int r, int h) {
             Args& b = kernel_args();
+            const uint32_t t = thread_here(), col = t & 15, quarter = t >> 4 & 3;
             const uint32_t first = key + h * 16 + quarter * 4, there = lowest_bits(int32_t(x.seq.total - first));
             const int32_t u = int32_t(first - x.seq.context);
             const uint32_t token = place_of_row(b, x, r * 16 + col).token;
@@ -717,6 +730,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         };
         // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
         auto hide = [&] {
+            const uint32_t quarter = thread_here() >> 4 & 3;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t there = lowest_bits(int32_t(x.seq.total - (key + h * 16 + quarter * 4)));
@@ -729,23 +743,27 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                     for (int w = 0; w < S::kWords; ++w) v[h][i].w[w] &= keep;
             }
         };
-#pragma unroll 1
-        while (key < x.key1) {
+        // One step; `more` is known where this is compiled, as the compiler would otherwise count on values that were not asked for
+        // behind keys that were, and wait for both.
+        auto run_step = [&](auto more) {
             const uint32_t next = key + WAVES * 32;
-            const bool more = next < x.key1;
             set_priority(x, key);
-            if (more) locate(next);
-            if constexpr (kInLds) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * S::kLoads) : "memory");    // (the scales: only values have been asked for since)
+            if constexpr (more()) locate(next);
+            if constexpr (kInLds) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * S::kLoads) : "memory");    // (the scales: only keys and values have been asked for since)
             // the keys' registers are free for the next once the scores are there, the others' at the end
             sums.step(key + 32 > x.all_see, get_k, get_v, get_q, get_unit, get_scales, sees, hide, [&] {
-                if (more) load_k();
+                if constexpr (more()) copy_scales(step + 1);
+                if constexpr (more()) load_k();
                 __builtin_amdgcn_sched_barrier(0);
             });
-            if (more) load_scales_and_v(step + 1);
+            if constexpr (more()) load_scales_and_v();
             __builtin_amdgcn_sched_barrier(0);
             key = next;
             ++step;
-        }
+        };
+#pragma unroll 1
+        while (key + WAVES * 32 < x.key1) run_step(std::true_type{});
+        if (key < x.key1) run_step(std::false_type{});
         join_waves<WAVES>(x, sums, space, joined_m, joined_l);
     });
 }
