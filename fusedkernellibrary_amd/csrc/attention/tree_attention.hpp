@@ -381,14 +381,21 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         float4_t y[2], next[2];
         // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of three parts of int8 take
         // all registers without that.)
+        constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * (CODES == FKLHIP_CODES_INT8 ? S::kLoads : S::kLoads / 2);
         constexpr bool kAhead = !(R == 4 && PARTS == 3 && CODES == FKLHIP_CODES_INT8);
+        constexpr bool kHeld = R < 4 || kRuns <= 4;
+        uint4_t q[kRuns];
+        auto ask_q = [&](int r) {
+#pragma unroll
+            for (int run = 0; run < kRuns; ++run) q[run] = get_q(r, run);
+        };
         if (kAhead) products(get_k, [&](int run) { return get_q(0, run); }, y);
         if (R == 1) after_scores();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (!kAhead) products(get_k, [&](int run) { return get_q(r, run); }, y);
-            else if (r + 1 < R) products(get_k, [&](int run) { return get_q(r + 1, run); }, next);
-            if (kAhead ? r + 2 == R : r + 1 == R) after_scores();
+            if (!kAhead && r + 1 == R) after_scores();
+            if (kAhead && kHeld && r + 1 < R) ask_q(r + 1);
             const float unit = get_unit(r);
             float4_t ks[2], vs[2];
             get_scales(ks, vs);
@@ -405,6 +412,7 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
                     }
                 }
             }
+            if (kAhead && r + 1 < R) products(get_k, [&](int run) { return kHeld ? q[run] : get_q(r + 1, run); }, next);
             // Weights, and a look at whether the reference has to move: where a weight is too large for half precision.
             float w[2][4], sum = 0.0f, top = 0.0f;
             auto weigh = [&](int h, int i, float score) {
@@ -419,6 +427,15 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
                     weigh(h, i, __builtin_fmaf(y[h][i], unit, -m[r]));
                     top = __builtin_fmaxf(top, w[h][i]);
                 }
+            if constexpr (kAhead && R > 1 && PARTS > 0) {
+                // one product of the next tile, then a share of this one's weights, again and again
+#pragma unroll
+                for (int i = 0; i < kProducts; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 40 / kProducts, 0);
+                }
+            }
+            if (kAhead && r + 2 == R) after_scores();
             if (__builtin_expect(__any(top > kLargest || sum > kMostSum), 0)) {
                 // the largest weight there would be, in units of log2
                 top = -__builtin_inff();
