@@ -49,7 +49,7 @@ int check_cache(const fklhip_kv_cache* c) {
     NEED(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scale, 16) && aligned(c->v_scale, 16), "a cache's arrays have to start at multiples of 16 bytes");
     NEED(c->codes == FKLHIP_CODES_INT8 || c->codes == FKLHIP_CODES_E4M3, "codes have to be FKLHIP_CODES_INT8 or FKLHIP_CODES_E4M3");
     NEED(c->page_tokens >= 16 && c->page_tokens <= 256 && (c->page_tokens & (c->page_tokens - 1)) == 0, "page_tokens has to be 16, 32, 64, 128 or 256");
-    NEED(c->pages >= 1 && c->pages * c->page_tokens <= std::numeric_limits<int32_t>::max(), "a cache has 1 to 2^31 - 1 slots");
+    NEED(c->pages >= 1 && c->pages <= std::numeric_limits<int32_t>::max() && c->pages * c->page_tokens <= std::numeric_limits<int32_t>::max(), "a cache has 1 to 2^31 - 1 slots");
     NEED(c->kv_heads >= 1 && c->kv_heads <= 65535, "kv_heads has to be 1 to 65535");
     NEED(c->head_dim >= 8 && c->head_dim <= 256 && c->head_dim % 8 == 0, "head_dim has to be a multiple of 8 up to 256");
     return FKLHIP_OK;
@@ -78,6 +78,7 @@ int run_heads(const fklhip_heads* h, const fklhip_kv_cache* cache, void* stream)
     NEED(h->pairs == 0 || h->pairs == 1, "pairs has to be 0 or 1");
     NEED(!h->rot_dim || !h->tokens || (h->cos && h->sin && h->positions && h->table_rows >= 1), "rot_dim without tables or positions");
     NEED(!h->rot_dim || (aligned(h->cos, 16) && aligned(h->sin, 16)), "tables have to start at multiples of 16 bytes");
+    NEED(aligned(h->positions, 4) && aligned(h->slots, 4), "positions and slots have to be aligned");
     NEED(h->table_rows >= 0 && h->table_rows <= std::numeric_limits<int32_t>::max(), "a table has up to 2^31 - 1 rows");
     NEED((h->q_weight == nullptr) == (h->k_weight == nullptr), "weights for both of q and k, or for none");
     NEED(!h->q_weight || (aligned(h->q_weight, 8) && aligned(h->k_weight, 8)), "weights have to start at multiples of 8 bytes");
@@ -124,7 +125,7 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, Attention
     const int64_t group = c->q_heads / cache->kv_heads;
     NEED(c->max_new * group * group < (int64_t(1) << 32) && c->max_new * group <= (int64_t(1) << 20), "more than 2^20 query rows to a key head");
     NEED(c->tokens * c->q_heads < (int64_t(1) << 31), "more than 2^31 - 1 query rows");
-    NEED(c->page_table_stride >= 0, "a negative page_table_stride");
+    NEED(c->page_table_stride >= 0 && c->page_table_stride <= std::numeric_limits<int32_t>::max(), "page_table_stride has to be 0 to 2^31 - 1");
     const uint32_t keys = uint32_t(std::min<int64_t>(int64_t(c->max_context) + c->max_new, c->page_table_stride * cache->page_tokens));
     plan = plan_attention(uint32_t(c->batch), uint32_t(cache->kv_heads), uint32_t(c->max_new * group), keys, uint32_t(cache->head_dim));
     return FKLHIP_OK;
@@ -157,6 +158,7 @@ int fklhip_kv_write(const fklhip_kv_cache* cache, const fklhip_rows* k, const fk
     CHECK(check_count(tokens));
     if (tokens == 0) return FKLHIP_OK;
     NEED(k && v && slots, "no rows or no slots");
+    NEED(aligned(slots, 4), "slots have to be aligned");
     CHECK(check_rows(*k, tokens, cache->kv_heads));
     CHECK(check_rows(*v, tokens, cache->kv_heads));
     HeadArgs a{};
@@ -172,6 +174,7 @@ int fklhip_kv_read(const fklhip_kv_cache* cache, const int32_t* slots, int64_t t
     CHECK(check_count(tokens));
     if (tokens == 0) return FKLHIP_OK;
     NEED(k && v && slots, "no rows or no slots");
+    NEED(aligned(slots, 4), "slots have to be aligned");
     CHECK(check_rows(*k, tokens, cache->kv_heads));
     CHECK(check_rows(*v, tokens, cache->kv_heads));
     ReadArgs a{to_cache(*cache), to_rows(*k), to_rows(*v), slots, uint32_t(tokens), uint32_t(cache->head_dim), 0};
@@ -196,6 +199,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     CHECK(check_rows(c->out, c->tokens, c->q_heads));
     NEED(c->context && c->q_start, "no context or no q_start");
     NEED(c->page_table || c->page_table_stride == 0, "no page_table");
+    NEED(aligned(c->context, 4) && aligned(c->q_start, 4) && aligned(c->page_table, 4) && aligned(c->lse, 4) && aligned(c->mask, 8), "lengths, page_table, lse and mask have to be aligned");
     NEED(!c->mask || (c->mask_words >= 1 && int64_t(c->mask_words) * 64 >= c->max_new), "mask_words has to be max_new / 64, rounded up, or more");
     const uint64_t bytes = workspace_of(*cache, plan);
     NEED(bytes == 0 || (c->workspace && c->workspace_bytes >= bytes), "the workspace is smaller than fklhip_tree_attention_workspace says");

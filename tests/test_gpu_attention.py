@@ -505,3 +505,97 @@ def test_last_launch_names_the_kernels(ops, device):
     assert fkl.last_launch()["form"] == "kv_read"
     ops.tree_attention(x, cache, ints(0, 1).view(1, 2), ints(0), ints(0, 1), max_new=1, max_context=0)
     assert fkl.last_launch()["form"] == "tree_attention_1x8"
+
+
+# ---- the step from C++, the example, refusals -------------------------------------------------------------------------
+
+def test_a_step_through_the_host_api(ops, device):
+    """The same kernels on the same inputs from the C++ host API: the same bits. Long contexts make its workspace grow."""
+    import ctypes as C
+    import os
+    import fusedkernellibrary_amd as fkl
+    fkl.lib()
+    step = C.CDLL(os.path.join(os.path.dirname(os.path.abspath(__file__)), "cases", "libattention_step.so"))
+    step.attention_step_error.restype = C.c_char_p
+    p, i64, i32 = C.c_void_p, C.c_int64, C.c_int32
+    step.attention_step_open.argtypes = [i64, i32, i32, i32, i32, C.POINTER(p)]
+    step.attention_step_close.argtypes = [p]
+    step.attention_step_run.argtypes = [p] * 9 + [i64] + [p] * 3 + [i64, p, p, i32, i64] + [i32] * 4 + [p]
+    server = p()
+    assert step.attention_step_open(0, 2, 16, 64, 0, C.byref(server)) == 2                      # no pages
+    hq, hkv, dim, page, entries = 8, 2, 64, 16, 400
+    assert step.attention_step_open(2 * entries, hkv, page, dim, 0, C.byref(server)) == 0, step.attention_step_error()
+    try:
+        g = gen(8)
+        cache = ops.KvCache.allocate(2 * entries, hkv, page, dim, device=device)
+        table = torch.randperm(2 * entries, generator=g).to(torch.int32).view(2, entries)
+        wq, wk = ((1 + 0.2 * torch.randn(dim, generator=g)).to(BF16).to(device) for _ in range(2))
+        cos, sin = (t.to(device) for t in tables(entries * page, dim))
+        ints = lambda v: torch.tensor(v, dtype=torch.int32, device=device)      # noqa: E731
+        on = table.to(device)
+        for context, new in (([0, 0], [5000, 70]), ([5000, 70], [1, 3])):
+            tokens = sum(new)
+            packed = torch.randn((tokens, hq + 2 * hkv, dim), generator=g).to(BF16).to(device)
+            of = torch.repeat_interleave(torch.arange(2), torch.tensor(new)).to(device)
+            start, have = ints([0, new[0], tokens]), ints(context)
+            j = have[of] + torch.arange(tokens, device=device) - start[of]
+            slots = (on[of, j.long() // page] * page + j % page).to(torch.int32)
+            positions = j.to(torch.int32)
+            again = packed.clone()
+            out, k_out, v_out = torch.empty_like(packed[:, :hq]).contiguous(), *(torch.empty((tokens, hkv, dim), dtype=BF16, device=device) for _ in range(2))
+            q = ops.qkv_to_cache(cache, packed[:, :hq], packed[:, hq:hq + hkv], packed[:, hq + hkv:], slots, wq, wk, cos, sin, positions)
+            want = ops.tree_attention(q, cache, on, have, start, max_new=max(new), max_context=max(context))
+            want_k, want_v = ops.kv_read(cache, slots)
+            rc = step.attention_step_run(server, again.data_ptr(), out.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                                         entries * page, positions.data_ptr(), slots.data_ptr(), on.data_ptr(), entries, have.data_ptr(), start.data_ptr(), 2, tokens, hq, max(new),
+                                         max(context), 0, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, step.attention_step_error()
+            torch.cuda.synchronize()
+            for got, expected in ((again[:, :hq], q), (out, want), (k_out, want_k), (v_out, want_v)):
+                assert torch.equal(got, expected)
+    finally:
+        torch.cuda.synchronize()
+        step.attention_step_close(server)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,codes", [(32, 8, 128, INT8), (6, 2, 64, E4M3)])
+def test_drafts_verified_as_trees_and_one_by_one(ops, device, heads, kv_heads, dim, codes):
+    """The example: both ways round a result (2^-8 of it) and their weights (2^-11 of the values) by themselves."""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("verify_drafts", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "verify_drafts.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    difference, largest = example.main(heads=heads, kv_heads=kv_heads, dim=dim, codes=codes)
+    assert 0 < largest and difference <= 2 * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -12) * largest
+
+
+def test_bindings_refuse_what_does_not_fit(ops, device):
+    cache = ops.KvCache.allocate(4, 2, 16, 64, device=device)
+    rows = lambda heads=4, tokens=3, dim=64, dtype=BF16, where=device: torch.zeros((tokens, heads, dim), dtype=dtype, device=where)      # noqa: E731
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)      # noqa: E731
+    table, lengths, start = ints(0, 1).view(1, 2), ints(4), ints(0, 3)
+    call = lambda **c: ops.tree_attention(**{**dict(q=rows(), cache=cache, page_table=table, context=lengths, q_start=start, max_new=3, max_context=4), **c})      # noqa: E731
+    call()
+    for change, word in ((dict(q=rows(dim=128)), "different sizes"), (dict(q=rows(dtype=torch.float32)), "bfloat16"), (dict(q=rows(where="cpu")), "device"), (dict(q=rows(heads=3)), "multiple of kv_heads"),
+                         (dict(page_table=table.long()), "page_table"), (dict(page_table=table[0]), "page_table"), (dict(context=ints(4, 4)), "context"), (dict(q_start=ints(0)), "q_start"),
+                         (dict(mask=torch.zeros((2, 1), dtype=torch.int64, device=device)), "mask"), (dict(mask=torch.zeros((3, 1), dtype=torch.int32, device=device)), "mask"),
+                         (dict(mask=torch.zeros((3, 0), dtype=torch.int64, device=device)), "word"), (dict(out=rows(heads=5)), "out"), (dict(lse=torch.zeros((3, 4), device=device).half()), "lse"),
+                         (dict(max_new=1 << 40), "max_new"), (dict(max_new=-1), "max_new"), (dict(q=rows().transpose(1, 2).contiguous().transpose(1, 2)), "tight"),
+                         (dict(q=rows().requires_grad_()), "gradient"), (dict(scale=float("inf")), "finite")):
+        with pytest.raises(ValueError, match=word):
+            call(**change)
+    with torch.no_grad():
+        call(q=rows().requires_grad_())
+    x, slots = rows(heads=2), ints(0, 1, 2)
+    for f, word in ((lambda: ops.kv_write(cache, x, x, slots[:2]), "slots"), (lambda: ops.kv_write(cache, x, rows(heads=3), slots), "v has to be"), (lambda: ops.kv_write(cache, x, x.half(), slots), "v has to be"),
+                    (lambda: ops.kv_read(cache, slots, dtype=torch.float32), "dtype"), (lambda: ops.kv_read(cache, slots.view(1, 3)), "one dimension"), (lambda: ops.kv_read(cache, slots, k_out=x.half()), "type"),
+                    (lambda: ops.qk_norm_rope(rows(), x, None, None, torch.zeros((9, 32), device=device), None, slots), "neither"),
+                    (lambda: ops.qk_norm_rope(rows(), x, torch.ones(64, device=device), torch.ones(64, device=device), None, None, None), "q_weight"),
+                    (lambda: ops.qkv_to_cache(cache, rows(heads=3), rows(heads=3), rows(heads=3), slots, None, None, None, None, None), "other heads"),
+                    (lambda: ops.KvCache(cache.k, cache.k, cache.k_scale, cache.v_scale), "v has to be"), (lambda: ops.KvCache(cache.k, cache.v, cache.k_scale.half(), cache.v_scale), "k_scale"),
+                    (lambda: ops.KvCache.allocate(4, 2, 24, 64, device=device) and ops.kv_write(ops.KvCache.allocate(4, 2, 24, 64, device=device), x, x, slots), "page_tokens")):
+        with pytest.raises(ValueError, match=word):
+            f()
+    with pytest.raises(ValueError, match="16 bytes"):
+        call(q=torch.zeros(3 * 4 * 64 + 1, dtype=BF16, device=device)[1:].view(3, 4, 64))
