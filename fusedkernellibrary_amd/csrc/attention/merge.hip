@@ -12,15 +12,8 @@ constexpr uint32_t kThreads = 256, kMostParts = 1025;         // (a row's parts 
 template <int D> struct Lanes { static constexpr uint32_t kRow = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = kThreads / kRow; };
 
 // The sequence of a token, with the granules in front of it.
-struct TokenOf { Sequence s; Found f; };
-__device__ __forceinline__ TokenOf sequence_of_token(Args& a, uint32_t token) {
-    TokenOf x;
-    x.f = find(a, threadIdx.x & 63, [&](uint32_t, uint32_t b, uint32_t, uint32_t) {
-        const Sequence s = sequence_of_lane(a, b);
-        return token >= s.first_token && token - s.first_token < s.fresh;
-    });
-    if (x.f.b < a.batch) x.s = sequence_at(a, x.f.b);
-    return x;
+__device__ __forceinline__ Found sequence_of_token(Args& a, uint32_t token) {
+    return find(a, threadIdx.x & 63, [&](uint32_t, const Sequence& s, uint32_t, uint32_t) { return token >= s.first_token && token - s.first_token < s.fresh; });
 }
 // A row's parts: those of shares share0 .. share0 + count. None: nobody had any of it. One: it has been written.
 struct Parts {
@@ -31,14 +24,14 @@ struct Parts {
         return share_begin(a, all, share0 + part) == share_begin(a, all, share0 + part + 1) ? -__builtin_inff() : a.partial_lse[place(a, part)];
     }
 };
-__device__ __forceinline__ Parts parts_of(Args& a, const TokenOf& x, uint32_t token, uint32_t head) {
-    const uint32_t n = granules_of(a, x.s);
-    const uint32_t kv_head = divide(head, a.group_magic), row = (token - x.s.first_token) * a.group + head - kv_head * a.group;
+__device__ __forceinline__ Parts parts_of(Args& a, const Found& f, uint32_t token, uint32_t head) {
+    const uint32_t n = granules_of(a, f.s);
+    const uint32_t kv_head = divide(head, a.group_magic), row = (token - f.s.first_token) * a.group + head - kv_head * a.group;
     const uint32_t block = row >> __builtin_ctz(a.unit_rows);
     if (n == 0) return {0, 0, 0};
-    const uint32_t first = x.f.before + (kv_head * blocks_of(a, x.s) + block) * n;
-    const uint32_t share0 = share_of(a, x.f.all, first);
-    return {share0, share_of(a, x.f.all, first + n - 1) - share0 + 1, row - block * a.unit_rows};
+    const uint32_t first = f.before + (kv_head * blocks_of(a, f.s) + block) * n;
+    const uint32_t share0 = share_of(a, f.all, first);
+    return {share0, share_of(a, f.all, first + n - 1) - share0 + 1, row - block * a.unit_rows};
 }
 // Four elements of a row, and its lse (in units of log2).
 __device__ __forceinline__ void put4(Args& a, uint32_t token, uint32_t head, uint32_t d, float4_t x) {
@@ -57,14 +50,14 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const A
     const uint32_t at = threadIdx.x % kLanes, head = blockIdx.x * Lanes<D>::kGroups + threadIdx.x / kLanes, d = at * 4;
     const uint32_t token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
-    const TokenOf x = sequence_of_token(a, token);
-    if (x.f.b >= a.batch || head >= a.q_heads) return;        // a row of no sequence, or none
-    const Parts p = parts_of(a, x, token, head);
+    const Found f = sequence_of_token(a, token);
+    if (f.b >= a.batch || head >= a.q_heads) return;          // a row of no sequence, or none
+    const Parts p = parts_of(a, f, token, head);
     if (p.count == 1) return;
     float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
     float top = -__builtin_inff(), sum = 0.0f;
     for (uint32_t i0 = 0; i0 < p.count; i0 += kLanes) {
-        const float mine = i0 + at < p.count ? p.lse(a, x.f.all, i0 + at) : -__builtin_inff();
+        const float mine = i0 + at < p.count ? p.lse(a, f.all, i0 + at) : -__builtin_inff();
         float most = mine;
 #pragma unroll
         for (uint32_t i = kLanes / 2; i; i >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, i, kLanes));
@@ -95,13 +88,13 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = at * 4;
     const uint32_t head = blockIdx.x, token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
-    const TokenOf t = sequence_of_token(a, token);
-    if (t.f.b >= a.batch) return;
-    const Parts p = parts_of(a, t, token, head);
+    const Found f = sequence_of_token(a, token);
+    if (f.b >= a.batch) return;
+    const Parts p = parts_of(a, f, token, head);
     if (p.count == 1) return;
     float top = -__builtin_inff();
     for (uint32_t i = threadIdx.x; i < p.count; i += kThreads) {
-        const float x = p.lse(a, t.f.all, i);
+        const float x = p.lse(a, f.all, i);
         weight[i] = x;
         top = __builtin_fmaxf(top, x);
     }

@@ -140,26 +140,29 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
     // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
     uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
     const bool shared = a.share_odd != 0;
+    Sequence s;
     if (shared) {
         const uint32_t share = own_share(a);
-        const Found f = find(a, lane, [&](uint32_t all, uint32_t, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
+        const Found f = find(a, lane, [&](uint32_t all, const Sequence&, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
         at = share_begin(a, f.all, share);
         end = share_begin(a, f.all, share + 1);
         b = f.b;
         in = at - f.before;
+        s = f.s;
+    } else {
+        s = sequence_at(a, b);
     }
     uint32_t whole = end - at;
     while (at < end && b < kernel_args().batch) {
         Args& a = kernel_args();
-        const Sequence s = sequence_at(a, b);
         const uint32_t n = granules_of(a, s), blocks = blocks_of(a, s);
         uint32_t head = blockIdx.x, block = blockIdx.y, g = 0, count = n;
         int part = -1;
         if (shared) {
             const uint32_t unit = n ? in / n : 0;
             if (unit >= blocks * a.cache.kv_heads || n == 0) {
-                ++b;
                 in = 0;
+                if (++b < a.batch) s = sequence_at(a, b);
                 continue;
             }
             head = unit / blocks;
@@ -184,6 +187,7 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         if (!shared) return;
         at = __builtin_amdgcn_readfirstlane(kept[0]); in = __builtin_amdgcn_readfirstlane(kept[1]); end = __builtin_amdgcn_readfirstlane(kept[2]);
         b = __builtin_amdgcn_readfirstlane(kept[3]); whole = __builtin_amdgcn_readfirstlane(kept[4]);
+        s = sequence_at(kernel_args(), b);
     }
 }
 

@@ -55,34 +55,44 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t v) {
     return add_dpp<0x143, 0xc>(v);                            // row_bcast 31: the upper half gets the lower
 }
 
-// (of the lane's own sequence)
-__device__ __forceinline__ Sequence sequence_of_lane(Args& a, uint32_t b) { return sequence_of(a, a.q_start[b], a.q_start[b + 1], a.context[b]); }
-__device__ __forceinline__ uint32_t weigh(Args& a, uint32_t b) { return b < a.batch ? weight_of(a, sequence_of_lane(a, b)) : 0u; }
-// The granules of all sequences, and the first of a sequence: that of granule at(all), or that of a token.
-struct Found { uint32_t all, b, before; };
+// (of the lane's own sequence; behind the last there are empty ones)
+__device__ __forceinline__ Sequence sequence_of_lane(Args& a, uint32_t b) {
+    return b < a.batch ? sequence_of(a, a.q_start[b], a.q_start[b + 1], a.context[b]) : Sequence{0, 0, 0, 0, 0};
+}
+__device__ __forceinline__ Sequence of_lane(const Sequence& s, uint32_t lane) {
+    const auto get = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), int(lane))); };
+    return {get(s.first_token), get(s.fresh), get(s.context), get(s.total), get(s.rows)};
+}
+// The granules of all sequences, and the first of a sequence: that of granule at(all), or that of a token; is_it(all, the lane's
+// sequence, its first granule, the one behind its last). b is the batch's size if there is none.
+struct Found { uint32_t all, b, before; Sequence s; };
 template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t lane, F is_it) {
     uint32_t before = 0;
-    Found f{0, a.batch, 0};
+    Found f{0, a.batch, 0, {0, 0, 0, 0, 0}};
     if (a.batch <= 64) {
-        const uint32_t own = weigh(a, lane), upto = scan_wave(own);
+        const Sequence s = sequence_of_lane(a, lane);
+        const uint32_t own = weight_of(a, s), upto = scan_wave(own);
         f.all = __builtin_amdgcn_readlane(int(upto), 63);
-        const uint64_t hits = __ballot(lane < a.batch && is_it(f.all, lane, upto - own, upto));
+        const uint64_t hits = __ballot(lane < a.batch && is_it(f.all, s, upto - own, upto));
         if (hits) {
             f.b = __builtin_ctzll(hits);
             f.before = __builtin_amdgcn_readlane(int(upto - own), int(f.b));
+            f.s = of_lane(s, f.b);
         }
         return f;
     }
     uint32_t sum = 0;
-    for (uint32_t b = lane; b < a.batch; b += 64) sum += weigh(a, b);
+    for (uint32_t b = lane; b < a.batch; b += 64) sum += weight_of(a, sequence_of_lane(a, b));
     f.all = __builtin_amdgcn_readlane(int(scan_wave(sum)), 63);
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint32_t own = weigh(a, b0 + lane), upto = before + scan_wave(own);
-        const uint64_t hits = __ballot(b0 + lane < a.batch && is_it(f.all, b0 + lane, upto - own, upto));
+        const Sequence s = sequence_of_lane(a, b0 + lane);
+        const uint32_t own = weight_of(a, s), upto = before + scan_wave(own);
+        const uint64_t hits = __ballot(b0 + lane < a.batch && is_it(f.all, s, upto - own, upto));
         if (hits) {
             const int hit = __builtin_ctzll(hits);
             f.b = b0 + hit;
             f.before = __builtin_amdgcn_readlane(int(upto - own), hit);
+            f.s = of_lane(s, hit);
             return f;
         }
         before = __builtin_amdgcn_readlane(int(upto), 63);
