@@ -44,6 +44,16 @@ __device__ __forceinline__ void put_lse(Args& a, uint32_t token, uint32_t head, 
     if (a.lse) a.lse[size_t(token) * a.q_heads + head] = lse * 0.6931471805599453f;
 }
 
+// Four elements of a part, weighted. A part without weight may hold anything; it is read all the same, as a branch around each
+// would have the parts come one after another.
+__device__ __forceinline__ float4_t part4(const float* from, float w) {
+    const float4_t x = *reinterpret_cast<const float4_t*>(from);
+    float4_t y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = w != 0.0f ? x[i] * w : 0.0f;
+    return y;
+}
+
 template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const AttentionArgs) {
     constexpr uint32_t kLanes = Lanes<D>::kRow;
     Args& a = kernel_args();
@@ -72,8 +82,8 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const A
         const uint32_t count = min(kLanes, p.count - i0);
 #pragma unroll 4
         for (uint32_t i = 0; i < count; ++i) {
-            const float w = __shfl(weight, i, kLanes);
-            if (d < D && w != 0.0f) o += *reinterpret_cast<const float4_t*>(a.partial + p.place(a, i0 + i) * D + d) * w;
+            const float w = __shfl(weight, i, kLanes);        // (of all lanes: those behind the row have weights too)
+            if (d < D) o += part4(a.partial + p.place(a, i0 + i) * D + d, w);
         }
     }
     if (d < D) put4(a, token, head, d, o * (sum == 0.0f ? 0.0f : 1.0f / sum));
@@ -117,11 +127,8 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     sum = sums[0] + sums[1] + sums[2] + sums[3];
     float4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
     if (d < D) {
-#pragma unroll 4
-        for (uint32_t i = group; i < p.count; i += kGroups) {
-            const float w = weight[i];
-            if (w != 0.0f) x += *reinterpret_cast<const float4_t*>(a.partial + p.place(a, i) * D + d) * w;
-        }
+#pragma unroll 8
+        for (uint32_t i = group; i < p.count; i += kGroups) x += part4(a.partial + p.place(a, i) * D + d, weight[i]);
         *reinterpret_cast<float4_t*>(&joined[group][d]) = x;
     }
     __syncthreads();
