@@ -3,7 +3,10 @@
 //
 // All are bound by memory (a head of 128 elements is 256 bytes in and 256 or 132 out for some 20 operations per element),
 // so what counts is that every access is wide, that all of a lane's rows are requested before the first is used, and
-// that one launch does everything a token needs.
+// that one launch does everything a token needs. A copy of 1 GiB runs at 5.1 TB/s here. Norm and rotation of 4099 tokens of 28 and 4
+// heads of 128 (71 MB) take 15.3 us, 4.7 TB/s; of 16384 tokens of 16 and 8 heads of 64 (105 MB) 21.8 us, 4.8 TB/s. 2048 tokens'
+// keys and values of 8 heads of 128 are written in 8.4 us (12.6 MB, a start and an end more than traffic), 30011 read back in
+// 30.7 us (186 MB, 6.1 TB/s). One token takes 3.3 us, which is a launch and three dependent trips to memory.
 #include "attention_device.hpp"
 
 namespace fkattn {
@@ -173,76 +176,74 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) w[k] = 1.0f;
     if (weights && p.live) { load4<TYPE>(weights, p.at[0], w); load4<TYPE>(weights, p.at[1], w + 4); }
-    {
-        const uint32_t token = tile * groups + group;
-        if (token >= a.tokens) return;
-        float x[HEADS][8];
-        const char* row = in.data + token * in.token_stride;
+    const uint32_t token = tile * groups + group;
+    if (token >= a.tokens) return;
+    float x[HEADS][8];
+    const char* row = in.data + token * in.token_stride;
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
+    for (int h = 0; h < HEADS; ++h) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[h][k] = 0.0f;
-            if (p.live && head0 + h < heads) {
-                load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[0], x[h]);
-                load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[1], x[h] + 4);
-            }
+        for (int k = 0; k < 8; ++k) x[h][k] = 0.0f;
+        if (p.live && head0 + h < heads) {
+            load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[0], x[h]);
+            load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[1], x[h] + 4);
         }
-        float4_t cosine = {1.0f, 1.0f, 1.0f, 1.0f}, sine = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float4_t cosine = {1.0f, 1.0f, 1.0f, 1.0f}, sine = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.rotated) {
+        const uint32_t position = uint32_t(a.positions[token]);
+        if (position < a.table_rows) {
+            const size_t at = size_t(position) * (a.rot_dim / 2) + p.turn;
+            cosine = *reinterpret_cast<const float4_t*>(a.cos + at);
+            sine = *reinterpret_cast<const float4_t*>(a.sin + at);
+        } else {
+            cosine = sine = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        }
+    }
+    uint32_t page = 0, off = 0;
+    bool stored = false;
+    if (TO_CACHE && !is_q) stored = locate(a.cache, a.slots[token], page, off);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        if (head0 + h >= heads) break;
+        if (weights) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(x[h][k], x[h][k], sum);
+            const float r = 1.0f / __builtin_sqrtf(sum_lanes<LANES>(sum) / float(dim) + a.eps);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[h][k] = x[h][k] * r * w[k];
+        }
         if (p.rotated) {
-            const uint32_t position = uint32_t(a.positions[token]);
-            if (position < a.table_rows) {
-                const size_t at = size_t(position) * (a.rot_dim / 2) + p.turn;
-                cosine = *reinterpret_cast<const float4_t*>(a.cos + at);
-                sine = *reinterpret_cast<const float4_t*>(a.sin + at);
-            } else {
-                cosine = sine = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // pairs are (k, k + 4) of the lane's elements as halves, (2k, 2k + 1) as neighbours
+                float& u = a.pairs ? x[h][2 * k] : x[h][k];
+                float& v = a.pairs ? x[h][2 * k + 1] : x[h][k + 4];
+                const float s = u, t = v;
+                u = s * cosine[k] - t * sine[k];
+                v = t * cosine[k] + s * sine[k];
             }
         }
-        uint32_t page = 0, off = 0;
-        bool stored = false;
-        if (TO_CACHE && !is_q) stored = locate(a.cache, a.slots[token], page, off);
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            if (head0 + h >= heads) break;
-            if (weights) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(x[h][k], x[h][k], sum);
-                const float r = 1.0f / __builtin_sqrtf(sum_lanes<LANES>(sum) / float(dim) + a.eps);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[h][k] = x[h][k] * r * w[k];
+        if (is_q || !TO_CACHE) {
+            if (p.live) {
+                char* to = out.data + token * out.token_stride + (head0 + h) * out.head_stride;
+                store4<TYPE>(to, p.at[0], x[h]);
+                store4<TYPE>(to, p.at[1], x[h] + 4);
             }
-            if (p.rotated) {
+        } else {
+            uint32_t top = 0, code[2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // pairs are (k, k + 4) of the lane's elements as halves, (2k, 2k + 1) as neighbours
-                    float& u = a.pairs ? x[h][2 * k] : x[h][k];
-                    float& v = a.pairs ? x[h][2 * k + 1] : x[h][k + 4];
-                    const float s = u, t = v;
-                    u = s * cosine[k] - t * sine[k];
-                    v = t * cosine[k] + s * sine[k];
-                }
-            }
-            if (is_q || !TO_CACHE) {
+            for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[h][k]));
+            const float scale = scale_of<CODES>(max_lanes<LANES>(top));
+            encode8<CODES>(x[h], scale, code);
+            if (stored) {
+                const size_t at = head_row(a.cache, page, head0 + h) + off;
+                if (lane == 0) a.cache.k_scale[at] = scale;
                 if (p.live) {
-                    char* to = out.data + token * out.token_stride + (head0 + h) * out.head_stride;
-                    store4<TYPE>(to, p.at[0], x[h]);
-                    store4<TYPE>(to, p.at[1], x[h] + 4);
-                }
-            } else {
-                uint32_t top = 0, code[2];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[h][k]));
-                const float scale = scale_of<CODES>(max_lanes<LANES>(top));
-                encode8<CODES>(x[h], scale, code);
-                if (stored) {
-                    const size_t at = head_row(a.cache, page, head0 + h) + off;
-                    if (lane == 0) a.cache.k_scale[at] = scale;
-                    if (p.live) {
-                        char* to = a.cache.k + at * dim;
-                        *reinterpret_cast<uint32_t*>(to + p.at[0]) = code[0];
-                        *reinterpret_cast<uint32_t*>(to + p.at[1]) = code[1];
-                    }
+                    char* to = a.cache.k + at * dim;
+                    *reinterpret_cast<uint32_t*>(to + p.at[0]) = code[0];
+                    *reinterpret_cast<uint32_t*>(to + p.at[1]) = code[1];
                 }
             }
         }
@@ -256,80 +257,78 @@ __global__ __launch_bounds__(256) void k_read(const ReadArgs a) {
     const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES, at = lane * 8;
     const uint32_t dim = a.head_dim, heads = a.cache.kv_heads, tile = tile_of_grid();
     const bool values = blockIdx.x >= a.k_chunks;
-    {
-        if (!values) {
-            const uint32_t token = tile * groups + group, head0 = blockIdx.x * HEADS;
-            if (token >= a.tokens || at >= dim) return;
-            uint32_t page, off;
-            const bool there = locate(a.cache, a.slots[token], page, off);
-            uint2_t code[HEADS];
-            float scale[HEADS];
+    if (!values) {
+        const uint32_t token = tile * groups + group, head0 = blockIdx.x * HEADS;
+        if (token >= a.tokens || at >= dim) return;
+        uint32_t page, off;
+        const bool there = locate(a.cache, a.slots[token], page, off);
+        uint2_t code[HEADS];
+        float scale[HEADS];
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                code[h] = uint2_t{0, 0};
-                scale[h] = 0.0f;
-                if (there && head0 + h < heads) {
-                    const size_t row = head_row(a.cache, page, head0 + h) + off;
-                    code[h] = *reinterpret_cast<const uint2_t*>(a.cache.k + row * dim + at);
-                    scale[h] = a.cache.k_scale[row];
-                }
+        for (int h = 0; h < HEADS; ++h) {
+            code[h] = uint2_t{0, 0};
+            scale[h] = 0.0f;
+            if (there && head0 + h < heads) {
+                const size_t row = head_row(a.cache, page, head0 + h) + off;
+                code[h] = *reinterpret_cast<const uint2_t*>(a.cache.k + row * dim + at);
+                scale[h] = a.cache.k_scale[row];
             }
+        }
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                if (head0 + h >= heads) break;
-                float x[8];
-                decode4<CODES>(code[h].x, x);
-                decode4<CODES>(code[h].y, x + 4);
-                uint4_t w;
+        for (int h = 0; h < HEADS; ++h) {
+            if (head0 + h >= heads) break;
+            float x[8];
+            decode4<CODES>(code[h].x, x);
+            decode4<CODES>(code[h].y, x + 4);
+            uint4_t w;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k] * scale[h], x[2 * k + 1] * scale[h]);
-                *reinterpret_cast<uint4_t*>(a.k.data + token * a.k.token_stride + (head0 + h) * a.k.head_stride + at * 2) = w;
+            for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k] * scale[h], x[2 * k + 1] * scale[h]);
+            *reinterpret_cast<uint4_t*>(a.k.data + token * a.k.token_stride + (head0 + h) * a.k.head_stride + at * 2) = w;
+        }
+    } else {
+        const uint32_t head = (blockIdx.x - a.k_chunks) * 4 + group % 4, first = tile * groups + (group / 4) * 4;
+        if (head >= heads || first >= a.tokens || at >= dim) return;
+        int32_t slot[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) slot[i] = first + i < a.tokens ? a.slots[first + i] : -1;
+        const bool run = (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+        uint32_t page, off;
+        float scale[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t code[8];                                  // of element k: the four tokens' bytes
+#pragma unroll
+        for (int k = 0; k < 8; ++k) code[k] = 0;
+        if (run) {
+            if (locate(a.cache, slot[0], page, off)) {
+                const size_t row = head_row(a.cache, page, head) + off;
+                const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + row * dim + size_t(at) * 4);
+                const uint4_t lo = from[0], hi = from[1];
+                const float4_t s = *reinterpret_cast<const float4_t*>(a.cache.v_scale + row);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { code[k] = lo[k]; code[k + 4] = hi[k]; scale[k] = s[k]; }
             }
         } else {
-            const uint32_t head = (blockIdx.x - a.k_chunks) * 4 + group % 4, first = tile * groups + (group / 4) * 4;
-            if (head >= heads || first >= a.tokens || at >= dim) return;
-            int32_t slot[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) slot[i] = first + i < a.tokens ? a.slots[first + i] : -1;
-            const bool run = (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
-            uint32_t page, off;
-            float scale[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t code[8];                                  // of element k: the four tokens' bytes
-#pragma unroll
-            for (int k = 0; k < 8; ++k) code[k] = 0;
-            if (run) {
-                if (locate(a.cache, slot[0], page, off)) {
-                    const size_t row = head_row(a.cache, page, head) + off;
-                    const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + row * dim + size_t(at) * 4);
-                    const uint4_t lo = from[0], hi = from[1];
-                    const float4_t s = *reinterpret_cast<const float4_t*>(a.cache.v_scale + row);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { code[k] = lo[k]; code[k + 4] = hi[k]; scale[k] = s[k]; }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!locate(a.cache, slot[i], page, off)) continue;
-                    const size_t row = head_row(a.cache, page, head) + off;
-                    scale[i] = a.cache.v_scale[row];
-                    // the whole dwords are read: the other bytes are other tokens' of the same page
-                    const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4);
-                    const uint4_t lo = from[0], hi = from[1];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) code[k] |= (((k < 4 ? lo[k & 3] : hi[k & 3]) >> (8 * (off & 3))) & 0xffu) << (8 * i);
-                }
-            }
-            float x[8][4];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) decode4<CODES>(code[k], x[k]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (first + i >= a.tokens) break;
-                uint4_t w;
+                if (!locate(a.cache, slot[i], page, off)) continue;
+                const size_t row = head_row(a.cache, page, head) + off;
+                scale[i] = a.cache.v_scale[row];
+                // the whole dwords are read: the other bytes are other tokens' of the same page
+                const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4);
+                const uint4_t lo = from[0], hi = from[1];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k][i] * scale[i], x[2 * k + 1][i] * scale[i]);
-                *reinterpret_cast<uint4_t*>(a.v.data + (first + i) * a.v.token_stride + head * a.v.head_stride + at * 2) = w;
+                for (int k = 0; k < 8; ++k) code[k] |= (((k < 4 ? lo[k & 3] : hi[k & 3]) >> (8 * (off & 3))) & 0xffu) << (8 * i);
             }
+        }
+        float x[8][4];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) decode4<CODES>(code[k], x[k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (first + i >= a.tokens) break;
+            uint4_t w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k][i] * scale[i], x[2 * k + 1][i] * scale[i]);
+            *reinterpret_cast<uint4_t*>(a.v.data + (first + i) * a.v.token_stride + head * a.v.head_stride + at * 2) = w;
         }
     }
 }

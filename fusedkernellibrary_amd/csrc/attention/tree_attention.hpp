@@ -2,26 +2,36 @@
 //
 // Mathematics. For the rows r of a key head (its query heads times the sequence's new tokens) and the keys j a row sees:
 //   s_rj = scale * ks_j * (q_r . kc_j),   o_r = sum_j e^(s_rj - m_r) vs_j vc_j / sum_j e^(s_rj - m_r)
-// with kc, vc the cache's codes and ks, vs their scales. The codes are exact in half precision (int8: 8 bits, e4m3: 4 bits of
-// 11), so the products run on the codes themselves and the scales enter as one factor per key: ks on the scores, vs on the
-// weights. A query row is brought to a largest magnitude in [1, 2) by a power of two, which is exact in half precision too,
-// but for elements 2^24 times smaller than the row's largest. The one rounding is that of the weights to half precision.
+// with kc, vc the cache's codes and ks, vs their scales. The products run on the codes themselves and the scales enter as one
+// factor per key: ks on the scores, vs on the weights. A query row is brought to a common size by a power of two, which is
+// exact, and held as a sum of 8-bit codes (kCodeProducts) or in half precision. Weights are rounded to half precision, and
+// values are exact in it (int8: 8 bits, e4m3: 4 bits of 11); all sums are in 32 bits.
 //
 // One pass over the keys, 32 at a time, everything in registers: S^T = K Q^T comes out of the matrix unit with a query row to
 // a lane column (lane % 16) and four keys to each of its four quarters (lane / 16), and O^T = V^T P^T wants its weights just
 // so if the contraction runs over the keys in that order; the cache keeps four tokens' bytes of a value element side by
 // side for that reason. So nothing moves between lanes, and the running maximum is per lane column.
 //
-// Two forms. Few rows to a key head (k_split_keys): the four waves of a workgroup take the same 16 or 32 rows and other keys,
-// which each loads into its registers, and the rows' parts are joined in LDS; the bound is reading the cache. Many rows
-// (k_split_rows): the waves take other rows and the same keys, which pass through LDS, copied there without registers and
-// several stages ahead; the bound is the arithmetic, of which turning codes into halves is shared by a wave's row tiles.
+// A workgroup takes R tiles of 16 rows of a key head, and its waves other keys of the same segment, 32 in turn; the waves' sums
+// are joined in LDS at the end. R is 1, 2 or 4: a key's conversion, its loads and its scales serve all R. One tile's queries
+// stay in registers; more are in LDS, as their sums take the registers. Four tiles of 128 elements are 128 registers of
+// sums, which leaves two waves to a SIMD.
+//
+// What bounds it. One tile: reading the cache. 64 sequences with 900 to 8191 keys (8 key heads of 128, int8, 616 MB) take 113 us
+// and 5.8 for joining, 5.5 TB/s; 48 with 4000 to 32700 (e4m3, 1.86 GB) 326 and 7.5 us, 5.7 TB/s; a kernel that only reads reaches
+// 6.3. Four tiles: the vector unit. 32 keys take a wave 38 instructions and 8 exponentials per tile (one scaling, one fused
+// subtraction, one exponential, one value scale, one sum and half a comparison per score), and the matrix unit 1024 cycles, of
+// which it hides about a third from two waves a SIMD: 16 trees of up to 61 tokens over 500 to 4100 keys (25.9 Gflop) take 63 us
+// and 9.8 for joining, where the products alone are 22 at the rate of a large matrix product. 131003 keys with 56 rows (277 MB)
+// take 68 and 6.7 us, where reading is 44. What was tried on four tiles: workgroups side by side that share a unit's keys in the
+// L2 cache (no faster per key, and slower for trees that leave some of them without rows), a touch of the lines two steps ahead
+// (88 us for 68), and 16 more rows' sums without queries read ahead (1 us slower).
 //
 // How the work is dealt out. The device alone knows the sequences' lengths, so every workgroup adds them up: the keys of all
 // (sequence, key head, block of rows), one behind the other, are cut into equal shares, one to a workgroup, all of which run
 // at the same time. A share may hold parts of two of them and whole ones in between; whole ones are written to the output,
-// parts to the workspace, from where k_merge takes them. Without shares (short sequences, or so many that the order of
-// launch evens them out) a workgroup takes one whole (sequence, key head, block of rows).
+// parts to the workspace, from where the kernels of merge.hip take them. Without shares (short sequences, or so many that the
+// order of launch evens them out) a workgroup takes one whole (sequence, key head, block of rows). plan_attention chooses.
 //
 // The running maximum is a reference m_r and not the exact maximum: weights are w = 2^(s - m) * vs, sums those of 2^(s - m), and
 // m moves only when a weight exceeds 2^kLead. Only then are scores compared across lanes and the sums rescaled. The largest
