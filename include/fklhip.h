@@ -131,7 +131,7 @@ int fklhip_last_form(const char **form);
 /*
  * Attention over a quantised key-value cache: the operators a language model's server runs for new or drafted tokens.
  * The reference has them as cooperative kernels of its own beside the fused path (FK/algorithms/attention/: attention,
- * split decoding, int8 and fp8 cache reads); here they are three kernels behind the five entry points below.
+ * split decoding, int8 and fp8 cache reads); here they are the kernels behind the five entry points below.
  *
  * All pointers are device pointers, all strides count elements, the last dimension of rows is contiguous. 16-bit rows
  * start at multiples of 16 bytes (head_dim is a multiple of 8; their strides have to be multiples of 8). The calls are
