@@ -140,23 +140,21 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     }
 }
 
-template <int D> int start_merge(const AttentionArgs& a, bool many_parts, hipStream_t s) {
+template <int D> int start_merge(const AttentionArgs& a, bool many_parts, void* stream) {
     const uint32_t y = a.tokens < 32768u ? a.tokens : 32768u, z = (a.tokens + 32767u) / 32768u;
-    if (many_parts) k_merge_many<D><<<dim3(a.q_heads, y, z), kThreads, 0, s>>>(a);
-    else k_merge_few<D><<<dim3((a.q_heads + Lanes<D>::kGroups - 1) / Lanes<D>::kGroups, y, z), kThreads, 0, s>>>(a);
-    return int(hipGetLastError());
+    if (many_parts) return launch(k_merge_many<D>, dim3(a.q_heads, y, z), dim3(kThreads), stream, a);
+    return launch(k_merge_few<D>, dim3((a.q_heads + Lanes<D>::kGroups - 1) / Lanes<D>::kGroups, y, z), dim3(kThreads), stream, a);
 }
 
 } // namespace
 
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream) {
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     switch (head_dim) {
-    case 64: return start_merge<64>(a, many_parts, s);
-    case 96: return start_merge<96>(a, many_parts, s);
-    case 128: return start_merge<128>(a, many_parts, s);
-    case 192: return start_merge<192>(a, many_parts, s);
-    default: return start_merge<256>(a, many_parts, s);
+    case 64: return start_merge<64>(a, many_parts, stream);
+    case 96: return start_merge<96>(a, many_parts, stream);
+    case 128: return start_merge<128>(a, many_parts, stream);
+    case 192: return start_merge<192>(a, many_parts, stream);
+    default: return start_merge<256>(a, many_parts, stream);
     }
 }
 

@@ -352,8 +352,7 @@ int start_heads(HeadArgs a, uint32_t threads, void* stream, Launched& info) {
     const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
     const dim3 grid(a.q_chunks + a.k_chunks + (TO_CACHE ? ceil_div(a.kv_heads, 4) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
     info = {"heads", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
-    k_heads<LANES, HEADS, TYPE, CODES, TO_CACHE><<<grid, dim3(threads), 0, static_cast<hipStream_t>(stream)>>>(a);
-    return int(hipGetLastError());
+    return launch(k_heads<LANES, HEADS, TYPE, CODES, TO_CACHE>, grid, dim3(threads), stream, a);
 }
 template <int LANES, int TYPE, int CODES, bool TO_CACHE> int start_heads(const HeadArgs& a, void* stream, Launched& info) {
     constexpr int kMany = TO_CACHE ? kManyToCache : kManyHeads;
@@ -371,8 +370,7 @@ template <int LANES, int HEADS, int TYPE, int CODES> int start_read(ReadArgs a, 
     const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
     const dim3 grid(a.k_chunks + ceil_div(a.cache.kv_heads, 4), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
     info = {"kv_read", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
-    k_read<LANES, HEADS, TYPE, CODES><<<grid, dim3(threads), 0, static_cast<hipStream_t>(stream)>>>(a);
-    return int(hipGetLastError());
+    return launch(k_read<LANES, HEADS, TYPE, CODES>, grid, dim3(threads), stream, a);
 }
 template <int LANES, int TYPE, int CODES> int start_read(const ReadArgs& a, void* stream, Launched& info) {
     if (a.tokens <= kFewTokens) return start_read<LANES, 1, TYPE, CODES>(a, smallest_group(LANES), stream, info);

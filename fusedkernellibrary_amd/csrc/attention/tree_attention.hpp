@@ -803,19 +803,13 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
 
 template <int D, int CODES, int PARTS> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
     const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(p.waves * 64);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     const char* name = p.tiles == 4 ? "tree_attention_4x4" : p.tiles == 2 ? "tree_attention_2x4" : p.waves == 8 ? "tree_attention_1x8" : "tree_attention_1x4";
     info = {name, {grid.x, grid.y, grid.z}, {block.x, 1, 1}, 0};
-    if (p.tiles == 4) {
-        if constexpr (D <= 128) k_tree_attention<D, CODES, 4, PARTS, 4><<<grid, block, 0, s>>>(a);
-    } else if (p.tiles == 2) {
-        k_tree_attention<D, CODES, 2, PARTS, 4><<<grid, block, 0, s>>>(a);
-    } else if (p.waves == 8) {
-        k_tree_attention<D, CODES, 1, PARTS, 8><<<grid, block, 0, s>>>(a);
-    } else {
-        k_tree_attention<D, CODES, 1, PARTS, 4><<<grid, block, 0, s>>>(a);
-    }
-    return int(hipGetLastError());
+    if constexpr (D <= 128)
+        if (p.tiles == 4) return launch(k_tree_attention<D, CODES, 4, PARTS, 4>, grid, block, stream, a);
+    if (p.tiles == 2) return launch(k_tree_attention<D, CODES, 2, PARTS, 4>, grid, block, stream, a);
+    if (p.waves == 8) return launch(k_tree_attention<D, CODES, 1, PARTS, 8>, grid, block, stream, a);
+    return launch(k_tree_attention<D, CODES, 1, PARTS, 4>, grid, block, stream, a);
 }
 template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
     if constexpr (kCodeProducts<D, CODES>) {

@@ -507,6 +507,31 @@ def test_last_launch_names_the_kernels(ops, device):
     assert fkl.last_launch()["form"] == "tree_attention_1x8"
 
 
+@pytest.mark.parametrize("kind,new,said", [(INT8, 1, None), (E4M3, 40, None), (INT8, 5, 60000)])
+def test_caches_beyond_4_gib(ops, device, kind, new, said):
+    """Pages whose keys and values lie beyond 2^32 bytes, and whose slots' elements are beyond 2^32: the same bits as in a small cache."""
+    g = gen(new)
+    heads, page, dim, tokens = 8, 128, 128, 700
+    pages = 2 ** 32 // (heads * page * dim) + 16
+    large, small = (ops.KvCache.allocate(n, heads, page, dim, codes=kind, device=device) for n in (pages, 16))
+    order = torch.randperm(8, generator=g)[:6]
+    k, v = torch.randn((2, tokens, heads, dim), generator=g).to(BF16).to(device)
+    q = torch.randn((new, 16, dim), generator=g).to(BF16).to(device)
+    j, got = torch.arange(tokens), []
+    for cache, first in ((large, pages - 8), (small, 4)):
+        table = (order + first).to(torch.int32)
+        slots = (table[j // page] * page + j % page).to(torch.int32).to(device)
+        if said is not None:
+            table = torch.nn.functional.pad(table, (0, said // page + 1 - len(table)), value=1 << 30)
+        ops.kv_write(cache, k, v, slots)
+        context, start = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([tokens - new], [0, new]))
+        out = ops.tree_attention(q, cache, table[None].to(device), context, start, max_new=new, max_context=tokens - new if said is None else said)
+        got.append((out, *ops.kv_read(cache, slots)))
+    assert (pages - 8) * heads * page * dim > 2 ** 32
+    for a, b in zip(*got):
+        assert a.abs().max() > 0 and torch.equal(a, b)
+
+
 # ---- the step from C++, the example, refusals -------------------------------------------------------------------------
 
 def test_a_step_through_the_host_api(ops, device):
