@@ -29,7 +29,7 @@ struct HeadArgs {
     Cache cache;
     uint32_t tokens, table_rows;
     uint32_t q_heads, kv_heads, head_dim, rot_dim;
-    uint32_t q_chunks, k_chunks;            // chunks of the kernel's heads; the chunks behind them are values, four heads each
+    uint32_t q_chunks, k_chunks;            // chunks of the kernel's heads; behind them come the values
     int pairs;
     float eps;
 };

@@ -73,12 +73,43 @@ __device__ __forceinline__ size_t head_row(const Cache& c, uint32_t page, uint32
 constexpr uint32_t kTilesY = 32768;
 __device__ __forceinline__ uint32_t tile_of_grid() { return blockIdx.z * kTilesY + blockIdx.y; }
 
+// One token's values of a head, byte by byte.
+template <int LANES, int TYPE, int CODES> __device__ __forceinline__ void write_value(const HeadArgs& a, uint32_t token, uint32_t head, uint32_t lane) {
+    const uint32_t at = lane * 8, dim = a.head_dim;
+    uint4_t raw = {0, 0, 0, 0};
+    if (at < dim) raw = *reinterpret_cast<const uint4_t*>(a.v.data + token * a.v.token_stride + head * a.v.head_stride + at * 2);
+    uint32_t page, off;
+    const bool stored = locate(a.cache, a.slots[token], page, off);
+    float x[8];
+    uint32_t top = 0, code[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) unpack2<TYPE>(raw[k], x[2 * k], x[2 * k + 1]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[k]));
+    const float scale = scale_of<CODES>(max_lanes<LANES>(top));
+    encode8<CODES>(x, scale, code);
+    if (!stored) return;
+    const size_t row = head_row(a.cache, page, head) + off;
+    if (lane == 0) a.cache.v_scale[row] = scale;
+    if (at < dim) {
+        char* to = a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4 + (off & 3);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to[k * 4] = char(code[k / 4] >> (8 * (k % 4)));
+    }
+}
+
 // LANES to a head of up to 8 * LANES elements, HEADS heads of one token to a group of lanes.
 template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE>
 __global__ __launch_bounds__(256) void k_heads(const HeadArgs a) {
     const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES;
     const uint32_t dim = a.head_dim, tile = tile_of_grid();
     if (TO_CACHE && blockIdx.x >= a.q_chunks + a.k_chunks) {
+        if constexpr (HEADS == 1) {
+            // few tokens: each by itself, as few are in neighbouring slots and four at a time take longer than one (32 of 8 heads: 4.8 us, and 3.0 so)
+            const uint32_t token = tile * groups + group;
+            if (token < a.tokens) write_value<LANES, TYPE, CODES>(a, token, blockIdx.x - a.q_chunks - a.k_chunks, lane);
+            return;
+        }
         // Values: four tokens in four neighbouring slots have their bytes side by side in the cache. A group looks after four tokens of a
         // head, and stores four at once that begin at one of them and at a slot that is a multiple of four, its own or the next group's;
         // tokens that are of no such four, byte by byte. (A chunk of a prompt begins at any slot: with own ones alone at once, 2048
@@ -285,6 +316,32 @@ __global__ __launch_bounds__(256) void k_read(const ReadArgs a) {
             for (int k = 0; k < 4; ++k) w[k] = pack2<TYPE>(x[2 * k] * scale[h], x[2 * k + 1] * scale[h]);
             *reinterpret_cast<uint4_t*>(a.k.data + token * a.k.token_stride + (head0 + h) * a.k.head_stride + at * 2) = w;
         }
+    } else if constexpr (HEADS == 1) {
+        // few tokens: each by itself
+        const uint32_t token = tile * groups + group, head = blockIdx.x - a.k_chunks;
+        if (token >= a.tokens || at >= dim) return;
+        uint32_t page, off;
+        uint4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+        float scale = 0.0f;
+        if (locate(a.cache, a.slots[token], page, off)) {
+            const size_t row = head_row(a.cache, page, head) + off;
+            // the whole dwords are read: the other bytes are other tokens' of the same page
+            const uint4_t* from = reinterpret_cast<const uint4_t*>(a.cache.v + (row - (off & 3)) * dim + size_t(at) * 4);
+            lo = from[0];
+            hi = from[1];
+            scale = a.cache.v_scale[row];
+            lo >>= 8 * (off & 3);
+            hi >>= 8 * (off & 3);
+        }
+        uint4_t w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint4_t& from = k < 2 ? lo : hi;
+            float x[4];
+            decode4<CODES>((from[2 * k & 3] & 0xffu) | (from[(2 * k & 3) + 1] & 0xffu) << 8, x);
+            w[k] = pack2<TYPE>(x[0] * scale, x[1] * scale);
+        }
+        *reinterpret_cast<uint4_t*>(a.v.data + token * a.v.token_stride + head * a.v.head_stride + at * 2) = w;
     } else {
         const uint32_t head = (blockIdx.x - a.k_chunks) * 4 + group % 4, first = tile * groups + (group / 4) * 4;
         if (head >= heads || first >= a.tokens || at >= dim) return;
@@ -341,7 +398,7 @@ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 // registers, of 32, 8 and 8 heads of 128 82.9 and 87.9 (one: 99.4), of 16, 8 and 8 of 64 28.1 and 33.6; reading 8 heads of
 // 64 10.0 and 11.2. Workgroups as small as values allow (four heads a group each) end more evenly: 28.1 us there, 28.6 with 256
 // threads; only reading, which waits for nothing but a slot, has 256 (17.8 us for 8 heads of 128, and 19.9 with 64).
-constexpr uint32_t kFewTokens = 256;
+constexpr uint32_t kFewTokens = 128;
 constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
@@ -350,7 +407,7 @@ int start_heads(HeadArgs a, uint32_t threads, void* stream, Launched& info) {
     a.q_chunks = ceil_div(a.q_heads, HEADS);
     a.k_chunks = ceil_div(a.kv_heads, HEADS);
     const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
-    const dim3 grid(a.q_chunks + a.k_chunks + (TO_CACHE ? ceil_div(a.kv_heads, 4) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
+    const dim3 grid(a.q_chunks + a.k_chunks + (TO_CACHE ? (HEADS == 1 ? a.kv_heads : ceil_div(a.kv_heads, 4)) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
     info = {"heads", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
     return launch(k_heads<LANES, HEADS, TYPE, CODES, TO_CACHE>, grid, dim3(threads), stream, a);
 }
@@ -368,7 +425,7 @@ template <int LANES, int TYPE> int start_heads(const HeadArgs& a, bool to_cache,
 template <int LANES, int HEADS, int TYPE, int CODES> int start_read(ReadArgs a, uint32_t threads, void* stream, Launched& info) {
     a.k_chunks = ceil_div(a.cache.kv_heads, HEADS);
     const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
-    const dim3 grid(a.k_chunks + ceil_div(a.cache.kv_heads, 4), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
+    const dim3 grid(a.k_chunks + (HEADS == 1 ? a.cache.kv_heads : ceil_div(a.cache.kv_heads, 4)), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
     info = {"kv_read", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
     return launch(k_read<LANES, HEADS, TYPE, CODES>, grid, dim3(threads), stream, a);
 }
