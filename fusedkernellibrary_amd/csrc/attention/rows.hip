@@ -392,13 +392,14 @@ __global__ __launch_bounds__(256) void k_read(const ReadArgs a) {
 
 uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
-// Few tokens: one head to a group of lanes, so that everything runs at once. Many: a group has several heads of a token, whose
+// Few rows of keys: one head of a token to a group of lanes, so that everything runs at once (504 tokens of 28 and 4 heads of 128
+// written 5.4 us, 7.0 in the form of many; 2048 tokens of 8 heads 11.1 and 8.4). Many: a group has several heads of a token, whose
 // rows it asks for together and which share its cosines, sines and slot. Values of 2 and 4 heads (16384 tokens): norm and rotation
 // of 40 heads of 128 71.3 and 68.8 us (one head: 86.2), of 24 of 64 20.8 and 19.7; with the write, whose quantising takes more
 // registers, of 32, 8 and 8 heads of 128 82.9 and 87.9 (one: 99.4), of 16, 8 and 8 of 64 28.1 and 33.6; reading 8 heads of
 // 64 10.0 and 11.2. Workgroups as small as values allow (four heads a group each) end more evenly: 28.1 us there, 28.6 with 256
 // threads; only reading, which waits for nothing but a slot, has 256 (17.8 us for 8 heads of 128, and 19.9 with 64).
-constexpr uint32_t kFewTokens = 128;
+constexpr uint32_t kFewRows = 6144;
 constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
@@ -413,7 +414,7 @@ int start_heads(HeadArgs a, uint32_t threads, void* stream, Launched& info) {
 }
 template <int LANES, int TYPE, int CODES, bool TO_CACHE> int start_heads(const HeadArgs& a, void* stream, Launched& info) {
     constexpr int kMany = TO_CACHE ? kManyToCache : kManyHeads;
-    if (a.tokens <= kFewTokens) return start_heads<LANES, 1, TYPE, CODES, TO_CACHE>(a, smallest_group(LANES), stream, info);
+    if (uint64_t(a.tokens) * a.kv_heads <= kFewRows) return start_heads<LANES, 1, TYPE, CODES, TO_CACHE>(a, smallest_group(LANES), stream, info);
     return start_heads<LANES, kMany, TYPE, CODES, TO_CACHE>(a, smallest_group(LANES), stream, info);
 }
 template <int LANES, int TYPE> int start_heads(const HeadArgs& a, bool to_cache, void* stream, Launched& info) {
@@ -430,7 +431,7 @@ template <int LANES, int HEADS, int TYPE, int CODES> int start_read(ReadArgs a, 
     return launch(k_read<LANES, HEADS, TYPE, CODES>, grid, dim3(threads), stream, a);
 }
 template <int LANES, int TYPE, int CODES> int start_read(const ReadArgs& a, void* stream, Launched& info) {
-    if (a.tokens <= kFewTokens) return start_read<LANES, 1, TYPE, CODES>(a, smallest_group(LANES), stream, info);
+    if (uint64_t(a.tokens) * a.cache.kv_heads <= kFewRows) return start_read<LANES, 1, TYPE, CODES>(a, smallest_group(LANES), stream, info);
     return start_read<LANES, kManyRead, TYPE, CODES>(a, 256, stream, info);
 }
 template <int LANES, int TYPE> int start_read(const ReadArgs& a, void* stream, Launched& info) {

@@ -33,7 +33,9 @@ def tables(rows, rot):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("tokens,hq,hkv,dim,rot,pairs", [
     (1, 8, 1, 64, 64, False), (3, 7, 1, 128, 64, True), (17, 5, 5, 96, 96, False), (64, 6, 3, 8, 8, True), (65, 4, 2, 256, 128, False),
-    (257, 9, 3, 128, 128, False), (300, 6, 2, 72, 40, True), (259, 5, 1, 192, 192, True), (1000, 3, 1, 64, 16, False)])
+    (257, 9, 3, 128, 128, False), (300, 6, 2, 72, 40, True), (259, 5, 1, 192, 192, True), (1000, 3, 1, 64, 16, False),
+    # rows enough for several heads of a token to a group of lanes
+    (2100, 5, 3, 64, 64, True), (1237, 6, 6, 128, 64, False), (1300, 5, 5, 256, 256, False), (6200, 2, 1, 96, 48, False)])
 def test_norm_and_rotation(ops, device, dtype, tokens, hq, hkv, dim, rot, pairs):
     g = gen(tokens * dim)
     packed = (3 * torch.randn((tokens, hq + hkv + 2, dim), generator=g)).to(dtype)
@@ -92,7 +94,9 @@ def some_slots(g, tokens, slots, order):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("tokens,heads,dim,page,order", [
     (1, 1, 64, 16, "run"), (5, 3, 128, 16, "odd run"), (32, 8, 128, 64, "any"), (301, 2, 96, 32, "run"), (303, 5, 256, 128, "odd run"),
-    (290, 4, 64, 256, "any"), (270, 1, 72, 32, "odd run"), (9, 2, 8, 16, "any")])
+    (290, 4, 64, 256, "any"), (270, 1, 72, 32, "odd run"), (9, 2, 8, 16, "any"),
+    # rows enough for several heads of a token, and four tokens' values, to a group of lanes
+    (2101, 3, 64, 64, "odd run"), (1237, 6, 128, 16, "any"), (1300, 5, 256, 128, "run"), (6203, 1, 96, 32, "odd run")])
 def test_cache_write_and_read(ops, device, kind, dtype, tokens, heads, dim, page, order):
     g = gen(tokens + dim)
     pages = -(-(tokens + 16) // page) + 1
@@ -122,11 +126,11 @@ def test_cache_write_and_read(ops, device, kind, dtype, tokens, heads, dim, page
         assert torch.equal(got.cpu(), want.float().to(dtype))                          # one rounding of a float32 product
 
 
-@pytest.mark.parametrize("kind,dim", [(INT8, 64), (E4M3, 128), (INT8, 192)])
-def test_writes_of_runs_that_begin_anywhere(ops, device, kind, dim):
+@pytest.mark.parametrize("kind,dim,pages", [(INT8, 64, 40), (E4M3, 128, 180), (INT8, 192, 160)])
+def test_writes_of_runs_that_begin_anywhere(ops, device, kind, dim, pages):
     """Stretches of all lengths that begin at any place of four, in any order, some slots outside, over the edges of workgroups."""
     g = gen(dim)
-    page, pages, heads = 16, 40, 3
+    page, heads = 16, 3
     left, slots = list(range(pages * page)), []
     while len(left) > 60:
         n, at = int(torch.randint(1, 24, (1,), generator=g)), int(torch.randint(0, len(left), (1,), generator=g))
@@ -418,6 +422,30 @@ def test_lengths_and_pages_beyond_what_was_said_are_cut_off(ops, device):
 
 
 # ---- the step ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,dtype,dim,rot,pairs,page", [(INT8, BF16, 128, 128, False, 64), (E4M3, F16, 64, 32, True, 16), (INT8, F16, 256, 256, False, 32), (E4M3, BF16, 96, 96, True, 16)])
+@pytest.mark.parametrize("tokens,heads", [(1237, 6), (6203, 1)])
+def test_many_tokens_to_the_cache(ops, device, kind, dtype, dim, rot, pairs, page, tokens, heads):
+    """One launch or two: the keys are quantised from 32 bits in one, so they are the norm's and rotation's, and the values as written."""
+    g = gen(tokens + dim)
+    pages = tokens // page + 3
+    packed = torch.randn((tokens, 4 * heads, dim), generator=g).to(dtype).to(device)
+    wq, wk = ((1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).to(device) for _ in range(2))
+    cos, sin = (t.to(device) for t in tables(tokens, rot))
+    positions = torch.arange(tokens, dtype=torch.int32, device=device)
+    slots = (torch.arange(tokens) + 5).to(torch.int32).to(device)
+    one, two = (ops.KvCache.allocate(pages, heads, page, dim, codes=kind, device=device) for _ in range(2))
+    q = ops.qkv_to_cache(one, packed[:, :2 * heads], packed[:, 2 * heads:3 * heads], packed[:, 3 * heads:], slots, wq, wk, cos, sin, positions, pairs=pairs)
+    q_alone, k_alone = ops.qk_norm_rope(packed[:, :2 * heads], packed[:, 2 * heads:3 * heads], wq, wk, cos, sin, positions, pairs=pairs)
+    ops.kv_write(two, k_alone, packed[:, 3 * heads:], slots)
+    assert torch.equal(q, q_alone)
+    (k1, v1), (k2, v2) = ops.kv_read(one, slots, dtype=dtype), ops.kv_read(two, slots, dtype=dtype)
+    assert torch.equal(v1, v2)
+    # the rounding of k_alone to 16 bits, a step of the codes (either way), and the last rounding of both
+    top = k_alone.double().abs().amax(-1, keepdim=True)
+    step = top / 127 if kind == INT8 else k_alone.double().abs() / 8 + top / 448 / 512
+    assert ((k1.double() - k2.double()).abs() <= 1.01 * step + 4 * ref.ROUND[dtype] * top).all()
+
 
 @pytest.mark.parametrize("kind,dtype,dim,rot,pairs,page", [(INT8, BF16, 128, 128, False, 64), (E4M3, F16, 64, 32, True, 16), (INT8, F16, 256, 256, False, 32), (E4M3, BF16, 96, 96, True, 16)])
 def test_a_whole_step(ops, device, kind, dtype, dim, rot, pairs, page):
