@@ -249,7 +249,7 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     // A workgroup to each row block, if all run at once and none is long: joining shares' parts costs 6 us and more. Small blocks
     // are the faster ones then, whose keys come from the L2 cache again; one tile's has eight waves if each has a compute unit.
     // Measured, 8 key heads of 128 (4 waves, 8 waves, shares, in us): one sequence of 1000 keys 12.1, 11.7, 14.4; 2000 17.8, 16.9,
-    // 16.3; 3000 23.4, 22.2, 16.2: a compute unit reads 50 GB/s and no more. 2 key heads of 64, 2000 keys: 14.5, 11.6, 14.5.
+    // 16.3; 3000 23.4, 22.2, 16.2: a compute unit reads 50 GB/s of what eight waves ask for. 2 key heads of 64, 2000 keys: 14.5, 11.6, 14.5.
     // 16 tokens, 16 sequences of 1000 keys: one tile 18.7, two 18.8, four 27.2, shares of two tiles 26.8; one sequence of
     // 1000: 12.5, 16.8, 25.3 and 16.8.
     p.tiles = 1;

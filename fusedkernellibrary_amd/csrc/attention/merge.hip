@@ -30,7 +30,7 @@ __device__ __forceinline__ Parts parts_of(Args& a, const Found& f, uint32_t toke
     const uint32_t block = row >> __builtin_ctz(a.unit_rows);
     if (n == 0) return {0, 0, 0};
     const uint32_t first = f.before + (kv_head * blocks_of(a, f.s) + block) * n;
-    const uint32_t share0 = share_of(a, f.all, first);
+    const uint32_t share0 = share_of(a, f.all, first + a.lead);  // (what stands in front of the keys is nobody's part)
     return {share0, share_of(a, f.all, first + n - 1) - share0 + 1, row - block * a.unit_rows};
 }
 // Four elements of a row, and its lse (in units of log2).

@@ -179,7 +179,7 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
             block = unit - head * blocks;
             g = in - unit * n;
             count = min(n - g, end - at);
-            part = count == n ? -1 : g == 0 ? 1 : 0;
+            part = g > a.lead ? 0 : g + count == n ? -1 : 1;
         } else if (block >= blocks) {
             return;
         }
@@ -188,12 +188,7 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         x.quarter = whole << a.granule_log >> 2;
         x.behind = (end - at - count) << a.granule_log;
         if (!shared) x.behind = 0, x.quarter = (x.key1 - x.key0) >> 2;
-        if (part >= 0 && g + count <= a.lead) {
-            // nothing but a block's beginning
-            if (threadIdx.x < x.rows) a.partial_lse[(size_t(own_share(a)) * 2 + part) * a.unit_rows + threadIdx.x] = -__builtin_inff();
-        } else {
-            run(x);
-        }
+        if (!shared || g + count > a.lead) run(x);            // (else there is nothing but a block's beginning)
         if (!shared) return;
         at = __builtin_amdgcn_readfirstlane(kept[0]); in = __builtin_amdgcn_readfirstlane(kept[1]); end = __builtin_amdgcn_readfirstlane(kept[2]);
         b = __builtin_amdgcn_readfirstlane(kept[3]); whole = __builtin_amdgcn_readfirstlane(kept[4]);
