@@ -650,7 +650,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         Args& a = kernel_args();
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
-        // The queries are asked for first, then keys and values, and while those are on their way the queries are made ready.
+        // The pages are asked for first, which keys and values wait for, then the queries, which are made ready while those are on their way.
+        uint32_t key = x.key0 + wave * 32, step = 0;
+        Pages pages{0, 0};
+        pages.fetch(a, x, key >> a.cache.page_log, lane);
         uint4_t raw[S::kSteps];
         const uint32_t tile = kInLds ? wave : 0;
         uint64_t mask = 0;                                         // (of one tile's rows, like the queries)
@@ -661,7 +664,6 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         size_t at[2];
         Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
         float4_t k_scales[2], v_scales[2];
-        Pages pages{0, 0};
         auto locate = [&](uint32_t key) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) at[h] = pages.place(a, x, key + h * 16, lane);
@@ -701,9 +703,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 for (int i = 0; i < S::kLoads; ++i) v[h][i] = load_words_at<S::kWords>(from + i * S::kChunk * 4, lane_v);
             }
         };
-        uint32_t key = x.key0 + wave * 32, step = 0;
         if (key < x.key1) {
-            pages.fetch(a, x, key >> a.cache.page_log, lane);
             locate(key);
             // (in the order of the steps to come: a first step that had asked for values first would have every step wait for its values)
             __builtin_amdgcn_sched_barrier(0);
