@@ -4,9 +4,9 @@
 // All are bound by memory (a head of 128 elements is 256 bytes in and 256 or 132 out for some 20 operations per element),
 // so what counts is that every access is wide, that all of a lane's rows are requested before the first is used, and
 // that one launch does everything a token needs. A copy of 1 GiB runs at 5.1 TB/s here. Norm and rotation of 4099 tokens of 28 and 4
-// heads of 128 (71 MB) take 15.3 us, 4.7 TB/s; of 16384 tokens of 16 and 8 heads of 64 (105 MB) 21.8 us, 4.8 TB/s. 2048 tokens'
-// keys and values of 8 heads of 128 are written in 8.4 us (12.6 MB, a start and an end more than traffic), 30011 read back in
-// 30.7 us (186 MB, 6.1 TB/s). One token takes 3.3 us, which is a launch and three dependent trips to memory.
+// heads of 128 (71 MB) take 15.2 us, 4.7 TB/s; of 16384 tokens of 16 and 8 heads of 64 (105 MB) 21.4 us, 4.9 TB/s. 2048 tokens'
+// keys and values of 8 heads of 128 are written in 8.3 us (12.7 MB, a start and an end more than traffic), 30011 read back in
+// 30.8 us (186 MB, 6.1 TB/s). One token takes 3.2 us, which is a launch and three dependent trips to memory.
 #include "attention_device.hpp"
 
 namespace fkattn {

@@ -18,14 +18,14 @@
 // sums, which leaves two waves to a SIMD.
 //
 // What bounds it. One tile: reading the cache. 64 sequences with 900 to 8191 keys (8 key heads of 128, int8, 616 MB) take 113 us
-// and 5.8 for joining, 5.5 TB/s; 48 with 4000 to 32700 (e4m3, 1.86 GB) 326 and 7.5 us, 5.7 TB/s; a kernel that only reads reaches
+// and 5.7 for joining, 5.4 TB/s; 48 with 4000 to 32700 (e4m3, 1.86 GB) 326 and 8 us, 5.7 TB/s; a kernel that only reads reaches
 // 6.3. Four tiles: the vector unit. 32 keys take a wave 38 instructions and 8 exponentials per tile (one scaling, one fused
 // subtraction, one exponential, one value scale, one sum and half a comparison per score), and the matrix unit 1024 cycles, of
-// which it hides about a third from two waves a SIMD: 16 trees of up to 61 tokens over 500 to 4100 keys (25.9 Gflop) take 63 us
-// and 9.8 for joining, where the products alone are 22 at the rate of a large matrix product. 131003 keys with 56 rows (277 MB)
-// take 68 and 6.7 us, where reading is 44. What was tried on four tiles: workgroups side by side that share a unit's keys in the
-// L2 cache (no faster per key, and slower for trees that leave some of them without rows), a touch of the lines two steps ahead
-// (88 us for 68), and 16 more rows' sums without queries read ahead (1 us slower).
+// which it hides about a third from two waves a SIMD: 16 trees of up to 61 tokens over 500 to 4100 keys (25.9 Gflop) take 62 us
+// and 9.3 for joining, where the products alone are 22 at the rate of a large matrix product. 131003 keys with 56 rows (277 MB)
+// take 67 and 6.5 us, where reading is 44. What was tried on four tiles: workgroups side by side that share a unit's keys in the
+// L2 cache (no faster per key, and slower for trees that leave some of them without rows), and a touch of the lines two steps ahead (88 us
+// for 68). Queries are read from LDS a tile ahead, between two tiles' products and weights (1.5 us of 64).
 //
 // How the work is dealt out. The device alone knows the sequences' lengths, so every workgroup adds them up: the keys of all
 // (sequence, key head, block of rows), one behind the other, are cut into equal shares, one to a workgroup, all of which run
