@@ -31,14 +31,20 @@ class KvCache:
     k        [pages, kv_heads, page_tokens, head_dim]          int8 or float8_e4m3fn
     v        [pages, kv_heads, page_tokens / 4, head_dim, 4]   four consecutive tokens of one element side by side
     k_scale  [pages, kv_heads, page_tokens] float32, v_scale the same
+
+    It is of these tensors for good: it holds them, and their places as the calls hand them on. Making one costs next to nothing.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "_described")
+    __slots__ = ("_tensors", "_described")
 
     def __init__(self, k, v, k_scale, v_scale):
         self._described = _native.describe_cache(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = k, v, k_scale, v_scale
 
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
     pages = property(lambda self: self.k.shape[0])
     kv_heads = property(lambda self: self.k.shape[1])
     page_tokens = property(lambda self: self.k.shape[2])

@@ -126,6 +126,7 @@ PyObject* describe_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.c.pages = pages; b.c.kv_heads = int32_t(heads); b.c.page_tokens = int32_t(page); b.c.head_dim = int32_t(dim);
     b.c.codes = int8 ? FKLHIP_CODES_INT8 : FKLHIP_CODES_E4M3;
     b.device = device.index();
+    check(fklhip_kv_read(&b.c, nullptr, 0, nullptr, nullptr, FKLHIP_BF16, nullptr), "KvCache");      // (of no tokens: looks at the cache alone)
     return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&b), sizeof b);
     END_HANDLE_TH_ERRORS
 }

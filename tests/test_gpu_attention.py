@@ -646,9 +646,12 @@ def test_bindings_refuse_what_does_not_fit(ops, device):
                     (lambda: ops.qk_norm_rope(rows(), x, None, None, torch.zeros((9, 32), device=device), None, slots), "neither"),
                     (lambda: ops.qk_norm_rope(rows(), x, torch.ones(64, device=device), torch.ones(64, device=device), None, None, None), "q_weight"),
                     (lambda: ops.qkv_to_cache(cache, rows(heads=3), rows(heads=3), rows(heads=3), slots, None, None, None, None, None), "other heads"),
-                    (lambda: ops.KvCache(cache.k, cache.k, cache.k_scale, cache.v_scale), "v has to be"), (lambda: ops.KvCache(cache.k, cache.v, cache.k_scale.half(), cache.v_scale), "k_scale"),
-                    (lambda: ops.KvCache.allocate(4, 2, 24, 64, device=device) and ops.kv_write(ops.KvCache.allocate(4, 2, 24, 64, device=device), x, x, slots), "page_tokens")):
+                    (lambda: ops.KvCache(cache.k, cache.k, cache.k_scale, cache.v_scale), "v has to be"), (lambda: ops.KvCache(cache.k, cache.v, cache.k_scale.half(), cache.v_scale), "k_scale")):
         with pytest.raises(ValueError, match=word):
             f()
+    with pytest.raises(ValueError, match="page_tokens"):
+        ops.KvCache.allocate(4, 2, 24, 64, device=device)
+    with pytest.raises(AttributeError):
+        cache.k = cache.k                                                          # a cache is of its tensors for good
     with pytest.raises(ValueError, match="16 bytes"):
         call(q=torch.zeros(3 * 4 * 64 + 1, dtype=BF16, device=device)[1:].view(3, 4, 64))
