@@ -270,11 +270,14 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     p.row_blocks = blocks(p.tiles);
     p.lead = p.tiles == 1 ? 1 : p.tiles == 2 ? 3 : 5;
     if (!whole) {
-        // as many shares as workgroups run at once, or a power of two that leaves two granules to each
+        // as many shares as workgroups run at once, or a power of two that leaves two granules to each; none where the order of launch
+        // evens things out, as many times more row blocks do, or a single sequence's that are twice as many (2048 tokens by
+        // themselves, 32 and 8 heads of 128: 65 us, and 90 in shares; behind 4000 others 195 and 225; several sequences may be of
+        // all lengths)
         const uint64_t all = units(p.tiles) * (p.lead + length);
         p.share_odd = slots == 512 && p.tiles == 1 ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
-        if (units(p.tiles) >= uint64_t(4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
+        if (units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
         else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
     }
     p.many_parts = p.shares() > 16 * units(p.tiles);

@@ -166,7 +166,8 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
     while (at < end && b < kernel_args().batch) {
         Args& a = kernel_args();
         const uint32_t n = granules_of(a, s), blocks = blocks_of(a, s);
-        uint32_t head = blockIdx.x, block = blockIdx.y, g = 0, count = n;
+        // (the last rows of a causal sequence see most: they begin first)
+        uint32_t head = blockIdx.x, block = gridDim.y - 1 - blockIdx.y, g = 0, count = n;
         int part = -1;
         if (shared) {
             const uint32_t unit = n ? in / n : 0;

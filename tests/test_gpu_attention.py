@@ -368,6 +368,17 @@ def test_every_form(ops, device, kind, dtype, form, dim, batch, new, hq, hkv, sa
     assert (last["grid"][1:] == [1, 1] and last["grid"][0] >= 64) if shared else last["grid"][2] == batch
 
 
+@pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, F16)])
+def test_one_sequence_of_many_rows(ops, device, kind, dtype):
+    """So many row blocks that none is shared, over a context that may be long and is not; every row sees every new token but one."""
+    import fusedkernellibrary_amd as fkl
+    mask = torch.full((256, 4), -1, dtype=torch.int64)
+    mask[100, 1] = ~(1 << 36)
+    run_attention(ops, device, context=[37], new=[256], hq=256, hkv=16, dim=64, page=32, kind=kind, dtype=dtype, seed=77, said=3000, mask=mask)
+    last = fkl.last_launch()
+    assert last["form"] == "tree_attention_4x4" and last["grid"] == [16, 64, 1]
+
+
 def test_results_do_not_change_from_call_to_call(ops, device):
     g = gen(21)
     table, pages = paged([4000, 3000], 16, g)
