@@ -25,7 +25,7 @@ ABI_SYMBOLS = (
     "fklhip_event_elapsed_ms", "fklhip_lookup", "fklhip_launch_handle", "fklhip_launch", "fklhip_last_launch", "fklhip_last_form",
     "fklhip_signature_count", "fklhip_signature_at", "fklhip_jit_log", "fklhip_strip_form",
     "fklhip_qk_norm_rope", "fklhip_qkv_to_cache", "fklhip_kv_write", "fklhip_kv_read", "fklhip_tree_attention",
-    "fklhip_tree_attention_workspace", "fklhip_argument_error",
+    "fklhip_tree_attention_workspace", "fklhip_argument_error", "fklhip_stream_is_capturing",
 )
 
 

@@ -90,6 +90,13 @@ int fklhip_stream_create(void** stream) {
 }
 int fklhip_stream_destroy(void* stream) { return int(hipStreamDestroy(static_cast<hipStream_t>(stream))); }
 int fklhip_stream_sync(void* stream) { return int(hipStreamSynchronize(static_cast<hipStream_t>(stream))); }
+int fklhip_stream_is_capturing(void* stream, int* capturing) {
+    if (!capturing) return FKLHIP_EINVAL;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status);
+    *capturing = status != hipStreamCaptureStatusNone;
+    return int(e);
+}
 
 int fklhip_malloc(void** ptr, size_t bytes) { return ptr ? int(hipMalloc(ptr, bytes)) : FKLHIP_EINVAL; }
 int fklhip_malloc_pitch(void** ptr, size_t* pitch, size_t width_bytes, size_t height) {

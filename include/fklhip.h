@@ -57,6 +57,8 @@ int fklhip_device_count(int *count);
 int fklhip_stream_create(void **stream);
 int fklhip_stream_destroy(void *stream);
 int fklhip_stream_sync(void *stream);
+/* 1 while a graph is being captured from the stream, else 0: nothing may be allocated for a call then. */
+int fklhip_stream_is_capturing(void *stream, int *capturing);
 
 /* Memory.  Replaces cudaMalloc / cudaMallocPitch / cudaFree / cudaMallocHost / cudaFreeHost in PtrImpl and Ptr:
  * FK/core/data/ptr_nd.h:47-126,154-250. */

@@ -16,6 +16,7 @@
 #include <stdexcept>
 #include <string>
 #include <utility>
+#include <vector>
 
 namespace fk {
 
@@ -97,20 +98,37 @@ inline void kvRead(const fklhip_kv_cache& cache, const int32_t* slots, const int
 }
 
 // Attention with a workspace that grows to what the calls so far have needed. One object serves one stream at a time: the calls
-// on a stream follow each other and may share it, calls on two streams at once may not.
+// on a stream follow each other and may share it, calls (and replays of graphs) on two streams at once may not.
+//
+// Calls may be captured into a graph, which then names the workspace: the object has to live as long as its graphs. It frees
+// none before its own end, so a later call that needs a larger one takes nothing from them (workspaces are of a few sizes, each
+// larger than the one before). Nothing can be allocated while a graph is captured: a call that would have to is refused with
+// std::logic_error, and reserve() is what comes before it.
 class TreeAttention {
-    attention_detail::DeviceMemory m_workspace;
-public:
-    void operator()(fklhip_attention call, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
+    std::vector<attention_detail::DeviceMemory> m_workspaces;  // the last is the one in use
+
+    size_t bytes() const { return m_workspaces.empty() ? 0 : m_workspaces.back().bytes(); }
+    static uint64_t needed(const fklhip_attention& call, const fklhip_kv_cache& cache) {
         uint64_t bytes = 0;
         FK_ATTENTION_CHECK(fklhip_tree_attention_workspace(&call, &cache, &bytes));
-        if (bytes > m_workspace.bytes()) {
-            stream.sync();                                     // (a call before this one may still use the smaller one)
-            m_workspace = attention_detail::DeviceMemory();
-            m_workspace = attention_detail::DeviceMemory(bytes);
+        return bytes;
+    }
+public:
+    // Makes the workspace large enough for calls of these sizes (its pointers are not looked at).
+    void reserve(const fklhip_attention& call, const fklhip_kv_cache& cache) {
+        const uint64_t need = needed(call, cache);
+        if (need > bytes()) m_workspaces.emplace_back(size_t(need));
+    }
+    void operator()(fklhip_attention call, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
+        const uint64_t need = needed(call, cache);
+        if (need > bytes()) {
+            int capturing = 0;
+            gpuErrchk(fklhip_stream_is_capturing(stream.getNativeStream(), &capturing));
+            if (capturing) throw std::logic_error("TreeAttention: a call that is captured needs its workspace beforehand (reserve)");
+            m_workspaces.emplace_back(size_t(need));
         }
-        call.workspace = m_workspace.data();
-        call.workspace_bytes = m_workspace.bytes();
+        call.workspace = m_workspaces.empty() ? nullptr : m_workspaces.back().data();
+        call.workspace_bytes = bytes();
         FK_ATTENTION_CHECK(fklhip_tree_attention(&call, &cache, stream.getNativeStream()));
     }
 };
