@@ -32,14 +32,16 @@ class KvCache:
     v        [pages, kv_heads, page_tokens / 4, head_dim, 4]   four consecutive tokens of one element side by side
     k_scale  [pages, kv_heads, page_tokens] float32, v_scale the same
 
-    It is of these tensors for good: it holds them, and their places as the calls hand them on. Making one costs next to nothing.
+    It is of these tensors for good, and holds nothing of them but the tensors: every call looks at where they are and at what
+    they are then. Making one costs next to nothing.
     """
 
-    __slots__ = ("_tensors", "_described")
+    __slots__ = ("_tensors",)
 
     def __init__(self, k, v, k_scale, v_scale):
-        self._described = _native.describe_cache(k, v, k_scale, v_scale)
-        self._tensors = k, v, k_scale, v_scale
+        tensors = k, v, k_scale, v_scale
+        _native.check_cache(tensors)
+        self._tensors = tensors
 
     k = property(lambda self: self._tensors[0])
     v = property(lambda self: self._tensors[1])
@@ -72,19 +74,19 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float = 
 def qkv_to_cache(cache: KvCache, q, k, v, slots, q_weight, k_weight, cos, sin, positions, *, eps: float = 1e-6, pairs: bool = False, q_out=None):
     """qk_norm_rope, with the keys and values [tokens, kv_heads, head_dim] quantised into the cache's slots (int32; one
     outside of the cache stores nothing) in the same launch. Returns q_out."""
-    return _native.qkv_to_cache(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, v, slots, cache._described, q_out)
+    return _native.qkv_to_cache(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, v, slots, cache._tensors, q_out)
 
 
 def kv_write(cache: KvCache, k, v, slots) -> None:
     """Quantises keys and values [tokens, kv_heads, head_dim] into the cache's slots."""
-    _native.kv_write(cache._described, k, v, slots)
+    _native.kv_write(cache._tensors, k, v, slots)
 
 
 def kv_read(cache: KvCache, slots, *, dtype=_torch.bfloat16, k_out=None, v_out=None):
     """The cache's slots as (keys, values) [len(slots), kv_heads, head_dim]."""
     if dtype not in _HALVES:
         raise ValueError("dtype has to be torch.bfloat16 or torch.float16")
-    return _native.kv_read(cache._described, slots, _HALVES[dtype], k_out, v_out)
+    return _native.kv_read(cache._tensors, slots, _HALVES[dtype], k_out, v_out)
 
 
 def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: int, max_context: int, mask=None, scale: float | None = None, out=None, lse=None):
@@ -95,4 +97,4 @@ def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: 
     mask[row, u // 64] (int64) says that a row sees new token u; without a mask new token t sees the new tokens 0 to t.
     All of them see the whole context. Rows that see nothing are zero. lse [tokens, q_heads] float32 receives the logarithm
     of the sum of exponentials if it is given. Returns out."""
-    return _native.tree_attention(q, cache._described, page_table, context, q_start, max_new, max_context, mask, scale, out, lse)
+    return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse)

@@ -47,18 +47,29 @@ void* stream_of(const Tensor& t, const char* name) {
     if (t.device().index() != c10::hip::current_device()) refuse(std::string(name) + " is on a device that is not the current one");
     return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
+// A storage may have been resized to less than its tensor needs (such tensors exist between a sharded model's steps).
+void holds(const Tensor& t, const char* name) {
+    int64_t last = t.storage_offset();
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) == 0) return;
+        last += (t.size(i) - 1) * t.stride(i);
+    }
+    if (int64_t(t.storage().nbytes() / t.element_size()) <= last) refuse(std::string(name) + "'s storage is smaller than the tensor");
+}
 fklhip_rows rows(const Tensor& t, const char* name, int64_t tokens, int64_t heads, int64_t dim, const Tensor& like) {
     if (t.dim() != 3 || t.size(0) != tokens || t.size(1) != heads || t.size(2) != dim || t.scalar_type() != like.scalar_type() || t.device() != like.device() ||
         (dim > 1 && t.stride(2) != 1))
         refuse(std::string(name) + " has to be " + shape_text({tokens, heads, dim}) + " of " + c10::toString(like.scalar_type()) + " on " + like.device().str() +
                " with a tight last dimension, not " + shape_text(t.sizes()) + " of " + c10::toString(t.scalar_type()) + " on " + t.device().str());
     if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " asks for a gradient, which these operators do not have (torch.no_grad())");
+    holds(t, name);
     return {t.data_ptr(), t.stride(0), t.stride(1)};
 }
 // A contiguous tensor of one type and shape on a device.
 void* plain(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, c10::Device device) {
     if (t.scalar_type() != type || t.sizes() != shape || t.device() != device || !t.is_contiguous())
         refuse(std::string(name) + " has to be " + shape_text(shape) + " of " + c10::toString(type) + " on " + device.str() + ", contiguous");
+    holds(t, name);
     return t.data_ptr();
 }
 bool none(PyObject* o) { return o == Py_None; }
@@ -101,23 +112,24 @@ void expect(Py_ssize_t have, Py_ssize_t want) {
     if (have != want) refuse("called with " + std::to_string(have) + " arguments and not " + std::to_string(want));
 }
 
-// ---- caches: a fklhip_kv_cache as bytes, made once for a cache --------------------------------------------------------
+// ---- caches: (k, v, k_scale, v_scale), read anew by every call ---------------------------------------------------------
 
-struct CacheBytes {
+// The description is of what the tensors are at the call: one that got other memory since the last call (through set_ or .data,
+// or because its storage was resized) is taken, or refused, as it is now.
+struct CacheView {
     fklhip_kv_cache c;
     int device;
 };
-PyObject* describe_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    expect(n, 4);
-    const Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &ks = tensor(a[2], "k_scale"), &vs = tensor(a[3], "v_scale");
+CacheView cache_of(PyObject* o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) refuse("not a cache's tensors");
+    const Tensor &k = tensor(PyTuple_GET_ITEM(o, 0), "k"), &v = tensor(PyTuple_GET_ITEM(o, 1), "v"), &ks = tensor(PyTuple_GET_ITEM(o, 2), "k_scale"), &vs = tensor(PyTuple_GET_ITEM(o, 3), "v_scale");
     const bool int8 = k.scalar_type() == at::kChar;
     if (k.dim() != 4 || !(int8 || k.scalar_type() == at::kFloat8_e4m3fn))
         refuse("k has to be [pages, kv_heads, page_tokens, head_dim] of torch.int8 or torch.float8_e4m3fn");
     if (!k.is_cuda()) refuse("k has to be on a GPU");
     const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), dim = k.size(3);
     const c10::Device device = k.device();
-    CacheBytes b{};
+    CacheView b{};
     b.c.k = plain(k, "k", k.scalar_type(), {pages, heads, page, dim}, device);
     b.c.v = plain(v, "v", k.scalar_type(), {pages, heads, page / 4, dim, 4}, device);
     b.c.k_scale = static_cast<float*>(plain(ks, "k_scale", at::kFloat, {pages, heads, page}, device));
@@ -126,15 +138,18 @@ PyObject* describe_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.c.pages = pages; b.c.kv_heads = int32_t(heads); b.c.page_tokens = int32_t(page); b.c.head_dim = int32_t(dim);
     b.c.codes = int8 ? FKLHIP_CODES_INT8 : FKLHIP_CODES_E4M3;
     b.device = device.index();
-    check(fklhip_kv_read(&b.c, nullptr, 0, nullptr, nullptr, FKLHIP_BF16, nullptr), "KvCache");      // (of no tokens: looks at the cache alone)
-    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&b), sizeof b);
+    return b;
+}
+// The check that a cache gets when it is made.
+PyObject* check_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 1);
+    const CacheView c = cache_of(a[0]);
+    check(fklhip_kv_read(&c.c, nullptr, 0, nullptr, nullptr, FKLHIP_BF16, nullptr), "KvCache");      // (of no tokens: looks at the cache alone)
+    Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
-const CacheBytes& cache_of(PyObject* o) {
-    if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != sizeof(CacheBytes)) refuse("not a cache's description");
-    return *reinterpret_cast<const CacheBytes*>(PyBytes_AS_STRING(o));
-}
-void on_device(const Tensor& t, const char* name, const CacheBytes& c) {
+void on_device(const Tensor& t, const char* name, const CacheView& c) {
     if (!t.is_cuda() || t.device().index() != c.device) refuse(std::string(name) + " is on another device than the cache");
 }
 
@@ -199,7 +214,7 @@ PyObject* qkv_to_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     fklhip_heads h{};
     heads_of(a, h);
     const Tensor& q = THPVariable_Unpack(a[0]);
-    const CacheBytes& c = cache_of(a[11]);
+    const CacheView c = cache_of(a[11]);
     on_device(q, "q", c);
     void* stream = stream_of(q, "q");
     h.v = rows(tensor(a[9], "v"), "v", h.tokens, h.kv_heads, h.head_dim, q);
@@ -217,7 +232,7 @@ PyObject* qkv_to_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 4);
-    const CacheBytes& c = cache_of(a[0]);
+    const CacheView c = cache_of(a[0]);
     const Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &slots = tensor(a[3], "slots");
     if (k.dim() != 3) refuse("k has to be [tokens, kv_heads, head_dim]");
     on_device(k, "k", c);
@@ -235,7 +250,7 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 5);
     at::AutoDispatchBelowAutograd quick;
-    const CacheBytes& c = cache_of(a[0]);
+    const CacheView c = cache_of(a[0]);
     const Tensor& slots = tensor(a[1], "slots");
     on_device(slots, "slots", c);
     if (slots.dim() != 1) refuse("slots has to have one dimension");
@@ -264,7 +279,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     expect(n, 11);
     at::AutoDispatchBelowAutograd quick;
     const Tensor& q = tensor(a[0], "q");
-    const CacheBytes& c = cache_of(a[1]);
+    const CacheView c = cache_of(a[1]);
     const Tensor& table = tensor(a[2], "page_table");
     fklhip_attention f{};
     if (q.dim() != 3) refuse("q has to be [tokens, q_heads, head_dim]");
@@ -308,7 +323,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
 #define FUNCTION(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    FUNCTION(describe_cache), FUNCTION(qk_norm_rope), FUNCTION(qkv_to_cache), FUNCTION(kv_write), FUNCTION(kv_read), FUNCTION(tree_attention),
+    FUNCTION(check_cache), FUNCTION(qk_norm_rope), FUNCTION(qkv_to_cache), FUNCTION(kv_write), FUNCTION(kv_read), FUNCTION(tree_attention),
 #undef FUNCTION
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attention", "Calls of fusedkernellibrary_amd.attention", -1, methods, nullptr, nullptr, nullptr, nullptr};

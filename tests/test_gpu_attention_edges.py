@@ -1,4 +1,5 @@
-"""Calls of the attention operators at the edges of what they accept, on the GPU: page tables without columns."""
+"""Calls of the attention operators at the edges of what they accept, on the GPU: page tables without columns, and caches whose
+tensors got other memory."""
 import math
 
 import pytest
@@ -39,3 +40,38 @@ def test_page_tables_without_columns(ops, device, batch, new, hq, hkv, dim, kind
             out = ops.tree_attention(q, cache, torch.zeros((batch, 0), dtype=torch.int32, device=device), ints(device, *[context] * batch), start, max_new=new, max_context=context, mask=mask,
                                      out=torch.full_like(q, 3.0), lse=lse)
             assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_a_cache_is_of_its_tensors_as_they_are(ops, device):
+    """Other memory for a cache's tensors is what the next call reads and writes; other shapes, or too little of it, are refused."""
+    g = gen(3)
+    x = torch.randn((2, 40, 2, 64), generator=g).to(BF16).to(device)
+    slots = torch.arange(40, dtype=torch.int32, device=device)
+    one, two = (ops.KvCache.allocate(4, 2, 16, 64, device=device) for _ in range(2))
+    ops.kv_write(one, x[0], x[0], slots)
+    ops.kv_write(two, x[1], x[1], slots)
+    first, second = (ops.kv_read(c, slots) for c in (one, two))
+    assert not torch.equal(first[0], second[0])
+    q, table, ends = x[0, :1, :1].repeat(1, 4, 1), torch.arange(4, dtype=torch.int32, device=device)[None], (ints(device, 39), ints(device, 0, 1))
+    attend = lambda c: ops.tree_attention(q, c, table, *ends, max_new=1, max_context=39)      # noqa: E731
+    want = attend(two)
+    for to, of in zip(one._tensors, two._tensors):
+        to.data = of.clone()
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv_read(one, slots), second)) and torch.equal(attend(one), want)
+    kept = [t.clone() for t in two._tensors]
+    ops.kv_write(one, x[0], x[0], slots)
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv_read(one, slots), first))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(two._tensors, kept))
+    calls = (lambda: ops.kv_write(one, x[0], x[0], slots), lambda: ops.kv_read(one, slots), lambda: attend(one),
+             lambda: ops.qkv_to_cache(one, x[0], x[0], x[0], slots, None, None, None, None, None))
+    good = one.k.data
+    for bad in (good[:, :, :, :32].contiguous(), good[:3].contiguous(), good.view(torch.uint8), good.cpu()):
+        one.k.data = bad
+        for call in calls:
+            with pytest.raises(ValueError):
+                call()
+    one.k.data = good
+    one.v_scale.untyped_storage().resize_(16)
+    for call in calls:
+        with pytest.raises(ValueError, match="storage"):
+            call()
