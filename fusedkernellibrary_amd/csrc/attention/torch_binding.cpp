@@ -56,12 +56,17 @@ void holds(const Tensor& t, const char* name) {
     }
     if (int64_t(t.storage().nbytes() / t.element_size()) <= last) refuse(std::string(name) + "'s storage is smaller than the tensor");
 }
+// A gradient or a tangent would be lost without a word.
+void serves(const Tensor& t, const char* name) {
+    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " asks for a gradient, which these operators do not have (torch.no_grad())");
+    if (t._fw_grad(0).defined()) refuse(std::string(name) + " carries a forward-mode tangent, which these operators do not have");
+}
 fklhip_rows rows(const Tensor& t, const char* name, int64_t tokens, int64_t heads, int64_t dim, const Tensor& like) {
     if (t.dim() != 3 || t.size(0) != tokens || t.size(1) != heads || t.size(2) != dim || t.scalar_type() != like.scalar_type() || t.device() != like.device() ||
         (dim > 1 && t.stride(2) != 1))
         refuse(std::string(name) + " has to be " + shape_text({tokens, heads, dim}) + " of " + c10::toString(like.scalar_type()) + " on " + like.device().str() +
                " with a tight last dimension, not " + shape_text(t.sizes()) + " of " + c10::toString(t.scalar_type()) + " on " + t.device().str());
-    if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(name) + " asks for a gradient, which these operators do not have (torch.no_grad())");
+    serves(t, name);
     holds(t, name);
     return {t.data_ptr(), t.stride(0), t.stride(1)};
 }
@@ -69,6 +74,7 @@ fklhip_rows rows(const Tensor& t, const char* name, int64_t tokens, int64_t head
 void* plain(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, c10::Device device) {
     if (t.scalar_type() != type || t.sizes() != shape || t.device() != device || !t.is_contiguous())
         refuse(std::string(name) + " has to be " + shape_text(shape) + " of " + c10::toString(type) + " on " + device.str() + ", contiguous");
+    serves(t, name);
     holds(t, name);
     return t.data_ptr();
 }

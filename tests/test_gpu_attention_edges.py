@@ -1,5 +1,5 @@
 """Calls of the attention operators at the edges of what they accept, on the GPU: page tables without columns, and caches whose
-tensors got other memory."""
+tensors got other memory, gradients that nobody would compute."""
 import math
 
 import pytest
@@ -75,3 +75,29 @@ def test_a_cache_is_of_its_tensors_as_they_are(ops, device):
     for call in calls:
         with pytest.raises(ValueError, match="storage"):
             call()
+
+
+def test_gradients_and_tangents_are_refused_wherever_they_are_asked_for(ops, device):
+    """Norm weights are parameters that ask for gradients in most models: under grad mode they are refused like rows, not detached."""
+    q, weight, table = torch.ones((3, 2, 64), dtype=BF16, device=device), torch.ones(64, dtype=BF16, device=device), torch.ones((4, 32), device=device)
+    positions = ints(device, 0, 1, 2)
+    cache = ops.KvCache.allocate(1, 2, 16, 64, device=device)
+    norm = lambda **c: ops.qk_norm_rope(**{**dict(q=q, k=q, q_weight=weight, k_weight=weight, cos=table, sin=table, positions=positions), **c})      # noqa: E731
+    store = lambda **c: ops.qkv_to_cache(**{**dict(cache=cache, q=q, k=q, v=q, slots=positions, q_weight=weight, k_weight=weight, cos=table, sin=table, positions=positions), **c})      # noqa: E731
+    for call, names in ((norm, ("q", "k", "q_weight", "k_weight", "cos", "sin", "q_out", "k_out")), (store, ("q", "k", "v", "q_weight", "k_weight", "cos", "sin", "q_out"))):
+        call()
+        for name in names:
+            given = {"q_weight": weight, "k_weight": weight, "cos": table, "sin": table}.get(name, q).clone()
+            with pytest.raises(ValueError, match=f"{name} asks for a gradient"):
+                call(**{name: torch.nn.Parameter(given)})
+            with torch.no_grad():
+                call(**{name: torch.nn.Parameter(given)})
+            with torch.autograd.forward_ad.dual_level():
+                with pytest.raises(ValueError, match=f"{name} carries a forward-mode tangent"):
+                    call(**{name: torch.autograd.forward_ad.make_dual(given, torch.ones_like(given))})
+    lse = torch.zeros((3, 2), device=device, requires_grad=True)
+    with pytest.raises(ValueError, match="lse asks for a gradient"):
+        ops.tree_attention(q, cache, ints(device, 0)[None], ints(device, 0), ints(device, 0, 3), max_new=3, max_context=0, lse=lse)
+    scales = torch.zeros((1, 2, 16), device=device, requires_grad=True)
+    with pytest.raises(ValueError, match="k_scale asks for a gradient"):
+        ops.KvCache(cache.k, cache.v, scales, cache.v_scale)
