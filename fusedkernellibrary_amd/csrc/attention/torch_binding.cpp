@@ -84,9 +84,14 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device device) { r
 Tensor output(PyObject* o, const char* name, at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
     return none(o) ? empty(shape, type, device) : tensor(o, name);
 }
+// What a call wrote to and the caller had before: autograd finds out by the version whether a tensor that it saved still is what it was.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // `given`, or a Python object of the tensor that was allocated.
 PyObject* result(PyObject* given, const Tensor& t) {
     if (none(given)) return THPVariable_Wrap(t);
+    written(t);
     Py_INCREF(given);
     return given;
 }
@@ -145,6 +150,9 @@ CacheView cache_of(PyObject* o) {
     b.c.codes = int8 ? FKLHIP_CODES_INT8 : FKLHIP_CODES_E4M3;
     b.device = device.index();
     return b;
+}
+void written(PyObject* cache) {
+    for (Py_ssize_t i = 0; i < 4; ++i) written(THPVariable_Unpack(PyTuple_GET_ITEM(cache, i)));
 }
 // The check that a cache gets when it is made.
 PyObject* check_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -228,6 +236,7 @@ PyObject* qkv_to_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor q_out = output(a[12], "q_out", q.sizes(), q.scalar_type(), q.device());
     h.q_out = rows(q_out, "q_out", h.tokens, h.q_heads, h.head_dim, q);
     check(fklhip_qkv_to_cache(&h, &c.c, stream), "qkv_to_cache");
+    written(a[11]);
     return result(a[12], q_out);
     END_HANDLE_TH_ERRORS
 }
@@ -247,6 +256,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const fklhip_rows kr = rows(k, "k", tokens, c.c.kv_heads, c.c.head_dim, k), vr = rows(v, "v", tokens, c.c.kv_heads, c.c.head_dim, k);
     const auto* s = static_cast<const int32_t*>(plain(slots, "slots", at::kInt, {tokens}, k.device()));
     check(fklhip_kv_write(&c.c, &kr, &vr, s, tokens, type, stream_of(k, "k")), "kv_write");
+    written(a[0]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -323,6 +333,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         f.workspace_bytes = bytes;
     }
     check(fklhip_tree_attention(&f, &c.c, stream), "tree_attention");
+    if (!none(a[10])) written(THPVariable_Unpack(a[10]));
     return result(a[9], out);
     END_HANDLE_TH_ERRORS
 }

@@ -1,5 +1,4 @@
-"""Calls of the attention operators at the edges of what they accept, on the GPU: page tables without columns, and caches whose
-tensors got other memory, gradients that nobody would compute."""
+"""Calls of the attention operators at the edges of what they accept, on the GPU."""
 import math
 
 import pytest
@@ -101,3 +100,30 @@ def test_gradients_and_tangents_are_refused_wherever_they_are_asked_for(ops, dev
     scales = torch.zeros((1, 2, 16), device=device, requires_grad=True)
     with pytest.raises(ValueError, match="k_scale asks for a gradient"):
         ops.KvCache(cache.k, cache.v, scales, cache.v_scale)
+
+
+def test_what_a_call_writes_to_is_known_to_autograd(ops, device):
+    """Outputs that the caller gives, and a cache's tensors, count as changed: a backward pass that had saved one refuses to run."""
+    q, positions = torch.ones((3, 2, 64), dtype=BF16, device=device), ints(device, 0, 1, 2)
+    cache = ops.KvCache.allocate(1, 2, 16, 64, device=device)
+    args = (ints(device, 0)[None], ints(device, 0), ints(device, 0, 3))
+    lse = torch.zeros((3, 2), device=device)
+    outs = [torch.zeros_like(q) for _ in range(7)]
+    before = [t._version for t in (*outs, *cache._tensors, lse, q)]
+    ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=outs[0], k_out=outs[1])
+    ops.qkv_to_cache(cache, q, q, q, positions, None, None, None, None, None, q_out=outs[2])
+    ops.kv_read(cache, positions, k_out=outs[3], v_out=outs[4])
+    ops.tree_attention(q, cache, *args, max_new=3, max_context=0, out=outs[5], lse=lse)
+    ops.kv_write(cache, q, q, positions)
+    after = [t._version for t in (*outs, *cache._tensors, lse, q)]
+    assert [a - b for a, b in zip(after, before)] == [1] * 6 + [0] + [2] * 4 + [1, 0]
+    saved, weight = torch.ones_like(q), torch.ones(64, dtype=BF16, device=device, requires_grad=True)
+    loss = (saved * weight).sum()
+    ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=saved)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        made_there = torch.zeros_like(q)
+        ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=made_there)
+    ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=made_there)
+    assert torch.equal(made_there, q)
