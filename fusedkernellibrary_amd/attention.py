@@ -8,8 +8,9 @@ each step's new or drafted tokens.
 Thin bindings of the C ABI (include/fklhip.h has the definitions of the operators and the cache's layout): tensors are passed
 on by address, the work runs on torch's current stream, and what does not fit raises ValueError before anything is launched.
 Outputs are allocated by torch unless they are given. The operators serve and do not train: under grad mode an argument that
-asks for a gradient is refused, a norm's weights too, and so is a forward-mode tangent. There is no other path: without the
-compiled library, or on CPU tensors, calls raise.
+asks for a gradient is refused, a norm's weights too, and so is a forward-mode tangent. The calls are no operators of torch's
+dispatcher, so tracers (torch.jit.trace, make_fx) cannot record them and are refused; a HIP graph can. There is no other path:
+without the compiled library, or on CPU tensors, calls raise.
 
 The library the C ABI answers to has these operators as FK/algorithms/attention/ (attention, split decoding, int8 and fp8
 cache reads).

@@ -7,9 +7,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
@@ -119,7 +121,12 @@ double number(PyObject* o) {
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
     return v;
 }
+// What every call begins with. The calls are no operators of torch's dispatcher: a tracer would record their outputs as they
+// happened to be, or as empty tensors.
 void expect(Py_ssize_t have, Py_ssize_t want) {
+    if (at::tracer::impl::is_dispatch_enabled() ||
+        (c10::impl::TorchDispatchModeTLS::any_modes_set() && c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
+        refuse("a tracer cannot record this call");
     if (have != want) refuse("called with " + std::to_string(have) + " arguments and not " + std::to_string(want));
 }
 

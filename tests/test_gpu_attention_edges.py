@@ -127,3 +127,18 @@ def test_what_a_call_writes_to_is_known_to_autograd(ops, device):
         ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=made_there)
     ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=made_there)
     assert torch.equal(made_there, q)
+
+
+def test_tracers_are_refused(ops, device):
+    """A tracer would record what a call happened to write, or an empty tensor, in place of the call."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    q = torch.ones((3, 2, 64), dtype=BF16, device=device)
+    call = lambda x: ops.qk_norm_rope(x, x, None, None, None, None, None)[0] + 1      # noqa: E731
+    with pytest.raises(ValueError, match="tracer"):
+        torch.jit.trace(call, (q,))
+    with pytest.raises(ValueError, match="tracer"):
+        make_fx(call)(q)
+    with FlopCounterMode(display=False):
+        assert torch.equal(call(q), q + 1)
+    assert torch.equal(torch.compile(call, backend="eager")(q), q + 1)
