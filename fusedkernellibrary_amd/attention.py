@@ -22,7 +22,10 @@ import torch as _torch
 from . import lib as _lib
 
 _lib()                          # says what is missing if nothing is built
-from . import _attention as _native  # noqa: E402  (csrc/attention/torch_binding.cpp; needs torch and the library loaded)
+try:
+    from . import _attention as _native  # noqa: E402  (csrc/attention/torch_binding.cpp; needs torch and the library loaded)
+except ImportError as e:
+    raise ImportError("_attention.so is not built, or not for this torch: python -m fusedkernellibrary_amd.build, with a torch for ROCm") from e
 
 _HALVES = {_torch.bfloat16: False, _torch.float16: True}
 

@@ -152,12 +152,14 @@ def build_library(verbose: bool = True) -> str:
 
 
 def build_torch_binding(verbose: bool = True) -> str | None:
-    """_attention.so: host code only, so the host compiler builds it. Without torch there is nothing to bind, and
-    libfklhip.so does not need it."""
+    """_attention.so: host code only, so the host compiler builds it. Without torch, or with one that is not ROCm's, there is
+    nothing to bind, and libfklhip.so does not need it."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    torch_dir = spec.submodule_search_locations[0] if spec else ""
+    if not spec or not os.path.exists(os.path.join(torch_dir, "lib", "libc10_hip.so")):
+        if verbose:
+            print("no torch for ROCm: fusedkernellibrary_amd.attention is not built")
         return None
-    torch_dir = spec.submodule_search_locations[0]
     out = os.path.join(PKG, "_attention.so")
     rocm = os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")
     include = [INCLUDE, os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), rocm,
