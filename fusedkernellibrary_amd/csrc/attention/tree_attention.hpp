@@ -406,21 +406,25 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
             if (!kAhead) products(get_k, [&](int run) { return get_q(r, run); }, y);
             if (!kAhead && r + 1 == R) after_scores();
             if (kAhead && kHeld && r + 1 < R) ask_q(r + 1);
-            const float unit = get_unit(r);
+            float unit = get_unit(r);
             float4_t ks[2], vs[2];
             get_scales(ks, vs);
 #pragma unroll
             for (int h = 0; h < 2; ++h) y[h] *= ks[h];
             if (__builtin_expect(masked, 0)) {
+                uint32_t some = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t seen = sees(r, h);
+                    some |= seen;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         y[h][i] = seen >> i & 1 ? y[h][i] : -__builtin_inff();
                         vs[h][i] = seen >> i & 1 ? vs[h][i] : 0.0f;          // (a hidden value's scale may be NaN)
                     }
                 }
+                // (of a row with an infinity or a NaN the unit is NaN, and -inf times that would be no score of a hidden key)
+                unit = some ? unit : 1.0f;
             }
             if (kAhead && r + 1 < R) products(get_k, [&](int run) { return kHeld ? q[run] : get_q(r + 1, run); }, next);
             // Weights, and a look at whether the reference has to move: where a weight is too large for half precision.

@@ -142,3 +142,39 @@ def test_tracers_are_refused(ops, device):
     with FlopCounterMode(display=False):
         assert torch.equal(call(q), q + 1)
     assert torch.equal(torch.compile(call, backend="eager")(q), q + 1)
+
+
+# keys' codes as they are, with two and three parts of a query, and keys as halves; one tile, two and four; whole blocks and shares
+every_product = pytest.mark.parametrize("kind,dtype,dim", [(INT8, BF16, 128), (INT8, F16, 64), (E4M3, BF16, 128), (E4M3, F16, 128), (E4M3, BF16, 64), (INT8, F16, 96), (INT8, BF16, 256)])
+every_form = pytest.mark.parametrize("new,said", [(4, 0), (9, 20000), (40, 20000)])
+
+
+def queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what):
+    """(out, lse, rows that see nothing, rows whose query holds `what` somewhere) of drafted tokens without a context."""
+    g, page, hkv, batch = gen(new + dim), 16, 2, 20
+    columns = max(new, said + new) // page + 1
+    cache = ops.KvCache.allocate(batch * (new // page + 1), hkv, page, dim, codes=kind, device=device)
+    table = torch.full((batch, columns), -1, dtype=torch.int32)
+    table[:, :new // page + 1] = torch.arange(table[:, :new // page + 1].numel()).view(batch, -1)
+    slots = (table[:, :new // page + 1, None] * page + torch.arange(page)).view(-1).to(torch.int32).to(device)
+    x = torch.randn((2, len(slots), hkv, dim), generator=g).to(dtype).to(device)
+    ops.kv_write(cache, x[0], x[1], slots)
+    q = torch.randn((batch * new, 4, dim), generator=g).to(dtype)
+    mask = torch.randint(0, 1 << new, (batch * new, 1), generator=g)
+    mask[torch.rand(batch * new, generator=g) < 0.4] = 0
+    bad = torch.rand((batch * new, 4), generator=g) < 0.5
+    q[bad, torch.randint(0, dim, (int(bad.sum()),), generator=g)] = what
+    lse = torch.zeros((batch * new, 4), device=device)
+    out = ops.tree_attention(q.to(device), cache, table.to(device), ints(device, *[0] * batch), ints(device, *range(0, batch * new + 1, new)), max_new=new, max_context=said, mask=mask.to(device),
+                             lse=lse)
+    blind = (mask == 0).expand(-1, 4)
+    assert (blind & bad).any() and (~blind & bad).any() and (~blind & ~bad).any()
+    return out.cpu(), lse.cpu(), blind, bad
+
+
+@every_product
+@every_form
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_rows_that_see_nothing_are_zero_whatever_their_queries_hold(ops, device, kind, dtype, dim, new, said, what):
+    out, lse, blind, _ = queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what)
+    assert (out[blind] == 0).all() and (lse[blind] == -math.inf).all()
