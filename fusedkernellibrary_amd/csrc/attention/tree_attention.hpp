@@ -256,6 +256,8 @@ template <int D, int CODES, int PARTS> __device__ __forceinline__ float prepare_
 #pragma unroll
         for (int k = 0; k < S::kSteps * 4; ++k)
             q[k] = pack2<FKLHIP_F16>(__builtin_amdgcn_ldexpf(e[2 * k], -p), __builtin_amdgcn_ldexpf(e[2 * k + 1], -p));
+        // (as with codes: an infinity makes NaN of its row's scores, not an infinity of either sign)
+        unit = top >= 0x7f800000u ? __builtin_nanf("") : unit;
     } else if constexpr (CODES == FKLHIP_CODES_INT8) {
         // A power of two in front of the largest magnitude that leaves it below 127.5 * 2^8 (or 2^14); a row with an
         // infinity or a NaN has scores that are NaN.

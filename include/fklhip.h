@@ -201,7 +201,7 @@ int fklhip_kv_read(const fklhip_kv_cache *cache, const int32_t *slots, int64_t t
  * page_table[b * page_table_stride + j / page_tokens] * page_tokens + j % page_tokens. Query row r sees the whole context
  * and new token u if bit u % 64 of mask[r * mask_words + u / 64] is set; without a mask, new token t sees 0..t. Query
  * heads are shared out to the key heads in order (q_heads a multiple of kv_heads). A row that sees nothing gives zeros and
- * lse -inf. Lengths above max_new and max_context, and tokens beyond the page table's row, are cut off; pages outside of
+ * lse -inf; a row that sees a key, and whose query holds an infinity or a NaN, gives NaN. Lengths above max_new and max_context, and tokens beyond the page table's row, are cut off; pages outside of
  * the cache are read as its last. head_dim: 64, 96, 128, 192 or 256. */
 typedef struct fklhip_attention {
     fklhip_rows q, out;

@@ -174,6 +174,16 @@ def queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what):
 
 @every_product
 @every_form
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_not_finite_make_their_rows_nan(ops, device, kind, dtype, dim, new, said, what):
+    """A row that sees a key is NaN with such a query, whatever the signs of its scores, and others are not."""
+    out, lse, blind, bad = queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what)
+    assert out[~blind & bad].isnan().all() and lse[~blind & bad].isnan().all()
+    assert out[~blind & ~bad].isfinite().all() and lse[~blind & ~bad].isfinite().all()
+
+
+@every_product
+@every_form
 @pytest.mark.parametrize("what", [math.nan, math.inf])
 def test_rows_that_see_nothing_are_zero_whatever_their_queries_hold(ops, device, kind, dtype, dim, new, said, what):
     out, lse, blind, _ = queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what)
