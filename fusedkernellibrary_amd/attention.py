@@ -100,6 +100,6 @@ def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: 
     Sequence b has context[b] (at most max_context) tokens in the cache and behind them its new ones, rows q_start[b] to
     q_start[b + 1] (at most max_new) of q; its token j is in page page_table[b, j // page_tokens]. Bit u % 64 of
     mask[row, u // 64] (int64) says that a row sees new token u; without a mask new token t sees the new tokens 0 to t.
-    All of them see the whole context. Rows that see nothing are zero. lse [tokens, q_heads] float32 receives the logarithm
-    of the sum of exponentials if it is given. Returns out."""
+    All of them see the whole context. Rows that see nothing are zero, and so are those of no sequence (a padded batch's).
+    lse [tokens, q_heads] float32 receives the logarithm of the sum of exponentials if it is given. Returns out."""
     return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse)

@@ -61,7 +61,12 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const A
     const uint32_t token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
     const Found f = sequence_of_token(a, token);
-    if (f.b >= a.batch || head >= a.q_heads) return;          // a row of no sequence, or none
+    if (head >= a.q_heads) return;
+    if (f.b >= a.batch) {                                     // a row of no sequence
+        if (d < D) put4(a, token, head, d, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
+        if (at == 0) put_lse(a, token, head, -__builtin_inff());
+        return;
+    }
     const Parts p = parts_of(a, f, token, head);
     if (p.count == 1) return;
     float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -99,7 +104,11 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     const uint32_t head = blockIdx.x, token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
     const Found f = sequence_of_token(a, token);
-    if (f.b >= a.batch) return;
+    if (f.b >= a.batch) {                                     // a row of no sequence
+        if (group == 0 && d < D) put4(a, token, head, d, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
+        if (threadIdx.x == 0) put_lse(a, token, head, -__builtin_inff());
+        return;
+    }
     const Parts p = parts_of(a, f, token, head);
     if (p.count == 1) return;
     float top = -__builtin_inff();

@@ -340,6 +340,10 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         f.workspace_bytes = bytes;
     }
     check(fklhip_tree_attention(&f, &c.c, stream), "tree_attention");
+    if (tokens != 0 && (f.batch == 0 || f.max_new == 0)) {     // (nothing was launched)
+        Tensor(out).zero_();
+        if (!none(a[10])) Tensor(THPVariable_Unpack(a[10])).fill_(-HUGE_VAL);
+    }
     if (!none(a[10])) written(THPVariable_Unpack(a[10]));
     return result(a[9], out);
     END_HANDLE_TH_ERRORS

@@ -144,9 +144,27 @@ __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32
     return x;
 }
 
+// Rows of the result that are of no sequence, in front of the first, above max_new or behind the last: zeros, as where a row sees
+// nothing. Those behind sequence b's, which end at `end`, and in front of the first's, one key head's. (With shares the kernels of
+// merge.hip, which come to every row, see to it.)
+template <int D, int THREADS> __device__ __forceinline__ void clear_rows(Args& a, const Sequence& s, uint32_t b, uint32_t head, int32_t end) {
+    const uint32_t front = b == 0 ? s.first_token : 0u, behind = s.first_token + s.fresh;
+    const uint32_t upto = b + 1 == a.batch ? a.tokens : end < 0 ? 0u : min(uint32_t(end), a.tokens);
+    if (__builtin_expect(front == 0 && upto <= behind, 1)) return;
+    const auto clear = [&](uint32_t token) {
+        char* to = a.out.data + int64_t(token) * a.out.token_stride + int64_t(head * a.group) * a.out.head_stride;
+        for (uint32_t i = threadIdx.x; i < a.group * (D / 8); i += THREADS)
+            *reinterpret_cast<uint4_t*>(to + int64_t(i / (D / 8)) * a.out.head_stride + i % (D / 8) * 16) = uint4_t{0, 0, 0, 0};
+        if (a.lse)
+            for (uint32_t i = threadIdx.x; i < a.group; i += THREADS) a.lse[size_t(token) * a.q_heads + head * a.group + i] = -__builtin_inff();
+    };
+    for (uint32_t token = 0; token < front; ++token) clear(token);
+    for (uint32_t token = behind; token < upto; ++token) clear(token);
+}
+
 // Calls `run` for every segment of the workgroup. `kept` is the wave's place in LDS for what the walk goes on with: a segment
 // needs all registers.
-template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, uint32_t* kept, F run) {
+template <int D, int THREADS, typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, uint32_t* kept, F run) {
     // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
     uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
     const bool shared = a.share_odd != 0;
@@ -160,7 +178,9 @@ template <typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lan
         in = at - f.before;
         s = f.s;
     } else {
-        s = sequence_at(a, b);
+        const int32_t rows_end = scalar(a.q_start + b + 1);
+        s = sequence_of(a, scalar(a.q_start + b), rows_end, scalar(a.context + b));
+        if (blockIdx.y == 0) clear_rows<D, THREADS>(a, s, b, blockIdx.x, rows_end);
     }
     uint32_t whole = end - at;
     while (at < end && b < kernel_args().batch) {
@@ -653,7 +673,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
     uint4_t* queries = reinterpret_cast<uint4_t*>(space);
 
     __shared__ uint32_t walks[WAVES][8];
-    walk(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
+    walk<D, WAVES * 64>(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
         Args& a = kernel_args();
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);

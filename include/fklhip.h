@@ -202,7 +202,9 @@ int fklhip_kv_read(const fklhip_kv_cache *cache, const int32_t *slots, int64_t t
  * and new token u if bit u % 64 of mask[r * mask_words + u / 64] is set; without a mask, new token t sees 0..t. Query
  * heads are shared out to the key heads in order (q_heads a multiple of kv_heads). A row that sees nothing gives zeros and
  * lse -inf; a row that sees a key, and whose query holds an infinity or a NaN, gives NaN. Lengths above max_new and max_context, and tokens beyond the page table's row, are cut off; pages outside of
- * the cache are read as its last. head_dim: 64, 96, 128, 192 or 256. */
+ * the cache are read as its last. Rows of q that are of no sequence (in front of q_start[0], cut off by max_new, at and behind
+ * q_start[batch]) are zeros with lse -inf as well; q_start has to rise. With tokens, batch or max_new 0 there is no row of a
+ * sequence: such a call launches nothing and leaves out and lse as they are. head_dim: 64, 96, 128, 192 or 256. */
 typedef struct fklhip_attention {
     fklhip_rows q, out;
     float *lse;                        /* [tokens][q_heads] log of the sum of exponentials, or NULL */

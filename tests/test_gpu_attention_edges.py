@@ -188,3 +188,46 @@ def test_queries_that_are_not_finite_make_their_rows_nan(ops, device, kind, dtyp
 def test_rows_that_see_nothing_are_zero_whatever_their_queries_hold(ops, device, kind, dtype, dim, new, said, what):
     out, lse, blind, _ = queries_that_are_not_finite(ops, device, kind, dtype, dim, new, said, what)
     assert (out[blind] == 0).all() and (lse[blind] == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, F16)])
+# whole blocks: one tile of eight waves and of four, two, four; shares whose parts groups of lanes join, and workgroups
+@pytest.mark.parametrize("dim,hq,hkv,copies,max_new,said", [(64, 4, 2, 1, 3, 0), (96, 6, 2, 1, 3, 0), (128, 4, 2, 40, 3, 0), (192, 40, 2, 40, 3, 0), (64, 32, 2, 40, 6, 0), (64, 4, 2, 1, 3, 60000),
+                                                            (96, 6, 2, 30, 3, 30000), (256, 10, 1, 1, 6, 60000), (128, 12, 1, 20, 6, 20000)])
+def test_rows_of_no_sequence_are_zero(ops, device, kind, dtype, dim, hq, hkv, copies, max_new, said):
+    """A padded batch: rows in front of the first sequence, behind the last, and above max_new, of sequences with and without others."""
+    new, cut = [2, 0, 9, 1, 4] * copies, lambda n: min(n, max_new)      # noqa: E731
+    g, page, front, behind = gen(dim), 16, 3, 21
+    starts = [front + sum(new[:b]) for b in range(len(new) + 1)]
+    tokens = starts[-1] + behind
+    context = torch.tensor([(b * 7) % 40 for b in range(len(new))], dtype=torch.int32)
+    if said == 0:
+        context.zero_()
+    cache = ops.KvCache.allocate(8, hkv, page, dim, codes=kind, device=device)
+    x = torch.randn((2, 8 * page, hkv, dim), generator=g).to(dtype).to(device)
+    ops.kv_write(cache, x[0], x[1], torch.arange(8 * page, dtype=torch.int32, device=device))
+    table = torch.randint(0, 8, (len(new), (said + max_new) // page + 1), generator=g, dtype=torch.int32).to(device)
+    q = torch.randn((tokens, hq, dim), generator=g).to(dtype).to(device)
+    wide = torch.full((tokens, hq + 1, dim + 8), math.nan, dtype=dtype, device=device)
+    lse = torch.full((tokens, hq), math.nan, device=device)
+    args = dict(page_table=table, context=context.to(device), max_new=max_new, max_context=said)
+    out = ops.tree_attention(q, cache, q_start=ints(device, *starts), out=wide[:, :hq, :dim], lse=lse, **args)
+    mine = torch.zeros(tokens, dtype=torch.bool)
+    for b, n in enumerate(new):
+        mine[starts[b]:starts[b] + cut(n)] = True
+    assert (~mine).sum() >= front + behind + copies * (9 - max_new)
+    assert (out[~mine] == 0).all() and (lse[~mine] == -math.inf).all() and out[mine].isfinite().all() and (out[mine] != 0).any(-1).all() and lse[mine].isfinite().all()
+    assert wide[:, hq:].isnan().all() and wide[:, :, dim:].isnan().all()
+    # the same rows by themselves
+    alone = ops.tree_attention(q[mine.to(device)], cache, q_start=ints(device, *[sum(map(cut, new[:b])) for b in range(len(new) + 1)]), **args)
+    assert torch.equal(out[mine.to(device)], alone)
+
+
+def test_calls_without_sequences_or_new_tokens_give_zeros(ops, device):
+    cache = ops.KvCache.allocate(1, 1, 16, 64, device=device)
+    q = torch.ones((5, 2, 64), dtype=BF16, device=device)
+    for batch, max_new in ((0, 3), (2, 0)):
+        lse = torch.zeros((5, 2), device=device)
+        out = ops.tree_attention(q, cache, torch.zeros((batch, 1), dtype=torch.int32, device=device), ints(device, *[1] * batch), ints(device, *range(batch + 1)), max_new=max_new, max_context=4,
+                                 out=torch.full_like(q, math.nan), lse=lse)
+        assert (out == 0).all() and (lse == -math.inf).all()
