@@ -8,7 +8,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <limits>
+#include <utility>
 
 using namespace fkattn;
 
@@ -30,6 +32,28 @@ int check_rows(const fklhip_rows& r, int64_t count, int64_t heads) {
     NEED(aligned(r.data, 16), "rows have to start at a multiple of 16 bytes");
     NEED(count <= 1 || r.token_stride % 8 == 0, "a token stride has to be a multiple of 8 elements");
     NEED(heads <= 1 || r.head_stride % 8 == 0, "a head stride has to be a multiple of 8 elements");
+    return FKLHIP_OK;
+}
+// Whether two of an output's rows share bytes: two workgroups would write there, in any order.
+bool overlaps(const fklhip_rows& r, int64_t count, int64_t heads, int64_t dim) {
+    // (a stride of a dimension of one row is not looked at)
+    int64_t step[2] = {std::abs(r.head_stride), std::abs(r.token_stride)}, n[2] = {heads, count};
+    if (n[0] <= 1 || (n[1] > 1 && step[1] < step[0])) std::swap(step[0], step[1]), std::swap(n[0], n[1]);
+    if (n[0] <= 1) return false;
+    if (step[0] < dim) return true;
+    if (n[1] <= 1 || (step[1] - dim) / step[0] >= n[0] - 1) return false;
+    // Rows in between others: i steps of the smaller stride against j of the larger. (Negative strides are the same places from
+    // another end.)
+    const __int128 small = step[0], large = step[1], end = small * (n[0] - 1) + dim;
+    for (int64_t j = 1; j < n[1] && large * j < end; ++j) {
+        const __int128 i = large * j / small, left = large * j - i * small;
+        if ((i < n[0] && left < dim) || (i + 1 < n[0] && small - left < dim)) return true;
+    }
+    return false;
+}
+int check_out(const fklhip_rows& r, int64_t count, int64_t heads, int64_t dim) {
+    if (const int rc = check_rows(r, count, heads); rc != FKLHIP_OK) return rc;
+    NEED(!overlaps(r, count, heads, dim), "rows of an output overlap");
     return FKLHIP_OK;
 }
 Rows to_rows(const fklhip_rows& r) { return {static_cast<char*>(r.data), r.token_stride * 2, r.head_stride * 2}; }
@@ -90,12 +114,12 @@ int run_heads(const fklhip_heads* h, const fklhip_kv_cache* cache, void* stream)
     if (h->tokens == 0) return FKLHIP_OK;
     CHECK(check_rows(h->q, h->tokens, h->q_heads));
     CHECK(check_rows(h->k, h->tokens, h->kv_heads));
-    CHECK(check_rows(h->q_out, h->tokens, h->q_heads));
+    CHECK(check_out(h->q_out, h->tokens, h->q_heads, h->head_dim));
     if (cache) {
         CHECK(check_rows(h->v, h->tokens, h->kv_heads));
         NEED(h->slots, "no slots");
     } else {
-        CHECK(check_rows(h->k_out, h->tokens, h->kv_heads));
+        CHECK(check_out(h->k_out, h->tokens, h->kv_heads, h->head_dim));
     }
     HeadArgs a{};
     a.q = to_rows(h->q); a.k = to_rows(h->k); a.q_out = to_rows(h->q_out);
@@ -175,8 +199,8 @@ int fklhip_kv_read(const fklhip_kv_cache* cache, const int32_t* slots, int64_t t
     if (tokens == 0) return FKLHIP_OK;
     NEED(k && v && slots, "no rows or no slots");
     NEED(aligned(slots, 4), "slots have to be aligned");
-    CHECK(check_rows(*k, tokens, cache->kv_heads));
-    CHECK(check_rows(*v, tokens, cache->kv_heads));
+    CHECK(check_out(*k, tokens, cache->kv_heads, cache->head_dim));
+    CHECK(check_out(*v, tokens, cache->kv_heads, cache->head_dim));
     ReadArgs a{to_cache(*cache), to_rows(*k), to_rows(*v), slots, uint32_t(tokens), uint32_t(cache->head_dim), 0};
     Launched info;
     return finish(launch_read(a, type, stream, info), info);
@@ -196,7 +220,7 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     NEED(std::isfinite(c->scale), "scale has to be finite");
     if (c->tokens == 0 || c->batch == 0 || c->max_new == 0) return FKLHIP_OK;
     CHECK(check_rows(c->q, c->tokens, c->q_heads));
-    CHECK(check_rows(c->out, c->tokens, c->q_heads));
+    CHECK(check_out(c->out, c->tokens, c->q_heads, cache->head_dim));
     NEED(c->context && c->q_start, "no context or no q_start");
     NEED(c->page_table || c->page_table_stride == 0, "no page_table");
     NEED(aligned(c->context, 4) && aligned(c->q_start, 4) && aligned(c->page_table, 4) && aligned(c->lse, 4) && aligned(c->mask, 8), "lengths, page_table, lse and mask have to be aligned");

@@ -136,10 +136,10 @@ int fklhip_last_form(const char **form);
  * split decoding, int8 and fp8 cache reads); here they are the kernels behind the five entry points below.
  *
  * All pointers are device pointers, all strides count elements, the last dimension of rows is contiguous. 16-bit rows
- * start at multiples of 16 bytes (head_dim is a multiple of 8; their strides have to be multiples of 8). The calls are
- * asynchronous on `stream`, allocate nothing, record no memset and may be captured into a graph. A call that returns
- * FKLHIP_EINVAL has launched nothing; fklhip_argument_error says what was wrong. What only the device can see (slots,
- * pages, lengths, positions) is held inside its bounds by the kernels, as described at each entry.
+ * start at multiples of 16 bytes (head_dim is a multiple of 8; their strides have to be multiples of 8). Rows of an output
+ * may not overlap each other. The calls are asynchronous on `stream`, allocate nothing, record no memset and may be captured
+ * into a graph. A call that returns FKLHIP_EINVAL has launched nothing; fklhip_argument_error says what was wrong. What only
+ * the device can see (slots, pages, lengths, positions) is held inside its bounds by the kernels, as described at each entry.
  */
 enum { FKLHIP_BF16 = 0, FKLHIP_F16 = 1 };
 enum { FKLHIP_CODES_INT8 = 0, FKLHIP_CODES_E4M3 = 1 };

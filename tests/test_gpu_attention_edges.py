@@ -231,3 +231,17 @@ def test_calls_without_sequences_or_new_tokens_give_zeros(ops, device):
         out = ops.tree_attention(q, cache, torch.zeros((batch, 1), dtype=torch.int32, device=device), ints(device, *[1] * batch), ints(device, *range(batch + 1)), max_new=max_new, max_context=4,
                                  out=torch.full_like(q, math.nan), lse=lse)
         assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_outputs_that_overlap_themselves_are_refused(ops, device):
+    cache = ops.KvCache.allocate(1, 2, 16, 64, device=device)
+    q, slots = torch.ones((3, 2, 64), dtype=BF16, device=device), ints(device, 0, 1, 2)
+    one = torch.zeros((1, 2, 64), dtype=BF16, device=device).expand(3, 2, 64)
+    ops.kv_write(cache, q, q, slots)
+    for call in (lambda: ops.qk_norm_rope(q, q, None, None, None, None, None, q_out=one), lambda: ops.qk_norm_rope(q, q, None, None, None, None, None, k_out=one),
+                 lambda: ops.kv_read(cache, slots, v_out=one), lambda: ops.qkv_to_cache(cache, q, q, q, slots, None, None, None, None, None, q_out=one),
+                 lambda: ops.tree_attention(q, cache, ints(device, 0)[None], ints(device, 0), ints(device, 0, 3), max_new=3, max_context=0, out=one)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    # inputs may overlap: one row for all tokens
+    assert torch.equal(ops.qk_norm_rope(one + 1, one, None, None, None, None, None)[1], one)
