@@ -669,7 +669,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
     __shared__ float joined_m[WAVES][R * 16], joined_l[WAVES][R * 16];
     __shared__ float units[R * 16];
     __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
-    __shared__ __attribute__((aligned(16))) float scales[WAVES][2][64];
+    __shared__ __attribute__((aligned(16))) float scales[WAVES][64];
     uint4_t* queries = reinterpret_cast<uint4_t*>(space);
 
     __shared__ uint32_t walks[WAVES][8];
@@ -678,7 +678,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
         // The pages are asked for first, which keys and values wait for, then the queries, which are made ready while those are on their way.
-        uint32_t key = x.key0 + wave * 32, step = 0;
+        uint32_t key = x.key0 + wave * 32;
         Pages pages{0, 0};
         // (a wave without keys asks for none: where the page table has no columns there is no entry to read)
         if (key < x.key1) pages.fetch(a, x, key >> a.cache.page_log, lane);
@@ -704,16 +704,23 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 for (int i = 0; i < S::kLoads; ++i) k[h][i] = load_words_at<S::kWords>(from + i * S::kChunk, lane_k);
             }
         };
-        // Scales of several tiles' steps are used again and again, and would take 16 registers: those go to LDS, two of the keys' and
-        // two of the values' blocks of 16 side by side, for this step and the next.
-        const uint32_t scales_at = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float*)&scales[wave][0][0])));
-        auto copy_scales = [&](uint32_t step) {
+        // Scales of several tiles' steps are used again and again, and would take 16 registers: those go through one register of each
+        // lane, asked for with the step's keys, to LDS, two of the keys' and two of the values' blocks of 16 side by side.
+        float scale_ahead = 0.0f;
+        auto ask_scales = [&] {
             if constexpr (kInLds) {
                 Args& b = kernel_args();
                 const uint32_t l = thread_here();
                 const size_t first = at[0], second = at[1];
-                const float* from = (l & 32 ? b.cache.v_scale : b.cache.k_scale) + (l & 16 ? second : first) + (l & 15);
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(scales_at + (step & 1) * 256), "v"(from) : "memory", "m0");
+                scale_ahead = ((l & 32 ? b.cache.v_scale : b.cache.k_scale) + (l & 16 ? second : first))[l & 15];
+            }
+        };
+        auto put_scales = [&] {
+            if constexpr (kInLds) {
+                // (the wave's own part of LDS, which it writes and reads in order)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+                scales[wave][lane] = scale_ahead;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
             }
         };
         auto load_scales_and_v = [&] {
@@ -735,7 +742,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             locate(key);
             // (in the order of the steps to come: a first step that had asked for values first would have every step wait for its values)
             __builtin_amdgcn_sched_barrier(0);
-            copy_scales(0);
+            ask_scales();
             load_k();
             __builtin_amdgcn_sched_barrier(0);
             load_scales_and_v();
@@ -767,8 +774,8 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         auto get_scales = [&](float4_t (&ks)[2], float4_t (&vs)[2]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                ks[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][step & 1][h * 16 + quarter * 4]) : k_scales[h];
-                vs[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][step & 1][32 + h * 16 + quarter * 4]) : v_scales[h];
+                ks[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][h * 16 + quarter * 4]) : k_scales[h];
+                vs[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][32 + h * 16 + quarter * 4]) : v_scales[h];
             }
         };
         // (from the thread's number anew, and so in the next: what both compute would be kept in registers through the loop)
@@ -803,17 +810,16 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             const uint32_t next = key + WAVES * 32;
             set_priority(x, key);
             if constexpr (more()) locate(next);
-            if constexpr (kInLds) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * S::kLoads) : "memory");    // (the scales: only keys and values have been asked for since)
+            put_scales();
             // the keys' registers are free for the next once the scores are there, the others' at the end
             sums.step(key + 32 > x.all_see, get_k, get_v, get_q, get_unit, get_scales, sees, hide, [&] {
-                if constexpr (more()) copy_scales(step + 1);
+                if constexpr (more()) ask_scales();
                 if constexpr (more()) load_k();
                 __builtin_amdgcn_sched_barrier(0);
             });
             if constexpr (more()) load_scales_and_v();
             __builtin_amdgcn_sched_barrier(0);
             key = next;
-            ++step;
         };
 #pragma unroll 1
         while (key + WAVES * 32 < x.key1) run_step(std::true_type{});
