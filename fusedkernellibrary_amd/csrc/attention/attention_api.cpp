@@ -237,6 +237,8 @@ int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cach
     a.mask_words = uint32_t(c->mask_words); a.q_heads = uint32_t(c->q_heads); a.group = uint32_t(c->q_heads / cache->kv_heads);
     a.group_magic = magic(a.group);
     a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
+    // (without room nobody sees anything: all rows are written like rows of no sequence, and nothing is read for them)
+    if (a.room == 0) a.max_new = 0;
     a.unit_rows = plan.unit_rows;
     a.granule_log = plan.granule_log; a.lead = plan.lead; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
     a.type = c->type; a.scale = c->scale;

@@ -680,8 +680,9 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         // The pages are asked for first, which keys and values wait for, then the queries, which are made ready while those are on their way.
         uint32_t key = x.key0 + wave * 32;
         Pages pages{0, 0};
-        // (a wave without keys asks for none: where the page table has no columns there is no entry to read)
-        if (key < x.key1) pages.fetch(a, x, key >> a.cache.page_log, lane);
+        // (There is an entry to read: a sequence with rows has a key at least, see sequence_of. A wave without keys asks for its last
+        // page's: with a branch around this, heads of 192 and 256 took 6 % longer.)
+        pages.fetch(a, x, key >> a.cache.page_log, lane);
         uint4_t raw[S::kSteps];
         const uint32_t tile = kInLds ? wave : 0;
         uint64_t mask = 0;                                         // (of one tile's rows, like the queries)

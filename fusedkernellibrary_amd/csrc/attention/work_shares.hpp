@@ -23,7 +23,8 @@ __device__ __forceinline__ uint32_t thread_here() {
 // What no kernel writes while it runs, at a place that is the same for the whole wave: a scalar load.
 template <typename T> __device__ __forceinline__ T scalar(const T* p) { return *(const __attribute__((address_space(4))) T*)(uintptr_t)p; }
 
-// A sequence as the device finds it, held inside what the host was told.
+// A sequence as the device finds it, held inside what the host was told. One with rows has keys: where the page table has room for
+// no token, max_new is 0 here.
 struct Sequence { uint32_t first_token, fresh, context, total, rows; };
 __device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t end, int32_t have) {
     Sequence s;
