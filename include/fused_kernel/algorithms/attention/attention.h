@@ -63,7 +63,8 @@ inline fklhip_rows headRows(void* data, const int32_t headsInRow, const int32_t 
     return {static_cast<char*>(data) + 2 * int64_t(firstHead) * headDim, int64_t(headsInRow) * headDim, headDim};
 }
 
-// A cache that owns its pages (see fklhip_kv_cache for the layout). Not copied, only moved.
+// A cache that owns its pages (see fklhip_kv_cache for the layout). Not copied, only moved: one that was moved from has no pages,
+// and calls refuse it.
 class KvCache {
     attention_detail::DeviceMemory m_k, m_v, m_kScale, m_vScale;
     fklhip_kv_cache m_cache{};
@@ -76,6 +77,17 @@ public:
         m_kScale = attention_detail::DeviceMemory(tokens * sizeof(float));
         m_vScale = attention_detail::DeviceMemory(tokens * sizeof(float));
         m_cache = {m_k.data(), m_v.data(), static_cast<float*>(m_kScale.data()), static_cast<float*>(m_vScale.data()), pages, kvHeads, pageTokens, headDim, static_cast<int32_t>(codes)};
+    }
+    KvCache(KvCache&& other) noexcept
+        : m_k(std::move(other.m_k)), m_v(std::move(other.m_v)), m_kScale(std::move(other.m_kScale)), m_vScale(std::move(other.m_vScale)),
+          m_cache(std::exchange(other.m_cache, {})) {}
+    KvCache& operator=(KvCache&& other) noexcept {
+        m_k = std::move(other.m_k);                            // (these change places, so the description does too)
+        m_v = std::move(other.m_v);
+        m_kScale = std::move(other.m_kScale);
+        m_vScale = std::move(other.m_vScale);
+        std::swap(m_cache, other.m_cache);
+        return *this;
     }
     const fklhip_kv_cache& get() const { return m_cache; }
     operator const fklhip_kv_cache&() const { return m_cache; }

@@ -1,4 +1,5 @@
-"""The objects of the C++ host API for attention: what a TreeAttention does with its workspace while graphs name it."""
+"""The objects of the C++ host API for attention: what a TreeAttention does with its workspace while graphs name it, and
+a moved cache with its pages."""
 import ctypes as C
 import os
 
@@ -130,3 +131,13 @@ def test_a_captured_call_that_needs_more_is_refused_and_the_capture_goes_on(ops,
     finally:
         torch.cuda.synchronize()
         objects.attend_close(attend)
+
+
+def test_a_cache_that_was_moved_from_has_no_pages_of_another(objects, device):
+    """Its description goes along: what is left behind has none, or the pages it got in exchange, and no pointer that somebody else owns."""
+    made, moves = (Cache * 2)(), (Cache * 4)()
+    assert objects.cache_moves(made, moves) == 0, objects.attention_objects_error()
+    fields = lambda c: tuple(getattr(c, name) for name, _ in Cache._fields_)      # noqa: E731
+    first, other = map(fields, made)
+    assert first[:4] != other[:4] and all(first[:4]) and all(other[:4])
+    assert [fields(c) for c in moves] == [fields(Cache()), first, other, first]
