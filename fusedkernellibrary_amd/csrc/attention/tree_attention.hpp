@@ -49,18 +49,18 @@ constexpr float kStart = 6.0f, kLead = 14.0f, kLargest = 16384.0f, kLeastScale =
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -1.0e30f;         // the reference of a row that has seen no key
 
-// How a key's product with the queries is taken. The matrix unit has products of 8-bit codes themselves, for runs of 64 (int8) or
-// 128 (e4m3) elements: a query row is then a sum of two or three rows of such codes, and no key is converted.
-//   int8: in fixed point, 256 * hi + lo (bfloat16: exact for elements from 2^-7 of the row's largest on) or with a third
-//         part behind them (half precision: exact from 2^-11 on); smaller elements are off by 2^-15 (2^-22) of the largest.
-//   e4m3: what four bits hold of each element, and of what is left, twice (8 bits, all that bfloat16 has) or three times;
-//         elements below 2^-9 of the largest are off by 2^-17 of it.
-// Heads of other sizes: keys as halves.
-template <int D, int CODES> constexpr bool kCodeProducts = CODES == FKLHIP_CODES_INT8 ? D % 64 == 0 : D % 128 == 0;
+// How a key's product with the queries is taken. int8, runs of 64 elements: the matrix unit has products of the codes themselves
+// whose sums are whole numbers of 32 bits; a query row is then a sum of two or three rows of codes, and no key is converted: in
+// fixed point, 256 * hi + lo (bfloat16: exact for elements from 2^-7 of the row's largest on) or with a third part behind them (half
+// precision: exact from 2^-11 on); smaller elements are off by 2^-15 (2^-22) of the largest.
+// Everything else: keys as halves, which hold their codes exactly, and sums in 32 bits. The matrix unit has products of e4m3 codes as
+// well, at a higher rate, but what it adds up of one instruction it cuts off 2^-13 below the largest product: next to one large
+// element of query and key others were lost (2^16 and 2^2 made 2^16; scores were off by up to 2^-12.5 of their largest product, and
+// are by 2^-22). That form took 67 us for trees of up to 61 (70 now), 57.5 for the step of trees in half precision (56.3).
+template <int D, int CODES> constexpr bool kCodeProducts = CODES == FKLHIP_CODES_INT8 && D % 64 == 0;
 
 using int2_t = int __attribute__((ext_vector_type(2)));
 using int4_t = int __attribute__((ext_vector_type(4)));
-using int8_t8 = int __attribute__((ext_vector_type(8)));
 
 template <int D> struct Shape {
     static constexpr int kChunk = D % 64 == 0 ? 64 : 32;   // elements of a row that one load of a lane's quarter row covers
@@ -249,7 +249,7 @@ template <int D> __device__ __forceinline__ void load_query(Args& a, const Segme
         raw[s] = *reinterpret_cast<const uint4_t*>(from + at * 2);
     }
 }
-template <int D, int CODES, int PARTS> __device__ __forceinline__ float prepare_query(Args& a, const uint4_t (&raw)[D / 32], uint32_t (&q)[kQueryRegs<D, PARTS>]) {
+template <int D, int PARTS> __device__ __forceinline__ float prepare_query(Args& a, const uint4_t (&raw)[D / 32], uint32_t (&q)[kQueryRegs<D, PARTS>]) {
     using S = Shape<D>;
     float e[S::kSteps * 8];
     uint32_t top = 0;
@@ -278,7 +278,7 @@ template <int D, int CODES, int PARTS> __device__ __forceinline__ float prepare_
             q[k] = pack2<FKLHIP_F16>(__builtin_amdgcn_ldexpf(e[2 * k], -p), __builtin_amdgcn_ldexpf(e[2 * k + 1], -p));
         // (as with codes: an infinity makes NaN of its row's scores, not an infinity of either sign)
         unit = top >= 0x7f800000u ? __builtin_nanf("") : unit;
-    } else if constexpr (CODES == FKLHIP_CODES_INT8) {
+    } else {
         // A power of two in front of the largest magnitude that leaves it below 127.5 * 2^8 (or 2^14); a row with an
         // infinity or a NaN has scores that are NaN.
         constexpr int kBits = PARTS == 2 ? 14 : 21;
@@ -301,24 +301,6 @@ template <int D, int CODES, int PARTS> __device__ __forceinline__ float prepare_
             }
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) q[part * S::kSteps * 2 + k] = w[part];
-        }
-    } else {
-        unit = top >= 0x7f800000u ? __builtin_nanf("") : unit * 0x1p-7f;
-#pragma unroll
-        for (int k = 0; k < S::kSteps * 2; ++k) {
-            float left[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) left[i] = __builtin_amdgcn_ldexpf(e[4 * k + i], 7 - p);
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                int w = __builtin_amdgcn_cvt_pk_fp8_f32(left[0], left[1], 0, false);
-                w = __builtin_amdgcn_cvt_pk_fp8_f32(left[2], left[3], w, true);
-                q[part * S::kSteps * 2 + k] = uint32_t(w);
-                float taken[4];
-                decode4<FKLHIP_CODES_E4M3>(uint32_t(w), taken);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) left[i] -= taken[i];
-            }
         }
     }
     unit = __builtin_amdgcn_ldexpf(unit, p);
@@ -359,7 +341,7 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
                 }
                 __builtin_amdgcn_sched_barrier(0);                  // (all codes at once as halves would take 32 registers)
             }
-        } else if constexpr (CODES == FKLHIP_CODES_INT8) {
+        } else {
             // the first two parts as one whole number, the third by itself: with it, 32 bits would not do
             int4_t sum[PARTS - 1][2];
 #pragma unroll
@@ -383,22 +365,6 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
                     y[h][i] = float(sum[0][h][i]);
                     if constexpr (PARTS == 3) y[h][i] = __builtin_fmaf(y[h][i], 256.0f, float(sum[1][h][i]));
                 }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::kLoads; i += 2)
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    const uint4_t u = get_q(part * S::kLoads + i), v = get_q(part * S::kLoads + i + 1);
-                    const int8_t8 row = {int(u[0]), int(u[1]), int(u[2]), int(u[3]), int(v[0]), int(v[1]), int(v[2]), int(v[3])};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const Words<S::kWords> lo = get_k(h, i), hi = get_k(h, i + 1);
-                        const int8_t8 codes = {int(lo.w[0]), int(lo.w[1]), int(lo.w[2]), int(lo.w[3]), int(hi.w[0]), int(hi.w[1]), int(hi.w[2]), int(hi.w[3])};
-                        const float4_t before = i == 0 && part == 0 ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : y[h];
-                        y[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, row, before, 0, 0, 0, 0, 0, 0);   // (e4m3 both, no scales)
-                    }
-                    if constexpr (PARTS == 3) __builtin_amdgcn_sched_barrier(0);    // (one part's registers at a time)
-                }
         }
     }
 
@@ -411,10 +377,10 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
     __device__ __forceinline__ void step(bool masked, K get_k, V get_v, Q get_q, U get_unit, G get_scales, M sees, H hide, A after_scores) {
         half8_t p[R];
         float4_t y[2], next[2];
-        // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of three parts of int8 take
-        // all registers without that.)
-        constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * (CODES == FKLHIP_CODES_INT8 ? S::kLoads : S::kLoads / 2);
-        constexpr bool kAhead = !(R == 4 && PARTS == 3 && CODES == FKLHIP_CODES_INT8);
+        // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of 128 elements take all registers
+        // without that if queries have three parts or keys are converted: trees of up to 61 took 73 us with it, and 70 without.)
+        constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * S::kLoads;
+        constexpr bool kAhead = !(R == 4 && (PARTS == 3 || (PARTS == 0 && D == 128)));
         constexpr bool kHeld = R < 4 || kRuns <= 4;
         uint4_t q[kRuns];
         auto ask_q = [&](int r) {
@@ -752,7 +718,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         uint32_t q[kRegs];
         float unit = 0.0f;
         if (tile < R) {
-            unit = prepare_query<D, CODES, PARTS>(kernel_args(), raw, q);
+            unit = prepare_query<D, PARTS>(kernel_args(), raw, q);
             if constexpr (kInLds) {
 #pragma unroll
                 for (int run = 0; run < kRuns; ++run) queries[(tile * kRuns + run) * 64 + lane] = uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};

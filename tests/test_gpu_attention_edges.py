@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import attention_reference as ref
+
 pytestmark = pytest.mark.gpu
 
 INT8, E4M3 = torch.int8, torch.float8_e4m3fn
@@ -245,3 +247,33 @@ def test_outputs_that_overlap_themselves_are_refused(ops, device):
             call()
     # inputs may overlap: one row for all tokens
     assert torch.equal(ops.qk_norm_rope(one + 1, one, None, None, None, None, None)[1], one)
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("large", [1.0, 40.0])
+@pytest.mark.parametrize("new", [1, 20])
+def test_scores_next_to_one_large_product(ops, device, kind, dtype, dim, large, new):
+    """One channel of queries and keys is larger than the rest, as in many models: the other channels' part of a score has to stay.
+    A row that sees one key has that key's score for its lse."""
+    g, batch, heads = gen(dim), 40, 16
+    x = torch.randn((batch * 32, 1, dim), generator=g)
+    x[..., 5] *= large
+    q = torch.randn((batch * new, heads, dim), generator=g)
+    q[..., 5] *= large
+    q, x = q.to(dtype), x.to(dtype)
+    cache = ops.KvCache.allocate(batch * 2, 1, 16, dim, codes=kind, device=device)
+    ops.kv_write(cache, x.to(device), x.to(device), torch.arange(batch * 32, dtype=torch.int32, device=device))
+    mask = torch.randint(0, new, (batch * new,), generator=g)
+    lse = torch.zeros((batch * new, heads), device=device)
+    ops.tree_attention(q.to(device), cache, torch.arange(batch * 2, dtype=torch.int32, device=device).view(batch, 2), ints(device, *[0] * batch), ints(device, *range(0, batch * new + 1, new)),
+                       max_new=new, max_context=0, mask=(1 << mask)[:, None].to(device), lse=lse, scale=0.25)
+    k = ref.Slots.of(cache).keys(torch.arange(batch * 32))[torch.arange(batch).repeat_interleave(new) * 32 + mask]                # [rows, 1, dim]
+    q = q.double()
+    want, size = (q * k).sum(-1) * 0.25, (q * k).abs().sum(-1) * 0.25
+    # what of a query's elements may be cut off, in parts of its row's largest (fixed point of 14 or 21 bits for int8, subnormal halves
+    # else); products and sums in 32 bits; the scaling by three factors and the two logarithms
+    cut = {(INT8, BF16): 2.0 ** -15, (INT8, F16): 2.0 ** -22}.get((kind, dtype), 2.0 ** -24) if kind == E4M3 or dim % 64 == 0 else 2.0 ** -24
+    bound = cut * q.abs().amax(-1) * k.abs().sum(-1) * 0.25 + (dim + 8) * 2.0 ** -24 * size + 2.0 ** -21 * want.abs() + 2.0 ** -20
+    ref.check(lse, want, bound)
