@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import attention_reference as ref
+from test_gpu_attention import run_attention, tree_mask
 
 pytestmark = pytest.mark.gpu
 
@@ -247,6 +248,26 @@ def test_outputs_that_overlap_themselves_are_refused(ops, device):
             call()
     # inputs may overlap: one row for all tokens
     assert torch.equal(ops.qk_norm_rope(one + 1, one, None, None, None, None, None)[1], one)
+
+
+@pytest.mark.parametrize("scale", [-0.1, -0.0, 0.0, 0.5])
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,new,said", [(64, 3, None), (96, 12, None), (128, 1, 9000), (128, 40, 9000), (256, 9, None)])
+def test_scales_of_all_signs(ops, device, scale, kind, dtype, dim, new, said):
+    """Below 0 the queries turn round, of 0 every key weighs the same."""
+    out = run_attention(ops, device, context=[40, 0, 77], new=[new] * 3, hq=4, hkv=2, dim=dim, page=16, kind=kind, dtype=dtype, seed=dim, said=said, scale=scale,
+                        mask=tree_mask([new] * 3, 1, gen(dim)) if new > 1 else None)
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, F16)])
+@pytest.mark.parametrize("new,dim,hq,words", [([65, 100, 3], 128, 2, 2), ([130, 64, 128], 64, 4, 3), ([200, 1, 70], 256, 1, 5)])
+def test_masks_of_several_words_over_shares(ops, device, kind, dtype, new, dim, hq, words):
+    """Words of masks are read again for each share of a row's keys; more words than the longest tree needs may be there."""
+    import fusedkernellibrary_amd as fkl
+    run_attention(ops, device, context=[300, 0, 61], new=new, hq=hq, hkv=1, dim=dim, page=32, kind=kind, dtype=dtype, seed=dim, said=20000, mask=tree_mask(new, words, gen(dim)))
+    assert fkl.last_launch()["grid"][1:] == [1, 1] and fkl.last_launch()["grid"][0] >= 64
 
 
 @pytest.mark.parametrize("kind", [INT8, E4M3])
