@@ -296,10 +296,12 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     p.row_blocks = blocks(p.tiles);
     p.lead = p.tiles == 1 ? 1 : p.tiles == 2 ? 3 : 5;
     if (!whole) {
-        // as many shares as workgroups run at once, or a power of two that leaves two granules to each; none where the order of launch
-        // evens things out, as many times more row blocks do, or a single sequence's that are twice as many (2048 tokens by
-        // themselves, 32 and 8 heads of 128: 65 us, and 90 in shares; behind 4000 others 195 and 225; several sequences may be of
-        // all lengths)
+        // As many shares as workgroups run at once, or a power of two that leaves two granules to each; none where the order of launch
+        // evens things out, as four times as many row blocks do, or a single sequence's that are twice as many. Measured, prompts over
+        // 32 and 8 heads of 128, int8 (whole blocks, shares, in us): 2048 tokens 75.5, 99.7; behind 4000 others 241, 267; 4096 tokens
+        // 228, 312; two of 2048 141, 212; three of 1500 134, 186; four of 1100 114, 171; 2048 and 300 85, 125; 1500, 200 and 700 67, 98.
+        // Both bounds are high: of what stays in shares, one of 1100 takes 59.2 and would take 33.7, two 98 and 63, three 124 and 87,
+        // two of 1500 137 and 92.
         const uint64_t all = units(p.tiles) * (p.lead + length);
         p.share_odd = slots == 512 && p.tiles == 1 ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;

@@ -393,7 +393,9 @@ __global__ __launch_bounds__(256) void k_read(const ReadArgs a) {
 uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
 // Few rows of keys: one head of a token to a group of lanes, so that everything runs at once (504 tokens of 28 and 4 heads of 128
-// written 5.4 us, 7.0 in the form of many; 2048 tokens of 8 heads 11.1 and 8.4). Many: a group has several heads of a token, whose
+// written 5.4 us, 7.0 in the form of many; 2048 tokens of 8 heads 11.1 and 8.4). Norm and rotation alone turn at about the same
+// number, whatever queries there are (few, many): 500 tokens of 28 and 4 heads 4.0 and 5.3, 1000 6.1 and 6.9, 1500 7.9 and 8.3, 760 of 64
+// and 8 8.4 and 9.1, 1500 of 64 and 4 12.9 and 12.5, 6000 of 8 and 1 9.5 and 9.0. Many: a group has several heads of a token, whose
 // rows it asks for together and which share its cosines, sines and slot. Values of 2 and 4 heads (16384 tokens): norm and rotation
 // of 40 heads of 128 71.3 and 68.8 us (one head: 86.2), of 24 of 64 20.8 and 19.7; with the write, whose quantising takes more
 // registers, of 32, 8 and 8 heads of 128 82.9 and 87.9 (one: 99.4), of 16, 8 and 8 of 64 28.1 and 33.6; reading 8 heads of

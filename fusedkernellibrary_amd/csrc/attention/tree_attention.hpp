@@ -2,9 +2,9 @@
 //
 // Mathematics. For the rows r of a key head (its query heads times the sequence's new tokens) and the keys j a row sees:
 //   s_rj = scale * ks_j * (q_r . kc_j),   o_r = sum_j e^(s_rj - m_r) vs_j vc_j / sum_j e^(s_rj - m_r)
-// with kc, vc the cache's codes and ks, vs their scales. The products run on the codes themselves and the scales enter as one
-// factor per key: ks on the scores, vs on the weights. A query row is brought to a common size by a power of two, which is
-// exact, and held as a sum of 8-bit codes (kCodeProducts) or in half precision. Weights are rounded to half precision, and
+// with kc, vc the cache's codes and ks, vs their scales. The products run on the codes, as they are or exactly in half precision,
+// and the scales enter as one factor per key: ks on the scores, vs on the weights. A query row is brought to a common size by a
+// power of two, which is exact, and held as a sum of 8-bit codes (kCodeProducts) or in half precision. Weights are rounded to half precision, and
 // values are exact in it (int8: 8 bits, e4m3: 4 bits of 11); all sums are in 32 bits.
 //
 // One pass over the keys, 32 at a time, everything in registers: S^T = K Q^T comes out of the matrix unit with a query row to
@@ -13,19 +13,21 @@
 // side for that reason. So nothing moves between lanes, and the running maximum is per lane column.
 //
 // A workgroup takes R tiles of 16 rows of a key head, and its waves other keys of the same segment, 32 in turn; the waves' sums
-// are joined in LDS at the end. R is 1, 2 or 4: a key's conversion, its loads and its scales serve all R. One tile's queries
+// are joined in LDS at the end. R is 1, 2 or 4: a key's loads and scales, and a value's conversion, serve all R. One tile's queries
 // stay in registers; more are in LDS, as their sums take the registers. Four tiles of 128 elements are 128 registers of
 // sums, which leaves two waves to a SIMD.
 //
-// What bounds it. One tile: reading the cache. 64 sequences with 900 to 8191 keys (8 key heads of 128, int8, 616 MB) take 113 us
-// and 5.7 for joining, 5.4 TB/s; 48 with 4000 to 32700 (e4m3, 1.86 GB) 326 and 8 us, 5.7 TB/s; a kernel that only reads reaches
-// 6.3. Four tiles: the vector unit. 32 keys take a wave 38 instructions and 8 exponentials per tile (one scaling, one fused
-// subtraction, one exponential, one value scale, one sum and half a comparison per score), and the matrix unit 1024 cycles, of
-// which it hides about a third from two waves a SIMD: 16 trees of up to 61 tokens over 500 to 4100 keys (25.9 Gflop) take 62 us
-// and 9.3 for joining, where the products alone are 22 at the rate of a large matrix product. 131003 keys with 56 rows (277 MB)
-// take 67 and 6.5 us, where reading is 44. What was tried on four tiles: workgroups side by side that share a unit's keys in the
-// L2 cache (no faster per key, and slower for trees that leave some of them without rows), and a touch of the lines two steps ahead (88 us
-// for 68). Queries are read from LDS a tile ahead, between two tiles' products and weights (1.5 us of 64).
+// What bounds it (times by kernel of a profile). One tile: reading the cache. 64 sequences with 900 to 8191 keys (8 key heads of 128,
+// int8, 616 MB) take 114 us and 5.8 for joining, 5.4 TB/s; 48 with 4000 to 32700 (e4m3, 1.86 GB) 326 and 8.4 us, 5.7 TB/s; a kernel
+// that only reads reaches 6.3. Four tiles: waits, with two waves to a SIMD to fill them. 16 trees of up to 61 tokens over 500 to 4100
+// keys (e4m3, 25.9 Gflop) take 67 us and 9.4 for joining, where the products alone are 22 at the rate of a large matrix product:
+// a wave's time is 40 % waits for memory and LDS, 21 % waits to issue, 28 % vector instructions (38 and 8 exponentials for a tile and
+// 32 keys: one scaling, one fused subtraction, one exponential, one value scale, one sum and half a comparison per score, besides
+// conversions); the matrix unit is busy a fifth of it. Each tile waits for what it reads from LDS: its queries, or, where the next
+// tile's are read ahead, its scales behind those. 131003 keys with 56 rows (int8, 277 MB) take 68 and 6.8 us, where reading is 44, with the same shares. What was tried
+// on four tiles: workgroups side by side that share a unit's keys in the L2 cache (no faster per key, and slower for trees that
+// leave some of them without rows), and a touch of the lines two steps ahead (88 us for 68). Two parts of int8 queries are read from
+// LDS in front of the weights of the tile before theirs (1.5 us of 64).
 //
 // How the work is dealt out. The device alone knows the sequences' lengths, so every workgroup adds them up: the keys of all
 // (sequence, key head, block of rows), one behind the other, are cut into equal shares, one to a workgroup, all of which run
