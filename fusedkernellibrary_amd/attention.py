@@ -17,6 +17,8 @@ cache reads).
 """
 from __future__ import annotations
 
+import typing as _typing
+
 import torch as _torch
 
 from . import lib as _lib
@@ -68,18 +70,20 @@ class KvCache:
         return cls(k, v, *scales)
 
 
-def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float = 1e-6, pairs: bool = False, q_out=None, k_out=None):
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, *, eps: float = 1e-6, pairs: bool = False, q_out=None, k_out=None, axes=None):
     """RMS norm of every head of q [tokens, q_heads, head_dim] and k [tokens, kv_heads, head_dim] and rotation by position.
 
     Weights None: no norm; cos and sin None: no rotation. cos and sin are [positions, rotated / 2]; elements i and
-    i + rotated / 2 turn together, or 2i and 2i + 1 with pairs. q_out and k_out may be q and k. Returns (q_out, k_out)."""
-    return _native.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, q_out, k_out)
+    i + rotated / 2 turn together, or 2i and 2i + 1 with pairs. With axes, a whole number for each of the rotated / 2 pairs,
+    positions is [axes, tokens], up to 4, and pair i turns by the positions of axes[i] (an image's or a video's time, height and
+    width). q_out and k_out may be q and k. Returns (q_out, k_out)."""
+    return _native.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, q_out, k_out, axes)
 
 
-def qkv_to_cache(cache: KvCache, q, k, v, slots, q_weight, k_weight, cos, sin, positions, *, eps: float = 1e-6, pairs: bool = False, q_out=None):
+def qkv_to_cache(cache: KvCache, q, k, v, slots, q_weight, k_weight, cos, sin, positions, *, eps: float = 1e-6, pairs: bool = False, q_out=None, axes=None):
     """qk_norm_rope, with the keys and values [tokens, kv_heads, head_dim] quantised into the cache's slots (int32; one
     outside of the cache stores nothing) in the same launch. Returns q_out."""
-    return _native.qkv_to_cache(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, v, slots, cache._tensors, q_out)
+    return _native.qkv_to_cache(q, k, q_weight, k_weight, cos, sin, positions, eps, pairs, v, slots, cache._tensors, q_out, axes)
 
 
 def kv_write(cache: KvCache, k, v, slots) -> None:
@@ -103,3 +107,54 @@ def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: 
     All of them see the whole context. Rows that see nothing are zero, and so are those of no sequence (a padded batch's).
     lse [tokens, q_heads] float32 receives the logarithm of the sum of exponentials if it is given. Returns out."""
     return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse)
+
+
+class StepTables(_typing.NamedTuple):
+    """What step_tables returns; the names are those of the arguments that take them."""
+    q_start: _torch.Tensor          # [batch + 1]
+    slots: _torch.Tensor            # [tokens]
+    positions: _torch.Tensor        # [tokens]
+    held: _torch.Tensor             # [batch]
+    available: _torch.Tensor        # [1]
+    mask: _torch.Tensor | None      # [tokens, words] int64, of trees
+
+
+def step_tables(page_table, held, context, new, free, available, *, page_tokens: int, tokens: int, max_new: int, parents=None) -> StepTables:
+    """The tables of a step from its requests' lengths, in one launch and without a look at them on the host. All are int32.
+
+    Request b has context[b] tokens in the cache, the first held[b] entries of page_table[b] and new[b] (at most max_new) new
+    tokens. The pages that those need are taken from the end of the first `available` [1] entries of free, request by request,
+    and written to page_table; held and available are returned as they are afterwards (available is negative by the pages that
+    were missing; a token without a page has slot -1). The step has `tokens` rows: rows behind the last request's have slot
+    -1, position 0 and an empty mask. With parents [tokens], new token t of a sequence follows its new token
+    parents[row] < t (-1: none): its position is context + the number of its ancestors, and its mask has them and itself."""
+    return StepTables(*_native.step_tables(page_table, held, context, new, free, available, page_tokens, tokens, max_new, parents))
+
+
+class Verified(_typing.NamedTuple):
+    """What verify_drafts returns, int32."""
+    path: _torch.Tensor             # [batch, max_new]: the accepted rows, counted from the sequence's first; then -1
+    count: _torch.Tensor            # [batch]: how many they are
+    out: _torch.Tensor              # [batch, max_new]: the tokens that were decided, as many; then -1
+
+
+def verify_drafts(target, tokens, q_start, uniforms, *, max_new: int, draft=None, parents=None) -> Verified:
+    """Drafted tokens against the target's probabilities, by random numbers that are given.
+
+    Sequence b's rows are q_start[b] to q_start[b + 1] (at most max_new, up to 1024): the first is of the last token that is
+    decided, the others of drafted ones, tokens[row] (int32). target [tokens, vocabulary] (float32, bfloat16 or float16) has the
+    probabilities of what follows each row. Row t follows row parents[row] < t, counted from its sequence's first, or row t - 1.
+    The children of the last accepted row are asked in their order: one with token x is accepted if target[parent, x] >
+    uniforms[row] * draft[row, x], draft being the probabilities that the tokens were drawn from (of chains), or without draft >
+    uniforms[row] * (1 - what the refused children in front of it had). Where none is accepted the next token is drawn from
+    max(target - draft, 0) of the refused row, from target without the refused tokens, or from target, by the uniform [0, 1) of
+    the sequence's first row. Tokens come out distributed as if drawn from target one by one."""
+    return Verified(*_native.verify_drafts(target, tokens, q_start, uniforms, max_new, draft, parents))
+
+
+def kv_keep(caches, page_table, context, path, count) -> None:
+    """Moves the rows of accepted tokens to where their sequences go on, in a cache or in those of several layers at once: what
+    is at place context[b] + path[b, i] of sequence b goes to place context[b] + i, for i from 1 up to count[b]. path (as
+    verify_drafts returns it) ascends. No cache is given twice, and no two sequences share a page where something moves."""
+    caches = (caches,) if isinstance(caches, KvCache) else caches
+    _native.kv_keep(tuple(c._tensors for c in caches), page_table, context, path, count)

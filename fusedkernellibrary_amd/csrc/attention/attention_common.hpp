@@ -34,6 +34,12 @@ struct HeadArgs {
     float eps;
 };
 
+// With positions of several axes, one array behind the other; two bits of of_pairs say a pair's.
+struct AxesHeadArgs : HeadArgs {
+    int64_t position_stride;
+    uint32_t axes, of_pairs[8];
+};
+
 struct ReadArgs {
     Cache cache;
     Rows k, v;
@@ -62,6 +68,7 @@ struct AttentionArgs {
 // Launchers (defined next to their kernels). Grids are laid out by the callers' arguments alone.
 struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
 int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
+int launch_heads(const AxesHeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream);
 // How a call is run: 16-row tiles (and so rows) and waves to a workgroup; row blocks of a sequence; share_odd << share_log

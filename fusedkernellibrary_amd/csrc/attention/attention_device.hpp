@@ -17,9 +17,9 @@ using uint4_t = uint32_t __attribute__((ext_vector_type(4)));
 constexpr float kTopInt8 = 127.0f, kTopE4M3 = 448.0f;
 
 // Launches a kernel of one argument; the runtime's code, of this launch and not of what was before it.
-template <typename A> int launch(void (*kernel)(A), dim3 grid, dim3 block, void* stream, A args) {
+template <typename A> int launch(void (*kernel)(A), dim3 grid, dim3 block, void* stream, A args, size_t lds = 0) {
     void* ptrs[] = {&args};
-    return int(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, 0, static_cast<hipStream_t>(stream)));
+    return int(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, lds, static_cast<hipStream_t>(stream)));
 }
 
 // ---- 16-bit types ----------------------------------------------------------------------------------------------------

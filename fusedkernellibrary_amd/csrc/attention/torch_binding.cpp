@@ -17,8 +17,12 @@
 
 #include <fklhip.h>
 
+#include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <memory>
 #include <string>
+#include <vector>
 
 namespace {
 
@@ -176,8 +180,29 @@ void on_device(const Tensor& t, const char* name, const CacheView& c) {
 
 // ---- heads ------------------------------------------------------------------------------------------------------------
 
-// q, k, q_weight, k_weight, cos, sin, positions, eps, pairs
-void heads_of(PyObject* const* a, fklhip_heads& h) {
+// Axes of pairs: None, or a sequence of whole numbers, and positions [axes, tokens] then.
+struct AxesView : fklhip_axes {
+    bool given = false;
+};
+AxesView axes_of(PyObject* o, int64_t pairs) {
+    AxesView x{};
+    if (none(o)) return x;
+    PyObject* items = PySequence_Fast(o, "axes has to be a sequence of whole numbers");
+    if (!items) throw python_error();
+    const std::unique_ptr<PyObject, void (*)(PyObject*)> held(items, [](PyObject* p) { Py_DECREF(p); });
+    if (PySequence_Fast_GET_SIZE(items) != pairs || pairs > 128) refuse("axes has to have an axis for each of " + std::to_string(pairs) + " pairs, up to 128");
+    for (int64_t i = 0; i < pairs; ++i) {
+        const int64_t axis = whole(PySequence_Fast_GET_ITEM(items, i));
+        if (axis < 0 || axis > 3) refuse("an axis has to be 0 to 3");
+        x.of_pair[i] = uint8_t(axis);
+    }
+    x.given = true;
+    return x;
+}
+
+// q, k, q_weight, k_weight, cos, sin, positions, eps, pairs; axes
+AxesView heads_of(PyObject* const* a, PyObject* of_pairs, fklhip_heads& h) {
+    AxesView axes{};
     const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k");
     if (q.dim() != 3 || k.dim() != 3) refuse("q and k have to be [tokens, heads, head_dim]");
     h.type = type_of(q, "q");
@@ -200,25 +225,37 @@ void heads_of(PyObject* const* a, fklhip_heads& h) {
         h.rot_dim = int32_t(2 * cos.size(1));
         h.cos = static_cast<const float*>(plain(cos, "cos", at::kFloat, cos.sizes(), q.device()));
         h.sin = static_cast<const float*>(plain(tensor(a[5], "sin"), "sin", at::kFloat, cos.sizes(), q.device()));
-        h.positions = static_cast<const int32_t*>(plain(tensor(a[6], "positions"), "positions", at::kInt, {tokens}, q.device()));
+        axes = axes_of(of_pairs, cos.size(1));
+        const Tensor& positions = tensor(a[6], "positions");
+        if (axes.given) {
+            if (positions.dim() != 2 || positions.size(0) < 1 || positions.size(0) > 4) refuse("positions has to be [axes, tokens] with axes, of 1 to 4");
+            axes.count = int32_t(positions.size(0));
+            axes.stride = tokens;
+            h.positions = static_cast<const int32_t*>(plain(positions, "positions", at::kInt, {positions.size(0), tokens}, q.device()));
+        } else {
+            h.positions = static_cast<const int32_t*>(plain(positions, "positions", at::kInt, {tokens}, q.device()));
+        }
+    } else if (!none(of_pairs)) {
+        refuse("axes without cos and sin");
     }
     h.eps = float(number(a[7]));
     h.pairs = PyObject_IsTrue(a[8]);
+    return axes;
 }
 
-// ..., q_out, k_out
+// ..., q_out, k_out, axes
 PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 11);
+    expect(n, 12);
     at::AutoDispatchBelowAutograd quick;
     fklhip_heads h{};
-    heads_of(a, h);
+    const AxesView axes = heads_of(a, a[11], h);
     const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]);
     void* stream = stream_of(q, "q");
     const Tensor q_out = output(a[9], "q_out", q.sizes(), q.scalar_type(), q.device()), k_out = output(a[10], "k_out", k.sizes(), q.scalar_type(), q.device());
     h.q_out = rows(q_out, "q_out", h.tokens, h.q_heads, h.head_dim, q);
     h.k_out = rows(k_out, "k_out", h.tokens, h.kv_heads, h.head_dim, q);
-    check(fklhip_qk_norm_rope(&h, stream), "qk_norm_rope");
+    check(axes.given ? fklhip_qk_norm_rope_axes(&h, &axes, stream) : fklhip_qk_norm_rope(&h, stream), "qk_norm_rope");
     PyObject* both = PyTuple_New(2);
     if (!both) throw python_error();
     PyTuple_SET_ITEM(both, 0, result(a[9], q_out));
@@ -227,13 +264,13 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// ..., v, slots, cache, q_out
+// ..., v, slots, cache, q_out, axes
 PyObject* qkv_to_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 13);
+    expect(n, 14);
     at::AutoDispatchBelowAutograd quick;
     fklhip_heads h{};
-    heads_of(a, h);
+    const AxesView axes = heads_of(a, a[13], h);
     const Tensor& q = THPVariable_Unpack(a[0]);
     const CacheView c = cache_of(a[11]);
     on_device(q, "q", c);
@@ -242,7 +279,7 @@ PyObject* qkv_to_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     h.slots = static_cast<const int32_t*>(plain(tensor(a[10], "slots"), "slots", at::kInt, {h.tokens}, q.device()));
     const Tensor q_out = output(a[12], "q_out", q.sizes(), q.scalar_type(), q.device());
     h.q_out = rows(q_out, "q_out", h.tokens, h.q_heads, h.head_dim, q);
-    check(fklhip_qkv_to_cache(&h, &c.c, stream), "qkv_to_cache");
+    check(axes.given ? fklhip_qkv_to_cache_axes(&h, &axes, &c.c, stream) : fklhip_qkv_to_cache(&h, &c.c, stream), "qkv_to_cache");
     written(a[11]);
     return result(a[12], q_out);
     END_HANDLE_TH_ERRORS
@@ -349,9 +386,143 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- a step's tables --------------------------------------------------------------------------------------------------
+
+int32_t* ints(PyObject* o, const char* name, at::IntArrayRef shape, c10::Device device) { return static_cast<int32_t*>(plain(tensor(o, name), name, at::kInt, shape, device)); }
+PyObject* tuple_of(std::initializer_list<const Tensor*> tensors) {
+    PyObject* all = PyTuple_New(Py_ssize_t(tensors.size()));
+    if (!all) throw python_error();
+    Py_ssize_t i = 0;
+    for (const Tensor* t : tensors) {
+        PyObject* o = Py_None;
+        if (t) o = THPVariable_Wrap(*t);
+        else Py_INCREF(o);
+        PyTuple_SET_ITEM(all, i++, o);
+    }
+    return all;
+}
+
+// page_table, held, context, new, free, available, page_tokens, tokens, max_new, parents
+PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 10);
+    at::AutoDispatchBelowAutograd quick;
+    const Tensor &table = tensor(a[0], "page_table"), &free = tensor(a[4], "free");
+    if (table.dim() != 2 || table.size(0) > 65535) refuse("page_table has to be [batch, pages of a sequence], batch up to 65535");
+    if (free.dim() != 1) refuse("free has to have one dimension");
+    void* stream = stream_of(table, "page_table");
+    const c10::Device device = table.device();
+    const int64_t batch = table.size(0), tokens = whole(a[7]);
+    if (tokens < 0 || tokens >= int64_t(1) << 30) refuse("tokens has to be 0 or more, below 2^30");
+    fklhip_tables t{};
+    t.page_table = ints(a[0], "page_table", table.sizes(), device);
+    t.held = ints(a[1], "held", {batch}, device);
+    t.context = ints(a[2], "context", {batch}, device);
+    t.fresh = ints(a[3], "new", {batch}, device);
+    t.free_pages = ints(a[4], "free", free.sizes(), device);
+    t.available = ints(a[5], "available", {1}, device);
+    t.page_table_stride = table.size(1); t.free_count = free.size(0); t.tokens = tokens; t.batch = int32_t(batch);
+    t.page_tokens = whole32(a[6], "page_tokens");
+    t.max_new = whole32(a[8], "max_new");
+    const bool trees = !none(a[9]);
+    if (trees) t.parents = ints(a[9], "parents", {tokens}, device);
+    if (t.max_new < 0) refuse("max_new has to be 0 or more");
+    t.mask_words = trees ? std::max(1, int32_t((int64_t(t.max_new) + 63) / 64)) : 0;
+    if (trees && int64_t(t.mask_words) * tokens >= int64_t(1) << 31) refuse("masks of more than 2^31 words");
+    const Tensor q_start = empty({batch + 1}, at::kInt, device), slots = empty({tokens}, at::kInt, device), positions = empty({tokens}, at::kInt, device), held = empty({batch}, at::kInt, device),
+                 left = empty({1}, at::kInt, device);
+    Tensor mask;
+    if (trees) {
+        mask = empty({tokens, t.mask_words}, at::kLong, device);
+        t.mask = static_cast<uint64_t*>(mask.data_ptr());
+    }
+    t.q_start = q_start.data_ptr<int32_t>(); t.slots = slots.data_ptr<int32_t>(); t.positions = positions.data_ptr<int32_t>();
+    t.held_out = held.data_ptr<int32_t>(); t.left = left.data_ptr<int32_t>();
+    check(fklhip_step_tables(&t, stream), "step_tables");
+    written(table);
+    return tuple_of({&q_start, &slots, &positions, &held, &left, trees ? &mask : nullptr});
+    END_HANDLE_TH_ERRORS
+}
+
+// target, tokens, q_start, uniforms, max_new, draft, parents
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7);
+    at::AutoDispatchBelowAutograd quick;
+    const Tensor &target = tensor(a[0], "target"), &q_start = tensor(a[2], "q_start");
+    fklhip_drafts d{};
+    if (target.dim() != 2 || target.size(1) < 1 || target.size(1) > 1 << 24) refuse("target has to be [tokens, vocabulary], of 1 to 2^24");
+    if (q_start.dim() != 1 || q_start.size(0) < 1 || q_start.size(0) > 65536) refuse("q_start has to be [batch + 1], batch up to 65535");
+    d.type = target.scalar_type() == at::kFloat ? FKLHIP_F32 : target.scalar_type() == at::kBFloat16 ? FKLHIP_BF16 : target.scalar_type() == at::kHalf ? FKLHIP_F16 : -1;
+    if (d.type < 0) refuse("target has to be torch.float32, torch.bfloat16 or torch.float16");
+    void* stream = stream_of(target, "target");
+    const c10::Device device = target.device();
+    const int64_t tokens = target.size(0), vocab = target.size(1), batch = q_start.size(0) - 1;
+    const auto table = [&](const Tensor& t, const char* name, int64_t& stride) -> const void* {
+        if (t.dim() != 2 || t.size(0) != tokens || t.size(1) != vocab || t.scalar_type() != target.scalar_type() || t.device() != device || (vocab > 1 && t.stride(1) != 1))
+            refuse(std::string(name) + " has to be " + shape_text({tokens, vocab}) + " of " + c10::toString(target.scalar_type()) + " on " + device.str() + " with a tight last dimension");
+        serves(t, name);
+        holds(t, name);
+        stride = t.stride(0);
+        return t.data_ptr();
+    };
+    d.target = table(target, "target", d.target_stride);
+    d.ids = ints(a[1], "tokens", {tokens}, device);
+    d.q_start = ints(a[2], "q_start", {batch + 1}, device);
+    d.uniforms = static_cast<const float*>(plain(tensor(a[3], "uniforms"), "uniforms", at::kFloat, {tokens}, device));
+    d.max_new = whole32(a[4], "max_new");
+    if (d.max_new < 0 || d.max_new > 1024) refuse("max_new has to be up to 1024");
+    if (!none(a[5])) d.draft = table(tensor(a[5], "draft"), "draft", d.draft_stride);
+    if (!none(a[6])) d.parents = ints(a[6], "parents", {tokens}, device);
+    if (!none(a[5]) && !none(a[6])) refuse("draft's probabilities are of chains: not with parents");
+    d.tokens = tokens; d.batch = int32_t(batch); d.vocab = int32_t(vocab);
+    const Tensor path = empty({batch, d.max_new}, at::kInt, device), count = empty({batch}, at::kInt, device), out = empty({batch, d.max_new}, at::kInt, device);
+    d.path = path.data_ptr<int32_t>(); d.count = count.data_ptr<int32_t>(); d.out = out.data_ptr<int32_t>();
+    uint64_t bytes = 0;
+    check(fklhip_verify_drafts_workspace(&d, &bytes), "verify_drafts");
+    Tensor workspace;                                          // (given back to torch's allocator, in the stream's order, on return)
+    if (bytes) {
+        workspace = empty({int64_t(bytes)}, at::kByte, device);
+        d.workspace = workspace.data_ptr();
+        d.workspace_bytes = bytes;
+    }
+    check(fklhip_verify_drafts(&d, stream), "verify_drafts");
+    if (batch != 0 && d.max_new == 0) Tensor(count).zero_();   // (nothing was launched)
+    return tuple_of({&path, &count, &out});
+    END_HANDLE_TH_ERRORS
+}
+
+// caches (a tuple of their tensors), page_table, context, path, count
+PyObject* kv_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 5);
+    if (!PyTuple_Check(a[0])) refuse("not caches");
+    const Py_ssize_t layers = PyTuple_GET_SIZE(a[0]);
+    if (layers > 1024) refuse("more than 1024 caches");
+    const Tensor &table = tensor(a[1], "page_table"), &path = tensor(a[3], "path");
+    if (table.dim() != 2 || table.size(0) > 65535) refuse("page_table has to be [batch, pages of a sequence], batch up to 65535");
+    if (path.dim() != 2 || path.size(1) > 1 << 20) refuse("path has to be [batch, max_new], max_new up to 2^20");
+    void* stream = stream_of(table, "page_table");
+    const c10::Device device = table.device();
+    const int64_t batch = table.size(0);
+    std::vector<fklhip_kv_cache> caches;
+    caches.reserve(size_t(layers));
+    for (Py_ssize_t i = 0; i < layers; ++i) {
+        const CacheView c = cache_of(PyTuple_GET_ITEM(a[0], i));
+        on_device(table, "page_table", c);
+        caches.push_back(c.c);
+    }
+    const int32_t *t = ints(a[1], "page_table", table.sizes(), device), *context = ints(a[2], "context", {batch}, device), *p = ints(a[3], "path", {batch, path.size(1)}, device),
+                  *count = ints(a[4], "count", {batch}, device);
+    check(fklhip_kv_keep(caches.data(), int32_t(layers), t, table.size(1), context, p, count, int32_t(batch), int32_t(path.size(1)), stream), "kv_keep");
+    for (Py_ssize_t i = 0; i < layers; ++i) written(PyTuple_GET_ITEM(a[0], i));
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
 #define FUNCTION(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-    FUNCTION(check_cache), FUNCTION(qk_norm_rope), FUNCTION(qkv_to_cache), FUNCTION(kv_write), FUNCTION(kv_read), FUNCTION(tree_attention),
+    FUNCTION(check_cache), FUNCTION(qk_norm_rope), FUNCTION(qkv_to_cache), FUNCTION(kv_write), FUNCTION(kv_read), FUNCTION(tree_attention), FUNCTION(step_tables), FUNCTION(verify_drafts), FUNCTION(kv_keep),
 #undef FUNCTION
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attention", "Calls of fusedkernellibrary_amd.attention", -1, methods, nullptr, nullptr, nullptr, nullptr};

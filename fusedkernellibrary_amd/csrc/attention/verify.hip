@@ -1,0 +1,343 @@
+// verify.hip -- drafted tokens against the target's probabilities, and the token that comes behind the accepted ones.
+//
+// Mathematics. From a sequence's first row on, the children of the row that the path has come to are asked in their order: child t
+// with token x is accepted if p(x) > u_t q_t(x), where p is the target's row of its parent and q_t the distribution it was drafted from; or,
+// without one, if p(x) > u_t (1 - what the refused children in front of it had). Behind the last accepted row a token is drawn from
+// w = max(p - q_t, 0) (t refused), p without the refused children's tokens, or p (nobody was asked): the first whose running
+// sum exceeds u times the whole sum. So the tokens are distributed as if drawn from the target's rows one by one.
+//
+// Sums are in 64 bits: a drawn token is a whole number, which a sum's rounding must not decide. (A sum of 10^5 float32 weights in
+// 32 bits is off by up to 10^-3 of itself in the worst order; in 64 bits a border is met with a chance of 10^-11.)
+//
+// Two launches. The first cuts a row into chunks, one to a workgroup; each finds the path for itself (a wave, by a few gathers that
+// the lanes make together: less than a launch of its own) and adds its chunk up. The second, a workgroup to a sequence, finds
+// the chunk and then the token in it. Bound by memory where the batch is large, else by the trips to memory one behind the other.
+#include <type_traits>
+
+#include "attention_device.hpp"
+#include "step_common.hpp"
+
+namespace fkattn {
+namespace {
+
+constexpr uint32_t kThreads = 256, kPerThread = 16, kChunk = kThreads * kPerThread;
+
+template <int TYPE> constexpr uint32_t kSize = TYPE == FKLHIP_F32 ? 4 : 2;
+template <int TYPE> constexpr uint32_t kRun = 16 / kSize<TYPE>;             // elements of a load
+template <int TYPE> constexpr uint32_t kRuns = kPerThread / kRun<TYPE>;
+
+// A probability: what is no number above 0 counts as 0.
+__device__ __forceinline__ float as_probability(float x) { return x > 0.0f && x < __builtin_inff() ? x : 0.0f; }
+template <int TYPE> __device__ __forceinline__ float element(const char* row, uint32_t i) {
+    if constexpr (TYPE == FKLHIP_F32) {
+        return as_probability(*reinterpret_cast<const float*>(row + size_t(i) * 4));
+    } else {
+        float a, b;
+        unpack2<TYPE>(*reinterpret_cast<const uint16_t*>(row + size_t(i) * 2), a, b);
+        return as_probability(a);
+    }
+}
+typedef uint4_t aligned4_t __attribute__((aligned(4)));
+typedef uint4_t aligned2_t __attribute__((aligned(2)));
+// A run of a row from element i on; elements behind the row are 0. (Rows begin at any element: 16 bytes at a time all the same.)
+template <int TYPE> __device__ __forceinline__ void load_run(const char* row, uint32_t i, uint32_t vocab, float (&x)[kRun<TYPE>]) {
+    using loose_t = std::conditional_t<TYPE == FKLHIP_F32, aligned4_t, aligned2_t>;
+    if (i + kRun<TYPE> <= vocab) {
+        const uint4_t w = *reinterpret_cast<const loose_t*>(row + size_t(i) * kSize<TYPE>);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (TYPE == FKLHIP_F32) x[k] = __builtin_bit_cast(float, uint32_t(w[k]));
+            else unpack2<TYPE>(w[k], x[2 * k], x[2 * k + 1]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kRun<TYPE>; ++k) x[k] = as_probability(x[k]);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < kRun<TYPE>; ++k) x[k] = i + k < vocab ? element<TYPE>(row, i + k) : 0.0f;
+    }
+}
+__device__ __forceinline__ float as_uniform(float u) { return u > 0.0f ? __builtin_fminf(u, 1.0f - 0x1p-24f) : 0.0f; }
+
+struct Place { uint32_t first, count; };
+__device__ __forceinline__ Place place_of(const VerifyArgs& a, uint32_t b) {
+    const int32_t lo = a.q_start[b], hi = a.q_start[b + 1];
+    Place p;
+    p.first = lo < 0 ? 0u : min(uint32_t(lo), a.tokens);
+    const int32_t n = hi - int32_t(p.first);
+    p.count = hi < 0 || n < 0 ? 0u : min(min(uint32_t(n), a.max_new), a.tokens - p.first);
+    return p;
+}
+
+// What the path of a sequence leads to: kept for the second launch in front of the refused children's tokens.
+struct Outcome { int32_t here, against, refused, count; };                   // `against`: the refused row whose q is taken off, or -1
+
+__device__ __forceinline__ double of_lane(double v, uint32_t lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(u)), int(lane)), hi = __builtin_amdgcn_readlane(int(uint32_t(u >> 32)), int(lane));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+
+// A wave's walk from a sequence's first row; path and refused are in LDS.
+template <int TYPE> __device__ __forceinline__ Outcome find_path(const VerifyArgs& a, const Place& p, uint32_t lane, int32_t* path, int32_t* refused) {
+    Outcome o{0, -1, 0, 1};
+    double rest = 1.0;
+    if (lane == 0) path[0] = 0;
+    for (uint32_t t0 = 0; t0 < p.count; t0 += 64) {
+        const uint32_t t = t0 + lane, row = p.first + t;
+        int32_t parent = -1, id = -1;
+        float u = 0.0f;
+        if (t > 0 && t < p.count) {
+            parent = a.parents ? a.parents[row] : int32_t(t) - 1;
+            id = a.ids[row];
+            u = as_uniform(a.uniforms[row]);
+            if (parent < 0 || uint32_t(parent) >= t) parent = -1;
+        }
+        float prob = 0.0f, drafted = 0.0f;
+        if (parent >= 0 && uint32_t(id) < a.vocab) {
+            prob = element<TYPE>(a.target + int64_t(p.first + parent) * a.target_stride, uint32_t(id));
+            if (a.draft) drafted = element<TYPE>(a.draft + int64_t(row) * a.draft_stride, uint32_t(id));
+        }
+        // (a token that an elder child had, among the 64 in front, was refused with it)
+        if (parent == o.here)
+            for (int32_t i = 0; i < o.refused; ++i)
+                if (refused[i] == id) prob = 0.0f;
+        uint64_t asked = __ballot(parent == o.here);
+        while (asked) {
+            const uint32_t s = __builtin_ctzll(asked);
+            const double pd = of_lane(double(prob), s), ud = of_lane(double(u), s), qd = of_lane(double(drafted), s);
+            const int32_t its = __builtin_amdgcn_readlane(id, int(s));
+            if (pd > ud * (a.draft ? qd : rest)) {
+                o.here = int32_t(t0 + s);
+                o.refused = 0;
+                o.against = -1;
+                rest = 1.0;
+                if (lane == 0) path[o.count] = o.here;
+                ++o.count;
+                asked = __ballot(parent == o.here);
+            } else {
+                if (a.draft) o.against = int32_t(t0 + s);
+                if (lane == 0) refused[o.refused] = its;
+                ++o.refused;
+                rest -= pd;
+                if (id == its && lane > s && parent == o.here) prob = 0.0f;
+                asked &= asked - 1;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    }
+    return o;
+}
+
+// A thread's weights of a chunk: run k holds elements chunk * kChunk + (k * kThreads + thread) * kRun ..
+template <int TYPE> struct Weights {
+    double w[kRuns<TYPE>][kRun<TYPE>];
+    static __device__ __forceinline__ uint32_t at(uint32_t chunk, uint32_t k) { return chunk * kChunk + (k * kThreads + threadIdx.x) * kRun<TYPE>; }
+    __device__ __forceinline__ void load(const char* p, const char* q, uint32_t chunk, uint32_t vocab) {
+        float x[kRuns<TYPE>][kRun<TYPE>], y[kRuns<TYPE>][kRun<TYPE>];
+#pragma unroll
+        for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
+            load_run<TYPE>(p, at(chunk, k), vocab, x[k]);
+            if (q) load_run<TYPE>(q, at(chunk, k), vocab, y[k]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kRuns<TYPE>; ++k)
+#pragma unroll
+            for (uint32_t i = 0; i < kRun<TYPE>; ++i) w[k][i] = q ? __builtin_fmax(double(x[k][i]) - double(y[k][i]), 0.0) : double(x[k][i]);
+    }
+    __device__ __forceinline__ void clear(uint32_t chunk, uint32_t id) {
+#pragma unroll
+        for (uint32_t k = 0; k < kRuns<TYPE>; ++k)
+#pragma unroll
+            for (uint32_t i = 0; i < kRun<TYPE>; ++i)
+                if (at(chunk, k) + i == id) w[k][i] = 0.0;
+    }
+    __device__ __forceinline__ double sum(uint32_t k) const {
+        double s = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kRun<TYPE>; ++i) s += w[k][i];
+        return s;
+    }
+};
+
+// The sum of a workgroup's values, for every thread.
+__device__ __forceinline__ double sum_of_all(double v, double* waves) {
+#pragma unroll
+    for (int i = 32; i; i >>= 1) v += __shfl_xor(v, i);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (waves[0] + waves[1]) + (waves[2] + waves[3]);
+}
+
+template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_sums(const VerifyArgs a) {
+    extern __shared__ int32_t lists[];                                       // path and refused tokens, max_new each
+    __shared__ Outcome shared;
+    __shared__ double waves[4];
+    const uint32_t chunk = blockIdx.x, b = blockIdx.y;
+    const Place p = place_of(a, b);
+    int32_t *path = lists, *refused = lists + a.max_new;
+    if (p.count == 0) {
+        if (chunk == 0) {
+            for (uint32_t i = threadIdx.x; i < a.max_new; i += kThreads) a.path[size_t(b) * a.max_new + i] = a.out[size_t(b) * a.max_new + i] = -1;
+            if (threadIdx.x == 0) a.count[b] = 0;
+        }
+        return;
+    }
+    if (threadIdx.x < 64) {
+        const Outcome o = find_path<TYPE>(a, p, threadIdx.x, path, refused);
+        if (threadIdx.x == 0) shared = o;
+    }
+    __syncthreads();
+    const Outcome o = shared;
+    if (chunk == 0) {
+        int32_t* record = a.record + size_t(b) * (4 + a.max_new);
+        for (uint32_t i = threadIdx.x; i < a.max_new; i += kThreads) {
+            const bool kept = int32_t(i) < o.count;
+            a.path[size_t(b) * a.max_new + i] = kept ? path[i] : -1;
+            a.out[size_t(b) * a.max_new + i] = int32_t(i) + 1 < o.count ? a.ids[p.first + path[i + 1]] : -1;
+            if (int32_t(i) < o.refused) record[4 + i] = refused[i];
+        }
+        if (threadIdx.x == 0) {
+            a.count[b] = o.count;
+            record[0] = o.here;
+            record[1] = o.against;
+            record[2] = o.refused;
+            record[3] = o.count;
+        }
+    }
+    Weights<TYPE> w;
+    w.load(a.target + int64_t(p.first + o.here) * a.target_stride, o.against >= 0 ? a.draft + int64_t(p.first + o.against) * a.draft_stride : nullptr, chunk, a.vocab);
+    if (!a.draft)
+        for (int32_t i = 0; i < o.refused; ++i) w.clear(chunk, uint32_t(refused[i]));
+    double s = 0.0;
+#pragma unroll
+    for (uint32_t k = 0; k < kRuns<TYPE>; ++k) s += w.sum(k);
+    s = sum_of_all(s, waves);
+    if (threadIdx.x == 0) a.sums[size_t(b) * a.chunks + chunk] = s;
+}
+
+template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_pick(const VerifyArgs a) {
+    __shared__ double waves[4], runs[kRuns<TYPE>][4];
+    __shared__ uint32_t found, last;
+    const uint32_t b = blockIdx.x, thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
+    const Place p = place_of(a, b);
+    if (p.count == 0) return;
+    const int32_t* record = a.record + size_t(b) * (4 + a.max_new);
+    const Outcome o{record[0], record[1], record[2], record[3]};
+    double* sums = a.sums + size_t(b) * a.chunks;
+    const char *target = a.target + int64_t(p.first + o.here) * a.target_stride, *draft = o.against >= 0 ? a.draft + int64_t(p.first + o.against) * a.draft_stride : nullptr;
+    const float u = as_uniform(a.uniforms[p.first]);
+    int32_t id = -1;
+    for (int plain = 0; plain < 2; ++plain) {
+        Weights<TYPE> w;
+        if (plain) {
+            // no weight is left: the target's row as it is
+            for (uint32_t c = 0; c < a.chunks; ++c) {
+                w.load(target, nullptr, c, a.vocab);
+                double s = 0.0;
+#pragma unroll
+                for (uint32_t k = 0; k < kRuns<TYPE>; ++k) s += w.sum(k);
+                s = sum_of_all(s, waves);
+                if (thread == 0) sums[c] = s;
+            }
+            __syncthreads();
+        }
+        // the chunk: each thread has some that are neighbours
+        const uint32_t each = (a.chunks + kThreads - 1) / kThreads, c0 = min(thread * each, a.chunks), c1 = min(c0 + each, a.chunks);
+        double own = 0.0;
+        for (uint32_t c = c0; c < c1; ++c) own += sums[c];
+        double upto = own;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) {
+            const double before = __shfl_up(upto, i);
+            if (lane >= uint32_t(i)) upto += before;
+        }
+        __syncthreads();
+        if (lane == 63) waves[wave] = upto;
+        if (thread == 0) {
+            found = 0xffffffffu;
+            last = 0;
+        }
+        __syncthreads();
+        double before = upto - own, all = 0.0;
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (i < wave) before += waves[i];
+            all += waves[i];
+        }
+        if (!(all > 0.0)) continue;
+        const double border = double(u) * all;
+        for (uint32_t c = c0; c < c1; ++c) {
+            const double s = sums[c];
+            before += s;
+            if (s > 0.0) {
+                atomicMax(&last, c);
+                if (before > border) {
+                    atomicMin(&found, c);
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        const uint32_t chunk = found != 0xffffffffu ? found : last;
+        // what is in front of it, in order
+        double front = 0.0;
+        for (uint32_t c = thread; c < chunk; c += kThreads) front += sums[c];
+        front = sum_of_all(front, waves);
+        w.load(target, plain ? nullptr : draft, chunk, a.vocab);
+        if (!a.draft && !plain)
+            for (int32_t i = 0; i < o.refused; ++i) w.clear(chunk, uint32_t(record[4 + i]));
+        double run[kRuns<TYPE>];
+#pragma unroll
+        for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
+            run[k] = w.sum(k);
+            double scan = run[k];
+#pragma unroll
+            for (int i = 1; i < 64; i <<= 1) {
+                const double x = __shfl_up(scan, i);
+                if (lane >= uint32_t(i)) scan += x;
+            }
+            if (lane == 63) runs[k][wave] = scan;
+            run[k] = scan - run[k];
+        }
+        __syncthreads();
+        if (thread == 0) {
+            found = 0xffffffffu;
+            last = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
+            double sum = front + run[k];
+            for (uint32_t i = 0; i < k * 4 + wave; ++i) sum += runs[i / 4][i % 4];
+#pragma unroll
+            for (uint32_t i = 0; i < kRun<TYPE>; ++i) {
+                sum += w.w[k][i];
+                if (w.w[k][i] > 0.0) {
+                    atomicMax(&last, w.at(chunk, k) + i);
+                    if (sum > border) atomicMin(&found, w.at(chunk, k) + i);
+                }
+            }
+        }
+        __syncthreads();
+        id = int32_t(found != 0xffffffffu ? found : last);
+        break;
+    }
+    if (thread == 0) a.out[size_t(b) * a.max_new + o.count - 1] = id;
+}
+
+template <int TYPE> int start_verify(const VerifyArgs& a, void* stream) {
+    if (const int rc = launch(k_verify_sums<TYPE>, dim3(a.chunks, a.batch), dim3(kThreads), stream, a, a.max_new * 8)) return rc;
+    return launch(k_verify_pick<TYPE>, dim3(a.batch), dim3(kThreads), stream, a);
+}
+
+} // namespace
+
+uint32_t verify_chunks(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
+
+int launch_verify(const VerifyArgs& a, int type, void* stream, Launched& info) {
+    info = {"verify_drafts", {a.chunks, a.batch, 1}, {kThreads, 1, 1}, a.max_new * 8};
+    if (type == FKLHIP_F32) return start_verify<FKLHIP_F32>(a, stream);
+    return type == FKLHIP_BF16 ? start_verify<FKLHIP_BF16>(a, stream) : start_verify<FKLHIP_F16>(a, stream);
+}
+
+} // namespace fkattn

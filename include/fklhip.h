@@ -141,7 +141,7 @@ int fklhip_last_form(const char **form);
  * into a graph. A call that returns FKLHIP_EINVAL has launched nothing; fklhip_argument_error says what was wrong. What only
  * the device can see (slots, pages, lengths, positions) is held inside its bounds by the kernels, as described at each entry.
  */
-enum { FKLHIP_BF16 = 0, FKLHIP_F16 = 1 };
+enum { FKLHIP_BF16 = 0, FKLHIP_F16 = 1, FKLHIP_F32 = 2 };      /* (F32: probabilities of fklhip_verify_drafts only) */
 enum { FKLHIP_CODES_INT8 = 0, FKLHIP_CODES_E4M3 = 1 };
 
 /* A paged cache. A cached value is code * scale with one float32 scale per token and head; codes are int8 (-127..127) or
@@ -186,6 +186,18 @@ int fklhip_qk_norm_rope(const fklhip_heads *heads, void *stream);
 /* The same, with the keys (in 32 bits) and the values quantised into the cache in the same launch instead of written out. */
 int fklhip_qkv_to_cache(const fklhip_heads *heads, const fklhip_kv_cache *cache, void *stream);
 
+/* Positions of several axes (time, height and width of an image's or a video's tokens). With these a token has `count` positions,
+ * heads->positions[axis * stride + token], and pair i turns by that of axis of_pair[i], i below rot_dim / 2. A position
+ * outside of the table makes the pairs of its axis NaN. */
+typedef struct fklhip_axes {
+    int64_t stride;
+    int32_t count;                     /* 1 to 4 */
+    uint8_t of_pair[128];
+} fklhip_axes;
+
+int fklhip_qk_norm_rope_axes(const fklhip_heads *heads, const fklhip_axes *axes, void *stream);
+int fklhip_qkv_to_cache_axes(const fklhip_heads *heads, const fklhip_axes *axes, const fklhip_kv_cache *cache, void *stream);
+
 /* Quantises rows into the cache: scale = max |x| / 127 (448 for e4m3), code = x / scale rounded to the nearest, ties to
  * even. A row of zeros has scale 0; a row with an infinity or a NaN is stored as NaN (scale NaN, codes 0). Tokens whose
  * slot is outside of the cache (a negative one, say) are skipped. No two tokens of a call may have the same slot. */
@@ -220,6 +232,67 @@ typedef struct fklhip_attention {
 
 int fklhip_tree_attention_workspace(const fklhip_attention *call, const fklhip_kv_cache *cache, uint64_t *bytes);
 int fklhip_tree_attention(const fklhip_attention *call, const fklhip_kv_cache *cache, void *stream);
+
+/* The tables of a server's step, from its requests' lengths. Request b has context[b] tokens in the cache, the first held[b]
+ * entries of its page table's row, and fresh[b] new tokens. Entries that the new tokens need are taken from the end of the
+ * first *available of free_pages, request by request, and written to page_table; held_out[b] and *left are what held and
+ * available are afterwards (*left is negative by the pages that were missing, and a request that got fewer than it needs has the
+ * first of them). The new tokens are rows q_start[b] .. of the step, as fklhip_attention takes them: each has the slot of its
+ * place in the sequence (-1 where it has no page) and position context + t for new token t. With parents, new token t
+ * follows new token parents[q_start[b] + t] < t (anything else: none), its position is context + the number of its ancestors
+ * among the new tokens, and its mask has the bits of those and its own. Rows behind the last request's: slot -1, position 0, an
+ * empty mask. Negative lengths count as 0, fresh above max_new and held above page_table_stride are cut off, and so are rows above `tokens`.
+ * held_out, left, slots, positions, mask and q_start may not overlap the other arrays. A launch. */
+typedef struct fklhip_tables {
+    int32_t *page_table;               /* [batch][page_table_stride], entries that are taken are written */
+    const int32_t *held, *context, *fresh;                 /* [batch] */
+    const int32_t *free_pages, *available;                 /* [free_count], [1] */
+    const int32_t *parents;            /* [tokens] or NULL */
+    int32_t *q_start, *slots, *positions, *held_out, *left;    /* [batch + 1], [tokens], [tokens], [batch], [1] */
+    uint64_t *mask;                    /* [tokens][mask_words], with parents */
+    int64_t tokens, page_table_stride, free_count;
+    int32_t batch, page_tokens, max_new, mask_words;
+} fklhip_tables;
+
+int fklhip_step_tables(const fklhip_tables *tables, void *stream);
+
+/* Drafted tokens against the target's probabilities, by random numbers that are given. Sequence b's rows are q_start[b] ..
+ * q_start[b + 1]: the first is of its last token that is decided, the others of drafted ones, row t's token being ids[t]. target's row
+ * t has the probabilities of what follows row t's token, and is taken to sum to 1. Row t follows row parents[t] < t of its
+ * sequence, counted from its first (without parents: t - 1; a parent that is not in front of its row: the row is never accepted).
+ * From the first row on, the children of the last accepted row are asked in their order. One with token x is accepted if
+ * target[its parent][x] > uniforms[t] * draft[t][x], where draft's row t has the probabilities that row t's token was drawn from. Without
+ * draft: if target[its parent][x] > uniforms[t] * (1 - what the tokens of the refused children in front of it had); a token
+ * that was refused already is refused again. Where no child is accepted the next token is drawn: from max(target - draft, 0) of the
+ * refused row, from target without the refused children's tokens, or from target where nobody was asked, always from the row
+ * that the path has come to; if nothing is left of the weights, from that row whole. It is the first token at which the running sum of
+ * the weights exceeds their sum times the uniform of the sequence's first row; -1 if that row has no number above 0.
+ * path[b] receives the accepted rows, counted from the sequence's first, that one in front; count[b] their number; out[b]
+ * the tokens that were decided: the accepted rows' and then the drawn one, count[b] in all. Behind them, and all of a sequence
+ * without rows (count 0): -1. Comparisons and sums are in 64 bits. Probabilities that are no finite number above 0 count as 0,
+ * uniforms as what is nearest in 0 .. 1 - 2^-24 (NaN: 0); a token outside of the vocabulary has probability 0. Sequences longer than
+ * max_new (up to 1024) and rows above `tokens` are cut off. With batch or max_new 0 nothing is launched. */
+typedef struct fklhip_drafts {
+    const void *target, *draft;        /* [tokens][vocab] of the type; draft may be NULL, and has to be with parents */
+    const int32_t *ids, *q_start, *parents;                /* [tokens], [batch + 1], [tokens] or NULL */
+    const float *uniforms;             /* [tokens] */
+    int32_t *path, *count, *out;       /* [batch][max_new], [batch], [batch][max_new] */
+    void *workspace;                   /* fklhip_verify_drafts_workspace bytes; not kept between calls */
+    uint64_t workspace_bytes;
+    int64_t tokens, target_stride, draft_stride;           /* strides: elements from row to row */
+    int32_t batch, max_new, vocab, type;
+} fklhip_drafts;
+
+int fklhip_verify_drafts_workspace(const fklhip_drafts *drafts, uint64_t *bytes);
+int fklhip_verify_drafts(const fklhip_drafts *drafts, void *stream);
+
+/* Moves the cache rows of accepted tokens to where their sequence goes on, in the caches of several layers at once: for
+ * 1 <= i < count[b], what is at place context[b] + path[b][i] of sequence b (its page table as in fklhip_attention) goes to place
+ * context[b] + i, codes and scales as they are. path[b] (of max_new entries) has to ascend; an entry that is at its place already, is
+ * not behind it or is max_new or more, and one whose place or page is outside of the table or the cache, moves nothing. All caches are
+ * of the same sizes, none is given twice, and no two sequences have a page in common where something moves. */
+int fklhip_kv_keep(const fklhip_kv_cache *caches, int32_t layers, const int32_t *page_table, int64_t page_table_stride,
+                   const int32_t *context, const int32_t *path, const int32_t *count, int32_t batch, int32_t max_new, void *stream);
 
 /* What the last of the calls above that returned FKLHIP_EINVAL on this thread found wrong; "" before the first. */
 int fklhip_argument_error(const char **text);
