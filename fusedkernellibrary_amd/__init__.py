@@ -26,6 +26,8 @@ ABI_SYMBOLS = (
     "fklhip_signature_count", "fklhip_signature_at", "fklhip_jit_log", "fklhip_strip_form",
     "fklhip_qk_norm_rope", "fklhip_qkv_to_cache", "fklhip_kv_write", "fklhip_kv_read", "fklhip_tree_attention",
     "fklhip_tree_attention_workspace", "fklhip_argument_error", "fklhip_stream_is_capturing",
+    "fklhip_qk_norm_rope_axes", "fklhip_qkv_to_cache_axes", "fklhip_shaped_attention", "fklhip_step_tables",
+    "fklhip_verify_drafts", "fklhip_verify_drafts_workspace", "fklhip_kv_keep",
 )
 
 

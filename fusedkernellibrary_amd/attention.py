@@ -98,15 +98,22 @@ def kv_read(cache: KvCache, slots, *, dtype=_torch.bfloat16, k_out=None, v_out=N
     return _native.kv_read(cache._tensors, slots, _HALVES[dtype], k_out, v_out)
 
 
-def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: int, max_context: int, mask=None, scale: float | None = None, out=None, lse=None):
+def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: int, max_context: int, mask=None, scale: float | None = None, out=None, lse=None,
+                   cap: float | None = None, slopes=None, positions=None, first=None, prefix=None):
     """Attention of new tokens' queries q [tokens, q_heads, head_dim] over the cache.
 
     Sequence b has context[b] (at most max_context) tokens in the cache and behind them its new ones, rows q_start[b] to
     q_start[b + 1] (at most max_new) of q; its token j is in page page_table[b, j // page_tokens]. Bit u % 64 of
     mask[row, u // 64] (int64) says that a row sees new token u; without a mask new token t sees the new tokens 0 to t.
     All of them see the whole context. Rows that see nothing are zero, and so are those of no sequence (a padded batch's).
-    lse [tokens, q_heads] float32 receives the logarithm of the sum of exponentials if it is given. Returns out."""
-    return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse)
+    lse [tokens, q_heads] float32 receives the logarithm of the sum of exponentials if it is given. Returns out.
+
+    Scores of another shape: cap (2^-6 to 2^9) makes them cap * tanh(score / cap); slopes [q_heads] float32 takes off slope * (the
+    row's position - the key's), which are places in the sequence or, of new tokens, positions [tokens] int32 (step_tables', of
+    trees). Rows that see other keys: none in front of place first[row] (int32; a window, the beginning of the row's document;
+    none of a sequence's rows sees what is in front of its first row's, and nothing of that is read), or, without a mask, all in
+    front of place prefix[b] (int32) besides those that they see anyway."""
+    return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse, cap, slopes, positions, first, prefix)
 
 
 class StepTables(_typing.NamedTuple):

@@ -95,6 +95,67 @@ uint64_t workspace_of(const fklhip_kv_cache& cache, const AttentionPlan& plan) {
     return uint64_t(plan.shares()) * 2 * plan.unit_rows * (cache.head_dim + 1) * 4;
 }
 
+template <typename A> int launch_any(const A& a, uint32_t head_dim, const AttentionPlan& plan, bool parts, void* stream, Launched& info) {
+    int rc;
+    switch (head_dim) {
+    case 64: rc = launch_attention<64>(a, plan, stream, info); break;
+    case 96: rc = launch_attention<96>(a, plan, stream, info); break;
+    case 128: rc = launch_attention<128>(a, plan, stream, info); break;
+    case 192: rc = launch_attention<192>(a, plan, stream, info); break;
+    default: rc = launch_attention<256>(a, plan, stream, info); break;
+    }
+    if (rc == FKLHIP_OK && parts) rc = launch_merge(a, head_dim, plan.many_parts, stream);
+    return rc;
+}
+
+int run_attention(const fklhip_attention* c, const fklhip_scores* h, const fklhip_kv_cache* cache, void* stream) {
+    AttentionPlan plan;
+    CHECK(plan_call(c, cache, plan));
+    NEED(std::isfinite(c->scale), "scale has to be finite");
+    if (h) {
+        NEED(h->cap == 0.0f || (h->cap >= 0x1p-6f && h->cap <= 0x1p9f), "cap has to be 0, or 2^-6 to 2^9");
+        NEED(!h->prefix || !c->mask, "a prefix and a mask");
+        NEED(aligned(h->slopes, 4) && aligned(h->positions, 4) && aligned(h->first, 4) && aligned(h->prefix, 4), "slopes, positions, first and prefix have to be aligned");
+    }
+    if (c->tokens == 0 || c->batch == 0 || c->max_new == 0) return FKLHIP_OK;
+    CHECK(check_rows(c->q, c->tokens, c->q_heads));
+    CHECK(check_out(c->out, c->tokens, c->q_heads, cache->head_dim));
+    NEED(c->context && c->q_start, "no context or no q_start");
+    NEED(c->page_table || c->page_table_stride == 0, "no page_table");
+    NEED(aligned(c->context, 4) && aligned(c->q_start, 4) && aligned(c->page_table, 4) && aligned(c->lse, 4) && aligned(c->mask, 8), "lengths, page_table, lse and mask have to be aligned");
+    NEED(!c->mask || (c->mask_words >= 1 && int64_t(c->mask_words) * 64 >= c->max_new), "mask_words has to be max_new / 64, rounded up, or more");
+    const uint64_t bytes = workspace_of(*cache, plan);
+    NEED(bytes == 0 || (c->workspace && c->workspace_bytes >= bytes), "the workspace is smaller than fklhip_tree_attention_workspace says");
+    NEED(bytes == 0 || aligned(c->workspace, 16), "the workspace has to start at a multiple of 16 bytes");
+    ShapedArgs a{};
+    a.q = to_rows(c->q); a.out = to_rows(c->out); a.lse = c->lse;
+    a.page_table = c->page_table; a.context = c->context; a.q_start = c->q_start; a.mask = c->mask;
+    a.cache = to_cache(*cache);
+    a.page_table_stride = c->page_table_stride;
+    a.tokens = uint32_t(c->tokens); a.batch = uint32_t(c->batch); a.max_new = uint32_t(c->max_new); a.max_context = uint32_t(c->max_context);
+    a.mask_words = uint32_t(c->mask_words); a.q_heads = uint32_t(c->q_heads); a.group = uint32_t(c->q_heads / cache->kv_heads);
+    a.group_magic = magic(a.group);
+    a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
+    // (without room nobody sees anything: all rows are written like rows of no sequence, and nothing is read for them)
+    if (a.room == 0) a.max_new = 0;
+    a.unit_rows = plan.unit_rows;
+    a.granule_log = plan.granule_log; a.lead = plan.lead; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
+    a.type = c->type; a.scale = c->scale;
+    if (bytes) {
+        a.partial = static_cast<float*>(c->workspace);
+        a.partial_lse = a.partial + uint64_t(plan.shares()) * 2 * plan.unit_rows * uint64_t(cache->head_dim);
+    }
+    Launched info;
+    const bool shaped = h && (h->cap != 0.0f || h->slopes || h->first || h->prefix);
+    if (!shaped) return finish(launch_any(static_cast<const AttentionArgs&>(a), uint32_t(cache->head_dim), plan, bytes != 0, stream, info), info);
+    a.slopes = h->slopes; a.positions = h->positions; a.first = h->first; a.prefix = h->prefix;
+    if (h->cap != 0.0f) {
+        a.cap_in = 2.0f / h->cap;
+        a.cap_out = h->cap * 1.4426950408889634f;
+    }
+    return finish(launch_any(a, uint32_t(cache->head_dim), plan, bytes != 0, stream, info), info);
+}
+
 } // namespace
 
 extern "C" {
@@ -161,49 +222,11 @@ int fklhip_tree_attention_workspace(const fklhip_attention* call, const fklhip_k
     return FKLHIP_OK;
 }
 
-int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cache, void* stream) {
-    AttentionPlan plan;
-    CHECK(plan_call(c, cache, plan));
-    NEED(std::isfinite(c->scale), "scale has to be finite");
-    if (c->tokens == 0 || c->batch == 0 || c->max_new == 0) return FKLHIP_OK;
-    CHECK(check_rows(c->q, c->tokens, c->q_heads));
-    CHECK(check_out(c->out, c->tokens, c->q_heads, cache->head_dim));
-    NEED(c->context && c->q_start, "no context or no q_start");
-    NEED(c->page_table || c->page_table_stride == 0, "no page_table");
-    NEED(aligned(c->context, 4) && aligned(c->q_start, 4) && aligned(c->page_table, 4) && aligned(c->lse, 4) && aligned(c->mask, 8), "lengths, page_table, lse and mask have to be aligned");
-    NEED(!c->mask || (c->mask_words >= 1 && int64_t(c->mask_words) * 64 >= c->max_new), "mask_words has to be max_new / 64, rounded up, or more");
-    const uint64_t bytes = workspace_of(*cache, plan);
-    NEED(bytes == 0 || (c->workspace && c->workspace_bytes >= bytes), "the workspace is smaller than fklhip_tree_attention_workspace says");
-    NEED(bytes == 0 || aligned(c->workspace, 16), "the workspace has to start at a multiple of 16 bytes");
-    AttentionArgs a{};
-    a.q = to_rows(c->q); a.out = to_rows(c->out); a.lse = c->lse;
-    a.page_table = c->page_table; a.context = c->context; a.q_start = c->q_start; a.mask = c->mask;
-    a.cache = to_cache(*cache);
-    a.page_table_stride = c->page_table_stride;
-    a.tokens = uint32_t(c->tokens); a.batch = uint32_t(c->batch); a.max_new = uint32_t(c->max_new); a.max_context = uint32_t(c->max_context);
-    a.mask_words = uint32_t(c->mask_words); a.q_heads = uint32_t(c->q_heads); a.group = uint32_t(c->q_heads / cache->kv_heads);
-    a.group_magic = magic(a.group);
-    a.room = uint32_t(std::min<int64_t>(c->page_table_stride * cache->page_tokens, int64_t(c->max_context) + c->max_new));
-    // (without room nobody sees anything: all rows are written like rows of no sequence, and nothing is read for them)
-    if (a.room == 0) a.max_new = 0;
-    a.unit_rows = plan.unit_rows;
-    a.granule_log = plan.granule_log; a.lead = plan.lead; a.share_log = plan.share_log; a.share_odd = plan.share_odd;
-    a.type = c->type; a.scale = c->scale;
-    if (bytes) {
-        a.partial = static_cast<float*>(c->workspace);
-        a.partial_lse = a.partial + uint64_t(plan.shares()) * 2 * plan.unit_rows * uint64_t(cache->head_dim);
-    }
-    Launched info;
-    int rc;
-    switch (cache->head_dim) {
-    case 64: rc = launch_attention<64>(a, plan, stream, info); break;
-    case 96: rc = launch_attention<96>(a, plan, stream, info); break;
-    case 128: rc = launch_attention<128>(a, plan, stream, info); break;
-    case 192: rc = launch_attention<192>(a, plan, stream, info); break;
-    default: rc = launch_attention<256>(a, plan, stream, info); break;
-    }
-    if (rc == FKLHIP_OK && bytes) rc = launch_merge(a, uint32_t(cache->head_dim), plan.many_parts, stream);
-    return finish(rc, info);
+int fklhip_tree_attention(const fklhip_attention* c, const fklhip_kv_cache* cache, void* stream) { return run_attention(c, nullptr, cache, stream); }
+
+int fklhip_shaped_attention(const fklhip_attention* c, const fklhip_scores* scores, const fklhip_kv_cache* cache, void* stream) {
+    NEED(scores, "no scores");
+    return run_attention(c, scores, cache, stream);
 }
 
 } // extern "C"

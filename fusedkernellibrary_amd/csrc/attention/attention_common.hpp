@@ -65,12 +65,20 @@ struct AttentionArgs {
 };
 // share_odd is 0 in a launch with a workgroup to each row block
 
+// With scores of another shape, and rows that see other keys (fklhip_scores).
+struct ShapedArgs : AttentionArgs {
+    const float* slopes;
+    const int32_t *positions, *first, *prefix;
+    float cap_in, cap_out;                  // 2 / cap, and cap in units of log2; 0 without
+};
+
 // Launchers (defined next to their kernels). Grids are laid out by the callers' arguments alone.
 struct Launched { const char* kernel; unsigned grid[3], block[3], lds; };
 int launch_heads(const HeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_heads(const AxesHeadArgs& a, int type, bool to_cache, void* stream, Launched& info);
 int launch_read(const ReadArgs& a, int type, void* stream, Launched& info);
 int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream);
+int launch_merge(const ShapedArgs& a, uint32_t head_dim, bool many_parts, void* stream);
 // How a call is run: 16-row tiles (and so rows) and waves to a workgroup; row blocks of a sequence; share_odd << share_log
 // shares, or none; whether rows have so many parts that a workgroup joins one.
 struct AttentionPlan {
@@ -80,5 +88,6 @@ struct AttentionPlan {
 };
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim);
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
+template <int D> int launch_attention(const ShapedArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
 
 } // namespace fkattn

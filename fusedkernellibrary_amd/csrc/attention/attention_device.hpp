@@ -10,6 +10,7 @@ namespace fkattn {
 
 using half2_t = _Float16 __attribute__((ext_vector_type(2)));
 using half8_t = _Float16 __attribute__((ext_vector_type(8)));
+using float2_t = float __attribute__((ext_vector_type(2)));
 using float4_t = float __attribute__((ext_vector_type(4)));
 using uint2_t = uint32_t __attribute__((ext_vector_type(2)));
 using uint4_t = uint32_t __attribute__((ext_vector_type(4)));

@@ -12,8 +12,8 @@ constexpr uint32_t kThreads = 256, kMostParts = 1025;         // (a row's parts 
 template <int D> struct Lanes { static constexpr uint32_t kRow = D <= 64 ? 16 : D <= 128 ? 32 : 64, kGroups = kThreads / kRow; };
 
 // The sequence of a token, with the granules in front of it.
-__device__ __forceinline__ Found sequence_of_token(Args& a, uint32_t token) {
-    return find(a, threadIdx.x & 63, [&](uint32_t, const Sequence& s, uint32_t, uint32_t) { return token >= s.first_token && token - s.first_token < s.fresh; });
+template <bool SHAPED> __device__ __forceinline__ Found sequence_of_token(Args& a, uint32_t token) {
+    return find<SHAPED>(a, threadIdx.x & 63, [&](uint32_t, const Sequence& s, uint32_t, uint32_t) { return token >= s.first_token && token - s.first_token < s.fresh; });
 }
 // A row's parts: those of shares share0 .. share0 + count. None: nobody had any of it. One: it has been written.
 struct Parts {
@@ -54,13 +54,13 @@ __device__ __forceinline__ float4_t part4(const float* from, float w) {
     return y;
 }
 
-template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const AttentionArgs) {
+template <int D, bool SHAPED> __global__ __launch_bounds__(kThreads) void k_merge_few(const ArgsOf<SHAPED>) {
     constexpr uint32_t kLanes = Lanes<D>::kRow;
     Args& a = kernel_args();
     const uint32_t at = threadIdx.x % kLanes, head = blockIdx.x * Lanes<D>::kGroups + threadIdx.x / kLanes, d = at * 4;
     const uint32_t token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
-    const Found f = sequence_of_token(a, token);
+    const Found f = sequence_of_token<SHAPED>(a, token);
     if (head >= a.q_heads) return;
     if (f.b >= a.batch) {                                     // a row of no sequence
         if (d < D) put4(a, token, head, d, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
@@ -95,7 +95,7 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_few(const A
     if (at == 0) put_lse(a, token, head, top + __builtin_log2f(sum));
 }
 
-template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const AttentionArgs) {
+template <int D, bool SHAPED> __global__ __launch_bounds__(kThreads) void k_merge_many(const ArgsOf<SHAPED>) {
     constexpr uint32_t kLanes = Lanes<D>::kRow, kGroups = Lanes<D>::kGroups;
     __shared__ float weight[kMostParts], tops[4], sums[4];
     __shared__ __attribute__((aligned(16))) float joined[kGroups][D];
@@ -103,7 +103,7 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = at * 4;
     const uint32_t head = blockIdx.x, token = blockIdx.y + blockIdx.z * 32768u;
     if (token >= a.tokens) return;
-    const Found f = sequence_of_token(a, token);
+    const Found f = sequence_of_token<SHAPED>(a, token);
     if (f.b >= a.batch) {                                     // a row of no sequence
         if (group == 0 && d < D) put4(a, token, head, d, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
         if (threadIdx.x == 0) put_lse(a, token, head, -__builtin_inff());
@@ -149,22 +149,24 @@ template <int D> __global__ __launch_bounds__(kThreads) void k_merge_many(const 
     }
 }
 
-template <int D> int start_merge(const AttentionArgs& a, bool many_parts, void* stream) {
+template <int D, bool SHAPED> int start_merge(const ArgsOf<SHAPED>& a, bool many_parts, void* stream) {
     const uint32_t y = a.tokens < 32768u ? a.tokens : 32768u, z = (a.tokens + 32767u) / 32768u;
-    if (many_parts) return launch(k_merge_many<D>, dim3(a.q_heads, y, z), dim3(kThreads), stream, a);
-    return launch(k_merge_few<D>, dim3((a.q_heads + Lanes<D>::kGroups - 1) / Lanes<D>::kGroups, y, z), dim3(kThreads), stream, a);
+    if (many_parts) return launch(k_merge_many<D, SHAPED>, dim3(a.q_heads, y, z), dim3(kThreads), stream, a);
+    return launch(k_merge_few<D, SHAPED>, dim3((a.q_heads + Lanes<D>::kGroups - 1) / Lanes<D>::kGroups, y, z), dim3(kThreads), stream, a);
+}
+template <bool SHAPED> int start_merge_of_any_size(const ArgsOf<SHAPED>& a, uint32_t head_dim, bool many_parts, void* stream) {
+    switch (head_dim) {
+    case 64: return start_merge<64, SHAPED>(a, many_parts, stream);
+    case 96: return start_merge<96, SHAPED>(a, many_parts, stream);
+    case 128: return start_merge<128, SHAPED>(a, many_parts, stream);
+    case 192: return start_merge<192, SHAPED>(a, many_parts, stream);
+    default: return start_merge<256, SHAPED>(a, many_parts, stream);
+    }
 }
 
 } // namespace
 
-int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream) {
-    switch (head_dim) {
-    case 64: return start_merge<64>(a, many_parts, stream);
-    case 96: return start_merge<96>(a, many_parts, stream);
-    case 128: return start_merge<128>(a, many_parts, stream);
-    case 192: return start_merge<192>(a, many_parts, stream);
-    default: return start_merge<256>(a, many_parts, stream);
-    }
-}
+int launch_merge(const AttentionArgs& a, uint32_t head_dim, bool many_parts, void* stream) { return start_merge_of_any_size<false>(a, head_dim, many_parts, stream); }
+int launch_merge(const ShapedArgs& a, uint32_t head_dim, bool many_parts, void* stream) { return start_merge_of_any_size<true>(a, head_dim, many_parts, stream); }
 
 } // namespace fkattn

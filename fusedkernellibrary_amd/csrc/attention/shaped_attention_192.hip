@@ -1,0 +1,6 @@
+// Kernels of attention with scores of another shape, for heads of 192 elements.
+#include "tree_attention.hpp"
+
+namespace fkattn {
+template <> int launch_attention<192>(const ShapedArgs& a, const AttentionPlan& plan, void* stream, Launched& info) { return start_attention<192, true>(a, plan, stream, info); }
+}

@@ -333,10 +333,10 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---- attention --------------------------------------------------------------------------------------------------------
 
-// q, cache, page_table, context, q_start, max_new, max_context, mask, scale, out, lse
+// q, cache, page_table, context, q_start, max_new, max_context, mask, scale, out, lse; cap, slopes, positions, first, prefix
 PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 11);
+    expect(n, 16);
     at::AutoDispatchBelowAutograd quick;
     const Tensor& q = tensor(a[0], "q");
     const CacheView c = cache_of(a[1]);
@@ -363,6 +363,17 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         f.mask_words = int32_t(mask.size(1));
         if (f.mask == nullptr && tokens != 0) refuse("mask has to have a word at least");
     }
+    fklhip_scores h{};
+    const bool shaped = !none(a[11]) || !none(a[12]) || !none(a[14]) || !none(a[15]);
+    if (!none(a[11])) {
+        h.cap = float(number(a[11]));
+        if (!(h.cap > 0.0f)) refuse("cap has to be above 0, or None");
+    }
+    if (!none(a[12])) h.slopes = static_cast<const float*>(plain(tensor(a[12], "slopes"), "slopes", at::kFloat, {heads}, q.device()));
+    const auto of_rows = [&](PyObject* o, const char* name, int64_t n) { return none(o) ? nullptr : static_cast<const int32_t*>(plain(tensor(o, name), name, at::kInt, {n}, q.device())); };
+    h.positions = of_rows(a[13], "positions", tokens);
+    h.first = of_rows(a[14], "first", tokens);
+    h.prefix = of_rows(a[15], "prefix", table.size(0));
     f.scale = none(a[8]) ? float(1.0 / std::sqrt(double(dim))) : float(number(a[8]));
     void* stream = stream_of(q, "q");
     const Tensor out = output(a[9], "out", q.sizes(), q.scalar_type(), q.device());
@@ -376,7 +387,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         f.workspace = workspace.data_ptr();
         f.workspace_bytes = bytes;
     }
-    check(fklhip_tree_attention(&f, &c.c, stream), "tree_attention");
+    check(shaped ? fklhip_shaped_attention(&f, &h, &c.c, stream) : fklhip_tree_attention(&f, &c.c, stream), "tree_attention");
     if (tokens != 0 && (f.batch == 0 || f.max_new == 0)) {     // (nothing was launched)
         Tensor(out).zero_();
         if (!none(a[10])) Tensor(THPVariable_Unpack(a[10])).fill_(-HUGE_VAL);

@@ -41,8 +41,6 @@
 // the first keys. (Value scales below kLeastScale count as that: values of 10^-22 and less lose accuracy.)
 #pragma once
 
-#include <type_traits>
-
 #include "work_shares.hpp"
 
 namespace fkattn {
@@ -125,6 +123,12 @@ __device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint64_t firs
     return (lowest_bits(int32_t(below)) | bits << below) & 15u;
 }
 
+// The place of the first key that a token's rows see.
+__device__ __forceinline__ uint32_t first_of(Args& a, const Sequence& s, uint32_t token) {
+    const int32_t first = shaped(a).first[s.first_token + token];
+    return max(s.front, first < 0 ? 0u : min(uint32_t(first), s.total));
+}
+
 // Keys key0 .. key1 of row block `block` and key head `head` of a sequence; where its parts go.
 struct Segment {
     Sequence seq;
@@ -132,17 +136,43 @@ struct Segment {
     uint32_t key0, key1, all_see;        // every row sees the keys in front of all_see
     int part;                            // -1: whole, 0 or 1: the share's part
     uint32_t behind, quarter;            // keys of the share behind the segment's, and a quarter of them all
+    uint32_t all_from = 0;               // every row may see the keys from there on (shaped)
 };
-__device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32_t b, uint32_t head, uint32_t block, uint32_t k0, uint32_t k1, int part) {
+template <bool SHAPED> __device__ __forceinline__ Segment segment_of(Args& a, const Sequence& s, uint32_t b, uint32_t head, uint32_t block, uint32_t k0, uint32_t k1, int part) {
     Segment x;
     x.seq = s; x.b = b; x.head = head; x.part = part;
     x.row0 = block * a.unit_rows;
     x.rows = min(a.unit_rows, s.rows - x.row0);
     const bool causal = a.mask == nullptr;
-    const uint32_t any_sees = causal ? min(s.context + divide(x.row0 + x.rows - 1, a.group_magic) + 1, s.total) : s.total;
+    uint32_t any_sees = causal ? min(s.context + divide(x.row0 + x.rows - 1, a.group_magic) + 1, s.total) : s.total;
     x.all_see = causal ? min(s.context + divide(x.row0, a.group_magic) + 1, s.total) : s.context;
+    if constexpr (SHAPED) {
+        Shaped& h = shaped(a);
+        if (causal && h.prefix) {
+            const int32_t prefix = scalar(h.prefix + b);
+            const uint32_t upto = prefix < 0 ? 0u : min(uint32_t(prefix), s.total);
+            any_sees = max(any_sees, upto);
+            x.all_see = max(x.all_see, upto);
+        }
+        k0 += s.skip;
+        k1 += s.skip;
+    }
     x.key0 = k0 << a.granule_log;
     x.key1 = min(k1 << a.granule_log, any_sees);
+    if constexpr (SHAPED) {
+        if (shaped(a).first) {
+            // what the block's rows see first, the first and the last of them: a row to a lane
+            const uint32_t token = divide(x.row0 + min(thread_here() & 63, x.rows - 1), a.group_magic);
+            uint32_t least = first_of(a, s, token), most = least;
+#pragma unroll
+            for (int i = 32; i; i >>= 1) {
+                least = min(least, uint32_t(__shfl_xor(int(least), i)));
+                most = max(most, uint32_t(__shfl_xor(int(most), i)));
+            }
+            x.all_from = __builtin_amdgcn_readfirstlane(most);
+            x.key0 = min(max(x.key0, __builtin_amdgcn_readfirstlane(least) & ~31u), max(x.key0, x.key1));
+        }
+    }
     return x;
 }
 
@@ -166,14 +196,14 @@ template <int D, int THREADS> __device__ __forceinline__ void clear_rows(Args& a
 
 // Calls `run` for every segment of the workgroup. `kept` is the wave's place in LDS for what the walk goes on with: a segment
 // needs all registers.
-template <int D, int THREADS, typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, uint32_t* kept, F run) {
+template <int D, int THREADS, bool SHAPED, typename F> __device__ __forceinline__ void walk(Args& a, uint32_t lane, uint32_t* kept, F run) {
     // granules at .. end of all are the share's, `in` of b's are in front of them; without shares: (sequence, head, block) of the grid
     uint32_t b = blockIdx.z, in = 0, at = 0, end = 1;
     const bool shared = a.share_odd != 0;
     Sequence s;
     if (shared) {
         const uint32_t share = own_share(a);
-        const Found f = find(a, lane, [&](uint32_t all, const Sequence&, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
+        const Found f = find<SHAPED>(a, lane, [&](uint32_t all, const Sequence&, uint32_t, uint32_t upto) { return upto > share_begin(a, all, share); });
         at = share_begin(a, f.all, share);
         end = share_begin(a, f.all, share + 1);
         b = f.b;
@@ -182,6 +212,8 @@ template <int D, int THREADS, typename F> __device__ __forceinline__ void walk(A
     } else {
         const int32_t rows_end = scalar(a.q_start + b + 1);
         s = sequence_of(a, scalar(a.q_start + b), rows_end, scalar(a.context + b));
+        if constexpr (SHAPED)
+            if (shaped(a).first && s.fresh) skip_front(a, s, scalar(shaped(a).first + s.first_token));
         if (blockIdx.y == 0) clear_rows<D, THREADS>(a, s, b, blockIdx.x, rows_end);
     }
     uint32_t whole = end - at;
@@ -195,7 +227,7 @@ template <int D, int THREADS, typename F> __device__ __forceinline__ void walk(A
             const uint32_t unit = n ? in / n : 0;
             if (unit >= blocks * a.cache.kv_heads || n == 0) {
                 in = 0;
-                if (++b < a.batch) s = sequence_at(a, b);
+                if (++b < a.batch) s = sequence_at<SHAPED>(a, b);
                 continue;
             }
             head = unit / blocks;
@@ -207,15 +239,15 @@ template <int D, int THREADS, typename F> __device__ __forceinline__ void walk(A
             return;
         }
         kept[0] = at + count; kept[1] = in + count; kept[2] = end; kept[3] = b; kept[4] = whole;
-        Segment x = segment_of(a, s, b, head, block, max(g, a.lead) - a.lead, max(g + count, a.lead) - a.lead, part);
+        Segment x = segment_of<SHAPED>(a, s, b, head, block, max(g, a.lead) - a.lead, max(g + count, a.lead) - a.lead, part);
         x.quarter = whole << a.granule_log >> 2;
         x.behind = (end - at - count) << a.granule_log;
-        if (!shared) x.behind = 0, x.quarter = (x.key1 - x.key0) >> 2;
+        if (!shared) x.behind = 0, x.quarter = (SHAPED && x.key1 < x.key0 ? 0 : x.key1 - x.key0) >> 2;
         if (!shared || g + count > a.lead) run(x);            // (else there is nothing but a block's beginning)
         if (!shared) return;
         at = __builtin_amdgcn_readfirstlane(kept[0]); in = __builtin_amdgcn_readfirstlane(kept[1]); end = __builtin_amdgcn_readfirstlane(kept[2]);
         b = __builtin_amdgcn_readfirstlane(kept[3]); whole = __builtin_amdgcn_readfirstlane(kept[4]);
-        s = sequence_at(kernel_args(), b);
+        s = sequence_at<SHAPED>(kernel_args(), b);
     }
 }
 
@@ -370,19 +402,21 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         }
     }
 
-    // 32 keys: get_k(block, load) and get_v have their codes, get_scales(ks, vs) the scales of the quarter's four keys of each
+    // 32 keys: get_k(block, load) and get_v have their codes, get_k_scales and get_v_scales the scales of the quarter's four keys of each
     // block, get_q(tile, run) the queries, get_unit(tile) what their scores are multiplied with. after_scores runs when the
     // keys are used up. Where `masked`, sees(tile, block) has a bit for each of the quarter's four keys that the lane's row
     // sees, and hide() clears the values that are no token's. (The masked way is a branch around the scores and no second copy
     // of the loop: between two loops the sums would be held twice.)
-    template <typename K, typename V, typename Q, typename U, typename G, typename M, typename H, typename A>
-    __device__ __forceinline__ void step(bool masked, K get_k, V get_v, Q get_q, U get_unit, G get_scales, M sees, H hide, A after_scores) {
+    // shape(tile, block, scores) makes products with the queries, multiplied with their unit, what the scores are; std::nullptr_t: they are.
+    template <typename K, typename V, typename Q, typename U, typename G, typename W, typename T, typename M, typename H, typename A>
+    __device__ __forceinline__ void step(bool masked, K get_k, V get_v, Q get_q, U get_unit, G get_k_scales, W get_v_scales, T shape, M sees, H hide, A after_scores) {
+        constexpr bool kShaped = !std::is_same_v<T, std::nullptr_t>;
         half8_t p[R];
         float4_t y[2], next[2];
         // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of 128 elements take all registers
         // without that if queries have three parts or keys are converted: trees of up to 61 took 73 us with it, and 70 without.)
         constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * S::kLoads;
-        constexpr bool kAhead = !(R == 4 && (PARTS == 3 || (PARTS == 0 && D == 128)));
+        constexpr bool kAhead = !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped)))) && !(kShaped && R == 2 && D == 256 && PARTS == 0);
         constexpr bool kHeld = R < 4 || kRuns <= 4;
         uint4_t q[kRuns];
         auto ask_q = [&](int r) {
@@ -398,9 +432,20 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
             if (kAhead && kHeld && r + 1 < R) ask_q(r + 1);
             float unit = get_unit(r);
             float4_t ks[2], vs[2];
-            get_scales(ks, vs);
+            get_k_scales(ks);
+            if constexpr (!kShaped) get_v_scales(vs);
 #pragma unroll
             for (int h = 0; h < 2; ++h) y[h] *= ks[h];
+            if constexpr (kShaped) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    y[h] *= unit;
+                    shape(r, h, y[h]);
+                    if constexpr (R == 4 || (R == 2 && D == 256)) __builtin_amdgcn_sched_barrier(0);    // (both blocks' at once take more registers than there are)
+                }
+                unit = 1.0f;
+                get_v_scales(vs);
+            }
             if (__builtin_expect(masked, 0)) {
                 uint32_t some = 0;
 #pragma unroll
@@ -626,8 +671,8 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
     __syncthreads();
 }
 
-template <int D, int CODES, int R, int PARTS, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_attention(const AttentionArgs) {
+template <int D, int CODES, int R, int PARTS, int WAVES, bool SHAPED>
+__global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_attention(const ArgsOf<SHAPED>) {
     using S = Shape<D>;
     constexpr int kRegs = kQueryRegs<D, PARTS>, kRuns = kRegs / 4;
     // One tile's rows: in registers. More: in LDS, whose place the joining of the waves takes afterwards.
@@ -638,10 +683,13 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
     __shared__ float units[R * 16];
     __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
     __shared__ __attribute__((aligned(16))) float scales[WAVES][64];
+    // of shaped rows: slope in units of log2 and position; the first key they see
+    __shared__ float2_t biases[SHAPED ? R * 16 : 1];
+    __shared__ uint32_t firsts[SHAPED ? R * 16 : 1];
     uint4_t* queries = reinterpret_cast<uint4_t*>(space);
 
     __shared__ uint32_t walks[WAVES][8];
-    walk<D, WAVES * 64>(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
+    walk<D, WAVES * 64, SHAPED>(kernel_args(), threadIdx.x & 63, walks[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)], [&](const Segment& x) {
         Args& a = kernel_args();
         const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
@@ -657,6 +705,19 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         if (tile < R) {
             load_query<D>(a, x, tile * 16 + col, quarter, raw);
             if (a.mask) mask = a.mask[int64_t(x.seq.first_token + place_of_row(a, x, tile * 16 + col).token) * a.mask_words];
+        }
+        float2_t bias = {0.0f, 0.0f};
+        uint32_t own_first = 0;
+        if constexpr (SHAPED) {
+            if (tile < R) {
+                const RowPlace place = place_of_row(a, x, tile * 16 + col);
+                if (shaped(a).slopes) {
+                    const uint32_t row = x.seq.first_token + place.token;
+                    bias.x = shaped(a).slopes[place.head] * kLog2e;
+                    bias.y = float(shaped(a).positions ? shaped(a).positions[row] : int32_t(x.seq.context + place.token));
+                }
+                if (shaped(a).first) own_first = first_of(a, x.seq, place.token);
+            }
         }
         size_t at[2];
         Words<S::kWords> k[2][S::kLoads], v[2][S::kLoads];
@@ -727,6 +788,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 if (quarter == 0) {
                     units[tile * 16 + col] = unit;
                     masks[tile * 16 + col] = mask;
+                    if constexpr (SHAPED) {
+                        biases[tile * 16 + col] = bias;
+                        firsts[tile * 16 + col] = own_first;
+                    }
                 }
             }
         }
@@ -740,12 +805,13 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             else return uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
         };
         auto get_unit = [&](int r) { return kInLds ? units[r * 16 + col] : unit; };
-        auto get_scales = [&](float4_t (&ks)[2], float4_t (&vs)[2]) {
+        auto get_k_scales = [&](float4_t (&s)[2]) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                ks[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][h * 16 + quarter * 4]) : k_scales[h];
-                vs[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][32 + h * 16 + quarter * 4]) : v_scales[h];
-            }
+            for (int h = 0; h < 2; ++h) s[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][h * 16 + quarter * 4]) : k_scales[h];
+        };
+        auto get_v_scales = [&](float4_t (&s)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][32 + h * 16 + quarter * 4]) : v_scales[h];
         };
         // (from the thread's number anew, and so in the next: what both compute would be kept in registers through the loop)
         auto sees = [&](int r, int h) {
@@ -754,16 +820,28 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             const uint32_t first = key + h * 16 + quarter * 4, there = lowest_bits(int32_t(x.seq.total - first));
             const int32_t u = int32_t(first - x.seq.context);
             const uint32_t token = place_of_row(b, x, r * 16 + col).token;
+            uint32_t from_first = 15u;
+            if constexpr (SHAPED) {
+                const uint32_t its_first = kInLds ? firsts[r * 16 + col] : own_first;
+                from_first = ~lowest_bits(int32_t(its_first - first));
+                if (b.mask == nullptr) {
+                    int32_t upto = int32_t(token) + 1;
+                    if (shaped(b).prefix) upto = max(upto, min(scalar(shaped(b).prefix + x.b), 1 << 30) - int32_t(x.seq.context));
+                    return lowest_bits(upto - u) & there & from_first;
+                }
+            }
             if (b.mask == nullptr) return lowest_bits(int32_t(token) + 1 - u) & there;
             const uint64_t word = kInLds ? masks[r * 16 + col] : mask;
-            return mask_bits(b.mask + int64_t(x.seq.first_token + token) * b.mask_words, word, b.mask_words, u) & there;
+            return mask_bits(b.mask + int64_t(x.seq.first_token + token) * b.mask_words, word, b.mask_words, u) & there & from_first;
         };
-        // what lies behind the last token is no token's: no code of it may reach a product, as 0 * NaN is NaN
+        // what lies behind the last token, or in front of the first that anybody sees, is no token's (its page may have gone to another):
+        // no code of it may reach a product, as 0 * NaN is NaN
         auto hide = [&] {
             const uint32_t quarter = thread_here() >> 4 & 3;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t there = lowest_bits(int32_t(x.seq.total - (key + h * 16 + quarter * 4)));
+                uint32_t there = lowest_bits(int32_t(x.seq.total - (key + h * 16 + quarter * 4)));
+                if constexpr (SHAPED) there &= ~lowest_bits(int32_t(x.seq.front - (key + h * 16 + quarter * 4)));
                 uint32_t keep = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) keep |= there >> i & 1 ? 0xffu << (8 * i) : 0u;
@@ -773,6 +851,41 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                     for (int w = 0; w < S::kWords; ++w) v[h][i].w[w] &= keep;
             }
         };
+        // Scores in units of log2: the tanh, cap (1 - 2 / (1 + e^(2 s / cap))), whose error is that of 1 / (1 + e), 2^-23 of the cap, so at
+        // most 2^-13 at the largest cap, 2^9 (in units of log2; half precision's rounding of weights is 2^-11); and the distance's part.
+        const auto shape = [&] {
+            if constexpr (!SHAPED) {
+                return nullptr;
+            } else {
+                return [&, cap_in = shaped(a).cap_in, cap_out = shaped(a).cap_out, biased = shaped(a).slopes != nullptr, placed = shaped(a).positions != nullptr](int r, int h, float4_t& s) {
+                    if (cap_in != 0.0f)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[i] * cap_in)), -2.0f * cap_out, cap_out);
+                    if (biased) {
+                        const uint32_t t = thread_here();
+                        const float2_t its = kInLds ? biases[r * 16 + (t & 15)] : bias;
+                        const int32_t first = int32_t(key + h * 16 + (t >> 4 & 3) * 4);
+                        const float at = float(first) - its.y;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(its.x, at + float(i), s[i]);
+                        if (placed && key + 32 > x.seq.context) {
+                            // new tokens are where they are said to be
+                            Args& b = kernel_args();
+#pragma unroll 1
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t j = uint32_t(first + i), u = j - x.seq.context;
+                                float more = 0.0f;
+                                if (j >= x.seq.context && j < x.seq.total) more = its.x * float(shaped(b).positions[x.seq.first_token + u] - int32_t(j));
+                                s[0] += i == 0 ? more : 0.0f;
+                                s[1] += i == 1 ? more : 0.0f;
+                                s[2] += i == 2 ? more : 0.0f;
+                                s[3] += i == 3 ? more : 0.0f;
+                            }
+                        }
+                    }
+                };
+            }
+        }();
         // One step; `more` is known where this is compiled, as the compiler would otherwise count on values that were not asked for
         // behind keys that were, and wait for both.
         auto run_step = [&](auto more) {
@@ -781,7 +894,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             if constexpr (more()) locate(next);
             put_scales();
             // the keys' registers are free for the next once the scores are there, the others' at the end
-            sums.step(key + 32 > x.all_see, get_k, get_v, get_q, get_unit, get_scales, sees, hide, [&] {
+            sums.step(key + 32 > x.all_see || (SHAPED && key < x.all_from), get_k, get_v, get_q, get_unit, get_k_scales, get_v_scales, shape, sees, hide, [&] {
                 if constexpr (more()) ask_scales();
                 if constexpr (more()) load_k();
                 __builtin_amdgcn_sched_barrier(0);
@@ -799,28 +912,28 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 
-template <int D, int CODES, int PARTS> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
+template <int D, int CODES, int PARTS, bool SHAPED> int start_attention(const ArgsOf<SHAPED>& a, const AttentionPlan& p, void* stream, Launched& info) {
     const dim3 grid = p.shares() == 0 ? dim3(a.cache.kv_heads, p.row_blocks, a.batch) : dim3(p.shares(), 1, 1), block(p.waves * 64);
-    const char* name = p.tiles == 4 ? "tree_attention_4x4" : p.tiles == 2 ? "tree_attention_2x4" : p.waves == 8 ? "tree_attention_1x8" : "tree_attention_1x4";
+    const char* name = SHAPED ? p.tiles == 4 ? "shaped_attention_4x4" : p.tiles == 2 ? "shaped_attention_2x4" : p.waves == 8 ? "shaped_attention_1x8" : "shaped_attention_1x4"
+                              : p.tiles == 4 ? "tree_attention_4x4" : p.tiles == 2 ? "tree_attention_2x4" : p.waves == 8 ? "tree_attention_1x8" : "tree_attention_1x4";
     info = {name, {grid.x, grid.y, grid.z}, {block.x, 1, 1}, 0};
     if constexpr (D <= 128)
-        if (p.tiles == 4) return launch(k_tree_attention<D, CODES, 4, PARTS, 4>, grid, block, stream, a);
-    if (p.tiles == 2) return launch(k_tree_attention<D, CODES, 2, PARTS, 4>, grid, block, stream, a);
-    if (p.waves == 8) return launch(k_tree_attention<D, CODES, 1, PARTS, 8>, grid, block, stream, a);
-    return launch(k_tree_attention<D, CODES, 1, PARTS, 4>, grid, block, stream, a);
+        if (p.tiles == 4) return launch(k_tree_attention<D, CODES, 4, PARTS, 4, SHAPED>, grid, block, stream, a);
+    if (p.tiles == 2) return launch(k_tree_attention<D, CODES, 2, PARTS, 4, SHAPED>, grid, block, stream, a);
+    if (p.waves == 8) return launch(k_tree_attention<D, CODES, 1, PARTS, 8, SHAPED>, grid, block, stream, a);
+    return launch(k_tree_attention<D, CODES, 1, PARTS, 4, SHAPED>, grid, block, stream, a);
 }
-template <int D, int CODES> int start_attention(const AttentionArgs& a, const AttentionPlan& p, void* stream, Launched& info) {
+template <int D, int CODES, bool SHAPED> int start_attention(const ArgsOf<SHAPED>& a, const AttentionPlan& p, void* stream, Launched& info) {
     if constexpr (kCodeProducts<D, CODES>) {
-        if (a.type == FKLHIP_F16) return start_attention<D, CODES, 3>(a, p, stream, info);
-        return start_attention<D, CODES, 2>(a, p, stream, info);
+        if (a.type == FKLHIP_F16) return start_attention<D, CODES, 3, SHAPED>(a, p, stream, info);
+        return start_attention<D, CODES, 2, SHAPED>(a, p, stream, info);
     } else {
-        return start_attention<D, CODES, 0>(a, p, stream, info);
+        return start_attention<D, CODES, 0, SHAPED>(a, p, stream, info);
     }
 }
-
-template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) {
-    if (a.cache.codes == FKLHIP_CODES_INT8) return start_attention<D, FKLHIP_CODES_INT8>(a, plan, stream, info);
-    return start_attention<D, FKLHIP_CODES_E4M3>(a, plan, stream, info);
+template <int D, bool SHAPED> int start_attention(const ArgsOf<SHAPED>& a, const AttentionPlan& plan, void* stream, Launched& info) {
+    if (a.cache.codes == FKLHIP_CODES_INT8) return start_attention<D, FKLHIP_CODES_INT8, SHAPED>(a, plan, stream, info);
+    return start_attention<D, FKLHIP_CODES_E4M3, SHAPED>(a, plan, stream, info);
 }
 
 } // namespace fkattn

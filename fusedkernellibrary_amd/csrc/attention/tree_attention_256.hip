@@ -2,5 +2,5 @@
 #include "tree_attention.hpp"
 
 namespace fkattn {
-template int launch_attention<256>(const AttentionArgs&, const AttentionPlan&, void*, Launched&);
+template <> int launch_attention<256>(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) { return start_attention<256, false>(a, plan, stream, info); }
 }

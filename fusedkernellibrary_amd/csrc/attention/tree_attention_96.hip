@@ -2,5 +2,5 @@
 #include "tree_attention.hpp"
 
 namespace fkattn {
-template int launch_attention<96>(const AttentionArgs&, const AttentionPlan&, void*, Launched&);
+template <> int launch_attention<96>(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info) { return start_attention<96, false>(a, plan, stream, info); }
 }

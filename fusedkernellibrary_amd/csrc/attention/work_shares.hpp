@@ -1,6 +1,8 @@
 // work_shares.hpp -- how attention's work is dealt out to workgroups: all of them count it the same way.
 #pragma once
 
+#include <type_traits>
+
 #include "attention_device.hpp"
 
 namespace fkattn {
@@ -13,6 +15,11 @@ __device__ __forceinline__ Args& kernel_args() {
     asm volatile("" : "+s"(p));
     return *p;
 }
+// The same of a kernel whose argument is ShapedArgs.
+using Shaped = const __attribute__((address_space(4))) ShapedArgs;
+__device__ __forceinline__ Shaped& shaped(Args& a) { return *(Shaped*)&a; }
+template <bool SHAPED> using ArgsOf = std::conditional_t<SHAPED, ShapedArgs, AttentionArgs>;
+
 // The thread's number, for a part of a kernel that is run again and again: what is computed from it stays in that part (the
 // compiler would move it in front of the loop over segments, and keep it in registers through everything).
 __device__ __forceinline__ uint32_t thread_here() {
@@ -25,7 +32,8 @@ template <typename T> __device__ __forceinline__ T scalar(const T* p) { return *
 
 // A sequence as the device finds it, held inside what the host was told. One with rows has keys: where the page table has room for
 // no token, max_new is 0 here.
-struct Sequence { uint32_t first_token, fresh, context, total, rows; };
+// (`front`: no row sees a key in front of that, and `skip` granules hold no other; 0 where nothing is shaped.)
+struct Sequence { uint32_t first_token, fresh, context, total, rows, front = 0, skip = 0; };
 __device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t end, int32_t have) {
     Sequence s;
     s.first_token = start < 0 ? 0u : min(uint32_t(start), a.tokens);
@@ -36,10 +44,21 @@ __device__ __forceinline__ Sequence sequence_of(Args& a, int32_t start, int32_t 
     s.rows = s.fresh * a.group;
     return s;
 }
-__device__ __forceinline__ Sequence sequence_at(Args& a, uint32_t b) { return sequence_of(a, scalar(a.q_start + b), scalar(a.q_start + b + 1), scalar(a.context + b)); }
+__device__ __forceinline__ uint32_t granules_of_keys(Args& a, uint32_t keys) { return (keys + (1u << a.granule_log) - 1) >> a.granule_log; }
+// A sequence's front, by what its first row sees first. (One granule is left at least: what has rows has them written.)
+__device__ __forceinline__ void skip_front(Args& a, Sequence& s, int32_t first) {
+    s.front = first < 0 ? 0u : min(uint32_t(first), s.total);
+    s.skip = s.total ? min(s.front >> a.granule_log, granules_of_keys(a, s.total) - 1) : 0u;
+}
+template <bool SHAPED> __device__ __forceinline__ Sequence sequence_at(Args& a, uint32_t b) {
+    Sequence s = sequence_of(a, scalar(a.q_start + b), scalar(a.q_start + b + 1), scalar(a.context + b));
+    if constexpr (SHAPED)
+        if (shaped(a).first && s.fresh) skip_front(a, s, scalar(shaped(a).first + s.first_token));
+    return s;
+}
 // Work is counted in granules: 2^granule_log keys of one key head and one block of its rows. In front of a block's keys stand
 // `lead` granules for what it takes to begin and to end it.
-__device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return s.total ? a.lead + ((s.total + (1u << a.granule_log) - 1) >> a.granule_log) : 0u; }
+__device__ __forceinline__ uint32_t granules_of(Args& a, const Sequence& s) { return s.total ? a.lead + granules_of_keys(a, s.total) - s.skip : 0u; }
 __device__ __forceinline__ uint32_t blocks_of(Args& a, const Sequence& s) { return (s.rows + a.unit_rows - 1) >> __builtin_ctz(a.unit_rows); }
 __device__ __forceinline__ uint32_t weight_of(Args& a, const Sequence& s) { return blocks_of(a, s) * a.cache.kv_heads * granules_of(a, s); }
 
@@ -57,43 +76,49 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t v) {
 }
 
 // (of the lane's own sequence; behind the last there are empty ones)
-__device__ __forceinline__ Sequence sequence_of_lane(Args& a, uint32_t b) {
-    return b < a.batch ? sequence_of(a, a.q_start[b], a.q_start[b + 1], a.context[b]) : Sequence{0, 0, 0, 0, 0};
+template <bool SHAPED> __device__ __forceinline__ Sequence sequence_of_lane(Args& a, uint32_t b) {
+    if (b >= a.batch) return Sequence{0, 0, 0, 0, 0};
+    Sequence s = sequence_of(a, a.q_start[b], a.q_start[b + 1], a.context[b]);
+    if constexpr (SHAPED)
+        if (shaped(a).first && s.fresh) skip_front(a, s, shaped(a).first[s.first_token]);
+    return s;
 }
-__device__ __forceinline__ Sequence of_lane(const Sequence& s, uint32_t lane) {
+template <bool SHAPED> __device__ __forceinline__ Sequence of_lane(const Sequence& s, uint32_t lane) {
     const auto get = [&](uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), int(lane))); };
-    return {get(s.first_token), get(s.fresh), get(s.context), get(s.total), get(s.rows)};
+    Sequence its{get(s.first_token), get(s.fresh), get(s.context), get(s.total), get(s.rows)};
+    if constexpr (SHAPED) its.front = get(s.front), its.skip = get(s.skip);
+    return its;
 }
 // The granules of all sequences, and the first of a sequence: that of granule at(all), or that of a token; is_it(all, the lane's
 // sequence, its first granule, the one behind its last). b is the batch's size if there is none.
 struct Found { uint32_t all, b, before; Sequence s; };
-template <typename F> __device__ __forceinline__ Found find(Args& a, uint32_t lane, F is_it) {
+template <bool SHAPED, typename F> __device__ __forceinline__ Found find(Args& a, uint32_t lane, F is_it) {
     uint32_t before = 0;
     Found f{0, a.batch, 0, {0, 0, 0, 0, 0}};
     if (a.batch <= 64) {
-        const Sequence s = sequence_of_lane(a, lane);
+        const Sequence s = sequence_of_lane<SHAPED>(a, lane);
         const uint32_t own = weight_of(a, s), upto = scan_wave(own);
         f.all = __builtin_amdgcn_readlane(int(upto), 63);
         const uint64_t hits = __ballot(lane < a.batch && is_it(f.all, s, upto - own, upto));
         if (hits) {
             f.b = __builtin_ctzll(hits);
             f.before = __builtin_amdgcn_readlane(int(upto - own), int(f.b));
-            f.s = of_lane(s, f.b);
+            f.s = of_lane<SHAPED>(s, f.b);
         }
         return f;
     }
     uint32_t sum = 0;
-    for (uint32_t b = lane; b < a.batch; b += 64) sum += weight_of(a, sequence_of_lane(a, b));
+    for (uint32_t b = lane; b < a.batch; b += 64) sum += weight_of(a, sequence_of_lane<SHAPED>(a, b));
     f.all = __builtin_amdgcn_readlane(int(scan_wave(sum)), 63);
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const Sequence s = sequence_of_lane(a, b0 + lane);
+        const Sequence s = sequence_of_lane<SHAPED>(a, b0 + lane);
         const uint32_t own = weight_of(a, s), upto = before + scan_wave(own);
         const uint64_t hits = __ballot(b0 + lane < a.batch && is_it(f.all, s, upto - own, upto));
         if (hits) {
             const int hit = __builtin_ctzll(hits);
             f.b = b0 + hit;
             f.before = __builtin_amdgcn_readlane(int(upto - own), hit);
-            f.s = of_lane(s, hit);
+            f.s = of_lane<SHAPED>(s, hit);
             return f;
         }
         before = __builtin_amdgcn_readlane(int(upto), 63);

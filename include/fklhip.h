@@ -233,6 +233,23 @@ typedef struct fklhip_attention {
 int fklhip_tree_attention_workspace(const fklhip_attention *call, const fklhip_kv_cache *cache, uint64_t *bytes);
 int fklhip_tree_attention(const fklhip_attention *call, const fklhip_kv_cache *cache, void *stream);
 
+/* The same with scores of another shape, s = cap tanh(scale q.k / cap) - slope distance, and rows that see other keys.
+ *   cap      0: no tanh; else 2^-6 to 2^9
+ *   slopes   one for each query head, or NULL. The distance is the row's position less the key's: places in the sequence, or, of
+ *            new tokens, positions[row] (a tree's tokens: context + depth) where they are given.
+ *   first    of each row: it sees no key in front of place first[row] (a window, the beginning of its document). No row of
+ *            a sequence sees a key in front of its first row's; what is in front of that is not read.
+ *   prefix   of each sequence, without a mask: all of its rows see all keys in front of place prefix[b].
+ * A row sees a key if the mask (or the order of tokens, or prefix) and first let it. The workspace is that of the call. */
+typedef struct fklhip_scores {
+    const float *slopes;               /* [q_heads] or NULL */
+    const int32_t *positions, *first;  /* [tokens] or NULL */
+    const int32_t *prefix;             /* [batch] or NULL */
+    float cap;
+} fklhip_scores;
+
+int fklhip_shaped_attention(const fklhip_attention *call, const fklhip_scores *scores, const fklhip_kv_cache *cache, void *stream);
+
 /* The tables of a server's step, from its requests' lengths. Request b has context[b] tokens in the cache, the first held[b]
  * entries of its page table's row, and fresh[b] new tokens. Entries that the new tokens need are taken from the end of the
  * first *available of free_pages, request by request, and written to page_table; held_out[b] and *left are what held and

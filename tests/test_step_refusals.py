@@ -9,7 +9,7 @@ import torch
 
 import fusedkernellibrary_amd as fkl
 from fusedkernellibrary_amd import attention as ops
-from test_attention_refusals import AT, I32, I64, P, Cache, a_cache, refused, some_heads
+from test_attention_refusals import AT, I32, I64, P, Cache, a_cache, an_attention, refused, some_heads, some_rows
 
 
 class Tables(C.Structure):
@@ -36,7 +36,11 @@ class Axes(C.Structure):
     _fields_ = [("stride", I64), ("count", I32), ("of_pair", C.c_uint8 * 128)]
 
 
-STRUCTURES = [("fklhip_tables", Tables, 144), ("fklhip_drafts", Drafts, 128), ("fklhip_axes", Axes, 144)]
+class Scores(C.Structure):
+    _fields_ = [(n, P) for n in ("slopes", "positions", "first", "prefix")] + [("cap", C.c_float)]
+
+
+STRUCTURES = [("fklhip_scores", Scores, 40), ("fklhip_tables", Tables, 144), ("fklhip_drafts", Drafts, 128), ("fklhip_axes", Axes, 144)]
 
 
 @pytest.mark.parametrize("name,mirror,size", STRUCTURES)
@@ -142,3 +146,19 @@ def test_axes(axes, word):
 def test_axes_of_pairs_that_do_not_turn_are_not_looked_at():
     assert fkl.lib().fklhip_qk_norm_rope_axes(C.byref(some_heads(tokens=0)), C.byref(some_axes(4, (0,) * 32 + (9,))), None) == 0
     refused(fkl.lib().fklhip_qkv_to_cache_axes(C.byref(some_heads()), C.byref(some_axes()), None, None), "no cache")
+
+
+@pytest.mark.parametrize("change,call,word", [
+    (dict(cap=-1.0), {}, "cap"), (dict(cap=2.0 ** -7), {}, "cap"), (dict(cap=513.0), {}, "cap"), (dict(cap=float("nan")), {}, "cap"), (dict(cap=float("inf")), {}, "cap"),
+    (dict(slopes=AT + 2), {}, "aligned"), (dict(positions=AT + 1), {}, "aligned"), (dict(first=AT + 2), {}, "aligned"), (dict(prefix=AT + 2), {}, "aligned"),
+    (dict(prefix=AT), dict(mask=AT, mask_words=1), "prefix and a mask"), (dict(cap=4.0), dict(type=3), "type"), (dict(cap=4.0), dict(q=some_rows(data=AT + 2)), "16 bytes"),
+    (dict(first=AT), dict(max_context=1 << 20, page_table_stride=1 << 18), "workspace")])
+def test_scores(change, call, word):
+    refused(fkl.lib().fklhip_shaped_attention(C.byref(an_attention(**call)), C.byref(Scores(**change)), C.byref(a_cache()), None), word)
+
+
+def test_shaping_nothing():
+    l = fkl.lib()
+    refused(l.fklhip_shaped_attention(C.byref(an_attention()), None, C.byref(a_cache()), None), "no scores")
+    for nothing in (dict(tokens=0), dict(batch=0), dict(max_new=0)):
+        assert l.fklhip_shaped_attention(C.byref(an_attention(**nothing)), C.byref(Scores(cap=3.0)), C.byref(a_cache()), None) == 0
