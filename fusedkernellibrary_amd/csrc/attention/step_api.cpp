@@ -28,7 +28,7 @@ int check_drafts(const fklhip_drafts* d) {
     return FKLHIP_OK;
 }
 uint64_t sums_of(const fklhip_drafts& d) { return uint64_t(d.batch) * verify_chunks(uint32_t(d.vocab)) * 8; }
-uint64_t workspace_of(const fklhip_drafts& d) { return d.max_new ? sums_of(d) + uint64_t(d.batch) * (4 + uint64_t(d.max_new)) * 4 : 0; }
+uint64_t workspace_of(const fklhip_drafts& d) { return d.max_new ? sums_of(d) + uint64_t(d.batch) * (kVerifyRecord + uint64_t(d.max_new)) * 4 : 0; }
 
 template <typename... P> bool all_aligned(size_t n, P... p) { return (aligned(p, n) && ...); }
 

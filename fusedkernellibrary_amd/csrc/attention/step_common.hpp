@@ -15,6 +15,7 @@ struct TablesArgs {
     uint32_t tokens, batch, width, page_log, max_new, mask_words, free_count;
 };
 
+constexpr uint32_t kVerifyRecord = 8;
 struct VerifyArgs {
     const char *target, *draft;
     int64_t target_stride, draft_stride;    // bytes
@@ -22,7 +23,7 @@ struct VerifyArgs {
     const float* uniforms;
     int32_t *path, *count, *out;
     double* sums;                           // [batch][chunks]
-    int32_t* record;                        // [batch][4 + max_new]
+    int32_t* record;                        // [batch][kVerifyRecord + max_new]
     uint32_t tokens, batch, max_new, vocab, chunks;
 };
 

@@ -68,8 +68,11 @@ __device__ __forceinline__ Place place_of(const VerifyArgs& a, uint32_t b) {
     return p;
 }
 
-// What the path of a sequence leads to: kept for the second launch in front of the refused children's tokens.
-struct Outcome { int32_t here, against, refused, count; };                   // `against`: the refused row whose q is taken off, or -1
+// What the path of a sequence leads to. `against`: the refused row whose q is taken off, or -1.
+struct Outcome { int32_t here, against, refused, count; };
+// What the second launch needs of it, rows counted from the first of all; the refused children's tokens stand behind.
+struct Record { int32_t here, against, refused, count; float u; int32_t none[3]; };
+static_assert(sizeof(Record) == kVerifyRecord * 4);
 
 __device__ __forceinline__ double of_lane(double v, uint32_t lane) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -179,7 +182,10 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_sums(co
     if (p.count == 0) {
         if (chunk == 0) {
             for (uint32_t i = threadIdx.x; i < a.max_new; i += kThreads) a.path[size_t(b) * a.max_new + i] = a.out[size_t(b) * a.max_new + i] = -1;
-            if (threadIdx.x == 0) a.count[b] = 0;
+            if (threadIdx.x == 0) {
+                a.count[b] = 0;
+                a.record[size_t(b) * (kVerifyRecord + a.max_new) + 3] = 0;
+            }
         }
         return;
     }
@@ -190,19 +196,17 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_sums(co
     __syncthreads();
     const Outcome o = shared;
     if (chunk == 0) {
-        int32_t* record = a.record + size_t(b) * (4 + a.max_new);
+        int32_t* record = a.record + size_t(b) * (kVerifyRecord + a.max_new);
         for (uint32_t i = threadIdx.x; i < a.max_new; i += kThreads) {
             const bool kept = int32_t(i) < o.count;
             a.path[size_t(b) * a.max_new + i] = kept ? path[i] : -1;
             a.out[size_t(b) * a.max_new + i] = int32_t(i) + 1 < o.count ? a.ids[p.first + path[i + 1]] : -1;
-            if (int32_t(i) < o.refused) record[4 + i] = refused[i];
+            if (int32_t(i) < o.refused) record[kVerifyRecord + i] = refused[i];
         }
         if (threadIdx.x == 0) {
             a.count[b] = o.count;
-            record[0] = o.here;
-            record[1] = o.against;
-            record[2] = o.refused;
-            record[3] = o.count;
+            const int32_t first = int32_t(p.first);
+            *reinterpret_cast<Record*>(record) = {first + o.here, o.against < 0 ? -1 : first + o.against, a.draft ? 0 : o.refused, o.count, as_uniform(a.uniforms[first]), {0, 0, 0}};
         }
     }
     Weights<TYPE> w;
@@ -216,113 +220,122 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_sums(co
     if (threadIdx.x == 0) a.sums[size_t(b) * a.chunks + chunk] = s;
 }
 
+// Sums of a wave's lanes up to and with each.
+__device__ __forceinline__ double scan_lanes(double v, uint32_t lane) {
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+        const double before = __shfl_up(v, i);
+        if (lane >= uint32_t(i)) v += before;
+    }
+    return v;
+}
+
+// Where a running sum exceeds `share` of them all: the chunk, the sum in front of it and the border; chunk < 0: all are 0.
+struct Chunk { int32_t chunk; double front, border; };
+__device__ __forceinline__ Chunk find_chunk(const double* sums, uint32_t chunks, float share, uint32_t lane) {
+    // (every wave for itself: there is nothing to wait for)
+    double own = lane < chunks ? sums[lane] : 0.0, upto = scan_lanes(own, lane), all = of_lane(upto, 63);
+    for (uint32_t c0 = 64; c0 < chunks; c0 += 64) all += of_lane(scan_lanes(c0 + lane < chunks ? sums[c0 + lane] : 0.0, lane), 63);
+    Chunk f{-1, 0.0, double(share) * all};
+    if (!(all > 0.0)) return f;
+    double before = 0.0;
+    for (uint32_t c0 = 0;;) {
+        const double in_front = before + (upto - own);
+        const uint64_t some = __ballot(own > 0.0), over = __ballot(own > 0.0 && before + upto > f.border);
+        if (over || some) {
+            const uint32_t at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+            f.chunk = int32_t(c0 + at);
+            f.front = of_lane(in_front, at);
+            if (over) return f;                                              // (else the last that has something, if none is over)
+        }
+        before += of_lane(upto, 63);
+        c0 += 64;
+        if (c0 >= chunks) return f;
+        own = c0 + lane < chunks ? sums[c0 + lane] : 0.0;
+        upto = scan_lanes(own, lane);
+    }
+}
+
 template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_pick(const VerifyArgs a) {
     __shared__ double waves[4], runs[kRuns<TYPE>][4];
-    __shared__ uint32_t found, last;
+    __shared__ uint32_t found[4], last[4];
     const uint32_t b = blockIdx.x, thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
-    const Place p = place_of(a, b);
-    if (p.count == 0) return;
-    const int32_t* record = a.record + size_t(b) * (4 + a.max_new);
-    const Outcome o{record[0], record[1], record[2], record[3]};
+    const int32_t* record = a.record + size_t(b) * (kVerifyRecord + a.max_new);
+    const Record o = *reinterpret_cast<const Record*>(record);
+    if (o.count == 0) return;
     double* sums = a.sums + size_t(b) * a.chunks;
-    const char *target = a.target + int64_t(p.first + o.here) * a.target_stride, *draft = o.against >= 0 ? a.draft + int64_t(p.first + o.against) * a.draft_stride : nullptr;
-    const float u = as_uniform(a.uniforms[p.first]);
-    int32_t id = -1;
-    for (int plain = 0; plain < 2; ++plain) {
-        Weights<TYPE> w;
-        if (plain) {
-            // no weight is left: the target's row as it is
-            for (uint32_t c = 0; c < a.chunks; ++c) {
-                w.load(target, nullptr, c, a.vocab);
-                double s = 0.0;
+    const char *target = a.target + int64_t(o.here) * a.target_stride, *draft = o.against >= 0 ? a.draft + int64_t(o.against) * a.draft_stride : nullptr;
+    Weights<TYPE> w;
+    Chunk f = find_chunk(sums, a.chunks, o.u, lane);
+    const bool whole = f.chunk < 0;
+    if (whole) {
+        // no weight is left: the target's row as it is
+        __syncthreads();
+        for (uint32_t c = 0; c < a.chunks; ++c) {
+            w.load(target, nullptr, c, a.vocab);
+            double s = 0.0;
 #pragma unroll
-                for (uint32_t k = 0; k < kRuns<TYPE>; ++k) s += w.sum(k);
-                s = sum_of_all(s, waves);
-                if (thread == 0) sums[c] = s;
-            }
-            __syncthreads();
-        }
-        // the chunk: each thread has some that are neighbours
-        const uint32_t each = (a.chunks + kThreads - 1) / kThreads, c0 = min(thread * each, a.chunks), c1 = min(c0 + each, a.chunks);
-        double own = 0.0;
-        for (uint32_t c = c0; c < c1; ++c) own += sums[c];
-        double upto = own;
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-            const double before = __shfl_up(upto, i);
-            if (lane >= uint32_t(i)) upto += before;
+            for (uint32_t k = 0; k < kRuns<TYPE>; ++k) s += w.sum(k);
+            s = sum_of_all(s, waves);
+            if (thread == 0) sums[c] = s;
         }
         __syncthreads();
-        if (lane == 63) waves[wave] = upto;
-        if (thread == 0) {
-            found = 0xffffffffu;
-            last = 0;
-        }
-        __syncthreads();
-        double before = upto - own, all = 0.0;
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (i < wave) before += waves[i];
-            all += waves[i];
-        }
-        if (!(all > 0.0)) continue;
-        const double border = double(u) * all;
-        for (uint32_t c = c0; c < c1; ++c) {
-            const double s = sums[c];
-            before += s;
-            if (s > 0.0) {
-                atomicMax(&last, c);
-                if (before > border) {
-                    atomicMin(&found, c);
-                    break;
-                }
-            }
-        }
-        __syncthreads();
-        const uint32_t chunk = found != 0xffffffffu ? found : last;
-        // what is in front of it, in order
-        double front = 0.0;
-        for (uint32_t c = thread; c < chunk; c += kThreads) front += sums[c];
-        front = sum_of_all(front, waves);
-        w.load(target, plain ? nullptr : draft, chunk, a.vocab);
-        if (!a.draft && !plain)
-            for (int32_t i = 0; i < o.refused; ++i) w.clear(chunk, uint32_t(record[4 + i]));
-        double run[kRuns<TYPE>];
-#pragma unroll
-        for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
-            run[k] = w.sum(k);
-            double scan = run[k];
-#pragma unroll
-            for (int i = 1; i < 64; i <<= 1) {
-                const double x = __shfl_up(scan, i);
-                if (lane >= uint32_t(i)) scan += x;
-            }
-            if (lane == 63) runs[k][wave] = scan;
-            run[k] = scan - run[k];
-        }
-        __syncthreads();
-        if (thread == 0) {
-            found = 0xffffffffu;
-            last = 0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
-            double sum = front + run[k];
-            for (uint32_t i = 0; i < k * 4 + wave; ++i) sum += runs[i / 4][i % 4];
-#pragma unroll
-            for (uint32_t i = 0; i < kRun<TYPE>; ++i) {
-                sum += w.w[k][i];
-                if (w.w[k][i] > 0.0) {
-                    atomicMax(&last, w.at(chunk, k) + i);
-                    if (sum > border) atomicMin(&found, w.at(chunk, k) + i);
-                }
-            }
-        }
-        __syncthreads();
-        id = int32_t(found != 0xffffffffu ? found : last);
-        break;
+        f = find_chunk(sums, a.chunks, o.u, lane);
     }
-    if (thread == 0) a.out[size_t(b) * a.max_new + o.count - 1] = id;
+    if (f.chunk < 0) {
+        if (thread == 0) a.out[size_t(b) * a.max_new + o.count - 1] = -1;
+        return;
+    }
+    const uint32_t chunk = uint32_t(f.chunk);
+    w.load(target, whole ? nullptr : draft, chunk, a.vocab);
+    if (!whole)
+        for (int32_t i = 0; i < o.refused; ++i) w.clear(chunk, uint32_t(record[kVerifyRecord + i]));
+    double front[kRuns<TYPE>];
+#pragma unroll
+    for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
+        const double run = w.sum(k), upto = scan_lanes(run, lane);
+        if (lane == 63) runs[k][wave] = upto;
+        front[k] = upto - run;
+    }
+    __syncthreads();
+    // the first element at which the sum is over the border; the last that has something, if rounding leaves none
+    uint32_t first = 0xffffffffu, some = 0;
+    double before = f.front;
+#pragma unroll
+    for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
+        double sum = before;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const double its = runs[k][i];
+            if (i < wave) sum += its;
+            before += its;
+        }
+        sum += front[k];
+#pragma unroll
+        for (uint32_t i = 0; i < kRun<TYPE>; ++i) {
+            sum += w.w[k][i];
+            const uint32_t at = w.at(chunk, k) + i;
+            if (w.w[k][i] > 0.0) {
+                some = at;
+                if (sum > f.border) first = min(first, at);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) {
+        first = min(first, uint32_t(__shfl_xor(int(first), i)));
+        some = max(some, uint32_t(__shfl_xor(int(some), i)));
+    }
+    if (lane == 0) {
+        found[wave] = first;
+        last[wave] = some;
+    }
+    __syncthreads();
+    if (thread == 0) {
+        first = min(min(found[0], found[1]), min(found[2], found[3]));
+        some = max(max(last[0], last[1]), max(last[2], last[3]));
+        a.out[size_t(b) * a.max_new + o.count - 1] = int32_t(first != 0xffffffffu ? first : some);
+    }
 }
 
 template <int TYPE> int start_verify(const VerifyArgs& a, void* stream) {

@@ -80,7 +80,7 @@ def test_bindings_of_tables():
     (dict(max_new=-1), "max_new"), (dict(max_new=1025), "max_new"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 24) + 1), "vocab"), (dict(q_start=None), "q_start"), (dict(path=None), "results"),
     (dict(count=None), "results"), (dict(out=None), "results"), (dict(target=None), "target"), (dict(ids=None), "ids"), (dict(uniforms=None), "uniforms"), (dict(draft=AT, parents=AT), "chains"),
     (dict(target=AT + 2), "aligned"), (dict(type=0, target=AT + 1), "aligned"), (dict(draft=AT + 2), "aligned"), (dict(parents=AT + 1), "aligned"), (dict(out=AT + 2), "aligned"),
-    (dict(workspace=None), "workspace"), (dict(workspace_bytes=71), "workspace"), (dict(workspace=AT + 4), "8 bytes")])
+    (dict(workspace=None), "workspace"), (dict(workspace_bytes=2 * 8 + 2 * 11 * 4 - 1), "workspace"), (dict(workspace=AT + 4), "8 bytes")])
 def test_drafts(change, word):
     refused(fkl.lib().fklhip_verify_drafts(C.byref(some_drafts(**change)), None), word)
     refused(fkl.lib().fklhip_verify_drafts(None, None), "no drafts")
@@ -89,7 +89,7 @@ def test_drafts(change, word):
 def test_workspaces_of_drafts():
     l, need = fkl.lib(), C.c_uint64()
     of = lambda **c: (l.fklhip_verify_drafts_workspace(C.byref(some_drafts(**c)), C.byref(need)), need.value)      # noqa: E731
-    assert of() == (0, 2 * 8 + 2 * 7 * 4) and of(vocab=4097) == (0, 4 * 8 + 2 * 7 * 4) and of(batch=0) == (0, 0) and of(max_new=0) == (0, 0)
+    assert of() == (0, 2 * 8 + 2 * 11 * 4) and of(vocab=4097) == (0, 4 * 8 + 2 * 11 * 4) and of(batch=0) == (0, 0) and of(max_new=0) == (0, 0)
     refused(l.fklhip_verify_drafts_workspace(C.byref(some_drafts()), None), "answer")
     refused(l.fklhip_verify_drafts_workspace(C.byref(some_drafts(vocab=0)), C.byref(need)), "vocab")
     for nothing in (dict(batch=0, workspace=None), dict(max_new=0, workspace=None)):
