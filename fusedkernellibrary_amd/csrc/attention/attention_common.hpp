@@ -38,6 +38,7 @@ struct HeadArgs {
 struct AxesHeadArgs : HeadArgs {
     int64_t position_stride;
     uint32_t axes, of_pairs[8];
+    uint32_t sweeps, chunks_each;           // of many tokens: groups of lanes to a token, and chunks of heads to each
 };
 
 struct ReadArgs {

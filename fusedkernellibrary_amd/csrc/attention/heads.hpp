@@ -107,25 +107,31 @@ __device__ __forceinline__ void turns_of(const AxesHeadArgs& a, uint32_t token, 
         word = turn / 16 == i ? its : word;
     }
     const uint32_t four = word >> (turn % 16 * 2) & 0xffu;
-    const auto pick = [](bool second, uint32_t a, uint32_t b) { return second ? b : a; };      // (of values: a choice of array elements is one of addresses)
-    const auto of = [&](uint32_t k) {
-        const uint32_t axis = four >> (2 * k) & 3u;
-        return pick(axis & 2, pick(axis & 1, position[0], position[1]), pick(axis & 1, position[2], position[3]));
-    };
-    if (four == (four & 3u) * 0x55u) {
-        const uint32_t at = of(0);
-        cosine = sine = float4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        if (at < a.table_rows) {
-            cosine = *reinterpret_cast<const float4_t*>(a.cos + size_t(at) * (a.rot_dim / 2) + turn);
-            sine = *reinterpret_cast<const float4_t*>(a.sin + size_t(at) * (a.rot_dim / 2) + turn);
-        }
-    } else {
+    // a row of the tables for each axis that one of the four pairs has (neighbours in every layout there is: four loads of one
+    // entry each take the cache four times as long)
+    float4_t c[4], s[4];
+    bool there[4];
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t at = of(k);
-            const size_t entry = size_t(min(at, a.table_rows - 1)) * (a.rot_dim / 2) + turn + k;
-            cosine[k] = at < a.table_rows ? a.cos[entry] : __builtin_nanf("");
-            sine[k] = at < a.table_rows ? a.sin[entry] : __builtin_nanf("");
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t hits = four ^ i * 0x55u;              // two zero bits where a pair's axis is i
+        const bool some = i < a.axes && ((hits | hits >> 1) & 0x55u) != 0x55u;
+        there[i] = position[i] < a.table_rows;
+        c[i] = s[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (some && there[i]) {
+            const size_t at = size_t(position[i]) * (a.rot_dim / 2) + turn;
+            c[i] = *reinterpret_cast<const float4_t*>(a.cos + at);
+            s[i] = *reinterpret_cast<const float4_t*>(a.sin + at);
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t axis = four >> (2 * k) & 3u;
+        cosine[k] = sine[k] = __builtin_nanf("");
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const bool its = axis == i && there[i];
+            cosine[k] = its ? c[i][k] : cosine[k];
+            sine[k] = its ? s[i][k] : sine[k];
         }
     }
 }
@@ -136,18 +142,20 @@ template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE, bool AXES>
 __global__ __launch_bounds__(256) void k_heads(const HeadArgsOf<AXES> a) {
     const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, groups = blockDim.x / LANES;
     const uint32_t dim = a.head_dim, tile = tile_of_grid();
-    if (TO_CACHE && blockIdx.x >= a.q_chunks + a.k_chunks) {
+    uint32_t first_value = a.q_chunks + a.k_chunks;           // of the grid's columns
+    if constexpr (AXES && HEADS > 1) first_value = a.sweeps;
+    if (TO_CACHE && blockIdx.x >= first_value) {
         if constexpr (HEADS == 1) {
             // few tokens: each by itself, as few are in neighbouring slots and four at a time take longer than one (32 of 8 heads: 4.8 us, and 3.0 so)
             const uint32_t token = tile * groups + group;
-            if (token < a.tokens) write_value<LANES, TYPE, CODES>(a, token, blockIdx.x - a.q_chunks - a.k_chunks, lane);
+            if (token < a.tokens) write_value<LANES, TYPE, CODES>(a, token, blockIdx.x - first_value, lane);
             return;
         }
         // Values: four tokens in four neighbouring slots have their bytes side by side in the cache. A group looks after four tokens of a
         // head, and stores four at once that begin at one of them and at a slot that is a multiple of four, its own or the next group's;
         // tokens that are of no such four, byte by byte. (A chunk of a prompt begins at any slot: with own ones alone at once, 2048
         // tokens of 8 heads of 128 that began at slot 3 took 17 us, and take 8.6.)
-        const uint32_t head = (blockIdx.x - a.q_chunks - a.k_chunks) * 4 + group % 4, at = lane * 8, first = tile * groups + (group / 4) * 4;
+        const uint32_t head = (blockIdx.x - first_value) * 4 + group % 4, at = lane * 8, first = tile * groups + (group / 4) * 4;
         if (head >= a.kv_heads || first >= a.tokens) return;
         const char* from = a.v.data + head * a.v.head_stride + at * 2;
         uint4_t raw[7];                                        // of tokens first ..
@@ -231,16 +239,116 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgsOf<AXES> a) {
         }
         return;
     }
-    const bool is_q = blockIdx.x < a.q_chunks;
-    const uint32_t head0 = (is_q ? blockIdx.x : blockIdx.x - a.q_chunks) * HEADS, heads = is_q ? a.q_heads : a.kv_heads;
-    const Rows in = is_q ? a.q : a.k, out = is_q ? a.q_out : a.k_out;
-    const char* weights = static_cast<const char*>(is_q ? a.q_weight : a.k_weight);
-    const LanePlace p = place_of(lane, dim, a.rot_dim, a.pairs);
+    // what of a token a group of lanes works on: chunk by chunk of its heads
+    bool is_q, stored = false;
+    uint32_t head0, heads, page = 0, off = 0;
+    Rows in, out;
+    const char* weights;
     float w[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = 1.0f;
-    if (weights && p.live) { load4<TYPE>(weights, p.at[0], w); load4<TYPE>(weights, p.at[1], w + 4); }
+    float4_t cosine = {1.0f, 1.0f, 1.0f, 1.0f}, sine = {0.0f, 0.0f, 0.0f, 0.0f};
+    const LanePlace p = place_of(lane, dim, a.rot_dim, a.pairs);
     const uint32_t token = tile * groups + group;
+    const auto choose = [&](uint32_t chunk) {
+        is_q = chunk < a.q_chunks;
+        head0 = (is_q ? chunk : chunk - a.q_chunks) * HEADS;
+        heads = is_q ? a.q_heads : a.kv_heads;
+        in = is_q ? a.q : a.k;
+        out = is_q ? a.q_out : a.k_out;
+        weights = static_cast<const char*>(is_q ? a.q_weight : a.k_weight);
+    };
+    const auto load_weights = [&] {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = 1.0f;
+        if (weights && p.live) { load4<TYPE>(weights, p.at[0], w); load4<TYPE>(weights, p.at[1], w + 4); }
+    };
+    // a head's elements normed, turned and written: to `out`, or as codes to the cache
+    const auto finish = [&](float (&x)[8], uint32_t head) {
+        if (weights) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(x[k], x[k], sum);
+            const float r = 1.0f / __builtin_sqrtf(sum_lanes<LANES>(sum) / float(dim) + a.eps);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = x[k] * r * w[k];
+        }
+        if (p.rotated) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // pairs are (k, k + 4) of the lane's elements as halves, (2k, 2k + 1) as neighbours
+                float& u = a.pairs ? x[2 * k] : x[k];
+                float& v = a.pairs ? x[2 * k + 1] : x[k + 4];
+                const float s = u, t = v;
+                u = s * cosine[k] - t * sine[k];
+                v = t * cosine[k] + s * sine[k];
+            }
+        }
+        if (is_q || !TO_CACHE) {
+            if (p.live) {
+                char* to = out.data + token * out.token_stride + head * out.head_stride;
+                store4<TYPE>(to, p.at[0], x);
+                store4<TYPE>(to, p.at[1], x + 4);
+            }
+        } else {
+            uint32_t top = 0, code[2];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[k]));
+            const float scale = scale_of<CODES>(max_lanes<LANES>(top));
+            encode8<CODES>(x, scale, code);
+            if (stored) {
+                const size_t at = head_row(a.cache, page, head) + off;
+                if (lane == 0) a.cache.k_scale[at] = scale;
+                if (p.live) {
+                    char* to = a.cache.k + at * dim;
+                    *reinterpret_cast<uint32_t*>(to + p.at[0]) = code[0];
+                    *reinterpret_cast<uint32_t*>(to + p.at[1]) = code[1];
+                }
+            }
+        }
+    };
+    if constexpr (AXES && HEADS > 1) {
+        // Many tokens: a group takes chunks_each of a token's chunks one after the other, and asks for the next while it works on one, so
+        // that the tables' rows are read for all of them at once.
+        if (token >= a.tokens) return;
+        const uint32_t begin = blockIdx.x * a.chunks_each, end = min(begin + a.chunks_each, a.q_chunks + a.k_chunks);
+        uint2_t raw[HEADS][2], next[HEADS][2];
+        const auto ask = [&](uint2_t (&raw)[HEADS][2]) {
+            const char* row = in.data + token * in.token_stride;
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    raw[h][i] = uint2_t{0, 0};
+                    if (p.live && head0 + h < heads) raw[h][i] = *reinterpret_cast<const uint2_t*>(row + (head0 + h) * in.head_stride + p.at[i] * 2);
+                }
+        };
+        choose(begin);
+        ask(raw);
+        if (p.rotated) turns_of(a, token, p.turn, cosine, sine);
+        if (TO_CACHE && end > a.q_chunks) stored = locate(a.cache, a.slots[token], page, off);
+        for (uint32_t chunk = begin; chunk < end; ++chunk) {
+            if (chunk + 1 < end) {
+                choose(chunk + 1);
+                ask(next);
+            }
+            choose(chunk);
+            load_weights();
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                if (head0 + h >= heads) break;
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) unpack2<TYPE>(raw[h][i / 2][i % 2], x[2 * i], x[2 * i + 1]);
+                finish(x, head0 + h);
+            }
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) raw[h][i] = next[h][i];
+        }
+        return;
+    }
+    choose(blockIdx.x);
+    load_weights();
     if (token >= a.tokens) return;
     float x[HEADS][8];
     const char* row = in.data + token * in.token_stride;
@@ -253,7 +361,6 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgsOf<AXES> a) {
             load4<TYPE>(row + (head0 + h) * in.head_stride, p.at[1], x[h] + 4);
         }
     }
-    float4_t cosine = {1.0f, 1.0f, 1.0f, 1.0f}, sine = {0.0f, 0.0f, 0.0f, 0.0f};
     if (p.rotated) {
         if constexpr (AXES) {
             turns_of(a, token, p.turn, cosine, sine);
@@ -268,53 +375,11 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgsOf<AXES> a) {
             }
         }
     }
-    uint32_t page = 0, off = 0;
-    bool stored = false;
     if (TO_CACHE && !is_q) stored = locate(a.cache, a.slots[token], page, off);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
         if (head0 + h >= heads) break;
-        if (weights) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(x[h][k], x[h][k], sum);
-            const float r = 1.0f / __builtin_sqrtf(sum_lanes<LANES>(sum) / float(dim) + a.eps);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[h][k] = x[h][k] * r * w[k];
-        }
-        if (p.rotated) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // pairs are (k, k + 4) of the lane's elements as halves, (2k, 2k + 1) as neighbours
-                float& u = a.pairs ? x[h][2 * k] : x[h][k];
-                float& v = a.pairs ? x[h][2 * k + 1] : x[h][k + 4];
-                const float s = u, t = v;
-                u = s * cosine[k] - t * sine[k];
-                v = t * cosine[k] + s * sine[k];
-            }
-        }
-        if (is_q || !TO_CACHE) {
-            if (p.live) {
-                char* to = out.data + token * out.token_stride + (head0 + h) * out.head_stride;
-                store4<TYPE>(to, p.at[0], x[h]);
-                store4<TYPE>(to, p.at[1], x[h] + 4);
-            }
-        } else {
-            uint32_t top = 0, code[2];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top = max(top, magnitude(x[h][k]));
-            const float scale = scale_of<CODES>(max_lanes<LANES>(top));
-            encode8<CODES>(x[h], scale, code);
-            if (stored) {
-                const size_t at = head_row(a.cache, page, head0 + h) + off;
-                if (lane == 0) a.cache.k_scale[at] = scale;
-                if (p.live) {
-                    char* to = a.cache.k + at * dim;
-                    *reinterpret_cast<uint32_t*>(to + p.at[0]) = code[0];
-                    *reinterpret_cast<uint32_t*>(to + p.at[1]) = code[1];
-                }
-            }
-        }
+        finish(x[h], head0 + h);
     }
 }
 
@@ -333,17 +398,27 @@ constexpr uint32_t kFewRows = 6144;
 constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
+// With several axes many tokens' heads are swept (sweep_heads), by about so many waves: the fewer, the fewer read the tables' rows; fewer
+// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB): 35.3 us with 8192 waves (10 heads each), 38.1 with 4096, 49.6 with
+// 2048, 39.4 with 14336, and 44.0 without sweeps, four heads to a group. 2048 tokens of 32 and 8: 14.5 with 2048, 13.9 with 5120.
+constexpr uint32_t kSweepWaves = 6144;
 template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE, bool AXES>
 int start_heads(HeadArgsOf<AXES> a, uint32_t threads, void* stream, Launched& info) {
     a.q_chunks = ceil_div(a.q_heads, HEADS);
     a.k_chunks = ceil_div(a.kv_heads, HEADS);
     const uint32_t tiles = ceil_div(a.tokens, threads / LANES);
-    const dim3 grid(a.q_chunks + a.k_chunks + (TO_CACHE ? (HEADS == 1 ? a.kv_heads : ceil_div(a.kv_heads, 4)) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
+    uint32_t columns = a.q_chunks + a.k_chunks;
+    if constexpr (AXES && HEADS > 1) {
+        const uint32_t waves = tiles * (threads / 64), most = (kSweepWaves + waves / 2) / waves;
+        a.chunks_each = ceil_div(columns, most < 1 ? 1 : most < columns ? most : columns);
+        columns = a.sweeps = ceil_div(columns, a.chunks_each);
+    }
+    const dim3 grid(columns + (TO_CACHE ? (HEADS == 1 ? a.kv_heads : ceil_div(a.kv_heads, 4)) : 0), tiles < kTilesY ? tiles : kTilesY, ceil_div(tiles, kTilesY));
     info = {"heads", {grid.x, grid.y, grid.z}, {threads, 1, 1}, 0};
     return launch(k_heads<LANES, HEADS, TYPE, CODES, TO_CACHE, AXES>, grid, dim3(threads), stream, a);
 }
 template <int LANES, int TYPE, int CODES, bool TO_CACHE, bool AXES> int start_heads(const HeadArgsOf<AXES>& a, void* stream, Launched& info) {
-    constexpr int kMany = TO_CACHE ? kManyToCache : kManyHeads;
+    constexpr int kMany = TO_CACHE || AXES ? kManyToCache : kManyHeads;
     if (uint64_t(a.tokens) * a.kv_heads <= kFewRows) return start_heads<LANES, 1, TYPE, CODES, TO_CACHE, AXES>(a, smallest_group(LANES), stream, info);
     return start_heads<LANES, kMany, TYPE, CODES, TO_CACHE, AXES>(a, smallest_group(LANES), stream, info);
 }
