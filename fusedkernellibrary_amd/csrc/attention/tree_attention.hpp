@@ -35,6 +35,9 @@
 // parts to the workspace, from where the kernels of merge.hip take them. Without shares (short sequences, or so many that the
 // order of launch evens them out) a workgroup takes one whole (sequence, key head, block of rows). plan_attention chooses.
 //
+// Shaped scores are taken from the last keys to the first: a bias by distance has them rise towards the row, and the reference
+// would have to move in every step (16 trees of up to 13 behind windows of 4096, 32 and 8 heads, e4m3: 68 us that way).
+//
 // The running maximum is a reference m_r and not the exact maximum: weights are w = 2^(s - m) * vs, sums those of 2^(s - m), and
 // m moves only when a weight exceeds 2^kLead. Only then are scores compared across lanes and the sums rescaled. The largest
 // weight starts at 2^kStart, so one is subnormal in half precision (below 2^-14) only 2^-(14 + kStart) below the largest of
@@ -163,14 +166,11 @@ template <bool SHAPED> __device__ __forceinline__ Segment segment_of(Args& a, co
         if (shaped(a).first) {
             // what the block's rows see first, the first and the last of them: a row to a lane
             const uint32_t token = divide(x.row0 + min(thread_here() & 63, x.rows - 1), a.group_magic);
-            uint32_t least = first_of(a, s, token), most = least;
-#pragma unroll
-            for (int i = 32; i; i >>= 1) {
-                least = min(least, uint32_t(__shfl_xor(int(least), i)));
-                most = max(most, uint32_t(__shfl_xor(int(most), i)));
-            }
-            x.all_from = __builtin_amdgcn_readfirstlane(most);
-            x.key0 = min(max(x.key0, __builtin_amdgcn_readfirstlane(least) & ~31u), max(x.key0, x.key1));
+            const uint32_t first = first_of(a, s, token);
+            const uint32_t low = reduce_lanes<32>(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; }), high = max_lanes<32>(first);
+            const uint32_t least = min(__builtin_amdgcn_readlane(low, 0), __builtin_amdgcn_readlane(low, 32));
+            x.all_from = max(__builtin_amdgcn_readlane(high, 0), __builtin_amdgcn_readlane(high, 32));
+            x.key0 = min(max(x.key0, least & ~31u), max(x.key0, x.key1));
         }
     }
     return x;
@@ -253,8 +253,8 @@ template <int D, int THREADS, bool SHAPED, typename F> __device__ __forceinline_
 
 // A wave's priority falls as its share gets done: left alone, the oldest of the workgroups on a compute unit runs ahead, and the
 // last one ends alone, without others to fill its gaps.
-__device__ __forceinline__ void set_priority(const Segment& x, uint32_t key) {
-    const uint32_t left = x.behind + x.key1 - key;
+template <bool DOWN> __device__ __forceinline__ void set_priority(const Segment& x, uint32_t key) {
+    const uint32_t left = x.behind + (DOWN ? key - x.key0 : x.key1 - key);
     if (left > 3 * x.quarter) __builtin_amdgcn_s_setprio(3);
     else if (left > 2 * x.quarter) __builtin_amdgcn_s_setprio(2);
     else if (left > x.quarter) __builtin_amdgcn_s_setprio(1);
@@ -407,7 +407,8 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
     // keys are used up. Where `masked`, sees(tile, block) has a bit for each of the quarter's four keys that the lane's row
     // sees, and hide() clears the values that are no token's. (The masked way is a branch around the scores and no second copy
     // of the loop: between two loops the sums would be held twice.)
-    // shape(tile, block, scores) makes products with the queries, multiplied with their unit, what the scores are; std::nullptr_t: they are.
+    // shape(block, row's slope and place, scores) makes products with the queries, multiplied with their unit, what the scores are;
+    // std::nullptr_t: they are. get_unit has slope and place behind the unit then.
     template <typename K, typename V, typename Q, typename U, typename G, typename W, typename T, typename M, typename H, typename A>
     __device__ __forceinline__ void step(bool masked, K get_k, V get_v, Q get_q, U get_unit, G get_k_scales, W get_v_scales, T shape, M sees, H hide, A after_scores) {
         constexpr bool kShaped = !std::is_same_v<T, std::nullptr_t>;
@@ -430,7 +431,15 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
             if (!kAhead) products(get_k, [&](int run) { return get_q(r, run); }, y);
             if (!kAhead && r + 1 == R) after_scores();
             if (kAhead && kHeld && r + 1 < R) ask_q(r + 1);
-            float unit = get_unit(r);
+            float unit;
+            float2_t bias = {0.0f, 0.0f};
+            if constexpr (kShaped) {
+                const float4_t its = get_unit(r);
+                unit = its[0];
+                bias = float2_t{its[1], its[2]};
+            } else {
+                unit = get_unit(r);
+            }
             float4_t ks[2], vs[2];
             get_k_scales(ks);
             if constexpr (!kShaped) get_v_scales(vs);
@@ -440,7 +449,7 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     y[h] *= unit;
-                    shape(r, h, y[h]);
+                    shape(h, bias, y[h]);
                     if constexpr (R == 4 || (R == 2 && D == 256)) __builtin_amdgcn_sched_barrier(0);    // (both blocks' at once take more registers than there are)
                 }
                 unit = 1.0f;
@@ -575,10 +584,11 @@ template <int WORDS> __device__ __forceinline__ Words<WORDS> load_words_at(Globa
 }
 
 // A wave's way through the page table: 64 entries at a time, one to a lane. (A scalar load for each block of keys would have
-// every wave wait for it; places are asked for in ascending order.)
-struct Pages {
+// every wave wait for it; places are asked for in ascending order, or, by twos, in descending order.)
+template <bool DOWN> struct Pages {
     uint32_t first, entry;
     __device__ __forceinline__ void fetch(Args& a, const Segment& x, uint32_t page, uint32_t lane) {
+        if constexpr (DOWN) page = max(page, 62u) - 62u;       // (the step's second place may be on the next page)
         first = page;
         const int32_t* entries = a.page_table + int64_t(x.b) * a.page_table_stride;
         entry = min(uint32_t(entries[min(page + lane, (x.seq.total - 1) >> a.cache.page_log)]), a.cache.pages - 1);
@@ -683,9 +693,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
     __shared__ float units[R * 16];
     __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
     __shared__ __attribute__((aligned(16))) float scales[WAVES][64];
-    // of shaped rows: slope in units of log2 and position; the first key they see
-    __shared__ float2_t biases[SHAPED ? R * 16 : 1];
+    // of shaped rows: unit, slope in units of log2 and position; the first key they see
+    __shared__ float4_t shapes[SHAPED ? R * 16 : 1];
     __shared__ uint32_t firsts[SHAPED ? R * 16 : 1];
+    __shared__ __attribute__((aligned(16))) float moves[SHAPED ? WAVES : 1][32];
     uint4_t* queries = reinterpret_cast<uint4_t*>(space);
 
     __shared__ uint32_t walks[WAVES][8];
@@ -695,7 +706,12 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
         const uint32_t lane_k = col * D + quarter * (S::kChunk / 4), lane_v = quarter * (4 * D) + col * (S::kChunk / 4);
         // The pages are asked for first, which keys and values wait for, then the queries, which are made ready while those are on their way.
         uint32_t key = x.key0 + wave * 32;
-        Pages pages{0, 0};
+        constexpr uint32_t kStride = WAVES * 32;
+        // (from the last step's keys to the first's: the loop counts up all the same, as another form of it would hold the sums twice)
+        uint32_t up = key, mirror = 0;
+        if constexpr (SHAPED)
+            if (key < x.key1) key += (x.key1 - key - 1) / kStride * kStride, mirror = up + key;
+        Pages<SHAPED> pages{0, 0};
         // (There is an entry to read: a sequence with rows has a key at least, see sequence_of. A wave without keys asks for its last
         // page's: with a branch around this, heads of 192 and 256 took 6 % longer.)
         pages.fetch(a, x, key >> a.cache.page_log, lane);
@@ -786,12 +802,13 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
 #pragma unroll
                 for (int run = 0; run < kRuns; ++run) queries[(tile * kRuns + run) * 64 + lane] = uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
                 if (quarter == 0) {
-                    units[tile * 16 + col] = unit;
-                    masks[tile * 16 + col] = mask;
                     if constexpr (SHAPED) {
-                        biases[tile * 16 + col] = bias;
+                        shapes[tile * 16 + col] = float4_t{unit, bias.x, bias.y, 0.0f};
                         firsts[tile * 16 + col] = own_first;
+                    } else {
+                        units[tile * 16 + col] = unit;
                     }
+                    masks[tile * 16 + col] = mask;
                 }
             }
         }
@@ -804,7 +821,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             if constexpr (kInLds) return queries[(r * kRuns + run) * 64 + lane];
             else return uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
         };
-        auto get_unit = [&](int r) { return kInLds ? units[r * 16 + col] : unit; };
+        auto get_unit = [&](int r) {
+            if constexpr (SHAPED) return kInLds ? shapes[r * 16 + col] : float4_t{unit, bias.x, bias.y, 0.0f};
+            else return kInLds ? units[r * 16 + col] : unit;
+        };
         auto get_k_scales = [&](float4_t (&s)[2]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) s[h] = kInLds ? *reinterpret_cast<const float4_t*>(&scales[wave][h * 16 + quarter * 4]) : k_scales[h];
@@ -857,42 +877,46 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             if constexpr (!SHAPED) {
                 return nullptr;
             } else {
-                return [&, cap_in = shaped(a).cap_in, cap_out = shaped(a).cap_out, biased = shaped(a).slopes != nullptr, placed = shaped(a).positions != nullptr](int r, int h, float4_t& s) {
+                return [&, cap_in = shaped(a).cap_in, cap_out = shaped(a).cap_out, biased = shaped(a).slopes != nullptr, placed = shaped(a).positions != nullptr](int h, float2_t its, float4_t& s) {
                     if (cap_in != 0.0f)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[i] * cap_in)), -2.0f * cap_out, cap_out);
                     if (biased) {
-                        const uint32_t t = thread_here();
-                        const float2_t its = kInLds ? biases[r * 16 + (t & 15)] : bias;
-                        const int32_t first = int32_t(key + h * 16 + (t >> 4 & 3) * 4);
+                        const int32_t first = int32_t(key + h * 16 + (thread_here() >> 4 & 3) * 4);
                         const float at = float(first) - its.y;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(its.x, at + float(i), s[i]);
                         if (placed && key + 32 > x.seq.context) {
-                            // new tokens are where they are said to be
-                            Args& b = kernel_args();
-#pragma unroll 1
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t j = uint32_t(first + i), u = j - x.seq.context;
-                                float more = 0.0f;
-                                if (j >= x.seq.context && j < x.seq.total) more = its.x * float(shaped(b).positions[x.seq.first_token + u] - int32_t(j));
-                                s[0] += i == 0 ? more : 0.0f;
-                                s[1] += i == 1 ? more : 0.0f;
-                                s[2] += i == 2 ? more : 0.0f;
-                                s[3] += i == 3 ? more : 0.0f;
-                            }
+                            const float4_t more = *reinterpret_cast<const float4_t*>(&moves[wave][h * 16 + (thread_here() >> 4 & 3) * 4]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(its.x, more[i], s[i]);
                         }
                     }
                 };
             }
         }();
+        // how far from their places new tokens are said to be, of a step's keys
+        auto put_moves = [&] {
+            if constexpr (SHAPED) {
+                Shaped& b = shaped(kernel_args());
+                if (b.slopes && b.positions && key + 32 > x.seq.context) {
+                    const uint32_t l = thread_here() & 63, j = key + l;
+                    float more = 0.0f;
+                    if (l < 32 && j >= x.seq.context && j < x.seq.total) more = float(b.positions[x.seq.first_token + j - x.seq.context] - int32_t(j));
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+                    if (l < 32) moves[wave][l] = more;
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+                }
+            }
+        };
         // One step; `more` is known where this is compiled, as the compiler would otherwise count on values that were not asked for
         // behind keys that were, and wait for both.
         auto run_step = [&](auto more) {
-            const uint32_t next = key + WAVES * 32;
-            set_priority(x, key);
+            const uint32_t next = SHAPED ? mirror - up - kStride : key + kStride;
+            set_priority<SHAPED>(x, key);
             if constexpr (more()) locate(next);
             put_scales();
+            put_moves();
             // the keys' registers are free for the next once the scores are there, the others' at the end
             sums.step(key + 32 > x.all_see || (SHAPED && key < x.all_from), get_k, get_v, get_q, get_unit, get_k_scales, get_v_scales, shape, sees, hide, [&] {
                 if constexpr (more()) ask_scales();
@@ -902,10 +926,11 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             if constexpr (more()) load_scales_and_v();
             __builtin_amdgcn_sched_barrier(0);
             key = next;
+            if constexpr (SHAPED) up += kStride;
         };
 #pragma unroll 1
-        while (key + WAVES * 32 < x.key1) run_step(std::true_type{});
-        if (key < x.key1) run_step(std::false_type{});
+        while ((SHAPED ? up : key) + kStride < x.key1) run_step(std::true_type{});
+        if ((SHAPED ? up : key) < x.key1) run_step(std::false_type{});
         join_waves<WAVES>(x, sums, space, joined_m, joined_l);
     });
 }
