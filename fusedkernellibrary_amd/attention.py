@@ -117,7 +117,7 @@ def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: 
 
 
 class StepTables(_typing.NamedTuple):
-    """What step_tables returns; the names are those of the arguments that take them."""
+    """What step_tables returns, in one allocation; the names are those of the arguments that take them."""
     q_start: _torch.Tensor          # [batch + 1]
     slots: _torch.Tensor            # [tokens]
     positions: _torch.Tensor        # [tokens]
@@ -135,11 +135,11 @@ def step_tables(page_table, held, context, new, free, available, *, page_tokens:
     were missing; a token without a page has slot -1). The step has `tokens` rows: rows behind the last request's have slot
     -1, position 0 and an empty mask. With parents [tokens], new token t of a sequence follows its new token
     parents[row] < t (-1: none): its position is context + the number of its ancestors, and its mask has them and itself."""
-    return StepTables(*_native.step_tables(page_table, held, context, new, free, available, page_tokens, tokens, max_new, parents))
+    return StepTables._make(_native.step_tables(page_table, held, context, new, free, available, page_tokens, tokens, max_new, parents))
 
 
 class Verified(_typing.NamedTuple):
-    """What verify_drafts returns, int32."""
+    """What verify_drafts returns, int32, in one allocation."""
     path: _torch.Tensor             # [batch, max_new]: the accepted rows, counted from the sequence's first; then -1
     count: _torch.Tensor            # [batch]: how many they are
     out: _torch.Tensor              # [batch, max_new]: the tokens that were decided, as many; then -1
@@ -156,7 +156,7 @@ def verify_drafts(target, tokens, q_start, uniforms, *, max_new: int, draft=None
     uniforms[row] * (1 - what the refused children in front of it had). Where none is accepted the next token is drawn from
     max(target - draft, 0) of the refused row, from target without the refused tokens, or from target, by the uniform [0, 1) of
     the sequence's first row. Tokens come out distributed as if drawn from target one by one."""
-    return Verified(*_native.verify_drafts(target, tokens, q_start, uniforms, max_new, draft, parents))
+    return Verified._make(_native.verify_drafts(target, tokens, q_start, uniforms, max_new, draft, parents))
 
 
 def kv_keep(caches, page_table, context, path, count) -> None:

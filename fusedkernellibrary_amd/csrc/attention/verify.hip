@@ -80,6 +80,21 @@ __device__ __forceinline__ double of_lane(double v, uint32_t lane) {
     return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
 }
 
+// Sums of a wave's lanes up to and with each.
+template <int CTRL, int ROWS> __device__ __forceinline__ double add_moved(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xf, false)), hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xf, false));
+    return v + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double scan_lanes(double v) {
+    v = add_moved<0x111, 0xf>(v);                              // row_shr 1, 2, 4, 8: within sixteen lanes
+    v = add_moved<0x112, 0xf>(v);
+    v = add_moved<0x114, 0xf>(v);
+    v = add_moved<0x118, 0xf>(v);
+    v = add_moved<0x142, 0xa>(v);                              // row_bcast 15: the second and fourth sixteen get the one before
+    return add_moved<0x143, 0xc>(v);                           // row_bcast 31: the upper half gets the lower
+}
+
 // A wave's walk from a sequence's first row; path and refused are in LDS.
 template <int TYPE> __device__ __forceinline__ Outcome find_path(const VerifyArgs& a, const Place& p, uint32_t lane, int32_t* path, int32_t* refused) {
     Outcome o{0, -1, 0, 1};
@@ -164,10 +179,9 @@ template <int TYPE> struct Weights {
 
 // The sum of a workgroup's values, for every thread.
 __device__ __forceinline__ double sum_of_all(double v, double* waves) {
-#pragma unroll
-    for (int i = 32; i; i >>= 1) v += __shfl_xor(v, i);
+    v = scan_lanes(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = v;
     __syncthreads();
     return (waves[0] + waves[1]) + (waves[2] + waves[3]);
 }
@@ -220,22 +234,12 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_sums(co
     if (threadIdx.x == 0) a.sums[size_t(b) * a.chunks + chunk] = s;
 }
 
-// Sums of a wave's lanes up to and with each.
-__device__ __forceinline__ double scan_lanes(double v, uint32_t lane) {
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-        const double before = __shfl_up(v, i);
-        if (lane >= uint32_t(i)) v += before;
-    }
-    return v;
-}
-
 // Where a running sum exceeds `share` of them all: the chunk, the sum in front of it and the border; chunk < 0: all are 0.
 struct Chunk { int32_t chunk; double front, border; };
 __device__ __forceinline__ Chunk find_chunk(const double* sums, uint32_t chunks, float share, uint32_t lane) {
     // (every wave for itself: there is nothing to wait for)
-    double own = lane < chunks ? sums[lane] : 0.0, upto = scan_lanes(own, lane), all = of_lane(upto, 63);
-    for (uint32_t c0 = 64; c0 < chunks; c0 += 64) all += of_lane(scan_lanes(c0 + lane < chunks ? sums[c0 + lane] : 0.0, lane), 63);
+    double own = lane < chunks ? sums[lane] : 0.0, upto = scan_lanes(own), all = of_lane(upto, 63);
+    for (uint32_t c0 = 64; c0 < chunks; c0 += 64) all += of_lane(scan_lanes(c0 + lane < chunks ? sums[c0 + lane] : 0.0), 63);
     Chunk f{-1, 0.0, double(share) * all};
     if (!(all > 0.0)) return f;
     double before = 0.0;
@@ -252,13 +256,13 @@ __device__ __forceinline__ Chunk find_chunk(const double* sums, uint32_t chunks,
         c0 += 64;
         if (c0 >= chunks) return f;
         own = c0 + lane < chunks ? sums[c0 + lane] : 0.0;
-        upto = scan_lanes(own, lane);
+        upto = scan_lanes(own);
     }
 }
 
 template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_pick(const VerifyArgs a) {
     __shared__ double waves[4], runs[kRuns<TYPE>][4];
-    __shared__ uint32_t found[4], last[4];
+    __shared__ uint32_t found[8], last[8];
     const uint32_t b = blockIdx.x, thread = threadIdx.x, lane = thread & 63, wave = thread >> 6;
     const int32_t* record = a.record + size_t(b) * (kVerifyRecord + a.max_new);
     const Record o = *reinterpret_cast<const Record*>(record);
@@ -293,7 +297,7 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_pick(co
     double front[kRuns<TYPE>];
 #pragma unroll
     for (uint32_t k = 0; k < kRuns<TYPE>; ++k) {
-        const double run = w.sum(k), upto = scan_lanes(run, lane);
+        const double run = w.sum(k), upto = scan_lanes(run);
         if (lane == 63) runs[k][wave] = upto;
         front[k] = upto - run;
     }
@@ -321,19 +325,19 @@ template <int TYPE> __global__ __launch_bounds__(kThreads) void k_verify_pick(co
             }
         }
     }
-#pragma unroll
-    for (int i = 32; i; i >>= 1) {
-        first = min(first, uint32_t(__shfl_xor(int(first), i)));
-        some = max(some, uint32_t(__shfl_xor(int(some), i)));
-    }
-    if (lane == 0) {
-        found[wave] = first;
-        last[wave] = some;
+    first = reduce_lanes<32>(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    some = max_lanes<32>(some);
+    if ((lane & 31) == 0) {
+        found[wave * 2 + lane / 32] = first;
+        last[wave * 2 + lane / 32] = some;
     }
     __syncthreads();
     if (thread == 0) {
-        first = min(min(found[0], found[1]), min(found[2], found[3]));
-        some = max(max(last[0], last[1]), max(last[2], last[3]));
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            first = min(first, found[i]);
+            some = max(some, last[i]);
+        }
         a.out[size_t(b) * a.max_new + o.count - 1] = int32_t(first != 0xffffffffu ? first : some);
     }
 }
