@@ -132,6 +132,28 @@ __device__ __forceinline__ uint32_t first_of(Args& a, const Sequence& s, uint32_
     return max(s.front, first < 0 ? 0u : min(uint32_t(first), s.total));
 }
 
+// What up to 64 rows of a sequence see: none a key in front of `from` or behind any_sees, all those from all_from to all_see. (Shaped.)
+struct Sight { uint32_t from, all_from, all_see, any_sees; };
+__device__ __forceinline__ Sight sight_of(Args& a, const Sequence& s, uint32_t b, uint32_t row0, uint32_t rows) {
+    Shaped& h = shaped(a);
+    const bool causal = a.mask == nullptr;
+    Sight x{s.front, s.front, causal ? min(s.context + divide(row0, a.group_magic) + 1, s.total) : s.context, causal ? min(s.context + divide(row0 + rows - 1, a.group_magic) + 1, s.total) : s.total};
+    if (causal && h.prefix) {
+        const int32_t prefix = scalar(h.prefix + b);
+        const uint32_t upto = prefix < 0 ? 0u : min(uint32_t(prefix), s.total);
+        x.any_sees = max(x.any_sees, upto);
+        x.all_see = max(x.all_see, upto);
+    }
+    if (h.first) {
+        // (a row to a lane)
+        const uint32_t first = first_of(a, s, divide(row0 + min(thread_here() & 63, rows - 1), a.group_magic));
+        const uint32_t low = reduce_lanes<32>(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; }), high = max_lanes<32>(first);
+        x.from = min(__builtin_amdgcn_readlane(low, 0), __builtin_amdgcn_readlane(low, 32));
+        x.all_from = max(__builtin_amdgcn_readlane(high, 0), __builtin_amdgcn_readlane(high, 32));
+    }
+    return x;
+}
+
 // Keys key0 .. key1 of row block `block` and key head `head` of a sequence; where its parts go.
 struct Segment {
     Sequence seq;
@@ -146,32 +168,19 @@ template <bool SHAPED> __device__ __forceinline__ Segment segment_of(Args& a, co
     x.seq = s; x.b = b; x.head = head; x.part = part;
     x.row0 = block * a.unit_rows;
     x.rows = min(a.unit_rows, s.rows - x.row0);
-    const bool causal = a.mask == nullptr;
-    uint32_t any_sees = causal ? min(s.context + divide(x.row0 + x.rows - 1, a.group_magic) + 1, s.total) : s.total;
-    x.all_see = causal ? min(s.context + divide(x.row0, a.group_magic) + 1, s.total) : s.context;
     if constexpr (SHAPED) {
-        Shaped& h = shaped(a);
-        if (causal && h.prefix) {
-            const int32_t prefix = scalar(h.prefix + b);
-            const uint32_t upto = prefix < 0 ? 0u : min(uint32_t(prefix), s.total);
-            any_sees = max(any_sees, upto);
-            x.all_see = max(x.all_see, upto);
-        }
-        k0 += s.skip;
-        k1 += s.skip;
-    }
-    x.key0 = k0 << a.granule_log;
-    x.key1 = min(k1 << a.granule_log, any_sees);
-    if constexpr (SHAPED) {
-        if (shaped(a).first) {
-            // what the block's rows see first, the first and the last of them: a row to a lane
-            const uint32_t token = divide(x.row0 + min(thread_here() & 63, x.rows - 1), a.group_magic);
-            const uint32_t first = first_of(a, s, token);
-            const uint32_t low = reduce_lanes<32>(first, [](uint32_t a, uint32_t b) { return a < b ? a : b; }), high = max_lanes<32>(first);
-            const uint32_t least = min(__builtin_amdgcn_readlane(low, 0), __builtin_amdgcn_readlane(low, 32));
-            x.all_from = max(__builtin_amdgcn_readlane(high, 0), __builtin_amdgcn_readlane(high, 32));
-            x.key0 = min(max(x.key0, least & ~31u), max(x.key0, x.key1));
-        }
+        const Sight sight = sight_of(a, s, b, x.row0, x.rows);
+        x.all_see = sight.all_see;
+        x.all_from = sight.all_from;
+        x.key0 = (k0 + s.skip) << a.granule_log;
+        x.key1 = min((k1 + s.skip) << a.granule_log, sight.any_sees);
+        x.key0 = min(max(x.key0, sight.from & ~31u), max(x.key0, x.key1));
+    } else {
+        const bool causal = a.mask == nullptr;
+        const uint32_t any_sees = causal ? min(s.context + divide(x.row0 + x.rows - 1, a.group_magic) + 1, s.total) : s.total;
+        x.all_see = causal ? min(s.context + divide(x.row0, a.group_magic) + 1, s.total) : s.context;
+        x.key0 = k0 << a.granule_log;
+        x.key1 = min(k1 << a.granule_log, any_sees);
     }
     return x;
 }
@@ -192,6 +201,52 @@ template <int D, int THREADS> __device__ __forceinline__ void clear_rows(Args& a
     };
     for (uint32_t token = 0; token < front; ++token) clear(token);
     for (uint32_t token = behind; token < upto; ++token) clear(token);
+}
+
+// The block of a sequence's rows that is nth by how many keys it sees, most first; up to 256 blocks. Windows, documents and prefixes
+// have blocks of all weights in any order, and one with many keys that begins last ends alone.
+__device__ __forceinline__ uint32_t nth_heaviest(Args& a, const Sequence& s, uint32_t b, uint32_t blocks, uint32_t nth, uint32_t lane) {
+    Shaped& h = shaped(a);
+    uint32_t prefix = 0;
+    if (h.prefix && !a.mask) {
+        const int32_t upto = scalar(h.prefix + b);
+        prefix = upto < 0 ? 0u : min(uint32_t(upto), s.total);
+    }
+    uint32_t weight[4];                                        // of blocks lane, lane + 64 ..: in units of 128 keys, from 1 on
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t block = k * 64 + lane, row0 = block * a.unit_rows;
+        weight[k] = 0;
+        if (block < blocks) {
+            const uint32_t last = divide(min(row0 + a.unit_rows, s.rows) - 1, a.group_magic);
+            const uint32_t from = h.first ? first_of(a, s, divide(row0, a.group_magic)) : 0u, upto = a.mask ? s.total : max(min(s.context + last + 1, s.total), prefix);
+            weight[k] = 1 + (upto > from ? (upto - from) >> 7 : 0u);
+        }
+    }
+    // the largest weight that more than nth blocks have or exceed, and which of those that have it
+    const auto having = [&](uint32_t w) {
+        uint32_t n = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) n += __builtin_popcountll(__ballot(weight[k] >= w));
+        return n;
+    };
+    uint32_t its = 0;
+    for (uint32_t bit = 1u << (32 - __builtin_clz((s.total >> 7) + 1)); bit; bit >>= 1)
+        if (having(its | bit) > nth) its |= bit;
+    uint32_t left = nth - having(its + 1), found = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        uint64_t same = __ballot(weight[k] == its);
+        const uint32_t n = __builtin_popcountll(same);
+        if (left < n) {
+            for (; left; --left) same &= same - 1;
+            found = k * 64 + __builtin_ctzll(same);
+            left = 0xffffffffu;
+        } else if (left != 0xffffffffu) {
+            left -= n;
+        }
+    }
+    return found;
 }
 
 // Calls `run` for every segment of the workgroup. `kept` is the wave's place in LDS for what the walk goes on with: a segment
@@ -237,6 +292,9 @@ template <int D, int THREADS, bool SHAPED, typename F> __device__ __forceinline_
             part = g > a.lead ? 0 : g + count == n ? -1 : 1;
         } else if (block >= blocks) {
             return;
+        } else if constexpr (SHAPED) {
+            // (a sequence's rows may be fewer than the grid's: its own blocks are the last of the grid's rows)
+            if ((shaped(a).first || shaped(a).prefix) && blocks > 1 && blocks <= 256) block = nth_heaviest(a, s, b, blocks, blocks - 1 - block, lane);
         }
         kept[0] = at + count; kept[1] = in + count; kept[2] = end; kept[3] = b; kept[4] = whole;
         Segment x = segment_of<SHAPED>(a, s, b, head, block, max(g, a.lead) - a.lead, max(g + count, a.lead) - a.lead, part);

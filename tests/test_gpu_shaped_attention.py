@@ -304,3 +304,109 @@ def test_what_does_not_fit_is_refused(ops, device):
                        (dict(slopes=torch.ones(4, device=device, requires_grad=True)), "gradient")):
         with pytest.raises(ValueError, match=word):
             call(**more)
+
+
+CHUNKS = [
+    # context, new tokens, options
+    ([0, 5, 31, 32, 33, 64, 100, 260], [65, 128, 64, 90, 1, 0, 127, 129], dict(cap=30.0)),
+    ([0, 5, 31, 32, 33, 64, 100, 260], [65, 128, 64, 90, 1, 0, 127, 129], dict(slopes=True, window=40)),
+    ([300, 0, 77, 16, 15, 0, 1, 500], [64, 200, 3, 64, 66, 17, 140, 100], dict(prefix=[310, 0, 2 ** 31 - 1, 60, 17, -1, 90, 555], window=123, cap=9.0)),
+    ([40, 41, 42, 43, 44, 45, 46, 47], [70, 71, 64, 5, 64, 66, 80, 0], dict(mask=True, positions=True, slopes=True, cap=20.0)),
+    ([200, 0, 0, 3, 90, 0, 7, 0], [64, 64, 90, 100, 101, 102, 1, 64], dict(first="any", slopes=True)),
+]
+
+
+@pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, F16), (INT8, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 64), (128, 32), (192, 16), (256, 256)])
+@pytest.mark.parametrize("case", range(len(CHUNKS)))
+def test_chunks_of_prompts(ops, device, kind, dtype, dim, page, case):
+    """Rows enough for workgroups whose waves share the keys: lengths around every edge of a tile, a step and a block of rows."""
+    import fusedkernellibrary_amd as fkl
+    context, new, options = CHUNKS[case]
+    g, options = gen(case), dict(options)
+    hq, hkv = (32, 16) if dim != 96 else (60, 20)
+    more = {n: options[n] for n in ("cap",) if n in options}
+    if "slopes" in options:
+        more["slopes"] = slopes_of(hq)
+    if "window" in options:
+        more["first"] = firsts(context, new, options["window"])
+    if "prefix" in options:
+        more["prefix"] = ints(options["prefix"])
+    if "mask" in options:
+        more["mask"] = tree_mask(new, 2, g)
+    if "positions" in options:
+        more["positions"] = ints([c + t // 3 for c, n in zip(context, new) for t in range(n)])
+    if "first" in options:
+        rng = random.Random(case)
+        more["first"] = ints([rng.choice([0, c, c + t, c + t + 1, c - 40, c + n, 2 ** 31 - 1, -1, 32, 33]) if t else min(c, 20) for c, n in zip(context, new) for t in range(n)])
+    run(ops, device, context=context, new=new, hq=hq, hkv=hkv, dim=dim, page=page, kind=kind, dtype=dtype, seed=case, **more)
+    last = fkl.last_launch()
+    assert last["form"] == "chunk_attention" and last["grid"] == [hkv, -(-max(new) * (hq // hkv) // 128), len(new)]
+
+
+@pytest.mark.parametrize("kind", [INT8, E4M3])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_chunks_with_queries_that_are_not_finite(ops, device, kind, bad):
+    import fusedkernellibrary_amd as fkl
+    g = gen(5)
+    q = torch.randn((300, 32, 64), generator=g).to(BF16)
+    q[7, :, 3], q[200, 5, 9], q[150, 1, 1] = bad, bad, bad
+    first = torch.zeros(300, dtype=torch.int32)
+    first[150] = 10 ** 9
+    table, pages = paged([400], 16, g)
+    slots = ref.Slots(pages * 16, 16, 64, kind, g)
+    out = ops.tree_attention(q.to(device), ops.KvCache(*slots.tensors(16, device)), table.to(device).expand(4, -1).contiguous(), ints([100, 100, 0, 0]).to(device), ints([0, 300, 300, 300, 300]).to(device),
+                             max_new=300, max_context=100, first=first.to(device)).cpu()
+    assert fkl.last_launch()["form"] == "chunk_attention"
+    want = torch.zeros((300, 32), dtype=torch.bool)
+    want[7], want[200, 5] = True, True
+    assert torch.equal(out.isnan().all(-1), want) and torch.equal(out.isnan().any(-1), want) and (out[150] == 0).all()
+
+
+def test_chunks_whose_scores_rise_and_scales_of_all_sizes(ops, device):
+    """The reference has to move, up and down the keys, over many orders of magnitude of values."""
+    for kind in (INT8, E4M3):
+        g = gen(9)
+        n, page = 700, 32
+        table, pages = paged([n], page, g)
+        slots = ref.Slots(pages * page, 16, 64, kind, g)
+        j = torch.arange(n)
+        at = table[0].long()[j // page] * page + j % page
+        slots.ks[at] *= (0.2 + (n - j) / 100.0).unsqueeze(1)
+        slots.vs[at] *= (10.0 ** ((j * 7 % 13) - 9.0)).unsqueeze(1)
+        slots.vs[at[::11]] = 0.0
+        q = (1.5 * torch.randn((600, 32, 64), generator=g)).to(BF16)
+        start, context = ints([0, 600]), ints([100])
+        out = ops.tree_attention(q.to(device), ops.KvCache(*slots.tensors(page, device)), table.to(device), context.to(device), start.to(device), max_new=600, max_context=100, cap=40.0)
+        want, bound, _, _ = shaped.attention(q, slots, page, table, context, start, 0.125, BF16, cap=40.0)
+        ref.check(out, want, bound, "out")
+
+
+def test_chunks_of_pages_that_are_no_pages_and_a_captured_call(ops, device):
+    g = gen(6)
+    table, pages = paged([900], 16, g)
+    cache = ops.KvCache(*ref.Slots(pages * 16, 16, 128, E4M3, g).tensors(16, device))
+    q = torch.randn((300, 32, 128), generator=g).to(BF16).to(device)
+    first = firsts([600], [300], 100).to(device)
+    call = lambda t: ops.tree_attention(q, cache, t, ints([600]).to(device), ints([0, 300]).to(device), max_new=300, max_context=600, first=first)      # noqa: E731
+    want = call(table.to(device))
+    for value in (-1, 2 ** 31 - 1):
+        stale = table.clone()
+        stale[0, :501 // 16] = value
+        assert torch.equal(call(stale.to(device)), want)
+    on, context, start = table.to(device), ints([600]).to(device), ints([0, 300]).to(device)
+    prefix = ints([0]).to(device)
+    again = lambda: ops.tree_attention(q, cache, on, context, start, max_new=300, max_context=600, first=first, prefix=prefix, cap=25.0)      # noqa: E731
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        again()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = again()
+    for i in range(3):
+        prefix.fill_(300 * i)
+        first.copy_(firsts([600], [300], 50 + 300 * i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, again())
