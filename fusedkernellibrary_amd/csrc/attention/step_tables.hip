@@ -106,7 +106,7 @@ template <bool TREES> __global__ __launch_bounds__(kWaves * 64) void k_step_tabl
             const bool live = t < count;
             const int32_t p = live ? a.parents[start + t] : -1;
             // the token's nearest ancestors within these 64, the next one behind them, and how many they are
-            uint64_t seen = uint64_t(1) << lane;
+            uint64_t seen = uint64_t(lane & 32 ? 1u << (lane & 31) : 0u) << 32 | (lane & 32 ? 0u : 1u << lane);
             int32_t next = p >= 0 && uint32_t(p) < t ? p : -1;
             uint32_t depth = next >= 0 ? 1 : 0;
 #pragma unroll 1

@@ -113,16 +113,25 @@ __device__ __forceinline__ float sum_quarters(float v) { return join_quarters(v,
 __device__ __forceinline__ uint32_t lowest_bits(int32_t n) { return n >= 4 ? 15u : n <= 0 ? 0u : (1u << n) - 1u; }
 // Bits u .. u + 3 of a row of a mask, where those below 0 (the context's) are set and those behind the row are not; `first` is
 // the row's first word.
-__device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint64_t first, uint32_t words, int32_t u) {
+template <bool HALVES> __device__ __forceinline__ uint32_t mask_bits(const uint64_t* row, uint64_t first, uint32_t words, int32_t u) {
     const uint32_t below = u >= 0 ? 0u : u <= -4 ? 4u : uint32_t(-u), from = u >= 0 ? uint32_t(u) : 0u;
-    const uint32_t shift = from & 63u;
     uint64_t lo = from < 64u ? first : 0, hi = 0;
     if (words > 1) {                                          // (the same for the whole wave)
         const uint32_t lo_at = from >> 6, hi_at = (from + 3) >> 6;
         lo = lo_at < words ? row[lo_at] : 0;
         hi = hi_at < words && hi_at != lo_at ? row[hi_at] : 0;
     }
-    const uint32_t bits = uint32_t(lo >> shift) | (shift ? uint32_t(hi << (64u - shift)) : 0u);
+    uint32_t bits;
+    if constexpr (HALVES) {
+        // By halves: a vector shift of 64 bits whose amount was in the last register that a wave has (v255 of 256) shifted by something
+        // else now and then. (Where shifts of 64 bits are taken, none is of that kind: tests/test_step_kernels_build.py; by halves, heads
+        // of 256 elements take more registers than there are.)
+        const uint32_t at = from & 32u ? uint32_t(lo >> 32) : uint32_t(lo), next = from & 32u ? uint32_t(hi) : uint32_t(lo >> 32);
+        bits = __builtin_amdgcn_alignbit(next, at, from & 31u);
+    } else {
+        const uint32_t shift = from & 63u;
+        bits = uint32_t(lo >> shift) | (shift ? uint32_t(hi << (64u - shift)) : 0u);
+    }
     return (lowest_bits(int32_t(below)) | bits << below) & 15u;
 }
 
@@ -910,7 +919,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             }
             if (b.mask == nullptr) return lowest_bits(int32_t(token) + 1 - u) & there;
             const uint64_t word = kInLds ? masks[r * 16 + col] : mask;
-            return mask_bits(b.mask + int64_t(x.seq.first_token + token) * b.mask_words, word, b.mask_words, u) & there & from_first;
+            return mask_bits<SHAPED && D < 256>(b.mask + int64_t(x.seq.first_token + token) * b.mask_words, word, b.mask_words, u) & there & from_first;
         };
         // what lies behind the last token, or in front of the first that anybody sees, is no token's (its page may have gone to another):
         // no code of it may reach a product, as 0 * NaN is NaN
