@@ -7,11 +7,13 @@
 //   fk::qkvToCache(heads, cache, stream);            // norm, rotation, quantising write: one launch
 //   fk::TreeAttention attend;                        // keeps its workspace
 //   attend(call, cache, stream);
+// and what is around it: fk::stepTables before, fk::VerifyDrafts and fk::kvKeep behind.
 #ifndef FK_AMD_ATTENTION_H
 #define FK_AMD_ATTENTION_H
 
 #include <fused_kernel/core/execution_model/stream.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -54,6 +56,24 @@ public:
     ~DeviceMemory() { if (m_data) fklhip_free(m_data); }
     void* data() const { return m_data; }
     size_t bytes() const { return m_bytes; }
+};
+
+// A workspace that grows. Those it has grown out of live as long as it does, for graphs that name them.
+class Workspace {
+    std::vector<DeviceMemory> m_memory;                        // the last is the one in use
+public:
+    size_t bytes() const { return m_memory.empty() ? 0 : m_memory.back().bytes(); }
+    void* data() const { return m_memory.empty() ? nullptr : m_memory.back().data(); }
+    void reserve(const uint64_t need) {
+        if (need > bytes()) m_memory.emplace_back(size_t(need));
+    }
+    void reserve(const uint64_t need, Stream_<ParArch::GPU_AMD>& stream, const char* of) {
+        if (need <= bytes()) return;
+        int capturing = 0;
+        gpuErrchk(fklhip_stream_is_capturing(stream.getNativeStream(), &capturing));
+        if (capturing) throw std::logic_error(std::string(of) + ": a call that is captured needs its workspace beforehand (reserve)");
+        reserve(need);
+    }
 };
 
 } // namespace attention_detail
@@ -99,6 +119,22 @@ inline void qkvToCache(const fklhip_heads& heads, const fklhip_kv_cache& cache, 
     FK_ATTENTION_CHECK(fklhip_qkv_to_cache(&heads, &cache, stream.getNativeStream()));
 }
 
+// The same with the positions of several axes, pair i turning by those of axis ofPair[i] (fklhip_axes).
+inline fklhip_axes ropeAxes(const std::vector<uint8_t>& ofPair, const int32_t count, const int64_t stride) {
+    fklhip_axes axes{stride, count, {}};
+    if (ofPair.size() > sizeof axes.of_pair) throw std::invalid_argument("a head has up to 128 pairs");
+    std::copy(ofPair.begin(), ofPair.end(), axes.of_pair);
+    return axes;
+}
+
+inline void qkNormRope(const fklhip_heads& heads, const fklhip_axes& axes, Stream_<ParArch::GPU_AMD>& stream) {
+    FK_ATTENTION_CHECK(fklhip_qk_norm_rope_axes(&heads, &axes, stream.getNativeStream()));
+}
+
+inline void qkvToCache(const fklhip_heads& heads, const fklhip_axes& axes, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
+    FK_ATTENTION_CHECK(fklhip_qkv_to_cache_axes(&heads, &axes, &cache, stream.getNativeStream()));
+}
+
 inline void kvWrite(const fklhip_kv_cache& cache, const fklhip_rows& k, const fklhip_rows& v, const int32_t* slots, const int64_t tokens, const RowType type,
                     Stream_<ParArch::GPU_AMD>& stream) {
     FK_ATTENTION_CHECK(fklhip_kv_write(&cache, &k, &v, slots, tokens, static_cast<int>(type), stream.getNativeStream()));
@@ -117,33 +153,60 @@ inline void kvRead(const fklhip_kv_cache& cache, const int32_t* slots, const int
 // larger than the one before). Nothing can be allocated while a graph is captured: a call that would have to is refused with
 // std::logic_error, and reserve() is what comes before it.
 class TreeAttention {
-    std::vector<attention_detail::DeviceMemory> m_workspaces;  // the last is the one in use
+    attention_detail::Workspace m_workspace;
 
-    size_t bytes() const { return m_workspaces.empty() ? 0 : m_workspaces.back().bytes(); }
     static uint64_t needed(const fklhip_attention& call, const fklhip_kv_cache& cache) {
         uint64_t bytes = 0;
         FK_ATTENTION_CHECK(fklhip_tree_attention_workspace(&call, &cache, &bytes));
         return bytes;
     }
+    void prepare(fklhip_attention& call, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
+        m_workspace.reserve(needed(call, cache), stream, "TreeAttention");
+        call.workspace = m_workspace.data();
+        call.workspace_bytes = m_workspace.bytes();
+    }
 public:
     // Makes the workspace large enough for calls of these sizes (its pointers are not looked at).
-    void reserve(const fklhip_attention& call, const fklhip_kv_cache& cache) {
-        const uint64_t need = needed(call, cache);
-        if (need > bytes()) m_workspaces.emplace_back(size_t(need));
-    }
+    void reserve(const fklhip_attention& call, const fklhip_kv_cache& cache) { m_workspace.reserve(needed(call, cache)); }
     void operator()(fklhip_attention call, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
-        const uint64_t need = needed(call, cache);
-        if (need > bytes()) {
-            int capturing = 0;
-            gpuErrchk(fklhip_stream_is_capturing(stream.getNativeStream(), &capturing));
-            if (capturing) throw std::logic_error("TreeAttention: a call that is captured needs its workspace beforehand (reserve)");
-            m_workspaces.emplace_back(size_t(need));
-        }
-        call.workspace = m_workspaces.empty() ? nullptr : m_workspaces.back().data();
-        call.workspace_bytes = bytes();
+        prepare(call, cache, stream);
         FK_ATTENTION_CHECK(fklhip_tree_attention(&call, &cache, stream.getNativeStream()));
     }
+    // With scores of another shape, or rows that see other keys (fklhip_scores).
+    void operator()(fklhip_attention call, const fklhip_scores& scores, const fklhip_kv_cache& cache, Stream_<ParArch::GPU_AMD>& stream) {
+        prepare(call, cache, stream);
+        FK_ATTENTION_CHECK(fklhip_shaped_attention(&call, &scores, &cache, stream.getNativeStream()));
+    }
 };
+
+// The tables of a step from its requests' lengths.
+inline void stepTables(const fklhip_tables& tables, Stream_<ParArch::GPU_AMD>& stream) { FK_ATTENTION_CHECK(fklhip_step_tables(&tables, stream.getNativeStream())); }
+
+// Drafted tokens against the target's probabilities, with a workspace for which all that TreeAttention says holds.
+class VerifyDrafts {
+    attention_detail::Workspace m_workspace;
+
+    static uint64_t needed(const fklhip_drafts& drafts) {
+        uint64_t bytes = 0;
+        FK_ATTENTION_CHECK(fklhip_verify_drafts_workspace(&drafts, &bytes));
+        return bytes;
+    }
+public:
+    void reserve(const fklhip_drafts& drafts) { m_workspace.reserve(needed(drafts)); }
+    void operator()(fklhip_drafts drafts, Stream_<ParArch::GPU_AMD>& stream) {
+        m_workspace.reserve(needed(drafts), stream, "VerifyDrafts");
+        drafts.workspace = m_workspace.data();
+        drafts.workspace_bytes = m_workspace.bytes();
+        FK_ATTENTION_CHECK(fklhip_verify_drafts(&drafts, stream.getNativeStream()));
+    }
+};
+
+// The cache rows of accepted tokens, moved to where their sequences go on, in all layers' caches. pageTable is [batch][entries],
+// path [batch][maxNew].
+inline void kvKeep(const std::vector<fklhip_kv_cache>& caches, const int32_t* pageTable, const int64_t entries, const int32_t* context, const int32_t* path, const int32_t* count, const int32_t batch,
+                   const int32_t maxNew, Stream_<ParArch::GPU_AMD>& stream) {
+    FK_ATTENTION_CHECK(fklhip_kv_keep(caches.data(), static_cast<int32_t>(caches.size()), pageTable, entries, context, path, count, batch, maxNew, stream.getNativeStream()));
+}
 
 #undef FK_ATTENTION_CHECK
 
