@@ -5,6 +5,8 @@
 // its lanes take a token each, 64 at a time. A token of a tree sees its ancestors: within 64 tokens by paths of 1, 2, 4 .. steps,
 // which the lanes hand each other, and beyond them what the first ancestor in front of the 64 sees, whose row is complete by then.
 // The batch's last wave takes what is behind the last request's rows. Bound by latency: a launch and three dependent trips to memory.
+#include <algorithm>
+
 #include "attention_device.hpp"
 #include "step_common.hpp"
 
@@ -95,10 +97,12 @@ template <bool TREES> __global__ __launch_bounds__(kWaves * 64) void k_step_tabl
     }
     const uint32_t count = min(r.fresh, a.tokens - start);
     if constexpr (!TREES) {
-        const uint32_t end = min(count, (blockIdx.y + 1) * kTileTokens);
-        for (uint32_t t = blockIdx.y * kTileTokens + lane; t < end; t += 64) {
-            a.slots[start + t] = slot_of(a, r, b, pages, free_now, r.context + t);
-            a.positions[start + t] = int32_t(r.context + t);
+        for (uint32_t t0 = blockIdx.y * kTileTokens; t0 < count; t0 += gridDim.y * kTileTokens) {
+            const uint32_t end = min(count, t0 + kTileTokens);
+            for (uint32_t t = t0 + lane; t < end; t += 64) {
+                a.slots[start + t] = slot_of(a, r, b, pages, free_now, r.context + t);
+                a.positions[start + t] = int32_t(r.context + t);
+            }
         }
     } else {
         for (uint32_t t0 = 0; t0 < count; t0 += 64) {
@@ -142,7 +146,8 @@ template <bool TREES> __global__ __launch_bounds__(kWaves * 64) void k_step_tabl
 
 int launch_step_tables(const TablesArgs& a, void* stream, Launched& info) {
     const bool trees = a.parents != nullptr;
-    const uint32_t tiles = trees || a.max_new == 0 ? 1 : (a.max_new + kTileTokens - 1) / kTileTokens;
+    const uint32_t most = std::min(std::min(a.max_new, a.tokens), 65535 * kTileTokens),
+                   tiles = trees || most == 0 ? 1 : (most + kTileTokens - 1) / kTileTokens;
     const dim3 grid(a.batch / kWaves + 1, tiles, 1), block(kWaves * 64);
     info = {"step_tables", {grid.x, grid.y, 1}, {block.x, 1, 1}, 0};
     return trees ? launch(k_step_tables<true>, grid, block, stream, a) : launch(k_step_tables<false>, grid, block, stream, a);

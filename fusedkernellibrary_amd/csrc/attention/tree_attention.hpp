@@ -760,7 +760,9 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
     __shared__ float units[R * 16];
     __shared__ uint64_t masks[R * 16];                             // the first word of each: all there is for trees of up to 64
     __shared__ __attribute__((aligned(16))) float scales[WAVES][64];
-    // of shaped rows: unit, slope in units of log2 and position; the first key they see
+    // Of shaped rows: unit, slope in units of log2, and where they are, from the end of the context and, for steps with new tokens, from the
+    // first one's position (floats have whole numbers up to 2^24: distances are exact up to that, places need not be); the first key they
+    // see. And what keys of a step with new tokens are away from where they would be by their places.
     __shared__ float4_t shapes[SHAPED ? R * 16 : 1];
     __shared__ uint32_t firsts[SHAPED ? R * 16 : 1];
     __shared__ __attribute__((aligned(16))) float moves[SHAPED ? WAVES : 1][32];
@@ -789,15 +791,20 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             load_query<D>(a, x, tile * 16 + col, quarter, raw);
             if (a.mask) mask = a.mask[int64_t(x.seq.first_token + place_of_row(a, x, tile * 16 + col).token) * a.mask_words];
         }
-        float2_t bias = {0.0f, 0.0f};
+        float slope = 0.0f, from_context = 0.0f, from_new = 0.0f;
         uint32_t own_first = 0;
         if constexpr (SHAPED) {
             if (tile < R) {
                 const RowPlace place = place_of_row(a, x, tile * 16 + col);
                 if (shaped(a).slopes) {
-                    const uint32_t row = x.seq.first_token + place.token;
-                    bias.x = shaped(a).slopes[place.head] * kLog2e;
-                    bias.y = float(shaped(a).positions ? shaped(a).positions[row] : int32_t(x.seq.context + place.token));
+                    slope = shaped(a).slopes[place.head] * kLog2e;
+                    uint32_t own = x.seq.context + place.token, first = x.seq.context;
+                    if (Shaped& b = shaped(kernel_args()); b.positions) {
+                        own = uint32_t(b.positions[x.seq.first_token + place.token]);
+                        first = uint32_t(b.positions[x.seq.first_token]);
+                    }
+                    from_context = float(int32_t(own - x.seq.context));
+                    from_new = float(int32_t(own - first));
                 }
                 if (shaped(a).first) own_first = first_of(a, x.seq, place.token);
             }
@@ -870,7 +877,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 for (int run = 0; run < kRuns; ++run) queries[(tile * kRuns + run) * 64 + lane] = uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
                 if (quarter == 0) {
                     if constexpr (SHAPED) {
-                        shapes[tile * 16 + col] = float4_t{unit, bias.x, bias.y, 0.0f};
+                        shapes[tile * 16 + col] = float4_t{unit, slope, from_context, from_new};
                         firsts[tile * 16 + col] = own_first;
                     } else {
                         units[tile * 16 + col] = unit;
@@ -889,8 +896,12 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
             else return uint4_t{q[run * 4], q[run * 4 + 1], q[run * 4 + 2], q[run * 4 + 3]};
         };
         auto get_unit = [&](int r) {
-            if constexpr (SHAPED) return kInLds ? shapes[r * 16 + col] : float4_t{unit, bias.x, bias.y, 0.0f};
-            else return kInLds ? units[r * 16 + col] : unit;
+            if constexpr (SHAPED) {
+                const float4_t its = kInLds ? shapes[r * 16 + col] : float4_t{unit, slope, from_context, from_new};
+                return float4_t{its[0], its[1], key + 32 > x.seq.context ? its[3] : its[2], 0.0f};
+            } else {
+                return kInLds ? units[r * 16 + col] : unit;
+            }
         };
         auto get_k_scales = [&](float4_t (&s)[2]) {
 #pragma unroll
@@ -913,7 +924,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 from_first = ~lowest_bits(int32_t(its_first - first));
                 if (b.mask == nullptr) {
                     int32_t upto = int32_t(token) + 1;
-                    if (shaped(b).prefix) upto = max(upto, min(scalar(shaped(b).prefix + x.b), 1 << 30) - int32_t(x.seq.context));
+                    if (shaped(b).prefix) upto = max(upto, max(0, min(scalar(shaped(b).prefix + x.b), 1 << 30)) - int32_t(x.seq.context));
                     return lowest_bits(upto - u) & there & from_first;
                 }
             }
@@ -948,12 +959,11 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                     if (cap_in != 0.0f)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + exp2_fast(s[i] * cap_in)), -2.0f * cap_out, cap_out);
-                    if (biased) {
-                        const int32_t first = int32_t(key + h * 16 + (thread_here() >> 4 & 3) * 4);
-                        const float at = float(first) - its.y;
+                    if (D < 256 ? biased : shaped(kernel_args()).slopes != nullptr) {      // (256: no register is left for it, nor for the next)
+                        const float at = float(int32_t(key + h * 16 + (thread_here() >> 4 & 3) * 4 - x.seq.context)) - its.y;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(its.x, at + float(i), s[i]);
-                        if (placed && key + 32 > x.seq.context) {
+                        if (key + 32 > x.seq.context && (D < 256 ? placed : shaped(kernel_args()).positions != nullptr)) {
                             const float4_t more = *reinterpret_cast<const float4_t*>(&moves[wave][h * 16 + (thread_here() >> 4 & 3) * 4]);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(its.x, more[i], s[i]);
@@ -962,16 +972,16 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
                 };
             }
         }();
-        // how far from their places new tokens are said to be, of a step's keys
         auto put_moves = [&] {
             if constexpr (SHAPED) {
                 Shaped& b = shaped(kernel_args());
                 if (b.slopes && b.positions && key + 32 > x.seq.context) {
                     const uint32_t l = thread_here() & 63, j = key + l;
-                    float more = 0.0f;
-                    if (l < 32 && j >= x.seq.context && j < x.seq.total) more = float(b.positions[x.seq.first_token + j - x.seq.context] - int32_t(j));
+                    const uint32_t ahead = uint32_t(scalar(b.positions + x.seq.first_token)) - x.seq.context;
+                    uint32_t more = 0u - ahead;
+                    if (l < 32 && j >= x.seq.context && j < x.seq.total) more += uint32_t(b.positions[x.seq.first_token + j - x.seq.context]) - j;
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-                    if (l < 32) moves[wave][l] = more;
+                    if (l < 32) moves[wave][l] = float(int32_t(more));
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
                 }
             }

@@ -121,8 +121,9 @@ int fklhip_strip_form(int enable);
  * kernel receives "rows", "gather" or "strip", each with "_jit" behind it for chains compiled at run time, or "rows_unaligned": the
  * kernel for rows that do not all start on dword boundaries, of the chains compiled ahead of time that have one of its own for
  * them (padding, deinterlacing, planar and circular reads; the others have one kernel for rows at every alignment).
- * The operators around a key-value cache are "heads" (norms, rotations and writes), "kv_read" and "tree_attention_TxW", with T tiles
- * of 16 rows and W waves to a workgroup; their lds_bytes are 0, as they ask for none at run time.
+ * The operators around a key-value cache are "heads" (norms, rotations and writes), "kv_read", "tree_attention_TxW", with T tiles
+ * of 16 rows and W waves to a workgroup, "shaped_attention_TxW" (with fklhip_scores), "step_tables", "verify_drafts" (its first launch)
+ * and "kv_keep"; their lds_bytes are 0 but for "verify_drafts", as they ask for none at run time.
  * grid/block receive 3 values each. */
 int fklhip_last_launch(const char **kernel, unsigned grid[3], unsigned block[3], unsigned *lds_bytes);
 /* The same launch's kernel by its own name, which fklhip_last_launch gives by the form it took the place of: "rows", "flat" (planes whose rows
@@ -236,7 +237,7 @@ int fklhip_tree_attention(const fklhip_attention *call, const fklhip_kv_cache *c
 /* The same with scores of another shape, s = cap tanh(scale q.k / cap) - slope distance, and rows that see other keys.
  *   cap      0: no tanh; else 2^-6 to 2^9
  *   slopes   one for each query head, or NULL. The distance is the row's position less the key's: places in the sequence, or, of
- *            new tokens, positions[row] (a tree's tokens: context + depth) where they are given.
+ *            new tokens, positions[row] (a tree's tokens: context + depth; 0 to 2^30) where they are given. Slopes are finite.
  *   first    of each row: it sees no key in front of place first[row] (a window, the beginning of its document). No row of
  *            a sequence sees a key in front of its first row's; what is in front of that is not read.
  *   prefix   of each sequence, without a mask: all of its rows see all keys in front of place prefix[b].
@@ -288,7 +289,8 @@ int fklhip_step_tables(const fklhip_tables *tables, void *stream);
  * the tokens that were decided: the accepted rows' and then the drawn one, count[b] in all. Behind them, and all of a sequence
  * without rows (count 0): -1. Comparisons and sums are in 64 bits. Probabilities that are no finite number above 0 count as 0,
  * uniforms as what is nearest in 0 .. 1 - 2^-24 (NaN: 0); a token outside of the vocabulary has probability 0. Sequences longer than
- * max_new (up to 1024) and rows above `tokens` are cut off. With batch or max_new 0 nothing is launched. */
+ * max_new (up to 1024) and rows above `tokens` are cut off. path, count, out and the workspace overlap nothing else. With batch or
+ * max_new 0 nothing is launched. */
 typedef struct fklhip_drafts {
     const void *target, *draft;        /* [tokens][vocab] of the type; draft may be NULL, and has to be with parents */
     const int32_t *ids, *q_start, *parents;                /* [tokens], [batch + 1], [tokens] or NULL */
