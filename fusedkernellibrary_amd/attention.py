@@ -5,6 +5,12 @@ each step's new or drafted tokens.
     q = qkv_to_cache(cache, q, k, v, slots, q_weight, k_weight, cos, sin, positions)       # norm, rotate, quantise, store
     o = tree_attention(q, cache, page_table, context, q_start, max_new=..., max_context=..., mask=...)
 
+and around the layers of a step of drafted tokens
+
+    t = step_tables(page_table, held, context, new, free, available, page_tokens=..., tokens=..., max_new=..., parents=...)
+    v = verify_drafts(target, tokens, t.q_start, uniforms, max_new=..., parents=...)
+    kv_keep(caches, page_table, context, v.path, v.count)
+
 Thin bindings of the C ABI (include/fklhip.h has the definitions of the operators and the cache's layout): tensors are passed
 on by address, the work runs on torch's current stream, and what does not fit raises ValueError before anything is launched.
 Outputs are allocated by torch unless they are given. The operators serve and do not train: under grad mode an argument that

@@ -399,8 +399,9 @@ constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
 // With several axes many tokens' heads are swept (sweep_heads), by about so many waves: the fewer, the fewer read the tables' rows; fewer
-// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB): 35.3 us with 8192 waves (10 heads each), 38.1 with 4096, 49.6 with
-// 2048, 39.4 with 14336, and 44.0 without sweeps, four heads to a group. 2048 tokens of 32 and 8: 14.5 with 2048, 13.9 with 5120.
+// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB), a pass: 36.8 us with 6144 waves (14 heads each), 37.2 with
+// 8192, 39.2 with 10240, 40.9 with 14336, 40.5 with 4096, 51.2 with 2048; 44.0 without sweeps, four heads to a group. 5000 tokens of 28 and 4:
+// 19.1, and 20.8, 21.1, 21.1, 19.8, 21.3; 3000 of 64 and 8: 25.4, and 24.3, 25.4, 25.6, 27.8, 29.8; 2048 of 32 and 8: 13.5 to 14.2 all.
 constexpr uint32_t kSweepWaves = 6144;
 template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE, bool AXES>
 int start_heads(HeadArgsOf<AXES> a, uint32_t threads, void* stream, Launched& info) {

@@ -11,7 +11,11 @@
 //
 // Two launches. The first cuts a row into chunks, one to a workgroup; each finds the path for itself (a wave, by a few gathers that
 // the lanes make together: less than a launch of its own) and adds its chunk up. The second, a workgroup to a sequence, finds
-// the chunk and then the token in it. Bound by memory where the batch is large, else by the trips to memory one behind the other.
+// the chunk and then the token in it. Bound by memory where the batch is large, else by the trips to memory one behind the other:
+// 4.6 + 4.8 us for one chain of 5 over 32000 tokens (float32), 5.6 + 4.7 for 24 trees over 100003 (bfloat16), 15.1 + 6.3 for 64 chains of
+// up to 8 over 131072 (67 MB at the most, 4.4 TB/s with the path in front). The second's scans are in registers, by moves between lanes:
+// with a wave's weights added in LDS it took 33 to 72 us. One launch, a workgroup of 1024 to a sequence, was slower but for many short
+// rows: 23.0 us for one sequence over 131072 (8.7 in two launches), 11.7 over 32000 (9.1), 18.5 for 256 over 32000 (21.3).
 #include <type_traits>
 
 #include "attention_device.hpp"
