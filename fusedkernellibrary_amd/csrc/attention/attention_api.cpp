@@ -71,7 +71,7 @@ int run_heads(const fklhip_heads* h, const fklhip_axes* axes, const fklhip_kv_ca
     return finish(launch_heads(a, h->type, cache != nullptr, stream, info), info);
 }
 
-int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, AttentionPlan& plan) {
+int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, bool shaped, bool fronts, AttentionPlan& plan) {
     NEED(c, "no call");
     CHECK(check_type(c->type));
     CHECK(check_cache(cache));
@@ -87,7 +87,8 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, Attention
     NEED(c->tokens * c->q_heads < (int64_t(1) << 31), "more than 2^31 - 1 query rows");
     NEED(c->page_table_stride >= 0 && c->page_table_stride <= std::numeric_limits<int32_t>::max(), "page_table_stride has to be 0 to 2^31 - 1");
     const uint32_t keys = uint32_t(std::min<int64_t>(int64_t(c->max_context) + c->max_new, c->page_table_stride * cache->page_tokens));
-    plan = plan_attention(uint32_t(c->batch), uint32_t(cache->kv_heads), uint32_t(c->max_new * group), keys, uint32_t(cache->head_dim));
+    plan = plan_attention(uint32_t(c->batch), uint32_t(cache->kv_heads), uint32_t(c->max_new * group), keys, uint32_t(cache->head_dim),
+                          {shaped ? uint32_t(std::max<int64_t>(1, c->tokens * group / std::max(1, c->batch))) : 0u, fronts});
     return FKLHIP_OK;
 }
 
@@ -110,7 +111,8 @@ template <typename A> int launch_any(const A& a, uint32_t head_dim, const Attent
 
 int run_attention(const fklhip_attention* c, const fklhip_scores* h, const fklhip_kv_cache* cache, void* stream) {
     AttentionPlan plan;
-    CHECK(plan_call(c, cache, plan));
+    const bool shaped = h && (h->cap != 0.0f || h->slopes || h->first || h->prefix);
+    CHECK(plan_call(c, cache, shaped, shaped && h->first, plan));
     NEED(std::isfinite(c->scale), "scale has to be finite");
     if (h) {
         NEED(h->cap == 0.0f || (h->cap >= 0x1p-6f && h->cap <= 0x1p9f), "cap has to be 0, or 2^-6 to 2^9");
@@ -146,7 +148,6 @@ int run_attention(const fklhip_attention* c, const fklhip_scores* h, const fklhi
         a.partial_lse = a.partial + uint64_t(plan.shares()) * 2 * plan.unit_rows * uint64_t(cache->head_dim);
     }
     Launched info;
-    const bool shaped = h && (h->cap != 0.0f || h->slopes || h->first || h->prefix);
     if (!shaped) return finish(launch_any(static_cast<const AttentionArgs&>(a), uint32_t(cache->head_dim), plan, bytes != 0, stream, info), info);
     a.slopes = h->slopes; a.positions = h->positions; a.first = h->first; a.prefix = h->prefix;
     if (h->cap != 0.0f) {
@@ -216,9 +217,10 @@ int fklhip_kv_read(const fklhip_kv_cache* cache, const int32_t* slots, int64_t t
 
 int fklhip_tree_attention_workspace(const fklhip_attention* call, const fklhip_kv_cache* cache, uint64_t* bytes) {
     NEED(bytes, "no place for the answer");
-    AttentionPlan plan;
-    CHECK(plan_call(call, cache, plan));
-    *bytes = workspace_of(*cache, plan);
+    AttentionPlan plan, shaped;
+    CHECK(plan_call(call, cache, false, false, plan));
+    CHECK(plan_call(call, cache, true, false, shaped));        // (with fronts there are shares, the same, or none)
+    *bytes = std::max(workspace_of(*cache, plan), workspace_of(*cache, shaped));
     return FKLHIP_OK;
 }
 
@@ -233,7 +235,7 @@ int fklhip_shaped_attention(const fklhip_attention* c, const fklhip_scores* scor
 
 namespace fkattn {
 
-AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim) {
+AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim, ScoreShape shape) {
     const auto log2_floor = [](uint64_t n) { uint32_t l = 0; while (n >>= 1) ++l; return l; };
     AttentionPlan p;
     p.granule_log = 7;
@@ -258,7 +260,10 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
     const bool whole = units(p.tiles) <= slots ? length * (2 * slots - units(p.tiles)) <= worth * 2 * slots : length <= 8;
     if (!whole) {
         // shares: the fewer blocks the less is converted and read, unless a share has so little that beginning and ending it counts more
-        p.tiles = most_tiles;
+        // Shaped scores of trees with up to 64 rows, 40 or fewer in the mean, have two tiles: most of four would be empty. 16 of 3 to 13 tokens
+        // behind windows of 4096, four query heads to a key head, two tiles and four, in us: e4m3 49.8, 53.8, int8 in half precision 53.8,
+        // 60.6; 5 to 13 over 500 to 4100, int8, 36.2, 43.1; but 16 tokens each 59.8, 56.6.
+        p.tiles = shape.mean_rows && rows <= 64 && shape.mean_rows <= 40 ? std::min(most_tiles, 2u) : most_tiles;
         p.waves = 4;
         while (p.tiles > 1 && units(p.tiles) * length < uint64_t(p.tiles == 4 ? 8 : 4) * slots) p.tiles /= 2;
     }
@@ -275,7 +280,15 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         const uint64_t all = units(p.tiles) * (p.lead + length);
         p.share_odd = slots == 512 && p.tiles == 1 ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
-        if (units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares() || all >= (uint64_t(1) << 30)) p.share_odd = 0;
+        bool enough = units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares();
+        // Of shaped scores fewer do: one and a half times as many, as many if none is long, half as many of prompts whose rows do not see what is
+        // in front (a block's keys are few then, and shares would end within them all the same). Measured, 32 and 8 heads of 128, e4m3, half
+        // precision (whole blocks, shares, in us): capped, one of 1100 tokens 39.2, 67.4, behind 3000 others 161, 140; one of 1500 62, 91, and
+        // 191, 195; two of 1100 67, 100; three of 500 behind 1000 to 3000 112, 124; windows of 512, one of 300 behind 3000 20.4, 29.4, of 700
+        // 32.1, 45.5, two of 1100 behind 1000 to 3000 62, 92; four documents, two of 700 49, 70, three of 1100 64.5, 98.4.
+        if (shape.mean_rows) enough |= 2 * units(p.tiles) >= 3 * uint64_t(p.shares()) || (units(p.tiles) >= p.shares() && length <= 16);
+        if (shape.fronts) enough |= 2 * units(p.tiles) >= p.shares() && rows >= 512 && length <= 64;
+        if (enough || all >= (uint64_t(1) << 30)) p.share_odd = 0;
         else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
     }
     p.many_parts = p.shares() > 16 * units(p.tiles);
