@@ -36,8 +36,9 @@
 // order of launch evens them out) a workgroup takes one whole (sequence, key head, block of rows). plan_attention chooses.
 //
 // Shaped scores are taken from the last keys to the first: a bias by distance has them rise towards the row, and the reference
-// would have to move in every step (16 trees of up to 13 behind windows of 4096, 32 and 8 heads, e4m3: 68 us that way, 50 this, and 6 for
-// joining, where reading the 138 MB takes 22: two waves to a SIMD are busy with vector instructions half of the time). A cap costs five of
+// would have to move in every step (16 trees of up to 13 behind windows of 4096, 32 and 8 heads, e4m3, four tiles: 68 us that way, 50 this;
+// with two tiles 46, and 6 for joining, where reading the 138 MB takes 22: two waves to a SIMD, vector instructions four tenths of the time,
+// waits the rest). A cap costs five of
 // those a score, two of them at a quarter of the rate: 64 sequences with 900 to 8191 keys take 115 us, as without one, and a chunk of 2048 tokens in three documents 77 us a pass,
 // vector instructions for six tenths of it (products alone: 19). There blocks of rows begin by how many keys they see, most first: 85.7 us in their order.
 // A workgroup of 128 rows with keys as halves in LDS, double buffered, took 123 us for it: all blocks are resident at once, the heaviest ends alone.
