@@ -33,11 +33,14 @@ template <int TYPE> __device__ __forceinline__ void load4(const char* row, uint3
     unpack2<TYPE>(w.x, x[0], x[1]);
     unpack2<TYPE>(w.y, x[2], x[3]);
 }
-template <int TYPE> __device__ __forceinline__ void store4(char* row, uint32_t at, const float* x) {
+// PAST: past the caches, which would keep what comes in for it.
+template <int TYPE, bool PAST> __device__ __forceinline__ void store4(char* row, uint32_t at, const float* x) {
     uint2_t w;
     w.x = pack2<TYPE>(x[0], x[1]);
     w.y = pack2<TYPE>(x[2], x[3]);
-    *reinterpret_cast<uint2_t*>(row + at * 2) = w;
+    uint2_t* const to = reinterpret_cast<uint2_t*>(row + at * 2);
+    if constexpr (PAST) __builtin_nontemporal_store(w, to);
+    else *to = w;
 }
 
 // Scale of a row from the bits of its largest magnitude: one that is infinite or NaN makes the row NaN.
@@ -285,8 +288,8 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgsOf<AXES> a) {
         if (is_q || !TO_CACHE) {
             if (p.live) {
                 char* to = out.data + token * out.token_stride + head * out.head_stride;
-                store4<TYPE>(to, p.at[0], x);
-                store4<TYPE>(to, p.at[1], x + 4);
+                store4<TYPE, AXES && HEADS != 1>(to, p.at[0], x);
+                store4<TYPE, AXES && HEADS != 1>(to, p.at[1], x + 4);
             }
         } else {
             uint32_t top = 0, code[2];
@@ -399,9 +402,11 @@ constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
 // With several axes many tokens' heads are swept (sweep_heads), by about so many waves: the fewer, the fewer read the tables' rows; fewer
-// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB), a pass: 36.8 us with 6144 waves (14 heads each), 37.2 with
-// 8192, 39.2 with 10240, 40.9 with 14336, 40.5 with 4096, 51.2 with 2048; 44.0 without sweeps, four heads to a group. 5000 tokens of 28 and 4:
-// 19.1, and 20.8, 21.1, 21.1, 19.8, 21.3; 3000 of 64 and 8: 25.4, and 24.3, 25.4, 25.6, 27.8, 29.8; 2048 of 32 and 8: 13.5 to 14.2 all.
+// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB), results kept until the next call's, a pass: 40.0 us with
+// 6144 waves (14 heads each), 40.0 with 8192, 42.4 with 10240, 42.0 with 14336, 42.8 with 4096, 52.7 with 2048. 5000 tokens of
+// 28 and 4: 18.7, and 20.6, 20.8, 20.7, 19.5, 20.3; 4000 of 32 and 8: 18.6, and 19.9 (the next three), 18.8, 21.0. Writing past the caches takes
+// 3 us off the 43 and 1.6 off 2048 tokens' 13.4, 0.9 off 5000's (but where all results go to the same place 39.5, and 36.8 without; there 44.0 without
+// sweeps). Attention of 300 to 4096 tokens reads such queries in the same time.
 constexpr uint32_t kSweepWaves = 6144;
 template <int LANES, int HEADS, int TYPE, int CODES, bool TO_CACHE, bool AXES>
 int start_heads(HeadArgsOf<AXES> a, uint32_t threads, void* stream, Launched& info) {
