@@ -474,6 +474,32 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         }
     }
 
+    // The same of all tiles, so that keys are converted once.
+    template <typename K, typename Q> __device__ __forceinline__ void products_of_all(K get_k, Q get_q, float4_t (&y)[R][2]) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) y[r][h] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i)
+#pragma unroll
+            for (int k = 0; k < S::kWords / 2; ++k) {
+                half8_t a[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Words<S::kWords> w = get_k(h, i);
+                    a[h] = halves8<CODES>(w.w[2 * k], w.w[2 * k + 1]);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const half8_t q = __builtin_bit_cast(half8_t, get_q(r, i * (S::kWords / 2) + k));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) y[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[h], q, y[r][h], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+
     // 32 keys: get_k(block, load) and get_v have their codes, get_k_scales and get_v_scales the scales of the quarter's four keys of each
     // block, get_q(tile, run) the queries, get_unit(tile) what their scores are multiplied with. after_scores runs when the
     // keys are used up. Where `masked`, sees(tile, block) has a bit for each of the quarter's four keys that the lane's row
@@ -489,7 +515,8 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of 128 elements take all registers
         // without that if queries have three parts or keys are converted: trees of up to 61 took 73 us with it, and 70 without.)
         constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * S::kLoads;
-        constexpr bool kAhead = !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped)))) && !(kShaped && R == 2 && D == 256 && PARTS == 0);
+        constexpr bool kTogether = kShaped && PARTS == 0 && R > 1;
+        constexpr bool kAhead = !kTogether && !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped)))) && !(kShaped && R == 2 && D == 256 && PARTS == 0);
         constexpr bool kHeld = R < 4 || kRuns <= 4;
         uint4_t q[kRuns];
         auto ask_q = [&](int r) {
@@ -498,10 +525,19 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         };
         if (kAhead) products(get_k, [&](int run) { return get_q(0, run); }, y);
         if (R == 1) after_scores();
+        float4_t all[kTogether ? R : 1][2];
+        if constexpr (kTogether) {
+            products_of_all(get_k, get_q, all);
+            after_scores();
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (!kAhead) products(get_k, [&](int run) { return get_q(r, run); }, y);
-            if (!kAhead && r + 1 == R) after_scores();
+            if constexpr (kTogether) {
+                y[0] = all[r][0];
+                y[1] = all[r][1];
+            }
+            if (!kAhead && !kTogether) products(get_k, [&](int run) { return get_q(r, run); }, y);
+            if (!kAhead && !kTogether && r + 1 == R) after_scores();
             if (kAhead && kHeld && r + 1 < R) ask_q(r + 1);
             float unit;
             float2_t bias = {0.0f, 0.0f};
