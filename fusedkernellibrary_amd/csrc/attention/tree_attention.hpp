@@ -515,8 +515,10 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of 128 elements take all registers
         // without that if queries have three parts or keys are converted: trees of up to 61 took 73 us with it, and 70 without.)
         constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * S::kLoads;
+        // Shaped, keys that are converted: all tiles' scores first, so that they are once (2048 tokens of a prompt 77.1 us, 77.8 tile by tile; 16 trees
+        // of 33 to 61 78.8, 80 to 84).
         constexpr bool kTogether = kShaped && PARTS == 0 && R > 1;
-        constexpr bool kAhead = !kTogether && !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped)))) && !(kShaped && R == 2 && D == 256 && PARTS == 0);
+        constexpr bool kAhead = !kTogether && !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped))));
         constexpr bool kHeld = R < 4 || kRuns <= 4;
         uint4_t q[kRuns];
         auto ask_q = [&](int r) {
