@@ -136,6 +136,32 @@ def flat(x):
     return [] if x is None else [t for t in x if t is not None] if isinstance(x, tuple) else [x]
 
 
+def test_nothing_to_do(ops, device):
+    """No tokens, no requests, no new ones, no entries: results of these sizes, and nothing else changes."""
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)      # noqa: E731
+    cache = ops.KvCache.allocate(2, 2, 16, 64, device=device)
+    for t in cache._tensors:
+        t.view(torch.uint8).fill_(5)
+    q, cos = torch.ones((0, 2, 64), dtype=BF16, device=device), torch.ones((4, 32), device=device)
+    assert [x.shape[0] for x in ops.qk_norm_rope(q, q, None, None, cos, cos, i(2, 0), axes=[0, 1] * 16)] == [0, 0]
+    assert ops.qkv_to_cache(cache, q, q, q, i(0), None, None, cos, cos, i(2, 0), axes=[0, 1] * 16).shape == q.shape
+    shaping = dict(cap=2.0, slopes=torch.ones(2, device=device), first=i(0), positions=i(0))
+    assert ops.tree_attention(q, cache, i(1, 2), i(1), i(2), max_new=1, max_context=3, **shaping).shape == q.shape
+    assert ops.tree_attention(q, cache, i(0, 2), i(0), i(1), max_new=1, max_context=3, prefix=i(0), **shaping).shape == q.shape
+    some = torch.ones((3, 2, 64), dtype=BF16, device=device)
+    for batch, max_new, width in ((0, 2, 2), (1, 0, 2), (1, 2, 0)):
+        out = ops.tree_attention(some, cache, i(batch, width), i(batch), i(batch + 1), max_new=max_new, max_context=3, cap=2.0, prefix=i(batch))
+        assert (out == 0).all()
+        t = ops.step_tables(i(batch, width), i(batch), i(batch), i(batch) + 2, i(0), i(1), page_tokens=16, tokens=3, max_new=max_new, parents=i(3))
+        assert t.q_start.tolist() == [0] * batch + [2 if batch and max_new else 0] and t.slots.tolist() == [-1] * 3 and t.held.tolist() == [0] * batch and t.available.tolist() == [0]
+        ops.kv_keep(cache, i(batch, width), i(batch), i(batch, max_new), i(batch) + 2)
+    for tokens, batch, max_new in ((0, 2, 3), (3, 0, 3), (3, 2, 0), (0, 0, 0)):
+        v = ops.verify_drafts(torch.ones((tokens, 7), device=device), i(tokens), i(batch + 1), torch.ones(tokens, device=device), max_new=max_new)
+        assert (v.count == 0).all() and v.path.shape == v.out.shape == (batch, max_new) and (v.path == -1).all() and (v.out == -1).all()
+    ops.kv_keep([], i(1, 2), i(1), i(1, 3), i(1) + 3)
+    assert all((t.view(torch.uint8) == 5).all() for t in cache._tensors)
+
+
 def test_gradients_and_tangents_are_refused(ops, device):
     calls = a_step(ops, device)
     for name, argument in (("axes", "q"), ("axes", "cos"), ("attend", "q"), ("attend", "slopes"), ("verify", "target"), ("verify", "draft"), ("verify", "uniforms")):
