@@ -474,7 +474,7 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         }
     }
 
-    // The same of all tiles, so that keys are converted once.
+    // The same of all tiles.
     template <typename K, typename Q> __device__ __forceinline__ void products_of_all(K get_k, Q get_q, float4_t (&y)[R][2]) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -515,8 +515,8 @@ template <int D, int CODES, int R, int PARTS> struct Sums {
         // The matrix unit works on the next tile's scores while this one's weights are taken. (Four tiles of 128 elements take all registers
         // without that if queries have three parts or keys are converted: trees of up to 61 took 73 us with it, and 70 without.)
         constexpr int kRuns = kQueryRegs<D, PARTS> / 4, kProducts = 2 * PARTS * S::kLoads;
-        // Shaped, keys that are converted: all tiles' scores first, so that they are once (2048 tokens of a prompt 77.1 us, 77.8 tile by tile; 16 trees
-        // of 33 to 61 78.8, 80 to 84).
+        // Shaped, keys that are converted: all tiles' products first, so that the next keys are asked for sooner (2048 tokens of a prompt 77.1 us, 77.8
+        // tile by tile; 16 trees of 33 to 61 78.8, 80 to 84; as many vector instructions, and 23 registers fewer for two tiles of 128 elements).
         constexpr bool kTogether = kShaped && PARTS == 0 && R > 1;
         constexpr bool kAhead = !kTogether && !(R == 4 && (PARTS == 3 || (D == 128 && (PARTS == 0 || kShaped))));
         constexpr bool kHeld = R < 4 || kRuns <= 4;
