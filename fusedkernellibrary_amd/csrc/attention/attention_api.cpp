@@ -88,7 +88,8 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, bool shap
     NEED(c->page_table_stride >= 0 && c->page_table_stride <= std::numeric_limits<int32_t>::max(), "page_table_stride has to be 0 to 2^31 - 1");
     const uint32_t keys = uint32_t(std::min<int64_t>(int64_t(c->max_context) + c->max_new, c->page_table_stride * cache->page_tokens));
     plan = plan_attention(uint32_t(c->batch), uint32_t(cache->kv_heads), uint32_t(c->max_new * group), keys, uint32_t(cache->head_dim),
-                          {shaped ? uint32_t(std::max<int64_t>(1, c->tokens * group / std::max(1, c->batch))) : 0u, fronts});
+                          {shaped ? uint32_t(std::max<int64_t>(1, c->tokens * group / std::max(1, c->batch))) : 0u, fronts,
+                           shaped && (cache->head_dim <= 96 || (cache->head_dim == 128 && cache->codes == FKLHIP_CODES_E4M3))});
     return FKLHIP_OK;
 }
 
@@ -263,7 +264,9 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         // Shaped scores of trees with up to 64 rows, 40 or fewer in the mean, have two tiles: most of four would be empty. 16 of 3 to 13 tokens
         // behind windows of 4096, four query heads to a key head, two tiles and four, in us: e4m3 49.8, 53.8, int8 in half precision 53.8,
         // 60.6; 5 to 13 over 500 to 4100, int8, 36.2, 43.1; but 16 tokens each 59.8, 56.6.
-        p.tiles = shape.mean_rows && rows <= 64 && shape.mean_rows <= 40 ? std::min(most_tiles, 2u) : most_tiles;
+        // All have two where three workgroups of two tiles fit a compute unit, e4m3, in us, two and four: 16 trees of 33 to 61 over 500 to 4100 74.1,
+        // 79.9; 20 to 29 behind windows 75.6, 81.4; four prompts of 100 to 130 over 2000 to 3000 51.1, 56.0; the first of the above 47.5.
+        p.tiles = shape.three || (shape.mean_rows && rows <= 64 && shape.mean_rows <= 40) ? std::min(most_tiles, 2u) : most_tiles;
         p.waves = 4;
         while (p.tiles > 1 && units(p.tiles) * length < uint64_t(p.tiles == 4 ? 8 : 4) * slots) p.tiles /= 2;
     }
@@ -278,7 +281,7 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         // Both bounds are high: of what stays in shares, one of 1100 takes 59.2 and would take 33.7, two 98 and 63, three 124 and 87,
         // two of 1500 137 and 92.
         const uint64_t all = units(p.tiles) * (p.lead + length);
-        p.share_odd = slots == 512 && p.tiles == 1 ? 3 : 1;
+        p.share_odd = slots == 512 && (p.tiles == 1 || (shape.three && p.tiles == 2)) ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
         bool enough = units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares();
         // Of shaped scores fewer do: one and a half times as many, as many if none is long, half as many of prompts whose rows do not see what is
@@ -287,7 +290,7 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         // 191, 195; two of 1100 67, 100; three of 500 behind 1000 to 3000 112, 124; windows of 512, one of 300 behind 3000 20.4, 29.4, of 700
         // 32.1, 45.5, two of 1100 behind 1000 to 3000 62, 92; four documents, two of 700 49, 70, three of 1100 64.5, 98.4.
         if (shape.mean_rows) enough |= 2 * units(p.tiles) >= 3 * uint64_t(p.shares()) || (units(p.tiles) >= p.shares() && length <= 16);
-        if (shape.fronts) enough |= 2 * units(p.tiles) >= p.shares() && rows >= 512 && length <= 64;
+        if (shape.fronts) enough |= units(p.tiles) >= 256 && rows >= 512 && length <= 64;
         if (enough || all >= (uint64_t(1) << 30)) p.share_odd = 0;
         else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
     }

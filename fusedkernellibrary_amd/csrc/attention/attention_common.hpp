@@ -88,8 +88,8 @@ struct AttentionPlan {
     uint32_t shares() const { return share_odd << share_log; }
 };
 // Of scores of another shape: a sequence's query rows to a key head in the mean (0: scores are as they are), and whether rows see nothing of
-// what is in front.
-struct ScoreShape { uint32_t mean_rows; bool fronts; };
+// what is in front, and whether a compute unit has room for three workgroups of two tiles (kThree in tree_attention.hpp).
+struct ScoreShape { uint32_t mean_rows; bool fronts, three; };
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim, ScoreShape shape);
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
 template <int D> int launch_attention(const ShapedArgs& a, const AttentionPlan& plan, void* stream, Launched& info);

@@ -715,18 +715,20 @@ template <bool DOWN> struct Pages {
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 
 // Workgroups of a compute unit. Their waves share out a segment's keys, 32 at a time.
-template <int D, int R, int WAVES> constexpr int kResident = D > 128 || WAVES == 8 ? 1 : R == 1 ? 3 : 2;
+// (Of shaped scores, two tiles: three where keys are converted or heads have 64 elements, as 168 registers do then.)
+template <int D, int R, int PARTS, bool SHAPED> constexpr bool kThree = SHAPED && R == 2 && (D <= 96 || (D == 128 && PARTS == 0));
+template <int D, int R, int PARTS, int WAVES, bool SHAPED> constexpr int kResident = D > 128 || WAVES == 8 ? 1 : R == 1 || kThree<D, R, PARTS, SHAPED> ? 3 : 2;
 
-// Joins a workgroup's waves, kAtOnce<D, R> tiles at a time, and writes the rows.
-template <int D, int R> constexpr int kAtOnce = R > 1 && D <= 128 ? 2 : 1;
+// Joins a workgroup's waves, kAtOnce tiles at a time, and writes the rows. (Of two tiles one, where LDS is for three workgroups.)
+template <int D, int R, int PARTS, bool SHAPED> constexpr int kAtOnce = R > 1 && D <= 128 && !kThree<D, R, PARTS, SHAPED> ? 2 : 1;
 template <int D> constexpr int kRowFloats = D + 4;                 // of a row in LDS: 16 bytes further round the banks than the last
-template <int WAVES, int D, int CODES, int R, int PARTS>
+template <int WAVES, bool SHAPED, int D, int CODES, int R, int PARTS>
 __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, PARTS>& sums, char* space, float (&joined_m)[WAVES][R * 16], float (&joined_l)[WAVES][R * 16]) {
     using S = Shape<D>;
     Args& a = kernel_args();
     const uint32_t thread = thread_here(), lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), col = lane & 15, quarter = lane >> 4;
     const uint32_t share = own_share(a);
-    constexpr int kTilesAtOnce = kAtOnce<D, R>, kRows = kTilesAtOnce * 16;
+    constexpr int kTilesAtOnce = kAtOnce<D, R, PARTS, SHAPED>, kRows = kTilesAtOnce * 16;
     float(*joined)[kRows * kRowFloats<D>] = reinterpret_cast<float(*)[kRows * kRowFloats<D>]>(space);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -792,12 +794,12 @@ __device__ __forceinline__ void join_waves(const Segment& x, Sums<D, CODES, R, P
 }
 
 template <int D, int CODES, int R, int PARTS, int WAVES, bool SHAPED>
-__global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_attention(const ArgsOf<SHAPED>) {
+__global__ __launch_bounds__(WAVES * 64, (kResident<D, R, PARTS, WAVES, SHAPED>)) void k_tree_attention(const ArgsOf<SHAPED>) {
     using S = Shape<D>;
     constexpr int kRegs = kQueryRegs<D, PARTS>, kRuns = kRegs / 4;
     // One tile's rows: in registers. More: in LDS, whose place the joining of the waves takes afterwards.
     constexpr bool kInLds = R > 1;
-    constexpr uint32_t kJoin = WAVES * kAtOnce<D, R> * 16 * kRowFloats<D> * 4, kQueries = kInLds ? R * kRuns * 1024 : 0;
+    constexpr uint32_t kJoin = WAVES * kAtOnce<D, R, PARTS, SHAPED> * 16 * kRowFloats<D> * 4, kQueries = kInLds ? R * kRuns * 1024 : 0;
     __shared__ __attribute__((aligned(16))) char space[kJoin > kQueries ? kJoin : kQueries];
     __shared__ float joined_m[WAVES][R * 16], joined_l[WAVES][R * 16];
     __shared__ float units[R * 16];
@@ -1051,7 +1053,7 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, WAVES>)) void k_tree_a
 #pragma unroll 1
         while ((SHAPED ? up : key) + kStride < x.key1) run_step(std::true_type{});
         if ((SHAPED ? up : key) < x.key1) run_step(std::false_type{});
-        join_waves<WAVES>(x, sums, space, joined_m, joined_l);
+        join_waves<WAVES, SHAPED>(x, sums, space, joined_m, joined_l);
     });
 }
 

@@ -208,6 +208,8 @@ def test_every_form(ops, device, kind, dtype, form, dim, batch, new, hq, hkv, sa
     run(ops, device, context=context, new=some, hq=hq, hkv=hkv, dim=dim, kind=kind, dtype=dtype, seed=batch, said=said, mask=mask, cap=8.0, slopes=slopes_of(hq),
         positions=ints([c + t // 2 for c, n in zip(context, some) for t in range(n)]), first=firsts(context, some, 150))
     last = fkl.last_launch()
+    if shared and form == "4x4" and (dim <= 96 or kind == E4M3):                   # (three workgroups of two tiles fit a compute unit)
+        form = "2x4"
     assert last["form"] == "shaped_attention_" + form
     assert (last["grid"][1:] == [1, 1] and last["grid"][0] >= 64) if shared else last["grid"][2] == batch
 

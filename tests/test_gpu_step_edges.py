@@ -72,19 +72,21 @@ def test_prefixes_and_first_places_at_the_ends_of_their_type(ops, device, kind, 
 
 
 @pytest.mark.parametrize("kind,dtype", [(INT8, BF16), (E4M3, F16)])
-@pytest.mark.parametrize("form,grid,new,context,hq,hkv,what", [
-    ("2x4", 512, [3, 13, 5, 8, 1, 13, 4, 9], [3000, 100, 4000, 7, 2500, 40, 0, 900], 32, 8, "window"),   # up to 52 rows, 28 in the mean
-    ("4x4", 512, [16, 13, 16, 15, 16, 16, 14, 16], [3000, 100, 4000, 7, 2500, 40, 0, 900], 32, 8, "window"),
-    ("2x4", 0, [290], [2900], 32, 8, "window"), ("4x4", 0, [1100], [130], 32, 8, "cap"), ("4x4", 0, [330, 500, 471], [1500, 1000, 1300], 32, 8, "cap"),
-    ("4x4", 512, [700], [2900], 32, 8, "cap"), ("4x4", 0, [700], [2900], 32, 8, "window"), ("4x4", 0, [700], [2900], 32, 8, "prefix")])
-def test_forms_that_shaped_scores_choose(ops, device, kind, dtype, form, grid, new, context, hq, hkv, what):
-    """Fewer tiles where most would be empty, whole blocks where shares end within them; `grid`: shares, or 0 for whole blocks."""
+@pytest.mark.parametrize("forms,new,context,what", [
+    ("2x4-512 2x4-768", [3, 13, 5, 8, 1, 13, 4, 9], [3000, 100, 4000, 7, 2500, 40, 0, 900], "window"),   # up to 52 rows, 28 in the mean
+    ("4x4-512 2x4-768", [16, 13, 16, 15, 16, 16, 14, 16], [3000, 100, 4000, 7, 2500, 40, 0, 900], "window"),
+    ("2x4-0 2x4-0", [290], [2900], "window"), ("4x4-0 2x4-0", [1100], [130], "cap"), ("4x4-0 2x4-0", [330, 500, 471], [1500, 1000, 1300], "cap"), ("4x4-512 2x4-768", [700], [2900], "cap"),
+    ("4x4-0 2x4-0", [700], [2900], "window"), ("4x4-0 2x4-0", [700], [2900], "prefix")])
+def test_forms_that_shaped_scores_choose(ops, device, kind, dtype, forms, new, context, what):
+    """Fewer tiles where most would be empty, whole blocks where shares end within them; of int8 and of e4m3, with the shares, or 0 for whole blocks."""
     import fusedkernellibrary_amd as fkl
+    hq, hkv = 32, 8
+    form, grid = forms.split()[kind == E4M3].split("-")
     first = ints([max(0, c + t + 1 - 200) for c, n in zip(context, new) for t in range(n)])
     more = dict(window=dict(first=first, slopes=slopes_of(hq)), cap=dict(cap=30.0), prefix=dict(first=first // 500 * 500, prefix=ints([c + n // 2 for c, n in zip(context, new)]), cap=10.0))[what]
-    run(ops, device, context=context, new=new, hq=hq, hkv=hkv, dim=64, page=32, kind=kind, dtype=dtype, seed=len(new), said=20000 if len(new) == 8 else None, **more)
+    run(ops, device, context=context, new=new, hq=hq, hkv=hkv, dim=128, page=32, kind=kind, dtype=dtype, seed=len(new), said=20000 if len(new) == 8 else None, **more)
     last = fkl.last_launch()
-    assert last["form"] == "shaped_attention_" + form and (last["grid"][0] == grid if grid else last["grid"][0] == hkv and last["grid"][2] == len(new))
+    assert last["form"] == "shaped_attention_" + form and (last["grid"][0] == int(grid) if int(grid) else last["grid"][0] == hkv and last["grid"][2] == len(new))
 
 
 # ---- tables -----------------------------------------------------------------------------------------------------------
