@@ -284,9 +284,9 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         p.share_odd = slots == 512 && (p.tiles == 1 || (shape.three && p.tiles == 2)) ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
         bool enough = units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares();
-        // Of shaped scores fewer do: one and a half times as many, as many if none is long, half as many of prompts whose rows do not see what is
+        // Of shaped scores fewer do: one and a half times as many, as many if none is long, 256 of prompts whose rows do not see what is
         // in front (a block's keys are few then, and shares would end within them all the same). Measured, 32 and 8 heads of 128, e4m3, half
-        // precision (whole blocks, shares, in us): capped, one of 1100 tokens 39.2, 67.4, behind 3000 others 161, 140; one of 1500 62, 91, and
+        // precision, four tiles (whole blocks, shares, in us): capped, one of 1100 tokens 39.2, 67.4, behind 3000 others 161, 140; one of 1500 62, 91, and
         // 191, 195; two of 1100 67, 100; three of 500 behind 1000 to 3000 112, 124; windows of 512, one of 300 behind 3000 20.4, 29.4, of 700
         // 32.1, 45.5, two of 1100 behind 1000 to 3000 62, 92; four documents, two of 700 49, 70, three of 1100 64.5, 98.4.
         if (shape.mean_rows) enough |= 2 * units(p.tiles) >= 3 * uint64_t(p.shares()) || (units(p.tiles) >= p.shares() && length <= 16);

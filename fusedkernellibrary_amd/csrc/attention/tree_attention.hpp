@@ -37,10 +37,10 @@
 //
 // Shaped scores are taken from the last keys to the first: a bias by distance has them rise towards the row, and the reference
 // would have to move in every step (16 trees of up to 13 behind windows of 4096, 32 and 8 heads, e4m3, four tiles: 68 us that way, 50 this;
-// with two tiles 46, and 6 for joining, where reading the 138 MB takes 22: two waves to a SIMD, vector instructions four tenths of the time,
-// waits the rest). A cap costs five of
-// those a score, two of them at a quarter of the rate: 64 sequences with 900 to 8191 keys take 115 us, as without one, and a chunk of 2048 tokens in three documents 77 us a pass,
-// vector instructions for six tenths of it (products alone: 19). There blocks of rows begin by how many keys they see, most first: 85.7 us in their order.
+// with two tiles 46, with three workgroups of them to a compute unit 42, and 6 for joining, where reading the 138 MB takes 22: vector instructions
+// 44 % of the time, waits the rest). A cap costs five of those a score, two of them at a quarter of the rate: 64 sequences with 900 to 8191
+// keys take 115 us, as without one, and a chunk of 2048 tokens in three documents 75 us a pass, vector instructions for 66 % of it (products
+// alone: 19). There blocks of rows begin by how many keys they see, most first: with four tiles 77.2, and 85.7 in their order.
 // A workgroup of 128 rows with keys as halves in LDS, double buffered, took 123 us for it: all blocks are resident at once, the heaviest ends alone.
 //
 // The running maximum is a reference m_r and not the exact maximum: weights are w = 2^(s - m) * vs, sums those of 2^(s - m), and
