@@ -109,7 +109,7 @@ def _draw(rng):
     if kind == "keep":
         new = rng.randint(2, 64)
         return case | {"batch": _log(rng, 1, 64), "new_lo": rng.randint(1, new), "new": new, "lo": rng.randint(0, 200), "hi": rng.randint(200, 1000), "hkv": hkv, "dim": dim, "page": page,
-                       "codes": rng.choice(["int8", "e4m3"]), "layers": _log(rng, 1, 16)}
+                       "codes": rng.choice(["int8", "e4m3"]), "layers": _log(rng, 1, 32)}
     new = rng.choice([1, 1, rng.randint(2, 64), _log(rng, 64, 2048)])
     tree = 1 < new <= 64 and rng.random() < 0.7
     hi = _log(rng, 16, 65536 if new <= 64 else 4096)
