@@ -168,6 +168,6 @@ def verify_drafts(target, tokens, q_start, uniforms, *, max_new: int, draft=None
 def kv_keep(caches, page_table, context, path, count) -> None:
     """Moves the rows of accepted tokens to where their sequences go on, in a cache or in those of several layers at once: what
     is at place context[b] + path[b, i] of sequence b goes to place context[b] + i, for i from 1 up to count[b]. path (as
-    verify_drafts returns it) ascends. No cache is given twice, and no two sequences share a page where something moves."""
+    verify_drafts returns it) ascends. No two caches overlap, and no two sequences share a page where something moves."""
     caches = (caches,) if isinstance(caches, KvCache) else caches
     _native.kv_keep(tuple(c._tensors for c in caches), page_table, context, path, count)

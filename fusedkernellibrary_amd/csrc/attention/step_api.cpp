@@ -16,7 +16,7 @@ int check_page(int32_t page_tokens) {
     return FKLHIP_OK;
 }
 uint32_t log_of(int32_t n) { return uint32_t(__builtin_ctz(uint32_t(n))); }
-constexpr int32_t kMostDrafts = 1024;
+constexpr int32_t kMostDrafts = 1024, kMostCaches = 1024;
 
 int check_drafts(const fklhip_drafts* d) {
     NEED(d, "no drafts");
@@ -29,6 +29,23 @@ int check_drafts(const fklhip_drafts* d) {
 }
 uint64_t sums_of(const fklhip_drafts& d) { return uint64_t(d.batch) * verify_chunks(uint32_t(d.vocab)) * 8; }
 uint64_t workspace_of(const fklhip_drafts& d) { return d.max_new ? sums_of(d) + uint64_t(d.batch) * (kVerifyRecord + uint64_t(d.max_new)) * 4 : 0; }
+
+// How far apart the nearest two of several caches' arrays of a kind begin, as a part of what such an array takes: 0 where one is given
+// twice, below 1 where two overlap. (Two waves would move the same rows.)
+double nearest_caches(const fklhip_kv_cache* caches, int32_t layers) {
+    const uint64_t rows = uint64_t(caches->pages) * uint64_t(caches->kv_heads) * uint64_t(caches->page_tokens), codes = rows * uint64_t(caches->head_dim);
+    uintptr_t at[kMostCaches];
+    double nearest = HUGE_VAL;
+    for (int kind = 0; kind < 4; ++kind) {
+        for (int32_t i = 0; i < layers; ++i) {
+            const fklhip_kv_cache& c = caches[i];
+            at[i] = reinterpret_cast<uintptr_t>(kind == 0 ? c.k : kind == 1 ? c.v : kind == 2 ? static_cast<void*>(c.k_scale) : static_cast<void*>(c.v_scale));
+        }
+        if (!std::is_sorted(at, at + layers)) std::sort(at, at + layers);
+        for (int32_t i = 1; i < layers; ++i) nearest = std::min(nearest, double(at[i] - at[i - 1]) / double(kind < 2 ? codes : rows * 4));
+    }
+    return nearest;
+}
 
 template <typename... P> bool all_aligned(size_t n, P... p) { return (aligned(p, n) && ...); }
 
@@ -98,7 +115,7 @@ int fklhip_verify_drafts(const fklhip_drafts* d, void* stream) {
 
 int fklhip_kv_keep(const fklhip_kv_cache* caches, int32_t layers, const int32_t* page_table, int64_t page_table_stride, const int32_t* context, const int32_t* path, const int32_t* count,
                    int32_t batch, int32_t max_new, void* stream) {
-    NEED(layers >= 0 && layers <= 1024, "layers has to be 0 to 1024");
+    NEED(layers >= 0 && layers <= kMostCaches, "layers has to be 0 to 1024");
     NEED(!layers || caches, "no caches");
     NEED(batch >= 0 && batch <= 65535, "batch has to be up to 65535");
     NEED(max_new >= 0 && max_new <= 1 << 20, "max_new has to be up to 2^20");
@@ -107,13 +124,13 @@ int fklhip_kv_keep(const fklhip_kv_cache* caches, int32_t layers, const int32_t*
         const fklhip_kv_cache &c = caches[i], &first = caches[0];
         CHECK(check_cache(&c));
         NEED(c.pages == first.pages && c.kv_heads == first.kv_heads && c.page_tokens == first.page_tokens && c.head_dim == first.head_dim && c.codes == first.codes, "caches of different sizes");
-        // (two waves would move the same rows)
-        for (int32_t j = 0; j < i; ++j)
-            NEED(c.k != caches[j].k && c.v != caches[j].v && c.k_scale != caches[j].k_scale && c.v_scale != caches[j].v_scale, "the same cache twice");
     }
+    const double nearest = layers ? nearest_caches(caches, layers) : HUGE_VAL;
+    NEED(nearest > 0.0, "the same cache twice");
     if (!layers || !batch || !max_new || !page_table_stride) return FKLHIP_OK;
     NEED(page_table && context && path && count, "no page_table, no context, no path or no count");
     NEED(all_aligned(4, page_table, context, path, count), "lengths, path and page_table have to be aligned");
+    NEED(nearest >= 1.0, "caches that overlap");
     KeepArgs a{};
     const Cache c = to_cache(caches[0]);
     a.page_table = page_table; a.context = context; a.path = path; a.count = count;

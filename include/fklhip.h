@@ -309,7 +309,7 @@ int fklhip_verify_drafts(const fklhip_drafts *drafts, void *stream);
  * 1 <= i < count[b], what is at place context[b] + path[b][i] of sequence b (its page table as in fklhip_attention) goes to place
  * context[b] + i, codes and scales as they are. path[b] (of max_new entries) has to ascend; an entry that is at its place already, is
  * not behind it or is max_new or more, and one whose place or page is outside of the table or the cache, moves nothing. All caches are
- * of the same sizes, none is given twice, and no two sequences have a page in common where something moves. */
+ * of the same sizes, none is given twice, no two overlap, and no two sequences have a page in common where something moves. */
 int fklhip_kv_keep(const fklhip_kv_cache *caches, int32_t layers, const int32_t *page_table, int64_t page_table_stride,
                    const int32_t *context, const int32_t *path, const int32_t *count, int32_t batch, int32_t max_new, void *stream);
 
