@@ -116,7 +116,7 @@ def tree_attention(q, cache: KvCache, page_table, context, q_start, *, max_new: 
 
     Scores of another shape: cap (2^-6 to 2^9) makes them cap * tanh(score / cap); slopes [q_heads] float32 takes off slope * (the
     row's position - the key's), which are places in the sequence or, of new tokens, positions [tokens] int32 (step_tables', of
-    trees). Rows that see other keys: none in front of place first[row] (int32; a window, the beginning of the row's document;
+    trees); a key behind its row, as a prefix has them, gains by it, as a bias of slope * (the key's position) has it. Rows that see other keys: none in front of place first[row] (int32; a window, the beginning of the row's document;
     none of a sequence's rows sees what is in front of its first row's, and nothing of that is read), or, without a mask, all in
     front of place prefix[b] (int32) besides those that they see anyway."""
     return _native.tree_attention(q, cache._tensors, page_table, context, q_start, max_new, max_context, mask, scale, out, lse, cap, slopes, positions, first, prefix)

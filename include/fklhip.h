@@ -237,7 +237,9 @@ int fklhip_tree_attention(const fklhip_attention *call, const fklhip_kv_cache *c
 /* The same with scores of another shape, s = cap tanh(scale q.k / cap) - slope distance, and rows that see other keys.
  *   cap      0: no tanh; else 2^-6 to 2^9
  *   slopes   one for each query head, or NULL. The distance is the row's position less the key's: places in the sequence, or, of
- *            new tokens, positions[row] (a tree's tokens: context + depth; 0 to 2^30) where they are given. Slopes are finite.
+ *            new tokens, positions[row] (a tree's tokens: context + depth; 0 to 2^30) where they are given. Slopes are finite. The
+ *            distance has a sign: of a key behind its row, which a prefix lets the row see, it is below 0, and such a key gains what one as
+ *            far in front loses. (A row's weights are those of slope * (the key's position) added to its scores.)
  *   first    of each row: it sees no key in front of place first[row] (a window, the beginning of its document). No row of
  *            a sequence sees a key in front of its first row's; what is in front of that is not read.
  *   prefix   of each sequence, without a mask: all of its rows see all keys in front of place prefix[b].
