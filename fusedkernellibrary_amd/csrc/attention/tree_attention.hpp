@@ -994,8 +994,10 @@ __global__ __launch_bounds__(WAVES * 64, (kResident<D, R, PARTS, WAVES, SHAPED>)
                     for (int w = 0; w < S::kWords; ++w) v[h][i].w[w] &= keep;
             }
         };
-        // Scores in units of log2: the tanh, cap (1 - 2 / (1 + e^(2 s / cap))), whose error is that of 1 / (1 + e), 2^-23 of the cap, so at
-        // most 2^-13 at the largest cap, 2^9 (in units of log2; half precision's rounding of weights is 2^-11); and the distance's part.
+        // Scores in units of log2: the tanh, cap (1 - 2 r), r = 1 / (1 + e^(2 s / cap)). Its sum, reciprocal (to a unit in the last place) and
+        // exponential leave r off by 3.5 2^-24 at most, so the result by twice that and what its own roundings add: 2^-20.5 of the cap (measured
+        // 2^-22), which is 2^-11 in units of log2 at the largest, 2^9, where half precision's rounding of weights is 2^-11 as well; and the
+        // distance's part.
         const auto shape = [&] {
             if constexpr (!SHAPED) {
                 return nullptr;
