@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_keep(const KeepArgs a) {
     const KeepCache& c = a.caches[blockIdx.z];
     const int32_t have = a.context[b], kept = a.count[b];
     const uint32_t context = have < 0 ? 0u : min(uint32_t(have), 1u << 30), count = kept < 0 ? 0u : min(uint32_t(kept), a.max_new);
-    const uint32_t dim = a.head_dim, pieces = dim / 8, quads = dim / 4;
+    const uint32_t dim = a.head_dim;
     for (uint32_t i0 = 1; i0 < count; i0 += kAtOnce) {
         // a lane finds a token's move
         Move m{0, 0};
