@@ -89,7 +89,7 @@ int plan_call(const fklhip_attention* c, const fklhip_kv_cache* cache, bool shap
     const uint32_t keys = uint32_t(std::min<int64_t>(int64_t(c->max_context) + c->max_new, c->page_table_stride * cache->page_tokens));
     plan = plan_attention(uint32_t(c->batch), uint32_t(cache->kv_heads), uint32_t(c->max_new * group), keys, uint32_t(cache->head_dim),
                           {shaped ? uint32_t(std::max<int64_t>(1, c->tokens * group / std::max(1, c->batch))) : 0u, fronts,
-                           shaped && (cache->head_dim <= 96 || (cache->head_dim == 128 && cache->codes == FKLHIP_CODES_E4M3))});
+                           shaped && three_of_two_tiles(cache->head_dim, !code_products(cache->head_dim, cache->codes))});
     return FKLHIP_OK;
 }
 

@@ -87,8 +87,13 @@ struct AttentionPlan {
     bool many_parts;
     uint32_t shares() const { return share_odd << share_log; }
 };
+// Whether attention's products are taken on a cache's codes as they are (kCodeProducts in tree_attention.hpp), or on keys as halves.
+constexpr bool code_products(int head_dim, int codes) { return codes == FKLHIP_CODES_INT8 && head_dim % 64 == 0; }
+// Whether a compute unit has room for three workgroups of two tiles with shaped scores: where keys are converted or heads have 64 elements, as
+// 168 registers do then.
+constexpr bool three_of_two_tiles(int head_dim, bool converted) { return head_dim <= 96 || (head_dim == 128 && converted); }
 // Of scores of another shape: a sequence's query rows to a key head in the mean (0: scores are as they are), and whether rows see nothing of
-// what is in front, and whether a compute unit has room for three workgroups of two tiles (kThree in tree_attention.hpp).
+// what is in front, and three_of_two_tiles.
 struct ScoreShape { uint32_t mean_rows; bool fronts, three; };
 AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t keys, uint32_t head_dim, ScoreShape shape);
 template <int D> int launch_attention(const AttentionArgs& a, const AttentionPlan& plan, void* stream, Launched& info);
