@@ -284,12 +284,16 @@ AttentionPlan plan_attention(uint32_t batch, uint32_t kv_heads, uint32_t rows, u
         p.share_odd = slots == 512 && (p.tiles == 1 || (shape.three && p.tiles == 2)) ? 3 : 1;
         p.share_log = p.share_odd == 3 || slots == 256 ? 8 : 9;
         bool enough = units(p.tiles) >= uint64_t(batch == 1 ? 2 : 4) * p.shares();
-        // Of shaped scores fewer do: one and a half times as many, as many if none is long, 256 of prompts whose rows do not see what is
-        // in front (a block's keys are few then, and shares would end within them all the same). Measured, 32 and 8 heads of 128, e4m3, half
-        // precision, four tiles (whole blocks, shares, in us): capped, one of 1100 tokens 39.2, 67.4, behind 3000 others 161, 140; one of 1500 62, 91, and
-        // 191, 195; two of 1100 67, 100; three of 500 behind 1000 to 3000 112, 124; windows of 512, one of 300 behind 3000 20.4, 29.4, of 700
-        // 32.1, 45.5, two of 1100 behind 1000 to 3000 62, 92; four documents, two of 700 49, 70, three of 1100 64.5, 98.4.
-        if (shape.mean_rows) enough |= 2 * units(p.tiles) >= 3 * uint64_t(p.shares()) || (units(p.tiles) >= p.shares() && length <= 16);
+        // Of shaped scores fewer do: as many if none is long; one and a half times as many of prompts, or where rows do not see what is in front; 256
+        // of prompts then (a block's keys are few, and shares would end within them all the same). Measured, 32 and 8 heads of 128, e4m3, half
+        // precision, four tiles, which such prompts had then (whole blocks, shares, in us): capped, one of 1100 tokens 39.2, 67.4, behind 3000 others
+        // 161, 140; one of 1500 62, 91, and 191, 195; two of 1100 67, 100; three of 500 behind 1000 to 3000 112, 124; windows of 512, one of 300 behind
+        // 3000 20.4, 29.4, of 700 32.1, 45.5, two of 1100 behind 1000 to 3000 62, 92; four documents, two of 700 49, 70, three of 1100 64.5, 98.4.
+        // Single tokens and trees that see all have shares, as one long sequence among short ones would end alone, and the host knows the
+        // longest only. Capped, bfloat16, in the forms that they have now: 64 tokens, 20 heads of 128, int8, one over 131072 and the others
+        // over 1000 967, 195; evenly up to 8000 271, 263; up to 2500 93, 97; 48, 16 and 8 heads of 256, evenly up to 20000 456, 393. 48 trees of 30, 32 and 8
+        // heads of 128, evenly up to 4000 152, 143, up to 2000 90, 95, one over 16000 and the others over 1000 331, 108; in windows of 512 60, 75.
+        if (shape.mean_rows) enough |= (2 * units(p.tiles) >= 3 * uint64_t(p.shares()) && (rows >= 512 || shape.fronts)) || (units(p.tiles) >= p.shares() && length <= 16);
         if (shape.fronts) enough |= units(p.tiles) >= 256 && rows >= 512 && length <= 64;
         if (enough || all >= (uint64_t(1) << 30)) p.share_odd = 0;
         else if (all < uint64_t(2) * p.shares()) p.share_log = log2_floor(all / 2), p.share_odd = 1;
