@@ -402,7 +402,7 @@ constexpr int kManyHeads = 4, kManyToCache = 2, kManyRead = 2;
 constexpr uint32_t smallest_group(uint32_t lanes) { return lanes * 4 < 64 ? 64 : lanes * 4; }
 
 // With several axes many tokens' heads are swept, chunk by chunk, by about so many waves: the fewer, the fewer read the tables' rows; fewer
-// than that wait. 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB), results kept until the next call's, a pass: 40.0 us with
+// than that wait. Without the write, 8191 tokens of 32 and 8 heads of 128, three axes in turn (172 MB), results kept until the next call's, a pass: 40.0 us with
 // 6144 waves (14 heads each), 40.0 with 8192, 42.4 with 10240, 42.0 with 14336, 42.8 with 4096, 52.7 with 2048. 5000 tokens of
 // 28 and 4: 18.7, and 20.6, 20.8, 20.7, 19.5, 20.3; 4000 of 32 and 8: 18.6, and 19.9 (the next three), 18.8, 21.0. Writing past the caches takes
 // 3 us off the 43 and 1.6 off 2048 tokens' 13.4, 0.9 off 5000's (but where all results go to the same place 39.5, and 36.8 without; there 44.0 without
